@@ -420,6 +420,25 @@ int mr_rope(void* x_bf16, int64_t ld, int64_t T, int S, int n_heads, int head_di
             const float* cos_sin, int backward, void* stream);
 
 /*
+ * Rotary positions of any layout on the first n_heads heads of the T rows of
+ * x (dtype; leading dimension ldx), row t at positions[t]:
+ *   theta = positions[t] frequencies[i],  i < rotary_dim / 2 (device float64),
+ *   (a, b) -> scale (a cos theta - b sin theta, a sin theta + b cos theta),
+ * pairs (a, b) = (x_i, x_{i + rotary_dim/2}) (MR_ROPE_HALF) or (x_2i, x_{2i+1})
+ * (MR_ROPE_INTERLEAVED) of a head's first rotary_dim elements, the rest of the
+ * head unchanged; backward = 1 negates theta (the gradient's map). Angles are
+ * reduced in float64, so positions may be any int32. Arithmetic in fp32, one
+ * rounding. out may be x with the same leading dimension (only the rotated
+ * part is then written) or share no memory with it (the whole heads are
+ * written); what lies beyond the n_heads heads is neither read nor written.
+ * Beside mr_rope: the mlx rope's traditional, dims, base/freqs and offset forms.
+ */
+enum { MR_ROPE_HALF = 0, MR_ROPE_INTERLEAVED = 1 };
+int mr_rope_positions(const void* x, int dtype, int64_t ldx, int64_t T, int n_heads, int head_dim,
+                      const int32_t* positions, const double* frequencies, int rotary_dim, int pairing,
+                      float scale, int backward, void* out, int64_t ldo, void* stream);
+
+/*
  * Split precision for the attention (the reference's three-product remedy,
  * DOCUMENTATION.md:885-925, carried through the scaled-dot-product attention
  * of mround/pipeline/blocks.py:605): fp32 q/k/v rows x [T, ldx] (the split

@@ -40,6 +40,7 @@ __all__ = [
     "pack_codes",
     "packed_width",
     "quantize_pack",
+    "rope_positions",
     "to_affine",
     "unpack_codes",
 ]
@@ -92,6 +93,7 @@ _SIGNATURES = {
     "mr_split_bf16": (_I, [_P, _L, _L, _L, _I, _P, _L, _P, _L, _P]),
     "mr_swiglu_split": (_I, [_P, _L, _L, _P, _P, _P, _P]),
     "mr_rope": (_I, [_P, _L, _L, _I, _I, _I, _P, _I, _P]),
+    "mr_rope_positions": (_I, [_P, _I, _L, _L, _I, _I, _P, _P, _I, _I, _F, _I, _P, _L, _P]),
     "mr_attn_fwd": (_I, [_P, _L, _I, _I, _I, _I, _I, _F, _P, _L, _P, _P]),
     "mr_attn_fwd_split": (_I, [_P, _P, _L, _I, _I, _I, _I, _I, _F, _P, _L, _P, _L, _P, _P]),
     "mr_rope_split": (_I, [_P, _L, _L, _I, _I, _I, _I, _P, _P, _P, _L, _P]),
@@ -192,6 +194,27 @@ def _rows_ptr(t: torch.Tensor | None) -> int | None:
     if t.dim() != 2 or t.stride(1) != 1:
         raise KernelError("a matrix operand must be 2-D with contiguous rows")
     return t.data_ptr()
+
+
+def _ld(t: torch.Tensor | None) -> int:
+    """A matrix operand's leading dimension (0 for None). A single row's stride
+    says nothing: torch leaves any value there."""
+    if t is None:
+        return 0
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _one_device(name: str, *tensors: torch.Tensor | None) -> None:
+    """Refuse operands that do not share the current device: the launch goes to
+    its stream, and the pointers would be another device's."""
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise KernelError("tensors passed to the HIP library must live on a ROCm device")
+        if t.get_device() != torch._C._cuda_getDevice():
+            raise KernelError(f"{name}: every tensor must live on the current device "
+                              f"(cuda:{torch._C._cuda_getDevice()}), got one on {t.device}")
 
 
 def _f32(t: torch.Tensor | None, name: str) -> torch.Tensor | None:
@@ -566,6 +589,35 @@ def rope(x, *, seq_len, n_heads, head_dim, cos_sin, backward=False) -> None:
     rc = lib().mr_rope(_ptr(x), x.stride(0), T, seq_len, n_heads, head_dim, _ptr(_f32(cos_sin, "cos_sin")),
                        int(backward), _stream(x))
     _check(rc, "mr_rope")
+
+
+ROPE_PAIRING = {"half": 0, "interleaved": 1}
+
+
+def rope_positions(x, positions, frequencies, *, n_heads, head_dim, pairing="half", scale=1.0, backward=False,
+                   out=None) -> None:
+    """``mr_rope_positions``: rotate the first ``n_heads`` heads of rows ``x``
+    ``[T, >= n_heads head_dim]`` (float32, bfloat16 or float16, rows may be
+    strided), token t at ``positions[t]`` (int32), by the angles ``positions[t] *
+    frequencies[i]`` (float64 ``[r/2]``, see
+    :func:`~mround_amd.pipeline.block.rope_frequencies`); the first r elements of
+    a head rotate, paired by halves or neighbours, times ``scale``. In place,
+    or into ``out`` (its heads whole). ``backward`` maps gradients."""
+    if pairing not in ROPE_PAIRING:
+        raise KernelError(f"rope_positions: pairing must be 'half' or 'interleaved', got {pairing!r}")
+    if positions.dtype != torch.int32 or frequencies.dtype != torch.float64:
+        raise KernelError("rope_positions: positions must be int32 and frequencies float64, got "
+                          f"{positions.dtype} and {frequencies.dtype}")
+    out = x if out is None else out
+    if x.dim() != 2 or out.dim() != 2 or x.shape[0] != positions.numel() or out.shape[0] != x.shape[0]:
+        raise KernelError("rope_positions: x and out are rows, one position each")
+    if out.dtype != x.dtype or min(x.shape[1], out.shape[1]) < n_heads * head_dim:
+        raise KernelError(f"rope_positions: x and out must share a dtype and hold {n_heads} heads of {head_dim}")
+    _one_device("rope_positions", x, positions, frequencies, out)
+    rc = lib().mr_rope_positions(
+        _rows_ptr(x), dtype_code(x.dtype), _ld(x), x.shape[0], n_heads, head_dim, _ptr(positions), _ptr(frequencies),
+        2 * frequencies.numel(), ROPE_PAIRING[pairing], scale, int(backward), _rows_ptr(out), _ld(out), _stream(x))
+    _check(rc, "mr_rope_positions")
 
 
 def attn_fwd(qkv, *, batch, seq_len, n_heads, n_kv_heads, head_dim, scale, out, lse) -> None:
