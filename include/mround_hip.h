@@ -261,6 +261,41 @@ int mr_cross_entropy(const void* logits, int64_t ld, int64_t T, int64_t V, const
                      void* stream);
 
 /*
+ * A teacher's list: per row of logits (T, V) (dtype, leading dimension ld) the k
+ * largest, 1 <= k <= min(V, 1024), in descending order, ties to the lower index
+ * (the zeros are equal; NaN counts as the largest), as fp32 values [T, k] and
+ * int32 ids [T, k], and, if lse is non-NULL, lse[t] = log sum_i exp(logits[t, i]
+ * / temperature).
+ */
+int mr_top_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, int k, float temperature,
+                  float* values, int32_t* ids, float* lse, void* stream);
+
+/*
+ * Distillation from a teacher's top logits: the divergence of the student's
+ * p = softmax(logits / temperature) from the teacher's list top_values at
+ * top_ids (both [T, k], k <= 1024; V <= 2^20). With top_lse (the teacher's
+ * log-sum-exp at this temperature, as mr_top_logits gives it)
+ *   q_j = exp(top_values_j / temperature - top_lse), q_R = max(0, 1 - sum q_j)
+ * and the unlisted vocabulary is one outcome more, of probabilities q_R and p_R;
+ * with top_lse NULL q is the softmax of the list alone and q_R = 0:
+ *   row_loss = sum_j q_j log(q_j / p_j) + q_R log(q_R / p_R).
+ * loss_out, if non-NULL, is scale * sum_t row_loss[t] (fixed-order fp64 sum);
+ * dlogits, if non-NULL, the gradient of that with respect to the logits, in
+ * their dtype, and may be the logits themselves (the same leading dimension).
+ * Negative ids are absent entries (a list may be shorter than k, and lie
+ * anywhere in its row); a row without entries has loss 0 and a zero gradient.
+ * An id >= V or one listed twice makes its row's loss and gradient NaN. Where no
+ * unlisted logit is above minus infinity the term of the rest is left out.
+ * Terms with q_j = 0 count nothing; a listed logit of minus infinity with
+ * q_j > 0 makes the loss infinite.
+ * Beside mr_cross_entropy as the objective the scores are gradients of
+ * (mround/pipeline/scoring.py:183-192).
+ */
+int mr_distill(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, const float* top_values,
+               const int32_t* top_ids, int k, const float* top_lse, float temperature, float scale,
+               float* row_loss, float* loss_out, void* dlogits, int64_t ldd, void* stream);
+
+/*
  * Embedding lookup into the fp32 residual stream: out[t, :] = table[ids[t], :]
  * (table (V, H) in dtype, leading dimension ldt; out leading dimension ldo).
  * An id outside [0, V) yields a NaN row. Replaces the model's embedding

@@ -1,0 +1,853 @@
+// A teacher's top logits and the distillation loss against them, for gfx950.
+//
+// Top logits: the k largest of a row in order, ties to the lower index, and the
+// row's log-sum-exp at a temperature. The teacher's list of a position.
+//
+// Distillation: with student logits z, u = z / T, p = softmax(u), and the
+// teacher's list t_j at ids S,
+//   whole = false (the teacher's log-sum-exp L at T is given):
+//     q_j = exp(t_j / T - L), q_R = max(0, 1 - sum q_j): the vocabulary off S is
+//     one outcome more, of probability p_R = sum_{i not in S} p_i;
+//   whole = true: q = softmax(t / T) over the list, q_R = 0;
+//   loss = sum_j q_j (log q_j - log p_j) + q_R (log q_R - log p_R),
+//   dloss/dz_i = (p_i Q - q_i) / T on S,  p_i (Q - q_R / p_R) / T off S,  Q = sum q + q_R.
+//
+// Both read rows of a vocabulary and are bound by memory: a row's logits move
+// once, and its gradient once. Row sums run in fp32; the list's terms, whose
+// differences are the loss, and 1 - sum q in fp64.
+#include <cmath>
+#include <limits>
+
+#include "mr_common.h"
+
+namespace mr {
+namespace {
+
+constexpr float kInf = __builtin_inff();
+constexpr int kMaxTop = 1024;
+
+__device__ __forceinline__ uint4 ld16(const uint8_t* p) {  // any alignment
+  uint4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+
+// Elements of a 16-byte piece of type DT, widened.
+template <int DT>
+constexpr int kPiece = DT == MR_F32 ? 4 : 8;
+
+template <int DT>
+__device__ __forceinline__ void widen(uint4 r, float (&v)[kPiece<DT>]) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (DT == MR_F32) {
+      v[k] = __uint_as_float(w[k]);
+    } else if constexpr (DT == MR_BF16) {
+      v[2 * k] = __uint_as_float(w[k] << 16);
+      v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+    } else {
+      v[2 * k] = f16_to_f32(static_cast<uint16_t>(w[k] & 0xffffu));
+      v[2 * k + 1] = f16_to_f32(static_cast<uint16_t>(w[k] >> 16));
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ uint4 narrow(const float (&v)[kPiece<DT>]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (DT == MR_F32) w[k] = __float_as_uint(v[k]);
+    else if constexpr (DT == MR_BF16) w[k] = pack_bf16x2(v[2 * k], v[2 * k + 1]);
+    else w[k] = static_cast<uint32_t>(f32_to_f16(v[2 * k])) | (static_cast<uint32_t>(f32_to_f16(v[2 * k + 1])) << 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Minus infinity in every element: no part in a maximum or a sum.
+template <int DT>
+__device__ __forceinline__ uint4 no_piece() {
+  constexpr uint32_t w = DT == MR_F32 ? 0xff800000u : DT == MR_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+  return make_uint4(w, w, w, w);
+}
+
+// Piece i of a row of V elements (piece V / E is the last, partial one).
+template <int DT>
+__device__ __forceinline__ uint4 load_piece(const uint8_t* row, int64_t i, int64_t V) {
+  constexpr int E = kPiece<DT>, ES = 16 / E;
+  if ((i + 1) * E <= V) return ld16(row + i * 16);
+  uint4 r = no_piece<DT>();
+  uint32_t w[4] = {r.x, r.y, r.z, r.w};
+  const int n = static_cast<int>(V - i * E);
+#pragma unroll
+  for (int k = 0; k < E - 1; ++k) {
+    if (k >= n) continue;
+    if constexpr (ES == 4) {
+      w[k] = reinterpret_cast<const uint32_t*>(row)[i * E + k];
+    } else {
+      const uint32_t x = reinterpret_cast<const uint16_t*>(row)[i * E + k];
+      w[k >> 1] = (k & 1) ? (w[k >> 1] & 0xffffu) | (x << 16) : (w[k >> 1] & 0xffff0000u) | x;
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// exp(d / T) for d = x - max: log2(e) / T in two floats, so that the exponent's
+// error is its rounding alone (the constant's own, up to 2^-25 of it, has one
+// sign and would add up over a row). Below 2^-126 the result is zero.
+struct ExpScale {
+  float hi, lo;
+};
+__device__ __forceinline__ float exp_t(float d, ExpScale c) {
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(d, c.hi, d * c.lo));
+}
+
+// A sum of exponentials about `from`, about `to` >= from. (About minus infinity it
+// is zero, or NaN, and stays.)
+__device__ __forceinline__ float rebase(float s, float from, float to, ExpScale c) {
+  return from == -kInf ? s : s * exp_t(from - to, c);
+}
+
+ExpScale exp_scale(double temperature) {
+  // hi from below and lo above zero: minus infinity times either is minus infinity
+  const double c = 1.4426950408889634073599 / temperature;
+  float hi = static_cast<float>(c);
+  if (hi > c) hi = std::nextafter(hi, 0.0f);
+  const float lo = static_cast<float>(c - hi);
+  return {hi, lo > 0.0f ? lo : std::numeric_limits<float>::min()};
+}
+
+// ------------------------------------------------------------------ top logits --
+
+// A float's place in the order of values: greater keys are greater, the zeros
+// are equal, NaN is above all. Zero is no float's key.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(x == 0.0f ? 0.0f : x);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k == 0xffffffffu ? 0x7fc00000u : k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+constexpr int kCandidates = 2048;
+
+struct TopParams {
+  const void* x;
+  int64_t ld, V;
+  int k;
+  ExpScale c;
+  double temperature;
+  float* values;
+  int32_t* ids;
+  float* lse;
+};
+
+// One workgroup per row, which it reads once. A thread keeps the largest of its
+// even and of its odd pieces: the k-th largest of these 2 THREADS maxima (of
+// their keys' upper halves) cannot exceed the row's k-th largest logit, and few
+// logits reach it. Those lie in the pieces of the maxima that reach it, which
+// are read again (a piece or two per thread, from cache) and filtered into a
+// list in LDS that is then ordered whole. A row with more candidates than the
+// list holds (many ties), a NaN or an infinity takes the radix selection.
+template <int DT, int THREADS>
+__global__ __launch_bounds__(THREADS) void top_rows(TopParams p) {
+  constexpr int E = kPiece<DT>, ES = 16 / E, W = THREADS / 64, U = 4;
+  __shared__ unsigned long long list[kCandidates];
+  __shared__ int owners[2 * THREADS];
+  __shared__ float s_m[W], s_s[W];
+  __shared__ int counts[2][4][W];
+  __shared__ int n_owners, n_list;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = blockIdx.x, V = p.V;
+  const uint8_t* x = static_cast<const uint8_t*>(p.x) + row * p.ld * ES;
+  const int64_t pieces = (V + E - 1) / E;
+  if (tid == 0) n_owners = n_list = 0;
+
+  float top[2] = {-kInf, -kInf}, m = -kInf, s = 0.0f;
+  bool has[2] = {false, false};
+  for (int64_t i0 = tid; i0 < pieces; i0 += U * THREADS) {
+    uint4 r[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int64_t i = i0 + j * THREADS;
+      r[j] = no_piece<DT>();
+      if (i < pieces) r[j] = load_piece<DT>(x, i, V);
+    }
+    float mx[2] = {-kInf, -kInf};
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      float v[E];
+      widen<DT>(r[j], v);
+#pragma unroll
+      for (int k = 0; k < E; ++k) mx[j & 1] = fmaxf(mx[j & 1], v[k]);
+    }
+    has[0] = true;
+    has[1] = has[1] || i0 + THREADS < pieces;
+    top[0] = fmaxf(top[0], mx[0]);
+    top[1] = fmaxf(top[1], mx[1]);
+    const float mn = fmaxf(m, fmaxf(mx[0], mx[1]));
+    const float base = mn == -kInf ? 0.0f : mn;
+    if (mn > m) s = rebase(s, m, base, p.c);
+    m = mn;
+    float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      float v[E];
+      widen<DT>(r[j], v);
+#pragma unroll
+      for (int k = 0; k < E; k += 2) {
+        s0 += exp_t(v[k] - base, p.c);
+        s1 += exp_t(v[k + 1] - base, p.c);
+      }
+    }
+    s += s0 + s1;
+  }
+  {
+    float mw = m;
+    for (int off = 32; off > 0; off >>= 1) mw = fmaxf(mw, __shfl_xor(mw, off, 64));
+    s = rebase(s, m, mw, p.c);
+    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+    if (lane == 0) {
+      s_m[wave] = mw;
+      s_s[wave] = s;
+    }
+  }
+  __syncthreads();
+  m = s_m[0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) m = fmaxf(m, s_m[w]);
+  s = 0.0f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) s += rebase(s_s[w], s_m[w], m, p.c);
+  const bool odd = !(s > 0.0f && s < kInf);  // a NaN, an infinity, or minus infinity throughout
+  if (tid == 0 && p.lse) {
+    float l = static_cast<float>(static_cast<double>(m) / p.temperature + log(static_cast<double>(s)));
+    if (odd) l = m;  // (a NaN is the list's first entry, which tells)
+    p.lse[row] = l;
+  }
+
+  // The largest 16-bit key that k of the maxima reach, two bits at a time.
+  uint32_t tau = 0;
+  {
+    const uint32_t k0 = has[0] ? order_key(top[0]) >> 16 : 0, k1 = has[1] ? order_key(top[1]) >> 16 : 0;
+    for (int shift = 14, step = 0; shift >= 0; shift -= 2, ++step) {
+      int(&cnt)[4][W] = counts[step & 1];
+#pragma unroll
+      for (uint32_t d = 1; d < 4; ++d) {
+        const uint32_t t = tau | (d << shift);
+        const int c = __popcll(__ballot(k0 >= t)) + __popcll(__ballot(k1 >= t));
+        if (lane == 0) cnt[d][wave] = c;
+      }
+      __syncthreads();
+      uint32_t best = 0;
+#pragma unroll
+      for (uint32_t d = 1; d < 4; ++d) {
+        int c = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) c += cnt[d][w];
+        if (c >= p.k) best = d;
+      }
+      tau |= best << shift;
+    }
+    if (!odd) {
+      if (k0 >= tau && has[0]) owners[atomicAdd(&n_owners, 1)] = 2 * tid;
+      if (k1 >= tau && has[1]) owners[atomicAdd(&n_owners, 1)] = 2 * tid + 1;
+    }
+  }
+  __syncthreads();
+  bool listed = false;
+  if (!odd) {
+    const int per = static_cast<int>((pieces + 2 * THREADS - 1) / (2 * THREADS));
+    const int total = n_owners * per;
+    for (int q = tid; q < total; q += THREADS) {
+      const int o = q / per, j = q - o * per, own = owners[o];
+      const int64_t i = (own >> 1) + static_cast<int64_t>(2 * j + (own & 1)) * THREADS;
+      if (i >= pieces) continue;
+      float v[E];
+      widen<DT>(load_piece<DT>(x, i, V), v);
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        const uint32_t key = order_key(v[k]);
+        if (key >> 16 >= tau && i * E + k < V) {
+          const int at = atomicAdd(&n_list, 1);
+          if (at < kCandidates)
+            list[at] = (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(i * E + k));
+        }
+      }
+    }
+    __syncthreads();
+    listed = n_list <= kCandidates;
+  }
+  int n = n_list;
+  if (!listed) {
+    // Radix selection of the k-th largest key, a byte at a time from the top;
+    // then every greater key and the first of the equal ones.
+    __shared__ int hist[256];
+    __shared__ uint32_t s_digit;
+    __shared__ int s_need;
+    uint32_t prefix = 0;
+    int need = p.k;
+    auto elem = [&](int64_t i) __attribute__((always_inline)) { return load_elem<DT>(x, i); };
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
+      __syncthreads();
+      for (int64_t i0 = 0; i0 < V; i0 += THREADS) {
+        const int64_t i = i0 + tid;
+        const uint32_t key = i < V ? order_key(elem(i)) : 0;
+        const bool in = i < V && (shift == 24 || key >> (shift + 8) == prefix);
+        const uint32_t digit = (key >> shift) & 255u;
+        // (lanes of one digit add once: rows of ties would queue at one counter)
+        const unsigned long long live = __ballot(in);
+        if (live) {
+          const uint32_t first = __shfl(static_cast<int>(digit), __ffsll(live) - 1, 64);
+          const unsigned long long same = __ballot(in && digit == first);
+          if (in && digit != first) atomicAdd(&hist[digit], 1);
+          if (lane == __ffsll(live) - 1) atomicAdd(&hist[first], __popcll(same));
+        }
+      }
+      __syncthreads();
+      if (tid == 0) {
+        int above = 0, d = 255;
+        while (above + hist[d] < need) above += hist[d--];
+        s_digit = d;
+        s_need = need - above;
+      }
+      __syncthreads();
+      prefix = (prefix << 8) | s_digit;
+      need = s_need;
+    }
+    if (tid == 0) {
+      n_list = 0;
+      n_owners = 0;  // of the equal keys
+    }
+    __syncthreads();
+    for (int64_t i0 = 0; i0 < V; i0 += THREADS) {
+      const int64_t i = i0 + tid;
+      const uint32_t key = i < V ? order_key(elem(i)) : 0;
+      const unsigned long long entry = (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(i));
+      if (key > prefix) list[atomicAdd(&n_list, 1)] = entry;
+      // equal keys in the order of their indexes
+      const bool equal = i < V && key == prefix;
+      const unsigned long long b = __ballot(equal);
+      if (lane == 0) counts[0][0][wave] = __popcll(b);
+      __syncthreads();
+      int before = n_owners, all = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if (w < wave) before += counts[0][0][w];
+        all += counts[0][0][w];
+      }
+      before += __popcll(b & ((1ull << lane) - 1));
+      if (equal && before < need) list[atomicAdd(&n_list, 1)] = entry;
+      __syncthreads();
+      if (tid == 0) n_owners += all;
+      __syncthreads();
+    }
+    n = p.k;
+  }
+  __syncthreads();
+  // The list in descending order. Short ones by counting, for each entry, those
+  // above it; longer ones by a bitonic network.
+  const int k_out = p.k;
+  float* values = p.values + row * k_out;
+  int32_t* ids = p.ids + row * k_out;
+  auto emit = [&](int at, unsigned long long e) __attribute__((always_inline)) {
+    values[at] = key_value(static_cast<uint32_t>(e >> 32));
+    ids[at] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(e));
+    if (at == 0 && odd && p.lse && static_cast<uint32_t>(e >> 32) == 0xffffffffu) p.lse[row] = __builtin_nanf("");
+  };
+  if (n <= 256) {
+    int* rank = owners;
+    for (int i = tid; i < 256; i += THREADS) rank[i] = 0;
+    __syncthreads();
+    // 64 entries a wave, the entries to compare with shared out among the waves
+    const int groups = (n + 63) / 64, parts = W / groups > 0 ? W / groups : 1;
+    for (int g = wave; g < groups * parts; g += W) {
+      const int i = (g % groups) * 64 + lane, part = g / groups;
+      const unsigned long long e = i < n ? list[i] : 0;
+      int above = 0;
+      for (int j = part; j < n; j += parts) above += list[j] > e;
+      if (i < n) atomicAdd(&rank[i], above);
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += THREADS)
+      if (rank[i] < k_out) emit(rank[i], list[i]);
+    return;
+  }
+  int size = 512;
+  while (size < n) size *= 2;
+  for (int i = n + tid; i < size; i += THREADS) list[i] = 0;
+  __syncthreads();
+  for (int width = 2; width <= size; width *= 2)
+    for (int stride = width / 2; stride > 0; stride /= 2) {
+      for (int q = tid; q < size / 2; q += THREADS) {
+        const int i = ((q & ~(stride - 1)) << 1) | (q & (stride - 1)), j = i + stride;
+        const unsigned long long a = list[i], b = list[j];
+        const bool down = (i & width) == 0;
+        if ((a < b) == down) {
+          list[i] = b;
+          list[j] = a;
+        }
+      }
+      __syncthreads();
+    }
+  for (int i = tid; i < k_out; i += THREADS) emit(i, list[i]);
+}
+
+// ---------------------------------------------------------------- distillation --
+
+constexpr int kBitmapMaxV = 1 << 20;
+
+struct DistillParams {
+  const void* z;
+  int64_t ldz;
+  int V, k;
+  const float* t;
+  const int32_t* ids;
+  const float* lse;  // null: the list is the whole distribution
+  ExpScale c;
+  double inv_t;
+  float scale;
+  float* row_loss;
+  void* dz;  // null: no gradient
+  int64_t ldd;
+};
+
+__device__ __forceinline__ float wave_max(float x) {
+  for (int off = 32; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
+  return x;
+}
+template <typename T>
+__device__ __forceinline__ T wave_sum(T x) {
+  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
+
+// The maximum or the sum of W waves' values, to every lane. (A lane reads one of
+// them: all W in every lane's registers at once, for eight such reductions,
+// made the held rows spill.)
+template <int W>
+__device__ __forceinline__ float waves_max(const float* v) {
+  float x = v[threadIdx.x % W];
+  for (int off = W / 2; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
+  return x;
+}
+template <int W, typename T>
+__device__ __forceinline__ T waves_sum(const T* v) {
+  T x = v[threadIdx.x % W];
+  for (int off = W / 2; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
+
+// One workgroup per row, the row held in registers (N pieces of 16 bytes per
+// thread, all loads in flight together) where HELD, else read twice. A bitmap of
+// the listed ids in LDS takes them out of the row (minus infinity), so the rest's
+// sum is formed of its own terms: as the total less the listed it would have no
+// digit left where the list has nearly all the mass. The listed logits are
+// gathered by the threads that hold their list entries, whose gradients are
+// written over the row's after it.
+template <int DT, int THREADS, int N, bool HELD>
+__global__ __launch_bounds__(THREADS, 4) void distill_rows(DistillParams p) {
+  constexpr int E = kPiece<DT>, ES = 16 / E, W = THREADS / 64, KE = kMaxTop / THREADS;
+  extern __shared__ uint32_t bitmap[];  // a bit per logit
+  __shared__ float s_rest[W], s_t[W], s_z[W];
+  __shared__ int s_n[W];
+  __shared__ double s_sum[W], s_list[W], s_q[W], s_a[W];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int64_t row = blockIdx.x;
+  const int V = p.V, pieces = (V + E - 1) / E;
+  const uint8_t* z = static_cast<const uint8_t*>(p.z) + row * p.ldz * ES;
+  uint8_t* dz = static_cast<uint8_t*>(p.dz) + row * p.ldd * ES;
+
+  // the list's entries of this thread
+  int id[KE];
+  float t[KE], zl[KE];
+#pragma unroll
+  for (int e = 0; e < KE; ++e) {
+    const int j = e * THREADS + tid;
+    id[e] = j < p.k ? p.ids[row * p.k + j] : -1;
+    t[e] = j < p.k ? p.t[row * p.k + j] : 0.0f;
+  }
+  for (int i = tid; i < (V + 31) / 32; i += THREADS) bitmap[i] = 0;
+  uint4 r[HELD ? N : 1] = {};
+  if constexpr (HELD) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = j * THREADS + tid;
+      r[j] = no_piece<DT>();
+      if (i < pieces) r[j] = load_piece<DT>(z, i, V);
+    }
+  }
+  __syncthreads();
+  // Entries past the vocabulary or listed twice make the row a NaN.
+  int n = 0;
+  bool bad = false;
+  float t_max = -kInf, z_max = -kInf;
+#pragma unroll
+  for (int e = 0; e < KE; ++e) {
+    zl[e] = 0.0f;
+    if (id[e] < 0) continue;
+    if (id[e] >= V) {
+      bad = true;
+      id[e] = -1;
+      continue;
+    }
+    const uint32_t bit = 1u << (id[e] & 31);
+    if (atomicOr(&bitmap[id[e] >> 5], bit) & bit) bad = true;
+    zl[e] = load_elem<DT>(z, id[e]);
+    ++n;
+    t_max = fmaxf(t_max, t[e]);
+    z_max = fmaxf(z_max, zl[e]);
+  }
+  __syncthreads();
+  // the row's pieces without the listed logits, and their maximum
+  const uint8_t* bits = reinterpret_cast<const uint8_t*>(bitmap);
+  auto unlisted = [&](uint4 q, int i, float (&v)[E]) __attribute__((always_inline)) {
+    widen<DT>(q, v);
+    const uint32_t b = E == 8 ? bits[i] : (bits[i >> 1] >> (4 * (i & 1))) & 15u;
+    if (b) {
+#pragma unroll
+      for (int k = 0; k < E; ++k)
+        if (b >> k & 1) v[k] = -kInf;
+    }
+  };
+  // (the values are unpacked anew in each pass, not kept: fresh hides that they are the same)
+  auto fresh = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < (HELD ? N : 1); ++j) asm volatile("" : "+v"(r[j].x), "+v"(r[j].y), "+v"(r[j].z), "+v"(r[j].w));
+  };
+  float rest_max = -kInf, sum = 0.0f;
+  if constexpr (HELD) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = j * THREADS + tid;
+      if (i >= pieces) continue;
+      float v[E];
+      unlisted(r[j], i, v);
+#pragma unroll
+      for (int k = 0; k < E; ++k) rest_max = fmaxf(rest_max, v[k]);
+      r[j] = narrow<DT>(v);
+    }
+  } else {
+    // (running maximum and sum, rescaled where the maximum grows)
+    constexpr int U = 4;
+    for (int i0 = tid; i0 < pieces; i0 += U * THREADS) {
+      uint4 q[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        q[j] = no_piece<DT>();
+        if (i0 + j * THREADS < pieces) q[j] = load_piece<DT>(z, i0 + j * THREADS, V);
+      }
+      float v[U][E];
+      float mx = rest_max;
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        unlisted(q[j], min(i0 + j * THREADS, pieces - 1), v[j]);
+#pragma unroll
+        for (int k = 0; k < E; ++k) mx = fmaxf(mx, v[j][k]);
+      }
+      const float base = mx == -kInf ? 0.0f : mx;
+      if (mx > rest_max) sum = rebase(sum, rest_max, base, p.c);
+      rest_max = mx;
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+#pragma unroll
+        for (int k = 0; k < E; ++k) sum += exp_t(v[j][k] - base, p.c);
+    }
+  }
+  const float own_max = rest_max;
+  rest_max = wave_max(rest_max);
+  t_max = wave_max(t_max);
+  z_max = wave_max(z_max);
+  n = __any(bad) ? -(1 << 20) : wave_sum(n);
+  if (lane == 0) {
+    s_rest[wave] = rest_max;
+    s_t[wave] = t_max;
+    s_z[wave] = z_max;
+    s_n[wave] = n;
+  }
+  __syncthreads();
+  rest_max = waves_max<W>(s_rest);
+  t_max = waves_max<W>(s_t);
+  z_max = waves_max<W>(s_z);
+  n = waves_sum<W>(s_n);
+  bad = n < 0;
+  const float rest_base = rest_max == -kInf ? 0.0f : rest_max, z_base = z_max == -kInf ? 0.0f : z_max;
+  if constexpr (HELD) {
+    float s1 = 0.0f;
+    fresh();
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float v[E];
+      widen<DT>(r[j], v);
+#pragma unroll
+      for (int k = 0; k < E; k += 2) {
+        sum += exp_t(v[k] - rest_base, p.c);
+        s1 += exp_t(v[k + 1] - rest_base, p.c);
+      }
+    }
+    sum += s1;
+  } else {
+    sum = rebase(sum, own_max, rest_max, p.c);
+  }
+  // the list: sum of q (or of its exponentials) and of q (log q - z / T)
+  double q_sum = 0.0, a_sum = 0.0;
+  double qe[KE];
+  float list_sum = 0.0f;
+  const double shift = p.lse ? static_cast<double>(p.lse[row]) : static_cast<double>(t_max) * p.inv_t;
+#pragma unroll
+  for (int e = 0; e < KE; ++e) {
+    qe[e] = 0.0;
+    if (id[e] < 0) continue;
+    const double log_q = static_cast<double>(t[e]) * p.inv_t - shift;
+    qe[e] = exp(log_q);
+    q_sum += qe[e];
+    if (qe[e] != 0.0) a_sum += qe[e] * (log_q - static_cast<double>(zl[e]) * p.inv_t);
+    list_sum += exp_t(zl[e] - z_base, p.c);
+  }
+  // (threads' sums meet in fp64: the loss is a small difference of logarithms, and
+  // a rounding of the total by 2^-24 is 2e-6 of a loss of 0.03)
+  double rest64 = wave_sum(static_cast<double>(sum)), list64 = wave_sum(static_cast<double>(list_sum));
+  q_sum = wave_sum(q_sum);
+  a_sum = wave_sum(a_sum);
+  if (lane == 0) {
+    s_sum[wave] = rest64;
+    s_list[wave] = list64;
+    s_q[wave] = q_sum;
+    s_a[wave] = a_sum;
+  }
+  __syncthreads();  // (and every read of the row's first pass is done)
+  rest64 = waves_sum<W>(s_sum);
+  list64 = waves_sum<W>(s_list);
+  sum = static_cast<float>(rest64);
+  list_sum = static_cast<float>(list64);
+  q_sum = waves_sum<W>(s_q);
+  a_sum = waves_sum<W>(s_a);
+  const float m = fmaxf(rest_max, z_max);
+  const float rest_part = rebase(sum, rest_max, m, p.c);
+  const float total = rest_part + rebase(list_sum, z_max, m, p.c);
+  const float p_rest = rest_part / total;
+  // (where no unlisted logit is above minus infinity there is no such outcome)
+  double q_rest = 0.0, q_norm = 1.0;
+  if (p.lse) {
+    q_rest = sum == 0.0f ? 0.0 : 1.0 - q_sum < 0.0 ? 0.0 : 1.0 - q_sum;
+  } else {
+    q_norm = 1.0 / q_sum;
+  }
+  const double q_all = p.lse ? q_sum + q_rest : 1.0;
+  // (last: its logarithms' registers are the row's until then)
+  auto write_loss = [&]() __attribute__((always_inline)) {
+    if (tid != 0) return;
+    double loss = 0.0;
+    if (bad) {
+      loss = __builtin_nan("");
+    } else if (n > 0) {
+      auto about_m = [&](double x, float from) { return x == 0.0 ? 0.0 : x * exp((static_cast<double>(from) - m) * p.inv_t); };
+      const double log_total = log(about_m(rest64, rest_max) + about_m(list64, z_max));
+      const double l = static_cast<double>(m) * p.inv_t + log_total;
+      loss = p.lse ? a_sum + q_sum * l : a_sum * q_norm - log(q_sum) + l;
+      if (q_rest > 0.0) {
+        const double log_rest = log(rest64) + (static_cast<double>(rest_max) - m) * p.inv_t - log_total;
+        loss += q_rest * (log(q_rest) - log_rest);
+      }
+    }
+    p.row_loss[row] = static_cast<float>(loss);
+  };
+  if (!p.dz) {
+    write_loss();
+    return;
+  }
+  const float gs = static_cast<float>(p.scale * p.inv_t);
+  // on the rest: exp(z - rest_max) g
+  float g = sum == 0.0f ? 0.0f : gs * (static_cast<float>(q_all * static_cast<double>(p_rest) - q_rest) / sum);
+  if (n == 0) g = 0.0f;
+  if (bad) g = __builtin_nanf("");
+  const bool none = n == 0;
+  auto put = [&](int i, float (&v)[E]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      v[k] = exp_t(v[k] - rest_base, p.c) * g;
+      if (none) v[k] = 0.0f;
+    }
+    const uint4 o = narrow<DT>(v);
+    if ((i + 1) * E <= V) {
+      __builtin_memcpy(dz + static_cast<int64_t>(i) * 16, &o, 16);
+    } else {
+#pragma unroll
+      for (int k = 0; k < E - 1; ++k)
+        if (i * E + k < V) store_elem<DT>(dz, static_cast<int64_t>(i) * E + k, v[k]);
+    }
+  };
+  if constexpr (HELD) {
+    fresh();
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int i = j * THREADS + tid;
+      if (i >= pieces) continue;
+      float v[E];
+      widen<DT>(r[j], v);
+      put(i, v);
+    }
+  } else {
+    constexpr int U = 4;
+    for (int i0 = tid; i0 < pieces; i0 += U * THREADS) {
+      uint4 q[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+        if (i0 + j * THREADS < pieces) q[j] = load_piece<DT>(z, i0 + j * THREADS, V);
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int i = i0 + j * THREADS;
+        if (i >= pieces) continue;
+        float v[E];
+        unlisted(q[j], i, v);
+        put(i, v);
+      }
+    }
+  }
+  __syncthreads();  // the rest's stores are done where the list's follow
+  write_loss();
+  if (none || bad) return;
+#pragma unroll
+  for (int e = 0; e < KE; ++e) {
+    if (id[e] < 0) continue;
+    const double pj = static_cast<double>(exp_t(zl[e] - m, p.c) / total);
+    store_elem<DT>(dz, id[e], gs * static_cast<float>(pj * q_all - qe[e] * q_norm));
+  }
+}
+
+// loss = scale * sum of the row losses, in a fixed order (fp64 partials).
+__global__ __launch_bounds__(1024) void sum_rows(const float* __restrict__ row_loss, int64_t T, float scale,
+                                                 float* __restrict__ loss_out) {
+  __shared__ double sm[16];
+  double acc = 0.0;
+  for (int64_t i = threadIdx.x; i < T; i += 1024) acc += static_cast<double>(row_loss[i]);
+  acc = wave_sum(acc);
+  if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (int w = 0; w < 16; ++w) t += sm[w];
+    loss_out[0] = static_cast<float>(t * static_cast<double>(scale));
+  }
+}
+
+bool element_aligned(const void* p, int es) { return reinterpret_cast<uintptr_t>(p) % es == 0; }
+
+}  // namespace
+}  // namespace mr
+
+extern "C" {
+
+int mr_top_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, int k, float temperature,
+                  float* values, int32_t* ids, float* lse, void* stream) {
+  using namespace mr;
+  clear_error();
+  if (T < 0 || V <= 0) return fail(MR_EINVAL, "mr_top_logits: bad sizes T=%lld V=%lld", static_cast<long long>(T),
+                                   static_cast<long long>(V));
+  if (!valid_dtype(dtype)) return fail(MR_EINVAL, "mr_top_logits: bad dtype %d", dtype);
+  if (k < 1 || k > kMaxTop || k > V)
+    return fail(MR_EINVAL, "mr_top_logits: k=%d must lie in [1, %d] and not pass V", k, kMaxTop);
+  if (!(temperature > 0.0f && temperature < __builtin_inff()))
+    return fail(MR_EINVAL, "mr_top_logits: the temperature must be positive and finite");
+  if (T == 0) return MR_OK;
+  if (!logits || !values || !ids) return fail(MR_EINVAL, "mr_top_logits: null pointer");
+  if (ld < V) return fail(MR_EINVAL, "mr_top_logits: the leading dimension is smaller than V");
+  if (T > 0x7fffffff || V > 0x7fffffff) return fail(MR_EINVAL, "mr_top_logits: too large");
+  const int es = dtype_bytes(dtype);
+  if (!element_aligned(logits, es) || !element_aligned(values, 4) || !element_aligned(ids, 4) || !element_aligned(lse, 4))
+    return fail(MR_EINVAL, "mr_top_logits: a pointer is not aligned to its elements");
+  {
+    const int64_t nx = ((T - 1) * ld + V) * es, no = T * k * 4;
+    if (overlap(values, no, logits, nx) || overlap(ids, no, logits, nx) || overlap(values, no, ids, no) ||
+        (lse && (overlap(lse, T * 4, logits, nx) || overlap(lse, T * 4, values, no) || overlap(lse, T * 4, ids, no))))
+      return fail(MR_EINVAL, "mr_top_logits: the outputs must not overlap the logits or each other");
+  }
+  TopParams p{logits, ld, V, k, exp_scale(temperature), temperature, values, ids, lse};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 g(static_cast<unsigned>(T));
+#define MR_TOP(DT) hipLaunchKernelGGL((top_rows<DT, 1024>), g, dim3(1024), 0, s, p)
+  if (dtype == MR_BF16) MR_TOP(MR_BF16);
+  else if (dtype == MR_F16) MR_TOP(MR_F16);
+  else MR_TOP(MR_F32);
+#undef MR_TOP
+  MR_LAUNCH_CHECK("mr_top_logits");
+  return MR_OK;
+}
+
+int mr_distill(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, const float* top_values,
+               const int32_t* top_ids, int k, const float* top_lse, float temperature, float scale, float* row_loss,
+               float* loss_out, void* dlogits, int64_t ldd, void* stream) {
+  using namespace mr;
+  clear_error();
+  if (T < 0 || V <= 0) return fail(MR_EINVAL, "mr_distill: bad sizes T=%lld V=%lld", static_cast<long long>(T),
+                                   static_cast<long long>(V));
+  if (V > kBitmapMaxV) return fail(MR_EINVAL, "mr_distill: vocabularies of more than %d", kBitmapMaxV);
+  if (!valid_dtype(dtype)) return fail(MR_EINVAL, "mr_distill: bad dtype %d", dtype);
+  if (k < 1 || k > kMaxTop) return fail(MR_EINVAL, "mr_distill: k=%d must lie in [1, %d]", k, kMaxTop);
+  if (!(temperature > 0.0f && temperature < __builtin_inff()))
+    return fail(MR_EINVAL, "mr_distill: the temperature must be positive and finite");
+  if (!row_loss || (T > 0 && (!logits || !top_values || !top_ids))) return fail(MR_EINVAL, "mr_distill: null pointer");
+  if (ld < V || (dlogits && ldd < V)) return fail(MR_EINVAL, "mr_distill: a leading dimension is smaller than V");
+  if (T > 0x7fffffff) return fail(MR_EINVAL, "mr_distill: too many rows");
+  const int es = dtype_bytes(dtype);
+  if (!element_aligned(logits, es) || !element_aligned(dlogits, es) || !element_aligned(top_values, 4) ||
+      !element_aligned(top_ids, 4) || !element_aligned(top_lse, 4) || !element_aligned(row_loss, 4) ||
+      !element_aligned(loss_out, 4))
+    return fail(MR_EINVAL, "mr_distill: a pointer is not aligned to its elements");
+  if (T > 0) {
+    // The gradient may be written over the logits (the same rows), else the
+    // outputs share nothing with what is read or each other.
+    const int64_t nz = ((T - 1) * ld + V) * es, nd = ((T - 1) * ldd + V) * es, nl = T * k * 4;
+    const void* reads[4] = {logits, top_values, top_ids, top_lse};
+    const int64_t nr[4] = {nz, nl, nl, T * 4};
+    const void* writes[3] = {dlogits, row_loss, loss_out};
+    const int64_t nw[3] = {nd, T * 4, 4};
+    for (int a = 0; a < 3; ++a) {
+      if (!writes[a]) continue;
+      for (int b = 0; b < 4; ++b) {
+        if (!reads[b] || (a == 0 && b == 0 && dlogits == logits && ldd == ld)) continue;
+        if (overlap(writes[a], nw[a], reads[b], nr[b]))
+          return fail(MR_EINVAL, "mr_distill: an output overlaps an input (the gradient may only be the logits themselves)");
+      }
+      for (int b = a + 1; b < 3; ++b)
+        if (writes[b] && overlap(writes[a], nw[a], writes[b], nw[b]))
+          return fail(MR_EINVAL, "mr_distill: the outputs overlap");
+    }
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (T > 0) {
+    DistillParams p{logits, ld, static_cast<int>(V), k, top_values, top_ids, top_lse, exp_scale(temperature),
+                    1.0 / static_cast<double>(temperature), scale, row_loss, dlogits, ldd};
+    const dim3 g(static_cast<unsigned>(T));
+    const size_t lds = static_cast<size_t>((V + 31) / 32) * 4;
+    const int64_t pieces = (V * es + 15) / 16;
+#define MR_DISTILL(DT, THREADS, N, HELD) hipLaunchKernelGGL((distill_rows<DT, THREADS, N, HELD>), g, dim3(THREADS), lds, s, p)
+    // the fewest threads that hold the row in at most 8 pieces each, then more pieces
+#define MR_DISTILL_D(DT)                                                \
+  do {                                                                  \
+    if (pieces <= 256 * 4) MR_DISTILL(DT, 256, 4, true);                \
+    else if (pieces <= 256 * 8) MR_DISTILL(DT, 256, 8, true);           \
+    else if (pieces <= 512 * 8) MR_DISTILL(DT, 512, 8, true);           \
+    else if (pieces <= 1024 * 8) MR_DISTILL(DT, 1024, 8, true);         \
+    else if (pieces <= 1024 * 14) MR_DISTILL(DT, 1024, 14, true);       \
+    else if (pieces <= 1024 * 20) MR_DISTILL(DT, 1024, 20, true);       \
+    else MR_DISTILL(DT, 1024, 1, false);                                \
+  } while (0)
+    if (dtype == MR_BF16) MR_DISTILL_D(MR_BF16);
+    else if (dtype == MR_F16) MR_DISTILL_D(MR_F16);
+    else MR_DISTILL_D(MR_F32);
+#undef MR_DISTILL_D
+#undef MR_DISTILL
+    MR_LAUNCH_CHECK("mr_distill");
+  }
+  if (loss_out) {
+    hipLaunchKernelGGL(sum_rows, dim3(1), dim3(1024), 0, s, row_loss, T, scale, loss_out);
+    MR_LAUNCH_CHECK("mr_distill");
+  }
+  return MR_OK;
+}
+
+}  // extern "C"

@@ -28,6 +28,7 @@ __all__ = [
     "cross_entropy",
     "delta_loss",
     "delta_loss_mapped",
+    "distill_loss",
     "dtype_code",
     "embed_rows",
     "fq_backward_signsgd",
@@ -42,6 +43,7 @@ __all__ = [
     "quantize_pack",
     "rope_positions",
     "to_affine",
+    "top_logits",
     "unpack_codes",
 ]
 
@@ -117,6 +119,8 @@ _SIGNATURES = {
     "mr_delta_loss_mapped": (_I, [_P, _I, _P, _L, _L, _I, _P, _I, _I, _F, _P, _L, _L, _L, _P, _P,
                                   _P]),
     "mr_cross_entropy": (_I, [_P, _L, _L, _L, _P, _F, _P, _P, _P, _L, _P]),
+    "mr_top_logits": (_I, [_P, _I, _L, _L, _L, _I, _F, _P, _P, _P, _P]),
+    "mr_distill": (_I, [_P, _I, _L, _L, _L, _P, _P, _I, _P, _F, _F, _P, _P, _P, _L, _P]),
     "mr_embed_rows": (_I, [_P, _I, _L, _L, _L, _P, _L, _P, _L, _P]),
 }
 
@@ -410,6 +414,50 @@ def cross_entropy(logits, labels, *, V, scale, row_loss, loss_out=None, dlogits=
                                 _ptr(dlogits), dlogits.stride(0) if dlogits is not None else 0,
                                 _stream(logits))
     _check(rc, "mr_cross_entropy")
+
+
+def top_logits(logits, *, V, values, ids, lse=None, temperature=1.0) -> None:
+    """``mr_top_logits``: the largest of the first ``V`` logits of each row
+    ``[T, >= V]`` (float32, bfloat16 or float16; rows may be strided) in
+    descending order, ties to the lower index: float32 ``values`` and int32
+    ``ids`` ``[T, k]``, and float32 ``lse`` ``[T]``, the row's log-sum-exp at
+    ``temperature``."""
+    T, k = values.shape
+    if ids.dtype != torch.int32 or ids.shape != values.shape:
+        raise KernelError("top_logits: ids must be int32 of the values' shape")
+    if logits.dim() != 2 or logits.shape[0] != T or logits.shape[1] < V or (lse is not None and lse.numel() != T):
+        raise KernelError(f"top_logits: logits must be [{T}, >= {V}], lse [{T}]")
+    _one_device("top_logits", logits, values, ids, lse)
+    rc = lib().mr_top_logits(_rows_ptr(logits), dtype_code(logits.dtype), _ld(logits), T, V, k, temperature,
+                             _ptr(_f32(values, "values")), _ptr(ids), _ptr(_f32(lse, "lse")), _stream(logits))
+    _check(rc, "mr_top_logits")
+
+
+def distill_loss(logits, values, ids, *, V, scale, row_loss, lse=None, temperature=1.0, loss_out=None,
+                 dlogits=None) -> None:
+    """``mr_distill``: the divergence of the softmax of ``logits`` ``[T, >= V]``
+    (float32, bfloat16 or float16; rows may be strided) from a teacher's list,
+    ``values`` at ``ids`` ``[T, k]`` as :func:`top_logits` gives them (negative
+    ids: no entry). With the teacher's ``lse`` the unlisted vocabulary is one
+    outcome more; without it the list is the whole distribution. ``dlogits`` (the
+    logits' dtype; may be ``logits``) receives the gradient of ``loss_out =
+    scale * sum(row_loss)``."""
+    T = logits.shape[0]
+    if logits.dim() != 2 or logits.shape[1] < V:
+        raise KernelError(f"distill_loss: logits must be [T, >= {V}]")
+    if values.dim() != 2 or values.shape[0] != T or ids.shape != values.shape or ids.dtype != torch.int32:
+        raise KernelError(f"distill_loss: values and int32 ids must be [{T}, k]")
+    if row_loss.numel() < T or (lse is not None and lse.numel() != T) or (loss_out is not None and loss_out.numel() < 1):
+        raise KernelError("distill_loss: one row loss and one lse per logits row, one element of loss_out")
+    if dlogits is not None and (dlogits.dtype != logits.dtype or dlogits.dim() != 2 or dlogits.shape[0] != T
+                                or dlogits.shape[1] < V):
+        raise KernelError(f"distill_loss: dlogits must be [{T}, >= {V}] of the logits' dtype")
+    _one_device("distill_loss", logits, values, ids, row_loss, lse, loss_out, dlogits)
+    rc = lib().mr_distill(_rows_ptr(logits), dtype_code(logits.dtype), _ld(logits), T, V,
+                          _ptr(_f32(values, "values")), _ptr(ids), values.shape[1], _ptr(_f32(lse, "lse")), temperature,
+                          scale, _ptr(_f32(row_loss, "row_loss")), _ptr(_f32(loss_out, "loss")), _rows_ptr(dlogits),
+                          _ld(dlogits), _stream(logits))
+    _check(rc, "mr_distill")
 
 
 def embed_rows(table, ids, out) -> None:

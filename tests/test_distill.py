@@ -1,0 +1,440 @@
+"""A row's top logits (``top_logits``) and the distillation loss against them
+(``distill_loss``), against their definitions in float64, and what they refuse.
+
+Bounds. An exponential is off by 2 units of its argument's rounding and one of
+its own; a thread adds at most V / 1024 + 8 of them in a row before the sums of
+threads meet in a tree of 10 levels: a row's sum is off by (V / 1024 + 40) 2^-24
+of itself (``unit``), its logarithm by as much. A probability carries besides
+4 |u - max| 2^-24 of its argument. Outputs round by half a unit of their type.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+import sys
+
+import numpy as np
+import pytest
+import torch
+
+from mround_amd import kernels as K
+from mround_amd.exceptions import KernelError
+from tests.helpers import dev
+
+DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def unit(V):
+    return (V / 1024 + 40) * 2.0 ** -24
+
+
+# ------------------------------------------------------------------ top logits --
+
+def ordered(z, k):
+    """ids of the k largest of each row, NaN first, ties to the lower index (a stable sort)."""
+    key = np.where(np.isnan(z), np.inf, z)
+    nan = np.isnan(z)
+    return np.stack([np.lexsort((np.arange(z.shape[1]), -key[r], ~nan[r]))[:k] for r in range(z.shape[0])])
+
+
+def run_top(z, V, k, temperature=1.0):
+    T = z.shape[0]
+    values = torch.empty(T, k, device=dev())
+    ids = torch.empty(T, k, dtype=torch.int32, device=dev())
+    lse = torch.empty(T, device=dev())
+    K.top_logits(z, V=V, values=values, ids=ids, lse=lse, temperature=temperature)
+    return values, ids, lse
+
+
+def check_top(z, k, temperature=1.0):
+    """``z`` on the CPU in its type; rows whose width is odd start off 16 bytes."""
+    values, ids, lse = run_top(z.to(dev()), z.shape[1], k, temperature)
+    z64 = z.double().numpy()
+    want = ordered(z64, k)
+    assert np.array_equal(ids.cpu().numpy(), want)
+    assert np.array_equal(values.cpu().double().numpy(), np.take_along_axis(z64, want, 1), equal_nan=True)
+    ref = torch.logsumexp(z.double() / temperature, 1)
+    got = lse.cpu().double()
+    assert torch.equal(torch.isnan(got), torch.isnan(ref))
+    finite = torch.isfinite(ref)
+    assert torch.equal(got[~finite & ~torch.isnan(ref)], ref[~finite & ~torch.isnan(ref)])
+    tol = unit(z.shape[1]) + 2.0 ** -24 * ref.abs()
+    assert bool(((got - ref).abs() <= tol)[finite].all()), float(((got - ref).abs() - tol)[finite].max())
+
+
+TOP_CASES = [(1, 1, 1), (3, 7, 7), (2, 8, 3), (5, 100, 100), (4, 1000, 1), (4, 2047, 300), (3, 2049, 1024),
+             (2, 3000, 1000), (3, 8191, 512), (2, 20000, 1024), (3, 70001, 64), (2, 151936, 64), (2, 151936, 700),
+             (1, 200001, 20)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("case", TOP_CASES, ids=lambda c: "x".join(map(str, c)))
+def test_top_logits(case, dtype):
+    T, V, k = case
+    print("case top", case, dtype, file=sys.stderr, flush=True)
+    z = (torch.randn(T, V, generator=torch.Generator().manual_seed(V + k)) * 3).to(DT[dtype])
+    check_top(z, k, temperature=1.0)
+    check_top(z, k, temperature=2.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("V", [30, 2048, 9000, 60001])
+@pytest.mark.parametrize("kind", ["equal", "two", "rising", "falling", "far", "infinite", "nan", "low", "zeros"])
+def test_top_logits_of_odd_rows(kind, V, dtype):
+    """Ties beyond any list, sorted rows, infinities, NaN, rows of the lowest values, zeros of both signs."""
+    k = min(V, 257)
+    print("case top odd", kind, V, dtype, file=sys.stderr, flush=True)
+    g = torch.Generator().manual_seed(4)
+    z = torch.randn(3, V, generator=g)
+    if kind == "equal":
+        z = torch.full((3, V), -1.5)
+    elif kind == "two":
+        z = (z > 0.3).float()
+    elif kind == "rising":
+        z = torch.arange(V).float().expand(3, V) / 64
+    elif kind == "falling":
+        z = -torch.arange(V).float().expand(3, V) / 64
+    elif kind == "far":
+        z = z * 1e4
+    elif kind == "infinite":
+        z[:, V // 3] = math.inf
+        z[1] = -math.inf
+        z[2, ::2] = -math.inf
+    elif kind == "nan":
+        z[0, V // 2] = z[0, 1] = math.nan
+        z[1, -1] = -math.nan
+        z[2, 0] = math.nan
+        z[2, 3] = math.inf
+    elif kind == "low":
+        z = torch.full((3, V), torch.finfo(DT[dtype]).min)
+        z[1, -1] = 0.0
+        z[2, : V // 2] = -math.inf
+    elif kind == "zeros":
+        z = torch.zeros(3, V)
+        z[:, 1::2] = -0.0
+    check_top(z.to(DT[dtype]), k)
+
+
+@pytest.mark.gpu
+def test_top_logits_of_strided_rows_and_offsets_past_32_bits():
+    """V of wider rows; the last row starts past 2^32 bytes."""
+    T, ld, V = 17, 1 << 27, 1001  # 4.5 GB of bfloat16
+    z = torch.full((T, ld), 50.0, dtype=torch.bfloat16, device=dev())
+    part = torch.randn(T, V, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    z[:, :V] = part.to(dev())
+    values, ids, lse = run_top(z, V, 9)
+    want = ordered(part.double().numpy(), 9)
+    assert np.array_equal(ids.cpu().numpy(), want)
+
+
+# ---------------------------------------------------------------- distillation --
+
+def reference(z, values, ids, *, scale, lse=None, temperature=1.0, upcast=torch.float64):
+    """row losses, dlogits and what bounds them need, in float64 on the CPU, by the formulas of the definition."""
+    z, t = z.to(upcast), values.to(upcast) / temperature
+    u = z / temperature
+    log_p = torch.log_softmax(u, 1)
+    p = log_p.exp()
+    T, V = z.shape
+    loss, grad = torch.zeros(T, dtype=upcast), torch.zeros(T, V, dtype=upcast)
+    size = torch.zeros(T, V, dtype=upcast)  # what of p a gradient's error scales with
+    weight = torch.zeros(T, dtype=upcast)
+    for r in range(T):
+        on = ids[r] >= 0
+        if not bool(on.any()):
+            continue
+        i = ids[r][on].long()
+        off = torch.ones(V, dtype=torch.bool)
+        off[i] = False
+        q = torch.exp(t[r][on] - lse[r].to(upcast)) if lse is not None else torch.softmax(t[r][on], 0)
+        q_rest, log_rest = 0.0, 0.0
+        if lse is not None and bool((z[r][off] > -math.inf).any()):
+            q_rest = max(0.0, float(1 - q.sum()))
+            log_rest = float(torch.logsumexp(u[r][off], 0) - torch.logsumexp(u[r], 0))
+        keep = q > 0
+        loss[r] = (q[keep] * (torch.log(q[keep]) - log_p[r][i][keep])).sum()
+        if q_rest > 0:
+            loss[r] += q_rest * (math.log(q_rest) - log_rest)
+        total = float(q.sum()) + q_rest
+        factor = total - (q_rest / math.exp(log_rest) if q_rest > 0 else 0.0)
+        grad[r] = p[r] * factor
+        size[r] = p[r] * (total + (q_rest / math.exp(log_rest) if q_rest > 0 else 0.0))
+        grad[r][i] = p[r][i] * total - q
+        size[r][i] = p[r][i] * total + q
+        weight[r] = total
+    gs = scale / temperature
+    far = (u - u.amax(1, keepdim=True)).abs()
+    return loss, grad * gs, size * gs, weight, torch.where(far < 1e30, far, torch.zeros_like(far))
+
+
+def make(T, V, k, dtype, *, seed=0, ragged=False, noise=0.5):
+    g = torch.Generator().manual_seed(seed)
+    teacher = torch.randn(T, V, generator=g) * 2 + torch.rand(T, V, generator=g) ** 64 * 8
+    z = (teacher + torch.randn(T, V, generator=g) * noise).to(DT[dtype])
+    values, ids = teacher.topk(k, 1)
+    ids = ids.int()
+    if ragged:
+        # entries absent anywhere, and rows without any
+        ids[torch.rand(T, k, generator=g) < 0.4] = -1
+        ids[::3] = -1
+    return z, values, ids, teacher
+
+
+def run(z, values, ids, *, scale, lse=None, temperature=1.0, grad=True, in_place=False, V=None):
+    zd = z.to(dev())
+    d = (zd if in_place else torch.full_like(zd, 3.0)) if grad else None
+    row, loss = torch.full((z.shape[0],), 9.0, device=dev()), torch.full((1,), 9.0, device=dev())
+    K.distill_loss(zd, values.to(dev()), ids.to(dev()), V=V or z.shape[1], scale=scale, row_loss=row,
+                   lse=None if lse is None else lse.to(dev()), temperature=temperature, loss_out=loss, dlogits=d)
+    return row, loss, d
+
+
+def check(z, values, ids, *, scale, lse=None, temperature=1.0):
+    V = z.shape[1]
+    want, grad, size, weight, far = reference(z, values, ids, scale=scale, lse=lse, temperature=temperature)
+    row, loss, d = run(z, values, ids, scale=scale, lse=lse, temperature=temperature)
+    tol = 2 * weight * unit(V) + 2.0 ** -24 * want.abs() + 1e-12
+    err = (row.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), f"loss: worst {float((err / tol).max())} of its bound"
+    assert abs(float(loss) - scale * float(row.double().sum())) <= 2.0 ** -23 * scale * float(row.double().abs().sum())
+    eps = torch.finfo(z.dtype).eps
+    gtol = 2 * size * (unit(V) + 4 * far * 2.0 ** -24) + eps / 2 * grad.abs() + 2.0 ** -25 * (z.dtype == torch.float16) \
+        + 2.0 ** -120 * scale
+    gerr = (d.cpu().double() - grad).abs()
+    assert bool((gerr <= gtol).all()), f"gradient: worst {float((gerr / gtol).max())} of its bound"
+    # the gradient over the logits, and no gradient: the same bits
+    row2, _, d2 = run(z, values, ids, scale=scale, lse=lse, temperature=temperature, in_place=True)
+    row3, _, _ = run(z, values, ids, scale=scale, lse=lse, temperature=temperature, grad=False)
+    assert torch.equal(row, row2) and torch.equal(row, row3) and torch.equal(d, d2)
+
+
+# rows, V, k: a piece, odd widths, each block size and registers a thread, rows read twice
+DISTILL_CASES = [(1, 1, 1), (3, 5, 2), (4, 100, 100), (5, 1001, 17), (2, 5000, 1024), (3, 8193, 64), (3, 16385, 300),
+                 (2, 40001, 33), (2, 90000, 8), (2, 151936, 64), (2, 151935, 64), (2, 200001, 100)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("tail", [True, False])
+@pytest.mark.parametrize("case", DISTILL_CASES, ids=lambda c: "x".join(map(str, c)))
+def test_distill(case, tail, dtype):
+    T, V, k = case
+    print("case distill", case, tail, dtype, file=sys.stderr, flush=True)
+    for temperature, ragged in ((1.0, False), (2.5, True)):
+        z, values, ids, teacher = make(T, V, k, dtype, seed=V, ragged=ragged)
+        lse = torch.logsumexp(teacher.double() / temperature, 1).float() if tail else None
+        check(z, values, ids, scale=256.0 if dtype == "f16" else 0.37, lse=lse, temperature=temperature)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_distill_with_nearly_all_mass_listed(dtype):
+    """A teacher whose rest is 1e-6 and a student whose rest is 1e-7 of the whole: formed as
+    differences of sums, neither would have a digit left."""
+    T, V, k = 4, 5000, 16
+    g = torch.Generator().manual_seed(2)
+    teacher = torch.randn(T, V, generator=g) - 25
+    teacher[:, :k] = torch.rand(T, k, generator=g) * 4
+    z = teacher.clone()
+    z[:, k:] -= 2.5
+    values, ids = teacher.topk(k, 1)
+    check(z.to(DT[dtype]), values, ids.int(), scale=1.0, lse=torch.logsumexp(teacher.double(), 1).float())
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences():
+    T, V, k, h = 3, 300, 12, 1e-4
+    for tail in (True, False):
+        z, values, ids, teacher = make(T, V, k, "f32", seed=9)
+        lse = torch.logsumexp(teacher.double() / 1.7, 1).float() if tail else None
+        kw = dict(scale=1.0, lse=lse, temperature=1.7)
+        _, _, d = run(z, values, ids, **kw)
+        cols = torch.cat([ids[0, :4].long(), torch.arange(0, V, 37)])
+        for c in cols.tolist():
+            up, down = z.double(), z.double()
+            up, down = up.clone(), down.clone()
+            up[:, c] += h
+            down[:, c] -= h
+            diff = (reference(up, values, ids, **kw)[0] - reference(down, values, ids, **kw)[0]) / (2 * h)
+            # third derivatives are below 1: h^2 / 6; float64 rounding 2^-52 / h of losses below 20
+            assert bool(((d[:, c].cpu().double() - diff).abs() <= h * h + 20 * 2.0 ** -52 / h + 4 * unit(V)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tail", [True, False])
+@pytest.mark.parametrize("V", [300, 100003])
+def test_rows_that_leave_nothing(tail, V):
+    """Empty lists, bad lists, lists of the whole vocabulary, logits of minus infinity, on and off the list."""
+    T, k = 7, 6
+    z, values, ids, teacher = make(T, V, k, "f32", seed=1)
+    ids[0] = -1                       # no entry: zero, whatever the logits
+    z[0, 5] = math.nan
+    ids[1, 3] = ids[1, 0]             # listed twice: NaN
+    ids[2, 2] = V                     # past the vocabulary: NaN
+    z[3] = -math.inf                  # the student allows the list alone
+    z[3, ids[3].long()] = 0.5
+    z[4, ids[4, 0].long()] = -math.inf  # the student excludes what the teacher expects: infinite loss
+    values[5, 1] = -math.inf          # the teacher excludes an entry
+    z[5, ids[5, 1].long()] = -math.inf
+    ids[6, 1:] = -1                   # a list of one
+    lse = torch.logsumexp(teacher.double(), 1).float() if tail else None
+    row, loss, d = run(z, values, ids, scale=1.0, lse=lse)
+    row, d = row.cpu().double(), d.cpu().double()
+    assert row[0] == 0 and bool((d[0] == 0).all())
+    for r in (1, 2):
+        assert math.isnan(row[r]) and bool(torch.isnan(d[r]).all())
+    good = [3, 4, 5, 6]
+    want, grad, size, weight, far = reference(z[good], values[good], ids[good], scale=1.0,
+                                              lse=None if lse is None else lse[good])
+    assert bool(torch.isinf(row[4])) and bool(torch.isinf(want[1]))
+    fin = [0, 2, 3]
+    err = (row[good].double() - want)[fin].abs()
+    assert bool((err <= 2 * weight[fin] * unit(V) + 2.0 ** -24 * want[fin].abs() + 1e-12).all())
+    gerr = (d[good] - grad).abs()
+    assert bool((gerr <= 2 * size * (unit(V) + 4 * far * 2.0 ** -24) + 2.0 ** -24 * grad.abs() + 2.0 ** -120).all())
+    assert bool((d[3][torch.isinf(z[3])] == 0).all())
+    assert math.isnan(float(loss))
+
+
+@pytest.mark.gpu
+def test_strided_rows_keep_what_lies_beside_them():
+    """Columns past V are neither read nor written; rows start off 16 bytes."""
+    T, V, k, ld = 5, 1003, 9, 1010
+    z, values, ids, teacher = make(T, V, k, "bf16", seed=3)
+    wide = torch.full((T, ld), math.nan, dtype=torch.bfloat16)
+    wide[:, :V] = z
+    lse = torch.logsumexp(teacher, 1)
+    row, _, d = run(wide, values, ids, scale=1.0, lse=lse, V=V)
+    want, _, dw = run(z, values, ids, scale=1.0, lse=lse)
+    assert torch.equal(row, want) and torch.equal(d[:, :V], dw) and bool((d[:, V:] == 3.0).all())
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    T, ld, V, k = 9, 1 << 27, 40001, 8  # float32: the last row starts at 4.3 GB
+    z, values, ids, teacher = make(T, V, k, "f32", seed=6)
+    wide = torch.zeros(T, ld, device=dev())
+    wide[:, :V] = z.to(dev())
+    row, loss = torch.empty(T, device=dev()), torch.empty(1, device=dev())
+    K.distill_loss(wide, values.to(dev()), ids.to(dev()), V=V, scale=1.0, row_loss=row, loss_out=loss, dlogits=wide)
+    want, _, d = run(z, values, ids, scale=1.0)
+    assert torch.equal(row, want) and torch.equal(wide[:, :V], d) and bool((wide[-1, V:] == 0).all())
+
+
+@pytest.mark.gpu
+def test_teacher_as_its_own_student():
+    """The list that ``top_logits`` gives, against the logits it came from: no divergence, no gradient."""
+    z = (torch.randn(6, 151936, generator=torch.Generator().manual_seed(12)) * 3).to(torch.bfloat16).to(dev())
+    for temperature in (1.0, 2.0):
+        values, ids, lse = run_top(z, 151936, 64, temperature)
+        row, loss, d = run(z, values, ids, scale=1.0, lse=lse, temperature=temperature)
+        # lse rounds to float32 (2^-24 of at most 16) and both sums are within their unit
+        bound = 4 * unit(151936) + 16 * 2.0 ** -24
+        assert float(row.abs().max()) <= bound
+        assert float(d.float().abs().max()) <= 2 * bound
+
+
+@pytest.mark.gpu
+def test_graph_and_side_stream():
+    """Both captured together and replayed on new logits between eager work; two streams at once."""
+    T, V, k = 33, 50257, 20
+    z = torch.empty(T, V, dtype=torch.bfloat16, device=dev())
+    values, ids, lse = torch.empty(T, k, device=dev()), torch.empty(T, k, dtype=torch.int32, device=dev()), torch.empty(T, device=dev())
+    student, row, loss, d = torch.empty_like(z), torch.empty(T, device=dev()), torch.empty(1, device=dev()), torch.empty_like(z)
+
+    def both(out):
+        K.top_logits(z, V=V, values=out[0], ids=out[1], lse=out[2])
+        K.distill_loss(student, out[0], out[1], V=V, scale=1.0 / T, row_loss=out[3], lse=out[2], loss_out=out[4],
+                       dlogits=out[5])
+
+    outs = (values, ids, lse, row, loss, d)
+    fill = lambda s: (z.copy_(torch.randn(T, V, generator=torch.Generator().manual_seed(s)) * 2),
+                      student.copy_(torch.randn(T, V, generator=torch.Generator().manual_seed(s + 1)) * 2))
+    fill(0)
+    both(outs)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        both(outs)
+    side = torch.cuda.Stream()
+    for s in (10, 20, 30):
+        fill(s)
+        want = tuple(torch.empty_like(o) for o in outs)
+        other = tuple(torch.empty_like(o) for o in outs)
+        side.wait_stream(torch.cuda.current_stream())
+        graph.replay()
+        with torch.cuda.stream(side):
+            both(other)
+        both(want)
+        torch.cuda.synchronize()
+        for a, b, c in zip(outs, want, other):
+            assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.gpu
+def test_no_rows():
+    e = lambda *s, dt=torch.float32: torch.empty(*s, dtype=dt, device=dev())
+    loss = torch.full((1,), 5.0, device=dev())
+    K.distill_loss(e(0, 10), e(0, 3), e(0, 3, dt=torch.int32), V=10, scale=1.0, row_loss=e(1), loss_out=loss)
+    assert float(loss) == 0.0
+    K.top_logits(e(0, 10), V=10, values=e(0, 3), ids=e(0, 3, dt=torch.int32))
+
+
+# ------------------------------------------------------------------- refusals --
+
+def test_top_logits_refusals_before_launch():
+    lib, P, f = K.lib(), ctypes.c_void_p, ctypes.c_float
+
+    def call(x=P(1 << 20), dt=1, ld=1000, T=4, V=1000, k=8, temp=1.0, values=P(1 << 24), ids=P(1 << 25), lse=P(1 << 26)):
+        return lib.mr_top_logits(x, dt, ld, T, V, k, f(temp), values, ids, lse, None)
+
+    for bad, word in ((dict(x=None), b"null"), (dict(values=None), b"null"), (dict(ids=None), b"null"),
+                      (dict(dt=5), b"dtype"), (dict(T=-1), b"sizes"), (dict(V=0), b"sizes"), (dict(k=0), b"k=0"),
+                      (dict(k=1025, V=2000, ld=2000), b"k=1025"), (dict(k=9, V=8), b"k=9"), (dict(ld=999), b"leading"),
+                      (dict(temp=0.0), b"temperature"), (dict(temp=math.nan), b"temperature"),
+                      (dict(temp=math.inf), b"temperature"), (dict(T=1 << 31), b"large"), (dict(x=P((1 << 20) + 1)), b"aligned"),
+                      (dict(values=P(1 << 20)), b"overlap"), (dict(ids=P(1 << 24)), b"overlap"),
+                      (dict(lse=P((1 << 25) + 4)), b"overlap")):
+        assert call(**bad) == -22, bad
+        assert word in lib.mr_last_error(), (bad, lib.mr_last_error())
+
+
+def test_distill_refusals_before_launch():
+    lib, P, f = K.lib(), ctypes.c_void_p, ctypes.c_float
+
+    def call(z=P(1 << 20), dt=0, ld=1000, T=4, V=1000, t=P(1 << 22), ids=P(1 << 23), k=8, lse=P(1 << 24), temp=1.0,
+             row=P(1 << 25), loss=P(1 << 26), d=P(1 << 27), ldd=1000):
+        return lib.mr_distill(z, dt, ld, T, V, t, ids, k, lse, f(temp), f(1.0), row, loss, d, ldd, None)
+
+    for bad, word in ((dict(z=None), b"null"), (dict(t=None), b"null"), (dict(ids=None), b"null"), (dict(row=None), b"null"),
+                      (dict(dt=-1), b"dtype"), (dict(T=-2), b"sizes"), (dict(V=0), b"sizes"),
+                      (dict(V=(1 << 20) + 1, ld=1 << 21, ldd=1 << 21), b"vocabularies"), (dict(k=0), b"k=0"),
+                      (dict(k=1025), b"k=1025"), (dict(ld=999), b"leading"), (dict(ldd=999), b"leading"),
+                      (dict(temp=-1.0), b"temperature"), (dict(T=1 << 31), b"rows"), (dict(z=P((1 << 20) + 2)), b"aligned"),
+                      (dict(d=P((1 << 20) + 4)), b"overlaps"), (dict(d=P(1 << 20), ldd=1001), b"overlaps"),
+                      (dict(row=P(1 << 22)), b"overlaps"), (dict(loss=P(1 << 25)), b"overlap"),
+                      (dict(row=P((1 << 27) + 16)), b"overlap")):
+        assert call(**bad) == -22, bad
+        assert word in lib.mr_last_error(), (bad, lib.mr_last_error())
+
+
+def test_bindings_refuse_on_the_host():
+    z, v, i = torch.zeros(4, 100), torch.zeros(4, 8), torch.zeros(4, 8, dtype=torch.int32)
+    with pytest.raises(KernelError, match="int32"):
+        K.top_logits(z, V=100, values=v, ids=i.long())
+    with pytest.raises(KernelError, match="logits must be"):
+        K.top_logits(z, V=101, values=v, ids=i)
+    with pytest.raises(KernelError, match="ROCm device"):
+        K.top_logits(z, V=100, values=v, ids=i)
+    kw = dict(V=100, scale=1.0, row_loss=torch.zeros(4))
+    with pytest.raises(KernelError, match="ids must be"):
+        K.distill_loss(z, v, i[:, :7], **kw)
+    with pytest.raises(KernelError, match="dlogits"):
+        K.distill_loss(z, v, i, dlogits=z.half(), **kw)
+    with pytest.raises(KernelError, match="one row loss"):
+        K.distill_loss(z, v, i, lse=torch.zeros(3), **kw)
+    with pytest.raises(KernelError, match="ROCm device"):
+        K.distill_loss(z, v, i, **kw)
