@@ -17,6 +17,7 @@
 // differences are the loss, and 1 - sum q in fp64.
 #include <cmath>
 #include <limits>
+#include <type_traits>
 
 #include "mr_common.h"
 
@@ -441,281 +442,503 @@ __device__ __forceinline__ T waves_sum(const T* v) {
   return x;
 }
 
-// One workgroup per row, the row held in registers (N pieces of 16 bytes per
-// thread, all loads in flight together) where HELD, else read twice. A bitmap of
-// the listed ids in LDS takes them out of the row (minus infinity), so the rest's
-// sum is formed of its own terms: as the total less the listed it would have no
-// digit left where the list has nearly all the mass. The listed logits are
-// gathered by the threads that hold their list entries, whose gradients are
-// written over the row's after it.
-template <int DT, int THREADS, int N, bool HELD>
-__global__ __launch_bounds__(THREADS, 4) void distill_rows(DistillParams p) {
-  constexpr int E = kPiece<DT>, ES = 16 / E, W = THREADS / 64, KE = kMaxTop / THREADS;
-  extern __shared__ uint32_t bitmap[];  // a bit per logit
-  __shared__ float s_rest[W], s_t[W], s_z[W];
-  __shared__ int s_n[W];
-  __shared__ double s_sum[W], s_list[W], s_q[W], s_a[W];
+// The list of a row: entry e THREADS + tid is thread tid's. Ids and teacher's
+// logits lie in LDS (behind the bitmap), a register each would not fit beside the
+// held rows; the student's logits are gathered into registers.
+template <int DT, int THREADS>
+struct List {
+  static constexpr int KE = kMaxTop / THREADS, W = THREADS / 64;
+  using Raw = typename std::conditional<DT == MR_F32, uint32_t, uint16_t>::type;
+  struct Shared {
+    float t[W], z[W];
+    int n[W];
+    double q[W], a[W], s[W], rest[W];
+  };
+  int* ids;
+  float* values;
+  Raw raw[KE];  // the listed logits, as they lie in memory
+  int n;        // entries; negative: a bad list
+  float t_max, z_max, lse;
+  double q_sum, a_sum, z_sum, shift;
+
+  __device__ __forceinline__ List(uint32_t* lds, int k) : ids(reinterpret_cast<int*>(lds)), values(reinterpret_cast<float*>(lds + k)) {}
+  // (not widened where it is loaded: that would wait for the row's pieces before it)
+  __device__ __forceinline__ float z(int e) const {
+    return DT == MR_F32 ? __uint_as_float(raw[e]) : DT == MR_BF16 ? bf16_to_f32(raw[e]) : f16_to_f32(raw[e]);
+  }
+  // f(e, id, t) for the thread's entries.
+  template <typename F>
+  __device__ __forceinline__ void each(const DistillParams& p, F f) const {
+#pragma unroll
+    for (int e = 0; e < KE; ++e) {
+      const int j = e * THREADS + static_cast<int>(threadIdx.x);
+      if (j < p.k) {
+        const int id = ids[j];
+        if (id >= 0) f(e, id, values[j]);
+      }
+    }
+  }
+  // The thread's entries, on their way while the row's loads are issued.
+  struct Entries {
+    int id[KE];
+    float t[KE];
+  };
+  __device__ __forceinline__ Entries load(const DistillParams& p, int64_t row) {
+    Entries x;
+    lse = p.lse ? p.lse[row] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < KE; ++e) {
+      const int j = e * THREADS + static_cast<int>(threadIdx.x);
+      x.id[e] = j < p.k ? p.ids[row * p.k + j] : -1;
+      x.t[e] = j < p.k ? p.t[row * p.k + j] : 0.0f;
+    }
+    return x;
+  }
+  // Marks the entries in the bitmap (clear, behind a barrier), gathers their logits
+  // and leaves the wave's counts and maximum in the block's. Entries past the
+  // vocabulary or listed twice make the row a NaN.
+  __device__ __forceinline__ void mark(const DistillParams& p, const Entries& x, const uint8_t* zrow, uint32_t* bitmap,
+                                       Shared& s) {
+    int count = 0;
+    bool bad = false;
+    float top = -kInf;
+#pragma unroll
+    for (int e = 0; e < KE; ++e) {
+      raw[e] = 0;
+      const int j = e * THREADS + static_cast<int>(threadIdx.x);
+      int id = x.id[e];
+      if (id >= p.V) {
+        bad = true;
+        id = -1;
+      }
+      if (j < p.k) {
+        ids[j] = id;
+        values[j] = x.t[e];
+      }
+      if (id < 0) continue;
+      const uint32_t bit = 1u << (id & 31);
+      if (atomicOr(&bitmap[id >> 5], bit) & bit) bad = true;
+      raw[e] = reinterpret_cast<const Raw*>(zrow)[id];
+      ++count;
+      top = fmaxf(top, x.t[e]);
+    }
+    top = wave_max(top);
+    count = __any(bad) ? -(1 << 20) : wave_sum(count);
+    if ((threadIdx.x & 63) == 0) {
+      s.t[threadIdx.x >> 6] = top;
+      s.n[threadIdx.x >> 6] = count;
+    }
+  }
+  // The wave's greatest listed logit into the block's, before a barrier; then what all came to.
+  __device__ __forceinline__ void publish(const DistillParams& p, Shared& s) {
+    float top = -kInf;
+    each(p, [&](int e, int, float) { top = fmaxf(top, z(e)); });
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0) s.z[threadIdx.x >> 6] = top;
+  }
+  __device__ __forceinline__ void collect(const Shared& s) {
+    t_max = waves_max<W>(s.t);
+    z_max = waves_max<W>(s.z);
+    n = waves_sum<W>(s.n);
+  }
+  // Sums of q (without lse: of its exponentials about the maximum), of
+  // q (log q - z / T) and of the student's exponentials about z_max. Into the
+  // block's sums with the thread's share of the rest, before a barrier; then from them.
+  __device__ __forceinline__ void sums(const DistillParams& p, float rest, Shared& s) {
+    q_sum = a_sum = 0.0;
+    float zs = 0.0f;
+    shift = p.lse ? static_cast<double>(lse) : static_cast<double>(t_max) * p.inv_t;
+    const float base = z_max == -kInf ? 0.0f : z_max;
+    each(p, [&](int e, int, float t) {
+      const double log_q = static_cast<double>(t) * p.inv_t - shift, q = exp(log_q);
+      q_sum += q;
+      if (q != 0.0) a_sum += q * (log_q - static_cast<double>(z(e)) * p.inv_t);
+      zs += exp_t(z(e) - base, p.c);
+    });
+    // (threads' sums meet in fp64: the loss is a small difference of logarithms, and
+    // a rounding of the total by 2^-24 is 2e-6 of a loss of 0.03)
+    const double r64 = wave_sum(static_cast<double>(rest)), z64 = wave_sum(static_cast<double>(zs));
+    q_sum = wave_sum(q_sum);
+    a_sum = wave_sum(a_sum);
+    if ((threadIdx.x & 63) == 0) {
+      s.rest[threadIdx.x >> 6] = r64;
+      s.s[threadIdx.x >> 6] = z64;
+      s.q[threadIdx.x >> 6] = q_sum;
+      s.a[threadIdx.x >> 6] = a_sum;
+    }
+  }
+  __device__ __forceinline__ void finish(const Shared& s) {
+    q_sum = waves_sum<W>(s.q);
+    a_sum = waves_sum<W>(s.a);
+    z_sum = waves_sum<W>(s.s);
+  }
+};
+
+// What a row comes to. The rest's exponentials are rest 2^base (base in powers of
+// two: exp(u) = 2^(u log2 e)), the list's z_sum 2^(z_max c).
+struct RowSums {
+  double rest, base, top, total;  // total: of both, times 2^-top
+  double q_rest, q_all, q_norm, p_rest, list_scale;
+  template <int DT, int THREADS>
+  __device__ __forceinline__ RowSums(const DistillParams& p, const List<DT, THREADS>& l, double rest_, double base_)
+      : rest(rest_), base(base_) {
+    const double c = static_cast<double>(p.c.hi) + p.c.lo;
+    const double dz = l.z_max == -kInf ? base : l.z_max * c;
+    top = rest > 0.0 ? fmax(base, dz) : dz;
+    const double r = rest > 0.0 ? rest * exp2(base - top) : rest;  // (NaN stays)
+    list_scale = exp2(dz - top);
+    total = r + l.z_sum * list_scale;
+    p_rest = r / total;
+    // (where no unlisted logit is above minus infinity there is no such outcome)
+    q_rest = 0.0;
+    q_norm = 1.0;
+    if (p.lse) q_rest = rest == 0.0 ? 0.0 : 1.0 - l.q_sum < 0.0 ? 0.0 : 1.0 - l.q_sum;
+    else q_norm = 1.0 / l.q_sum;
+    q_all = p.lse ? l.q_sum + q_rest : 1.0;
+  }
+  template <int DT, int THREADS>
+  __device__ __forceinline__ float loss(const DistillParams& p, const List<DT, THREADS>& l) const {
+    if (l.n < 0) return __builtin_nanf("");
+    if (l.n == 0) return 0.0f;
+    constexpr double ln2 = 0.69314718055994530942;
+    const double log_total = log(total) + top * ln2;
+    double x = p.lse ? l.a_sum + l.q_sum * log_total : l.a_sum * q_norm - log(l.q_sum) + log_total;
+    if (q_rest > 0.0) x += q_rest * (log(q_rest) - (log(rest) + base * ln2 - log_total));
+    return static_cast<float>(x);
+  }
+  // The gradient on the rest is rest_gradient * (term of the rest's sum).
+  __device__ __forceinline__ double rest_gradient(const DistillParams& p) const {
+    return rest == 0.0 ? 0.0 : p.scale * p.inv_t * (q_all * p_rest - q_rest) / rest;
+  }
+  template <int DT, int THREADS>
+  __device__ __forceinline__ void list_gradients(const DistillParams& p, const List<DT, THREADS>& l, uint8_t* dz) const {
+    const double gs = p.scale * p.inv_t, f = list_scale / total * q_all;
+    const float base_z = l.z_max == -kInf ? 0.0f : l.z_max;
+    l.each(p, [&](int e, int id, float t) {
+      const double q = exp(static_cast<double>(t) * p.inv_t - l.shift) * q_norm;
+      store_elem<DT>(dz, id, static_cast<float>(gs * (static_cast<double>(exp_t(l.z(e) - base_z, p.c)) * f - q)));
+    });
+  }
+};
+
+// A barrier for what the block's threads have written to LDS; loads from memory
+// stay in flight (__syncthreads waits for them).
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The listed ones of a piece's E logits, a bit each.
+template <int E>
+__device__ __forceinline__ uint32_t listed_bits(const uint32_t* bitmap, int i) {
+  const uint8_t* b = reinterpret_cast<const uint8_t*>(bitmap);
+  return E == 8 ? b[i] : (b[i >> 1] >> (4 * (i & 1))) & 15u;
+}
+
+// A piece with the elements of `bits` at minus infinity.
+template <int DT>
+__device__ __forceinline__ void take_out(uint4& q, uint32_t bits) {
+  uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (DT == MR_F32) {
+      if (bits >> k & 1) w[k] = 0xff800000u;
+    } else {
+      constexpr uint32_t inf = DT == MR_BF16 ? 0xff80u : 0xfc00u;
+      if (bits >> (2 * k) & 1) w[k] = (w[k] & 0xffff0000u) | inf;
+      if (bits >> (2 * k + 1) & 1) w[k] = (w[k] & 0xffffu) | (inf << 16);
+    }
+  }
+  q = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Piece i of a gradient row.
+template <int DT>
+__device__ __forceinline__ void store_piece(uint8_t* row, int i, int V, uint4 o) {
+  constexpr int E = kPiece<DT>, ES = 16 / E;
+  if ((i + 1) * E <= V) {
+    __builtin_memcpy(row + static_cast<int64_t>(i) * 16, &o, 16);
+    return;
+  }
+  const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+  for (int k = 0; k < E - 1; ++k) {
+    if (i * E + k >= V) continue;
+    if constexpr (ES == 4) reinterpret_cast<uint32_t*>(row)[i * E + k] = w[k];
+    else reinterpret_cast<uint16_t*>(row)[i * E + k] = static_cast<uint16_t>((k & 1) ? w[k >> 1] >> 16 : w[k >> 1]);
+  }
+}
+
+// One workgroup per row, the row held in registers: N pieces of 16 bytes per
+// thread, all loads in flight together, the row read once. A bitmap of the listed
+// ids in LDS takes them out of it (minus infinity), so the rest's sum is formed of
+// its own terms: as the total less the listed it would have no digit left where
+// the list has nearly all the mass. The listed logits are gathered by the threads
+// that hold their list entries, whose gradients are written over the row's.
+//
+// With one row of 16-bit logits to a CU's registers nothing overlaps a row but
+// itself, and 2 exponentials a logit (4 issue slots each) take as long as the
+// row's loads. So the sum does not wait for the row's maximum: it runs about the
+// maximum of the first pieces to arrive, piece by piece as the others do, and
+// only a sum outside 2^-64 .. 2^64 is formed again about the maximum itself.
+// exp(v / T) is 2^(v hi - b), one fused multiply-add: b is any number, and what
+// hi lacks of log2(e) / T is made up in the sum's base, to first order, by the
+// mean of v (over one in E of the terms).
+template <int DT, int THREADS, int N>
+__global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
+  constexpr int E = kPiece<DT>, ES = 16 / E, W = THREADS / 64;
+  extern __shared__ uint32_t bitmap[];  // a bit per logit, a word more, and the list
+  __shared__ typename List<DT, THREADS>::Shared s;
+  __shared__ float s_first[W], s_ve[W], s_e[W];
+  __shared__ float s_g;
+  __shared__ uint32_t s_sign;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int64_t row = blockIdx.x;
   const int V = p.V, pieces = (V + E - 1) / E;
   const uint8_t* z = static_cast<const uint8_t*>(p.z) + row * p.ldz * ES;
   uint8_t* dz = static_cast<uint8_t*>(p.dz) + row * p.ldd * ES;
 
-  // the list's entries of this thread
-  int id[KE];
-  float t[KE], zl[KE];
-#pragma unroll
-  for (int e = 0; e < KE; ++e) {
-    const int j = e * THREADS + tid;
-    id[e] = j < p.k ? p.ids[row * p.k + j] : -1;
-    t[e] = j < p.k ? p.t[row * p.k + j] : 0.0f;
-  }
-  for (int i = tid; i < (V + 31) / 32; i += THREADS) bitmap[i] = 0;
-  uint4 r[HELD ? N : 1] = {};
-  if constexpr (HELD) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int i = j * THREADS + tid;
-      r[j] = no_piece<DT>();
-      if (i < pieces) r[j] = load_piece<DT>(z, i, V);
-    }
-  }
-  __syncthreads();
-  // Entries past the vocabulary or listed twice make the row a NaN.
-  int n = 0;
-  bool bad = false;
-  float t_max = -kInf, z_max = -kInf;
-#pragma unroll
-  for (int e = 0; e < KE; ++e) {
-    zl[e] = 0.0f;
-    if (id[e] < 0) continue;
-    if (id[e] >= V) {
-      bad = true;
-      id[e] = -1;
-      continue;
-    }
-    const uint32_t bit = 1u << (id[e] & 31);
-    if (atomicOr(&bitmap[id[e] >> 5], bit) & bit) bad = true;
-    zl[e] = load_elem<DT>(z, id[e]);
-    ++n;
-    t_max = fmaxf(t_max, t[e]);
-    z_max = fmaxf(z_max, zl[e]);
-  }
-  __syncthreads();
-  // the row's pieces without the listed logits, and their maximum
-  const uint8_t* bits = reinterpret_cast<const uint8_t*>(bitmap);
-  auto unlisted = [&](uint4 q, int i, float (&v)[E]) __attribute__((always_inline)) {
-    widen<DT>(q, v);
-    const uint32_t b = E == 8 ? bits[i] : (bits[i >> 1] >> (4 * (i & 1))) & 15u;
-    if (b) {
-#pragma unroll
-      for (int k = 0; k < E; ++k)
-        if (b >> k & 1) v[k] = -kInf;
-    }
+  List<DT, THREADS> l(bitmap + (V + 31) / 32 + 1, p.k);
+  const typename List<DT, THREADS>::Entries entries = l.load(p, row);
+  // Every load is whole and unconditional (a branch around a load makes each wait
+  // for the last): pieces past the end are the row's last 16 bytes, of which
+  // take_out leaves what no other piece has.
+  uint4 r[N];
+  auto first = [&](int t, int j) __attribute__((always_inline)) { return min((j * THREADS + t) * E, V - E); };
+  // (anew: a copy of the thread's index whose products no earlier pass has kept)
+  auto anew = [&]() __attribute__((always_inline)) {
+    int t = tid;
+    asm volatile("" : "+v"(t));
+    return t;
   };
+#pragma unroll
+  for (int j = 0; j < N; ++j) r[j] = ld16(z + static_cast<uint32_t>(first(tid, j) * ES));
+  for (int i = tid; i <= (V + 31) / 32; i += THREADS) bitmap[i] = 0;
+  lds_barrier();
+  l.mark(p, entries, z, bitmap, s);
+  {
+    float v[E], mx = -kInf;
+    widen<DT>(r[0], v);
+#pragma unroll
+    for (int k = 0; k < E; ++k) mx = fmaxf(mx, v[k]);
+    mx = wave_max(mx);
+    if (lane == 0) s_first[wave] = mx;
+  }
+  lds_barrier();
   // (the values are unpacked anew in each pass, not kept: fresh hides that they are the same)
   auto fresh = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < (HELD ? N : 1); ++j) asm volatile("" : "+v"(r[j].x), "+v"(r[j].y), "+v"(r[j].z), "+v"(r[j].w));
+    for (int j = 0; j < N; ++j) asm volatile("" : "+v"(r[j].x), "+v"(r[j].y), "+v"(r[j].z), "+v"(r[j].w));
   };
-  float rest_max = -kInf, sum = 0.0f;
-  if constexpr (HELD) {
+  float about = waves_max<W>(s_first);
+  float sum, ve, se;
+  auto add_up = [&](auto takes) __attribute__((always_inline)) {
+    if (!(about > -kInf && about < kInf)) about = 0.0f;
+    const float b = -about * p.c.hi;
+    const int t = anew();
+    float s0 = 0.0f, s1 = 0.0f;
+    ve = se = 0.0f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int i = j * THREADS + tid;
-      if (i >= pieces) continue;
-      float v[E];
-      unlisted(r[j], i, v);
-#pragma unroll
-      for (int k = 0; k < E; ++k) rest_max = fmaxf(rest_max, v[k]);
-      r[j] = narrow<DT>(v);
-    }
-  } else {
-    // (running maximum and sum, rescaled where the maximum grows)
-    constexpr int U = 4;
-    for (int i0 = tid; i0 < pieces; i0 += U * THREADS) {
-      uint4 q[U];
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        q[j] = no_piece<DT>();
-        if (i0 + j * THREADS < pieces) q[j] = load_piece<DT>(z, i0 + j * THREADS, V);
+      if constexpr (decltype(takes)::value) {
+        const int at = first(t, j), drop = min((j * THREADS + t) * E - at, E);
+        const uint32_t bits = __builtin_amdgcn_alignbit(bitmap[(at >> 5) + 1], bitmap[at >> 5], at & 31) | ((1u << drop) - 1);
+        if (bits & ((1u << E) - 1)) take_out<DT>(r[j], bits);
       }
-      float v[U][E];
-      float mx = rest_max;
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        unlisted(q[j], min(i0 + j * THREADS, pieces - 1), v[j]);
-#pragma unroll
-        for (int k = 0; k < E; ++k) mx = fmaxf(mx, v[j][k]);
-      }
-      const float base = mx == -kInf ? 0.0f : mx;
-      if (mx > rest_max) sum = rebase(sum, rest_max, base, p.c);
-      rest_max = mx;
-#pragma unroll
-      for (int j = 0; j < U; ++j)
-#pragma unroll
-        for (int k = 0; k < E; ++k) sum += exp_t(v[j][k] - base, p.c);
-    }
-  }
-  const float own_max = rest_max;
-  rest_max = wave_max(rest_max);
-  t_max = wave_max(t_max);
-  z_max = wave_max(z_max);
-  n = __any(bad) ? -(1 << 20) : wave_sum(n);
-  if (lane == 0) {
-    s_rest[wave] = rest_max;
-    s_t[wave] = t_max;
-    s_z[wave] = z_max;
-    s_n[wave] = n;
-  }
-  __syncthreads();
-  rest_max = waves_max<W>(s_rest);
-  t_max = waves_max<W>(s_t);
-  z_max = waves_max<W>(s_z);
-  n = waves_sum<W>(s_n);
-  bad = n < 0;
-  const float rest_base = rest_max == -kInf ? 0.0f : rest_max, z_base = z_max == -kInf ? 0.0f : z_max;
-  if constexpr (HELD) {
-    float s1 = 0.0f;
-    fresh();
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
       float v[E];
       widen<DT>(r[j], v);
 #pragma unroll
       for (int k = 0; k < E; k += 2) {
-        sum += exp_t(v[k] - rest_base, p.c);
-        s1 += exp_t(v[k + 1] - rest_base, p.c);
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(v[k], p.c.hi, b));
+        if (k == 0) {
+          ve = __builtin_fmaf(fmaxf(v[0], -1e30f), e0, ve);
+          se += e0;
+        }
+        s0 += e0;
+        s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(v[k + 1], p.c.hi, b));
       }
+      // Here, as the pieces arrive: left alone the sums move behind the next barrier,
+      // and the bitmap's words of every piece are read ahead (40 registers).
+      asm volatile("" : "+v"(s0), "+v"(s1), "+v"(ve), "+v"(se));
+      if (j & 1) __builtin_amdgcn_sched_barrier(0);
     }
-    sum += s1;
-  } else {
-    sum = rebase(sum, own_max, rest_max, p.c);
-  }
-  // the list: sum of q (or of its exponentials) and of q (log q - z / T)
-  double q_sum = 0.0, a_sum = 0.0;
-  double qe[KE];
-  float list_sum = 0.0f;
-  const double shift = p.lse ? static_cast<double>(p.lse[row]) : static_cast<double>(t_max) * p.inv_t;
-#pragma unroll
-  for (int e = 0; e < KE; ++e) {
-    qe[e] = 0.0;
-    if (id[e] < 0) continue;
-    const double log_q = static_cast<double>(t[e]) * p.inv_t - shift;
-    qe[e] = exp(log_q);
-    q_sum += qe[e];
-    if (qe[e] != 0.0) a_sum += qe[e] * (log_q - static_cast<double>(zl[e]) * p.inv_t);
-    list_sum += exp_t(zl[e] - z_base, p.c);
-  }
-  // (threads' sums meet in fp64: the loss is a small difference of logarithms, and
-  // a rounding of the total by 2^-24 is 2e-6 of a loss of 0.03)
-  double rest64 = wave_sum(static_cast<double>(sum)), list64 = wave_sum(static_cast<double>(list_sum));
-  q_sum = wave_sum(q_sum);
-  a_sum = wave_sum(a_sum);
-  if (lane == 0) {
-    s_sum[wave] = rest64;
-    s_list[wave] = list64;
-    s_q[wave] = q_sum;
-    s_a[wave] = a_sum;
-  }
-  __syncthreads();  // (and every read of the row's first pass is done)
-  rest64 = waves_sum<W>(s_sum);
-  list64 = waves_sum<W>(s_list);
-  sum = static_cast<float>(rest64);
-  list_sum = static_cast<float>(list64);
-  q_sum = waves_sum<W>(s_q);
-  a_sum = waves_sum<W>(s_a);
-  const float m = fmaxf(rest_max, z_max);
-  const float rest_part = rebase(sum, rest_max, m, p.c);
-  const float total = rest_part + rebase(list_sum, z_max, m, p.c);
-  const float p_rest = rest_part / total;
-  // (where no unlisted logit is above minus infinity there is no such outcome)
-  double q_rest = 0.0, q_norm = 1.0;
-  if (p.lse) {
-    q_rest = sum == 0.0f ? 0.0 : 1.0 - q_sum < 0.0 ? 0.0 : 1.0 - q_sum;
-  } else {
-    q_norm = 1.0 / q_sum;
-  }
-  const double q_all = p.lse ? q_sum + q_rest : 1.0;
-  // (last: its logarithms' registers are the row's until then)
-  auto write_loss = [&]() __attribute__((always_inline)) {
-    if (tid != 0) return;
-    double loss = 0.0;
-    if (bad) {
-      loss = __builtin_nan("");
-    } else if (n > 0) {
-      auto about_m = [&](double x, float from) { return x == 0.0 ? 0.0 : x * exp((static_cast<double>(from) - m) * p.inv_t); };
-      const double log_total = log(about_m(rest64, rest_max) + about_m(list64, z_max));
-      const double l = static_cast<double>(m) * p.inv_t + log_total;
-      loss = p.lse ? a_sum + q_sum * l : a_sum * q_norm - log(q_sum) + l;
-      if (q_rest > 0.0) {
-        const double log_rest = log(rest64) + (static_cast<double>(rest_max) - m) * p.inv_t - log_total;
-        loss += q_rest * (log(q_rest) - log_rest);
-      }
-    }
-    p.row_loss[row] = static_cast<float>(loss);
-  };
-  if (!p.dz) {
-    write_loss();
-    return;
-  }
-  const float gs = static_cast<float>(p.scale * p.inv_t);
-  // on the rest: exp(z - rest_max) g
-  float g = sum == 0.0f ? 0.0f : gs * (static_cast<float>(q_all * static_cast<double>(p_rest) - q_rest) / sum);
-  if (n == 0) g = 0.0f;
-  if (bad) g = __builtin_nanf("");
-  const bool none = n == 0;
-  auto put = [&](int i, float (&v)[E]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int k = 0; k < E; ++k) {
-      v[k] = exp_t(v[k] - rest_base, p.c) * g;
-      if (none) v[k] = 0.0f;
-    }
-    const uint4 o = narrow<DT>(v);
-    if ((i + 1) * E <= V) {
-      __builtin_memcpy(dz + static_cast<int64_t>(i) * 16, &o, 16);
-    } else {
-#pragma unroll
-      for (int k = 0; k < E - 1; ++k)
-        if (i * E + k < V) store_elem<DT>(dz, static_cast<int64_t>(i) * E + k, v[k]);
+    sum = s0 + s1;
+    ve = wave_sum(ve);
+    se = wave_sum(se);
+    if (lane == 0) {
+      s_ve[wave] = ve;
+      s_e[wave] = se;
     }
   };
-  if constexpr (HELD) {
+  add_up(std::true_type{});
+  l.publish(p, s);
+  __syncthreads();
+  l.collect(s);
+  l.sums(p, sum, s);
+  __syncthreads();  // (and every read of the row is done)
+  const double rest0 = waves_sum<W>(s.rest);
+  if (!(rest0 > 0x1p-64 && rest0 < 0x1p64)) {  // (or a NaN)
+    fresh();
+    float mx = -kInf;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float v[E];
+      widen<DT>(r[j], v);
+#pragma unroll
+      for (int k = 0; k < E; ++k) mx = fmaxf(mx, v[k]);
+    }
+    mx = wave_max(mx);
+    if (lane == 0) s_first[wave] = mx;
+    __syncthreads();
+    about = waves_max<W>(s_first);
+    fresh();
+    add_up(std::false_type{});
+    const double r64 = wave_sum(static_cast<double>(sum));
+    if (lane == 0) s.rest[wave] = r64;
+    __syncthreads();
+  }
+  // What the row comes to, from the block's sums (a wave or all).
+  auto row_sums = [&]() __attribute__((always_inline)) {
+    const double lo = static_cast<double>(p.c.lo);
+    const float v = waves_sum<W>(s_ve), e = waves_sum<W>(s_e);
+    l.finish(s);
+    return RowSums(p, l, waves_sum<W>(s.rest),
+                   static_cast<double>(about * p.c.hi) + lo * (e > 0.0f ? static_cast<double>(v / e) : about));
+  };
+  const bool none = l.n == 0;
+  if (p.dz) {
+    // (one wave works the factor out: in every wave its float64 registers would
+    // not fit beside the row)
+    if (wave == 0) {
+      const RowSums x = row_sums();
+      const double g = l.n < 0 ? __builtin_nan("") : x.rest_gradient(p);
+      if (lane == 0) {
+        // f32: term and gradient to its precision, (v - about) log2(e) / T in two
+        // parts; else the factor goes into the exponent, its sign onto the pairs
+        s_g = static_cast<float>(DT == MR_F32 ? g * exp2(about * (static_cast<double>(p.c.hi) + p.c.lo) - x.base)
+                                              : log2(fabs(g)) - x.base);
+        s_sign = g < 0.0 ? 0x80008000u : 0u;
+      }
+    }
+    __syncthreads();
+    const float g = s_g;
+    const uint32_t sign = s_sign;
+    const int t = anew();
     fresh();
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int i = j * THREADS + tid;
+      const int i = j * THREADS + t;
       if (i >= pieces) continue;
       float v[E];
       widen<DT>(r[j], v);
-      put(i, v);
-    }
-  } else {
-    constexpr int U = 4;
-    for (int i0 = tid; i0 < pieces; i0 += U * THREADS) {
-      uint4 q[U];
 #pragma unroll
-      for (int j = 0; j < U; ++j)
-        if (i0 + j * THREADS < pieces) q[j] = load_piece<DT>(z, i0 + j * THREADS, V);
+      for (int k = 0; k < E; ++k)
+        v[k] = DT == MR_F32 ? exp_t(v[k] - about, p.c) * g : __builtin_amdgcn_exp2f(__builtin_fmaf(v[k], p.c.hi, g));
+      uint4 o = narrow<DT>(v);
+      if constexpr (DT != MR_F32) o = make_uint4(o.x ^ sign, o.y ^ sign, o.z ^ sign, o.w ^ sign);
+      if (none) o = make_uint4(0, 0, 0, 0);
+      if ((i + 1) * E <= V) {
+        __builtin_memcpy(dz + static_cast<int64_t>(i) * 16, &o, 16);
+      } else {
+        const uint32_t w[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int i = i0 + j * THREADS;
-        if (i >= pieces) continue;
-        float v[E];
-        unlisted(q[j], i, v);
-        put(i, v);
+        for (int k = 1; k < E; ++k) {
+          if (V - E + k < i * E) continue;
+          if constexpr (ES == 4) reinterpret_cast<uint32_t*>(dz)[V - E + k] = w[k];
+          else reinterpret_cast<uint16_t*>(dz)[V - E + k] = static_cast<uint16_t>((k & 1) ? w[k >> 1] >> 16 : w[k >> 1]);
+        }
       }
+    }
+    __syncthreads();  // the rest's stores are done where the list's follow
+  }
+  const RowSums x = row_sums();
+  if (tid == 0) p.row_loss[row] = x.loss(p, l);
+  if (p.dz && l.n > 0) x.list_gradients(p, l, dz);
+}
+
+// Longer rows (and those shorter than a piece), read twice: the sum about a running maximum, then the gradient.
+template <int DT>
+__global__ __launch_bounds__(1024) void distill_twice(DistillParams p) {
+  constexpr int THREADS = 1024, U = 4;
+  constexpr int E = kPiece<DT>, ES = 16 / E, W = THREADS / 64;
+  extern __shared__ uint32_t bitmap[];
+  __shared__ typename List<DT, THREADS>::Shared s;
+  __shared__ float s_max[W];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int64_t row = blockIdx.x;
+  const int V = p.V, pieces = (V + E - 1) / E;
+  const uint8_t* z = static_cast<const uint8_t*>(p.z) + row * p.ldz * ES;
+  uint8_t* dz = static_cast<uint8_t*>(p.dz) + row * p.ldd * ES;
+  List<DT, THREADS> l(bitmap + (V + 31) / 32 + 1, p.k);
+  const typename List<DT, THREADS>::Entries entries = l.load(p, row);
+  for (int i = tid; i <= (V + 31) / 32; i += THREADS) bitmap[i] = 0;
+  __syncthreads();
+  l.mark(p, entries, z, bitmap, s);
+  __syncthreads();
+  float mx = -kInf, sum = 0.0f;
+  for (int i0 = tid; i0 < pieces; i0 += U * THREADS) {
+    uint4 q[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      q[j] = no_piece<DT>();
+      if (i0 + j * THREADS < pieces) q[j] = load_piece<DT>(z, i0 + j * THREADS, V);
+    }
+    float v[U][E];
+    float m = mx;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const uint32_t bits = i0 + j * THREADS < pieces ? listed_bits<E>(bitmap, i0 + j * THREADS) : 0;
+      if (bits) take_out<DT>(q[j], bits);
+      widen<DT>(q[j], v[j]);
+#pragma unroll
+      for (int k = 0; k < E; ++k) m = fmaxf(m, v[j][k]);
+    }
+    const float about = m == -kInf ? 0.0f : m;
+    if (m > mx) sum = rebase(sum, mx, about, p.c);
+    mx = m;
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+#pragma unroll
+      for (int k = 0; k < E; ++k) sum += exp_t(v[j][k] - about, p.c);
+  }
+  const float m = wave_max(mx);
+  if (lane == 0) s_max[wave] = m;
+  l.publish(p, s);
+  __syncthreads();
+  l.collect(s);
+  float about = waves_max<W>(s_max);
+  sum = rebase(sum, mx, about, p.c);
+  if (about == -kInf) about = 0.0f;
+  l.sums(p, sum, s);
+  __syncthreads();  // (and the list's reads of the row are done)
+  l.finish(s);
+  const double base = static_cast<double>(about) * (static_cast<double>(p.c.hi) + p.c.lo);
+  const RowSums x(p, l, waves_sum<W>(s.rest), base);
+  if (tid == 0) p.row_loss[row] = x.loss(p, l);
+  if (!p.dz) return;
+  const bool none = l.n == 0;
+  const float g = l.n < 0 ? __builtin_nanf("") : static_cast<float>(x.rest_gradient(p));
+  for (int i0 = tid; i0 < pieces; i0 += U * THREADS) {
+    uint4 q[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+      if (i0 + j * THREADS < pieces) q[j] = load_piece<DT>(z, i0 + j * THREADS, V);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = i0 + j * THREADS;
+      if (i >= pieces) continue;
+      const uint32_t bits = listed_bits<E>(bitmap, i);
+      if (bits) take_out<DT>(q[j], bits);
+      float v[E];
+      widen<DT>(q[j], v);
+#pragma unroll
+      for (int k = 0; k < E; ++k) v[k] = none ? 0.0f : exp_t(v[k] - about, p.c) * g;
+      store_piece<DT>(dz, i, V, narrow<DT>(v));
     }
   }
   __syncthreads();  // the rest's stores are done where the list's follow
-  write_loss();
-  if (none || bad) return;
-#pragma unroll
-  for (int e = 0; e < KE; ++e) {
-    if (id[e] < 0) continue;
-    const double pj = static_cast<double>(exp_t(zl[e] - m, p.c) / total);
-    store_elem<DT>(dz, id[e], gs * static_cast<float>(pj * q_all - qe[e] * q_norm));
-  }
+  if (l.n > 0) x.list_gradients(p, l, dz);
 }
 
 // loss = scale * sum of the row losses, in a fixed order (fp64 partials).
@@ -822,19 +1045,20 @@ int mr_distill(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, 
     DistillParams p{logits, ld, static_cast<int>(V), k, top_values, top_ids, top_lse, exp_scale(temperature),
                     1.0 / static_cast<double>(temperature), scale, row_loss, dlogits, ldd};
     const dim3 g(static_cast<unsigned>(T));
-    const size_t lds = static_cast<size_t>((V + 31) / 32) * 4;
+    const size_t lds = static_cast<size_t>((V + 31) / 32 + 1) * 4 + static_cast<size_t>(k) * 8;
     const int64_t pieces = (V * es + 15) / 16;
-#define MR_DISTILL(DT, THREADS, N, HELD) hipLaunchKernelGGL((distill_rows<DT, THREADS, N, HELD>), g, dim3(THREADS), lds, s, p)
+#define MR_DISTILL(DT, THREADS, N) hipLaunchKernelGGL((distill_held<DT, THREADS, N>), g, dim3(THREADS), lds, s, p)
     // the fewest threads that hold the row in at most 8 pieces each, then more pieces
-#define MR_DISTILL_D(DT)                                                \
-  do {                                                                  \
-    if (pieces <= 256 * 4) MR_DISTILL(DT, 256, 4, true);                \
-    else if (pieces <= 256 * 8) MR_DISTILL(DT, 256, 8, true);           \
-    else if (pieces <= 512 * 8) MR_DISTILL(DT, 512, 8, true);           \
-    else if (pieces <= 1024 * 8) MR_DISTILL(DT, 1024, 8, true);         \
-    else if (pieces <= 1024 * 14) MR_DISTILL(DT, 1024, 14, true);       \
-    else if (pieces <= 1024 * 20) MR_DISTILL(DT, 1024, 20, true);       \
-    else MR_DISTILL(DT, 1024, 1, false);                                \
+#define MR_DISTILL_D(DT)                                                                   \
+  do {                                                                                     \
+    if (V * es < 16) hipLaunchKernelGGL((distill_twice<DT>), g, dim3(1024), lds, s, p);     \
+    else if (pieces <= 256 * 4) MR_DISTILL(DT, 256, 4);                                    \
+    else if (pieces <= 256 * 8) MR_DISTILL(DT, 256, 8);                                    \
+    else if (pieces <= 512 * 8) MR_DISTILL(DT, 512, 8);                                    \
+    else if (pieces <= 1024 * 8) MR_DISTILL(DT, 1024, 8);                                  \
+    else if (pieces <= 1024 * 14) MR_DISTILL(DT, 1024, 14);                                \
+    else if (pieces <= 1024 * 20) MR_DISTILL(DT, 1024, 20);                                \
+    else hipLaunchKernelGGL((distill_twice<DT>), g, dim3(1024), lds, s, p);                \
   } while (0)
     if (dtype == MR_BF16) MR_DISTILL_D(MR_BF16);
     else if (dtype == MR_F16) MR_DISTILL_D(MR_F16);
