@@ -407,6 +407,37 @@ int mr_gemm_swiglu_bwd(int64_t M, int64_t N, int64_t K, const void* dd, int64_t 
                        int64_t lddgu, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Products with an activation f in their epilogue (MR_ACT_*; relu squared,
+ * x sigmoid(x), x Phi(x) and its tanh approximation), for ungated MLPs and
+ * residual branches. Operands bf16 as mr_gemm's; any M, N % 8 == 0, K % 64 == 0.
+ *   mr_gemm_act      C [M, N] (c_dtype) = f(X [M, K] W^T + bias[N]) (+ resid, C
+ *                    then fp32 and resid itself allowed); pre, if non-NULL,
+ *                    receives X W^T + bias as bf16 [M, N], what a backward reads
+ *   mr_gemm_act_bwd  dpre [M, N] bf16 = (dd [M, K] Wd [K, N]) f'(pre), from the
+ *                    gradient of the next product's output; pre itself allowed
+ *   mr_act_bwd       dpre = dout f'(pre), from the output's own gradient (fp32 or
+ *                    bf16; M <= 2,097,120); over pre or a bf16 dout allowed
+ * and, if dbias is non-NULL, dbias[n] = sum over rows of dpre before it is
+ * rounded (fp32, a fixed order), for which partials holds
+ * mr_bias_partials_bytes(M, N). relu' is 0 at 0. The gradients of X and W are
+ * mr_gemm's products of dpre. workspace: as mr_gemm's, of (M, N, K).
+ * The relus, silu and gelus of mlx.nn beside the gated mr_gemm_swiglu.
+ */
+enum { MR_ACT_RELU = 0, MR_ACT_RELU2 = 1, MR_ACT_SILU = 2, MR_ACT_GELU = 3, MR_ACT_GELU_TANH = 4 };
+int mr_gemm_act(int64_t M, int64_t N, int64_t K, const void* X, int64_t ldx, const void* W, int64_t ldw,
+                int act, const float* bias, const float* resid, int64_t ldr, void* C, int c_dtype,
+                int64_t ldc, void* pre, int64_t ldpre, void* workspace, size_t workspace_bytes,
+                void* stream);
+size_t mr_bias_partials_bytes(int64_t M, int64_t N);
+int mr_gemm_act_bwd(int64_t M, int64_t N, int64_t K, const void* dd, int64_t ldd, const void* Wd,
+                    int64_t ldw, const void* pre, int64_t ldpre, int act, void* dpre, int64_t lddpre,
+                    float* dbias, float* partials, size_t partials_bytes, void* workspace,
+                    size_t workspace_bytes, void* stream);
+int mr_act_bwd(int64_t M, int64_t N, const void* dout, int dout_dtype, int64_t ldo, const void* pre,
+               int64_t ldpre, int act, void* dpre, int64_t lddpre, float* dbias, float* partials,
+               size_t partials_bytes, void* stream);
+
+/*
  * RMSNorm over rows of the fp32 residual stream, y = h rsqrt(mean(h^2) + eps) w
  * as bf16 (the next GEMM's operand) plus the per-row rsqrt for the backward;
  * the backward adds the residual gradient: dh = dres + d(rmsnorm)/dh^T dy.

@@ -24,6 +24,7 @@ from mround_amd.exceptions import KernelError, KernelUnavailableError
 
 __all__ = [
     "MODE",
+    "act_bwd",
     "copy_bytes",
     "cross_entropy",
     "delta_loss",
@@ -33,6 +34,8 @@ __all__ = [
     "embed_rows",
     "fq_backward_signsgd",
     "fq_forward",
+    "gemm_act",
+    "gemm_act_bwd",
     "lib",
     "lib_path",
     "loss_mse",
@@ -89,6 +92,11 @@ _SIGNATURES = {
     "mr_gemm_swiglu": (_I, [_L, _L, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, ctypes.c_size_t, _P]),
     "mr_gemm_swiglu_split": (_I, [_L, _L, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, ctypes.c_size_t, _P]),
     "mr_gemm_swiglu_bwd": (_I, [_L, _L, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, ctypes.c_size_t, _P]),
+    "mr_gemm_act": (_I, [_L, _L, _L, _P, _L, _P, _L, _I, _P, _P, _L, _P, _I, _L, _P, _L, _P, ctypes.c_size_t, _P]),
+    "mr_bias_partials_bytes": (ctypes.c_size_t, [_L, _L]),
+    "mr_gemm_act_bwd": (_I, [_L, _L, _L, _P, _L, _P, _L, _P, _L, _I, _P, _L, _P, _P, ctypes.c_size_t, _P,
+                             ctypes.c_size_t, _P]),
+    "mr_act_bwd": (_I, [_L, _L, _P, _I, _L, _P, _L, _I, _P, _L, _P, _P, ctypes.c_size_t, _P]),
     "mr_rmsnorm_fwd": (_I, [_P, _P, _L, _L, _F, _P, _P, _P]),
     "mr_rmsnorm_bwd": (_I, [_P, _P, _P, _P, _P, _L, _L, _P, _P, _P]),
     "mr_rmsnorm_fwd_split": (_I, [_P, _P, _L, _L, _F, _P, _P, _P, _P]),
@@ -578,6 +586,103 @@ def gemm_swiglu_bwd(dd, wd, gu, dgu, *, workspace=None) -> None:
     rc = lib().mr_gemm_swiglu_bwd(M, N, K, _ptr(dd), dd.stride(0), _ptr(wd), wd.stride(0), _ptr(gu),
                                   gu.stride(0), _ptr(dgu), dgu.stride(0), ws_ptr, ws_bytes, _stream(dd))
     _check(rc, "mr_gemm_swiglu_bwd")
+
+
+ACTIVATIONS = {"relu": 0, "relu2": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+
+def _activation(name: str, act: str) -> int:
+    if act not in ACTIVATIONS:
+        raise KernelError(f"{name}: the activation must be one of {', '.join(ACTIVATIONS)}, got {act!r}")
+    return ACTIVATIONS[act]
+
+
+def _bf16_matrix(name: str, what: str, t, shape=None) -> None:
+    if t.dtype != torch.bfloat16 or t.dim() != 2 or (shape is not None and tuple(t.shape) != shape):
+        raise KernelError(f"{name}: {what} must be a bfloat16 matrix" + (f" {list(shape)}" if shape else "")
+                          + f", got {t.dtype} {list(t.shape)}")
+
+
+def _vector(name: str, what: str, t, n: int) -> None:
+    if t is not None and (t.dtype != torch.float32 or t.numel() != n):
+        raise KernelError(f"{name}: {what} must be float32 of {n} elements")
+
+
+def _partials(dbias, M: int, N: int, device):
+    """The column sums' workspace of a bias gradient: a tensor of the call's own,
+    which the allocator ties to the current stream."""
+    if dbias is None:
+        return None
+    return torch.empty(max(int(lib().mr_bias_partials_bytes(M, N)), 16), dtype=torch.uint8, device=device)
+
+
+def gemm_act(x, w, out, *, act, bias=None, pre=None, resid=None, workspace=None) -> None:
+    """``mr_gemm_act``: ``out = f(x w^T + bias) (+ resid)`` for bfloat16 ``x``
+    ``[M, K]`` and ``w`` ``[N, K]``, float32 ``bias`` ``[N]`` and ``resid`` ``[M,
+    N]`` (``out`` then float32, and may be ``resid``); ``out`` bfloat16 or float32.
+    ``act``: "relu", "relu2" (squared), "silu", "gelu" or "gelu_tanh". ``pre``
+    (bfloat16 ``[M, N]``) receives ``x w^T + bias`` for the backward. ``workspace``
+    as :func:`gemm`'s. M is any size; N is a multiple of 8, K of 64."""
+    code = _activation("gemm_act", act)
+    _bf16_matrix("gemm_act", "x", x)
+    (M, K), N = x.shape, w.shape[0]
+    _bf16_matrix("gemm_act", "w", w, (N, K))
+    if out.dtype not in (torch.bfloat16, torch.float32) or tuple(out.shape) != (M, N):
+        raise KernelError(f"gemm_act: out must be bfloat16 or float32 [{M}, {N}], got {out.dtype} {list(out.shape)}")
+    if pre is not None:
+        _bf16_matrix("gemm_act", "pre", pre, (M, N))
+    if resid is not None and (resid.dtype != torch.float32 or tuple(resid.shape) != (M, N)):
+        raise KernelError(f"gemm_act: resid must be float32 [{M}, {N}]")
+    _vector("gemm_act", "bias", bias, N)
+    _one_device("gemm_act", x, w, out, bias, pre, resid, workspace)
+    ws = _gemm_ws(x.device, M, N, K, workspace)
+    ws_ptr, ws_bytes = _ws_args(ws)
+    rc = lib().mr_gemm_act(M, N, K, _rows_ptr(x), _ld(x), _rows_ptr(w), _ld(w), code, _ptr(bias), _rows_ptr(resid),
+                           _ld(resid), _rows_ptr(out), dtype_code(out.dtype), _ld(out), _rows_ptr(pre), _ld(pre),
+                           ws_ptr, ws_bytes, _stream(x))
+    _check(rc, "mr_gemm_act")
+
+
+def gemm_act_bwd(dd, wd, pre, dpre, *, act, dbias=None, workspace=None) -> None:
+    """``mr_gemm_act_bwd``: ``dpre = (dd wd) f'(pre)`` from the gradient ``dd``
+    ``[M, K]`` of the next product's output and its weight ``wd`` ``[K, N]``, all
+    bfloat16 (``dpre`` may be ``pre``); float32 ``dbias`` ``[N]`` receives the sums
+    over rows."""
+    code = _activation("gemm_act_bwd", act)
+    _bf16_matrix("gemm_act_bwd", "dd", dd)
+    (M, K), N = dd.shape, wd.shape[1]
+    _bf16_matrix("gemm_act_bwd", "wd", wd, (K, N))
+    _bf16_matrix("gemm_act_bwd", "pre", pre, (M, N))
+    _bf16_matrix("gemm_act_bwd", "dpre", dpre, (M, N))
+    _vector("gemm_act_bwd", "dbias", dbias, N)
+    _one_device("gemm_act_bwd", dd, wd, pre, dpre, dbias, workspace)
+    # (both held until the launch: the one freed, the other could take its place)
+    ws, part = _gemm_ws(dd.device, M, N, K, workspace), _partials(dbias, M, N, dd.device)
+    (ws_ptr, ws_bytes), (part_ptr, part_bytes) = _ws_args(ws), _ws_args(part)
+    rc = lib().mr_gemm_act_bwd(M, N, K, _rows_ptr(dd), _ld(dd), _rows_ptr(wd), _ld(wd), _rows_ptr(pre), _ld(pre), code,
+                               _rows_ptr(dpre), _ld(dpre), _ptr(dbias), part_ptr, part_bytes, ws_ptr, ws_bytes,
+                               _stream(dd))
+    _check(rc, "mr_gemm_act_bwd")
+
+
+def act_bwd(dout, pre, dpre, *, act, dbias=None) -> None:
+    """``mr_act_bwd``: ``dpre = dout f'(pre)`` from the gradient ``dout`` ``[M, N]``
+    (float32 or bfloat16) of an output whose last step is the activation; ``pre``
+    and ``dpre`` bfloat16 (``dpre`` may be ``pre``, or a bfloat16 ``dout``); float32
+    ``dbias`` ``[N]`` receives the sums over rows."""
+    code = _activation("act_bwd", act)
+    if dout.dtype not in (torch.float32, torch.bfloat16) or dout.dim() != 2:
+        raise KernelError(f"act_bwd: dout must be a float32 or bfloat16 matrix, got {dout.dtype} {list(dout.shape)}")
+    M, N = dout.shape
+    _bf16_matrix("act_bwd", "pre", pre, (M, N))
+    _bf16_matrix("act_bwd", "dpre", dpre, (M, N))
+    _vector("act_bwd", "dbias", dbias, N)
+    _one_device("act_bwd", dout, pre, dpre, dbias)
+    part = _partials(dbias, M, N, dout.device)
+    part_ptr, part_bytes = _ws_args(part)
+    rc = lib().mr_act_bwd(M, N, _rows_ptr(dout), dtype_code(dout.dtype), _ld(dout), _rows_ptr(pre), _ld(pre), code,
+                          _rows_ptr(dpre), _ld(dpre), _ptr(dbias), part_ptr, part_bytes, _stream(dout))
+    _check(rc, "mr_act_bwd")
 
 
 def rmsnorm_fwd(h, w, eps, y, rstd=None) -> None:
