@@ -73,21 +73,52 @@ __device__ __forceinline__ uint4 no_piece() {
   return make_uint4(w, w, w, w);
 }
 
-// Piece i of a row of V elements (piece V / E is the last, partial one).
+// The listed or left out ones of a piece at minus infinity, a bit each.
 template <int DT>
-__device__ __forceinline__ uint4 load_piece(const uint8_t* row, int64_t i, int64_t V) {
+__device__ __forceinline__ void take_out(uint4& q, uint32_t bits) {
+  uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (DT == MR_F32) {
+      if (bits >> k & 1) w[k] = 0xff800000u;
+    } else {
+      constexpr uint32_t inf = DT == MR_BF16 ? 0xff80u : 0xfc00u;
+      if (bits >> (2 * k) & 1) w[k] = (w[k] & 0xffff0000u) | inf;
+      if (bits >> (2 * k + 1) & 1) w[k] = (w[k] & 0xffffu) | (inf << 16);
+    }
+  }
+  q = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Piece i of a row of V >= E elements, any i: what no earlier piece has of the 16
+// bytes that start at its first element or end the row, whichever is sooner; the
+// rest is minus infinity. The load is whole and without a branch (a branch around
+// a load makes each wait for the last).
+template <int DT>
+__device__ __forceinline__ uint4 piece_bytes(const uint8_t* row, int64_t i, int64_t V) {
   constexpr int E = kPiece<DT>, ES = 16 / E;
-  if ((i + 1) * E <= V) return ld16(row + i * 16);
+  return ld16(row + min(i * E, V - E) * ES);
+}
+template <int DT>
+__device__ __forceinline__ uint32_t piece_drop(int64_t i, int64_t V) {  // bits of the elements that are not the piece's
+  constexpr int E = kPiece<DT>;
+  const int64_t over = i * E - (V - E);
+  return over <= 0 ? 0u : (1u << (over < E ? static_cast<int>(over) : E)) - 1;
+}
+
+// The same of a row shorter than a piece, element by element.
+template <int DT>
+__device__ __forceinline__ uint4 short_row(const uint8_t* row, int64_t V) {
+  constexpr int E = kPiece<DT>, ES = 16 / E;
   uint4 r = no_piece<DT>();
   uint32_t w[4] = {r.x, r.y, r.z, r.w};
-  const int n = static_cast<int>(V - i * E);
 #pragma unroll
   for (int k = 0; k < E - 1; ++k) {
-    if (k >= n) continue;
+    if (k >= V) continue;
     if constexpr (ES == 4) {
-      w[k] = reinterpret_cast<const uint32_t*>(row)[i * E + k];
+      w[k] = reinterpret_cast<const uint32_t*>(row)[k];
     } else {
-      const uint32_t x = reinterpret_cast<const uint16_t*>(row)[i * E + k];
+      const uint32_t x = reinterpret_cast<const uint16_t*>(row)[k];
       w[k >> 1] = (k & 1) ? (w[k >> 1] & 0xffffu) | (x << 16) : (w[k >> 1] & 0xffff0000u) | x;
     }
   }
@@ -117,6 +148,32 @@ ExpScale exp_scale(double temperature) {
   if (hi > c) hi = std::nextafter(hi, 0.0f);
   const float lo = static_cast<float>(c - hi);
   return {hi, lo > 0.0f ? lo : std::numeric_limits<float>::min()};
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+  for (int off = 32; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
+  return x;
+}
+template <typename T>
+__device__ __forceinline__ T wave_sum(T x) {
+  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
+
+// The maximum or the sum of W waves' values, to every lane. (A lane reads one of
+// them: all W in every lane's registers at once, for eight such reductions,
+// made the held rows spill.)
+template <int W>
+__device__ __forceinline__ float waves_max(const float* v) {
+  float x = v[threadIdx.x % W];
+  for (int off = W / 2; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
+  return x;
+}
+template <int W, typename T>
+__device__ __forceinline__ T waves_sum(const T* v) {
+  T x = v[threadIdx.x % W];
+  for (int off = W / 2; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+  return x;
 }
 
 // ------------------------------------------------------------------ top logits --
@@ -153,11 +210,11 @@ struct TopParams {
 // list in LDS that is then ordered whole. A row with more candidates than the
 // list holds (many ties), a NaN or an infinity takes the radix selection.
 template <int DT, int THREADS>
-__global__ __launch_bounds__(THREADS) void top_rows(TopParams p) {
+__global__ __launch_bounds__(THREADS, 8) void top_rows(TopParams p) {
   constexpr int E = kPiece<DT>, ES = 16 / E, W = THREADS / 64, U = 4;
   __shared__ unsigned long long list[kCandidates];
   __shared__ int owners[2 * THREADS];
-  __shared__ float s_m[W], s_s[W];
+  __shared__ float s_m[W], s_b[W], s_s[W], s_v[W], s_n[W];
   __shared__ int counts[2][4][W];
   __shared__ int n_owners, n_list;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -166,16 +223,9 @@ __global__ __launch_bounds__(THREADS) void top_rows(TopParams p) {
   const int64_t pieces = (V + E - 1) / E;
   if (tid == 0) n_owners = n_list = 0;
 
-  float top[2] = {-kInf, -kInf}, m = -kInf, s = 0.0f;
-  bool has[2] = {false, false};
-  for (int64_t i0 = tid; i0 < pieces; i0 += U * THREADS) {
-    uint4 r[U];
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int64_t i = i0 + j * THREADS;
-      r[j] = no_piece<DT>();
-      if (i < pieces) r[j] = load_piece<DT>(x, i, V);
-    }
+  float top[2] = {-kInf, -kInf}, m = -kInf, base = 0.0f, s = 0.0f, dv = 0.0f, dn = 0.0f;
+  const bool has[2] = {tid < pieces, tid + THREADS < pieces};
+  auto add_up = [&](uint4(&r)[U]) __attribute__((always_inline)) {
     float mx[2] = {-kInf, -kInf};
 #pragma unroll
     for (int j = 0; j < U; ++j) {
@@ -184,14 +234,20 @@ __global__ __launch_bounds__(THREADS) void top_rows(TopParams p) {
 #pragma unroll
       for (int k = 0; k < E; ++k) mx[j & 1] = fmaxf(mx[j & 1], v[k]);
     }
-    has[0] = true;
-    has[1] = has[1] || i0 + THREADS < pieces;
     top[0] = fmaxf(top[0], mx[0]);
     top[1] = fmaxf(top[1], mx[1]);
     const float mn = fmaxf(m, fmaxf(mx[0], mx[1]));
-    const float base = mn == -kInf ? 0.0f : mn;
-    if (mn > m) s = rebase(s, m, base, p.c);
+    if (mn > m) {
+      const float grown = mn * p.c.hi, f = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(base - grown);
+      base = grown;
+      s *= f;
+      dv *= f;
+      dn *= f;
+    }
     m = mn;
+    // exp(v / T) about 2^base: one fused multiply-add and the exponential. What hi
+    // lacks of log2(e) / T comes back with the mean of v, from one in E of the terms.
+    const float b = -base;
     float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
     for (int j = 0; j < U; ++j) {
@@ -199,34 +255,70 @@ __global__ __launch_bounds__(THREADS) void top_rows(TopParams p) {
       widen<DT>(r[j], v);
 #pragma unroll
       for (int k = 0; k < E; k += 2) {
-        s0 += exp_t(v[k] - base, p.c);
-        s1 += exp_t(v[k + 1] - base, p.c);
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(v[k], p.c.hi, b));
+        if (k == 0) {
+          dv = __builtin_fmaf(fmaxf(v[0], -1e30f), e, dv);
+          dn += e;
+        }
+        s0 += e;
+        s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(v[k + 1], p.c.hi, b));
       }
     }
     s += s0 + s1;
+  };
+  if (V >= E) {
+    for (int64_t i0 = tid; i0 < pieces; i0 += U * THREADS) {
+      uint4 r[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) r[j] = piece_bytes<DT>(x, i0 + j * THREADS, V);
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+        if (const uint32_t drop = piece_drop<DT>(i0 + j * THREADS, V)) take_out<DT>(r[j], drop);
+      add_up(r);
+    }
+  } else if (tid == 0) {
+    uint4 r[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) r[j] = no_piece<DT>();
+    r[0] = short_row<DT>(x, V);
+    add_up(r);
   }
   {
-    float mw = m;
-    for (int off = 32; off > 0; off >>= 1) mw = fmaxf(mw, __shfl_xor(mw, off, 64));
-    s = rebase(s, m, mw, p.c);
-    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+    const float about = wave_max(m == -kInf ? -kInf : base);
+    const float f = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(base - about);
+    m = wave_max(m);
+    s = wave_sum(s * f);
+    dv = wave_sum(dv * f);
+    dn = wave_sum(dn * f);
     if (lane == 0) {
-      s_m[wave] = mw;
+      s_m[wave] = m;
+      s_b[wave] = about;
       s_s[wave] = s;
+      s_v[wave] = dv;
+      s_n[wave] = dn;
     }
   }
   __syncthreads();
-  m = s_m[0];
-#pragma unroll
-  for (int w = 1; w < W; ++w) m = fmaxf(m, s_m[w]);
-  s = 0.0f;
-#pragma unroll
-  for (int w = 0; w < W; ++w) s += rebase(s_s[w], s_m[w], m, p.c);
-  const bool odd = !(s > 0.0f && s < kInf);  // a NaN, an infinity, or minus infinity throughout
-  if (tid == 0 && p.lse) {
-    float l = static_cast<float>(static_cast<double>(m) / p.temperature + log(static_cast<double>(s)));
-    if (odd) l = m;  // (a NaN is the list's first entry, which tells)
-    p.lse[row] = l;
+  m = waves_max<W>(s_m);
+  bool odd;  // a NaN, an infinity, minus infinity throughout, or a maximum whose exponent is no float32
+  {
+    const float about = waves_max<W>(s_b), own = s_b[tid % W];
+    const float f = own == -kInf ? 1.0f : __builtin_amdgcn_exp2f(own - about);
+    double sum = static_cast<double>(s_s[tid % W] * f);
+    float v = s_v[tid % W] * f, n = s_n[tid % W] * f;
+    for (int off = W / 2; off > 0; off >>= 1) {
+      sum += __shfl_xor(sum, off, 64);
+      v += __shfl_xor(v, off, 64);
+      n += __shfl_xor(n, off, 64);
+    }
+    odd = !(sum > 0.0 && sum < static_cast<double>(kInf) && m < kInf);
+    if (tid == 0 && p.lse) {
+      const float mean = n > 0.0f && v < kInf && v > -kInf ? v / n : m;
+      const double l = 0.69314718055994530942 * (static_cast<double>(about) + static_cast<double>(p.c.lo) * mean) + log(sum);
+      // (odd: the maximum alone, an infinity or past what its terms reach; a NaN is
+      // the list's first entry, which tells)
+      p.lse[row] = static_cast<float>(odd ? m / p.temperature : l);
+    }
   }
 
   // The largest 16-bit key that k of the maxima reach, two bits at a time.
@@ -266,15 +358,17 @@ __global__ __launch_bounds__(THREADS) void top_rows(TopParams p) {
       const int o = q / per, j = q - o * per, own = owners[o];
       const int64_t i = (own >> 1) + static_cast<int64_t>(2 * j + (own & 1)) * THREADS;
       if (i >= pieces) continue;
+      const int64_t start = V >= E ? min(i * E, V - E) : 0;
+      const uint32_t drop = V >= E ? piece_drop<DT>(i, V) : 0xffffffffu << V;
       float v[E];
-      widen<DT>(load_piece<DT>(x, i, V), v);
+      widen<DT>(V >= E ? piece_bytes<DT>(x, i, V) : short_row<DT>(x, V), v);
 #pragma unroll
       for (int k = 0; k < E; ++k) {
         const uint32_t key = order_key(v[k]);
-        if (key >> 16 >= tau && i * E + k < V) {
+        if (key >> 16 >= tau && !(drop >> k & 1)) {
           const int at = atomicAdd(&n_list, 1);
           if (at < kCandidates)
-            list[at] = (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(i * E + k));
+            list[at] = (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - static_cast<uint32_t>(start + k));
         }
       }
     }
@@ -415,32 +509,6 @@ struct DistillParams {
   void* dz;  // null: no gradient
   int64_t ldd;
 };
-
-__device__ __forceinline__ float wave_max(float x) {
-  for (int off = 32; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
-  return x;
-}
-template <typename T>
-__device__ __forceinline__ T wave_sum(T x) {
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-  return x;
-}
-
-// The maximum or the sum of W waves' values, to every lane. (A lane reads one of
-// them: all W in every lane's registers at once, for eight such reductions,
-// made the held rows spill.)
-template <int W>
-__device__ __forceinline__ float waves_max(const float* v) {
-  float x = v[threadIdx.x % W];
-  for (int off = W / 2; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
-  return x;
-}
-template <int W, typename T>
-__device__ __forceinline__ T waves_sum(const T* v) {
-  T x = v[threadIdx.x % W];
-  for (int off = W / 2; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-  return x;
-}
 
 // The list of a row: entry e THREADS + tid is thread tid's. Ids and teacher's
 // logits lie in LDS (behind the bitmap), a register each would not fit beside the
@@ -629,44 +697,21 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// The listed ones of a piece's E logits, a bit each.
-template <int E>
-__device__ __forceinline__ uint32_t listed_bits(const uint32_t* bitmap, int i) {
-  const uint8_t* b = reinterpret_cast<const uint8_t*>(bitmap);
-  return E == 8 ? b[i] : (b[i >> 1] >> (4 * (i & 1))) & 15u;
-}
-
-// A piece with the elements of `bits` at minus infinity.
-template <int DT>
-__device__ __forceinline__ void take_out(uint4& q, uint32_t bits) {
-  uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if constexpr (DT == MR_F32) {
-      if (bits >> k & 1) w[k] = 0xff800000u;
-    } else {
-      constexpr uint32_t inf = DT == MR_BF16 ? 0xff80u : 0xfc00u;
-      if (bits >> (2 * k) & 1) w[k] = (w[k] & 0xffff0000u) | inf;
-      if (bits >> (2 * k + 1) & 1) w[k] = (w[k] & 0xffffu) | (inf << 16);
-    }
-  }
-  q = make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// Piece i of a gradient row.
+// Piece i of a gradient row, laid out as piece_bytes reads it.
 template <int DT>
 __device__ __forceinline__ void store_piece(uint8_t* row, int i, int V, uint4 o) {
   constexpr int E = kPiece<DT>, ES = 16 / E;
   if ((i + 1) * E <= V) {
-    __builtin_memcpy(row + static_cast<int64_t>(i) * 16, &o, 16);
+    __builtin_memcpy(row + static_cast<uint32_t>(i * 16), &o, 16);
     return;
   }
   const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+  const int start = V >= E ? V - E : 0;
 #pragma unroll
-  for (int k = 0; k < E - 1; ++k) {
-    if (i * E + k >= V) continue;
-    if constexpr (ES == 4) reinterpret_cast<uint32_t*>(row)[i * E + k] = w[k];
-    else reinterpret_cast<uint16_t*>(row)[i * E + k] = static_cast<uint16_t>((k & 1) ? w[k >> 1] >> 16 : w[k >> 1]);
+  for (int k = 0; k < E; ++k) {
+    if (start + k < i * E || start + k >= V) continue;
+    if constexpr (ES == 4) reinterpret_cast<uint32_t*>(row)[start + k] = w[k];
+    else reinterpret_cast<uint16_t*>(row)[start + k] = static_cast<uint16_t>((k & 1) ? w[k >> 1] >> 16 : w[k >> 1]);
   }
 }
 
@@ -701,9 +746,7 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
 
   List<DT, THREADS> l(bitmap + (V + 31) / 32 + 1, p.k);
   const typename List<DT, THREADS>::Entries entries = l.load(p, row);
-  // Every load is whole and unconditional (a branch around a load makes each wait
-  // for the last): pieces past the end are the row's last 16 bytes, of which
-  // take_out leaves what no other piece has.
+  // (pieces past the end are the row's last 16 bytes, none of them its own)
   uint4 r[N];
   auto first = [&](int t, int j) __attribute__((always_inline)) { return min((j * THREADS + t) * E, V - E); };
   // (anew: a copy of the thread's index whose products no earlier pass has kept)
@@ -838,17 +881,7 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
       uint4 o = narrow<DT>(v);
       if constexpr (DT != MR_F32) o = make_uint4(o.x ^ sign, o.y ^ sign, o.z ^ sign, o.w ^ sign);
       if (none) o = make_uint4(0, 0, 0, 0);
-      if ((i + 1) * E <= V) {
-        __builtin_memcpy(dz + static_cast<int64_t>(i) * 16, &o, 16);
-      } else {
-        const uint32_t w[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-        for (int k = 1; k < E; ++k) {
-          if (V - E + k < i * E) continue;
-          if constexpr (ES == 4) reinterpret_cast<uint32_t*>(dz)[V - E + k] = w[k];
-          else reinterpret_cast<uint16_t*>(dz)[V - E + k] = static_cast<uint16_t>((k & 1) ? w[k >> 1] >> 16 : w[k >> 1]);
-        }
-      }
+      store_piece<DT>(dz, i, V, o);
     }
     __syncthreads();  // the rest's stores are done where the list's follow
   }
@@ -876,20 +909,23 @@ __global__ __launch_bounds__(1024) void distill_twice(DistillParams p) {
   __syncthreads();
   l.mark(p, entries, z, bitmap, s);
   __syncthreads();
+  auto get = [&](int i) __attribute__((always_inline)) { return V >= E ? piece_bytes<DT>(z, i, V) : short_row<DT>(z, V); };
+  // the listed elements of a piece and those that are not its own
+  auto left_out = [&](int i) __attribute__((always_inline)) {
+    if (V < E) return i ? 0xffu : bitmap[0] & 0xffu;
+    const int at = min(i * E, V - E);
+    return (__builtin_amdgcn_alignbit(bitmap[(at >> 5) + 1], bitmap[at >> 5], at & 31) | piece_drop<DT>(i, V)) & ((1u << E) - 1);
+  };
   float mx = -kInf, sum = 0.0f;
   for (int i0 = tid; i0 < pieces; i0 += U * THREADS) {
     uint4 q[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      q[j] = no_piece<DT>();
-      if (i0 + j * THREADS < pieces) q[j] = load_piece<DT>(z, i0 + j * THREADS, V);
-    }
+    for (int j = 0; j < U; ++j) q[j] = get(i0 + j * THREADS);
     float v[U][E];
     float m = mx;
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const uint32_t bits = i0 + j * THREADS < pieces ? listed_bits<E>(bitmap, i0 + j * THREADS) : 0;
-      if (bits) take_out<DT>(q[j], bits);
+      if (const uint32_t bits = left_out(i0 + j * THREADS)) take_out<DT>(q[j], bits);
       widen<DT>(q[j], v[j]);
 #pragma unroll
       for (int k = 0; k < E; ++k) m = fmaxf(m, v[j][k]);
@@ -922,14 +958,12 @@ __global__ __launch_bounds__(1024) void distill_twice(DistillParams p) {
   for (int i0 = tid; i0 < pieces; i0 += U * THREADS) {
     uint4 q[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j)
-      if (i0 + j * THREADS < pieces) q[j] = load_piece<DT>(z, i0 + j * THREADS, V);
+    for (int j = 0; j < U; ++j) q[j] = get(i0 + j * THREADS);
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const int i = i0 + j * THREADS;
       if (i >= pieces) continue;
-      const uint32_t bits = listed_bits<E>(bitmap, i);
-      if (bits) take_out<DT>(q[j], bits);
+      if (const uint32_t bits = left_out(i)) take_out<DT>(q[j], bits);
       float v[E];
       widen<DT>(q[j], v);
 #pragma unroll

@@ -18,44 +18,46 @@ int act_forward(const GemmParams& p, bool bf16, hipStream_t s) {
   return bf16 ? dispatch<true, true, EPI_ACT + F, true>(p, s) : dispatch<true, true, EPI_ACT + F, false>(p, s);
 }
 
-// dpre = dout f'(pre) over 32 rows and 512 columns a block (64 lanes of 8 columns,
-// 4 waves of 8 rows, all of a thread's loads in flight), and the rows' column sums.
+// dpre = dout f'(pre) over 32 rows and 256 columns a block (32 lanes of 8 columns, a
+// wave 2 rows at a time and 8 in all, all of a thread's loads in flight), and the
+// rows' column sums. Bound by memory; blocks of 512 columns left 4 waves a CU at
+// 4005 x 896.
 template <int F, int DT>
 __global__ __launch_bounds__(256) void act_bwd_rows(const void* __restrict__ dout, int64_t ldo, const uint16_t* pre,
                                                     int64_t ldpre, uint16_t* dpre, int64_t ldd, int64_t M, int N,
                                                     float* colsum) {
-  __shared__ float part[4][512];
+  __shared__ float part[4][256];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * 32 + wave * 8;
-  const int col = blockIdx.x * 512 + lane * 8;
-  const bool in = col < N;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * 32 + wave * 8 + (lane >> 5);
+  const int col = blockIdx.x * 256 + (lane & 31) * 8, cb = min(col, N - 8);
+  float d[4][8], x[4][8];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int64_t row = row0 + 2 * r < M ? row0 + 2 * r : M - 1;
+    load8<DT>(dout, row * ldo + cb, d[r]);
+    load8<MR_BF16>(pre, row * ldpre + cb, x[r]);
+  }
   float sums[8] = {};
-  if (in) {
-    float d[8][8], x[8][8];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const int64_t row = row0 + r < M ? row0 + r : M - 1;
-      load8<DT>(dout, row * ldo + col, d[r]);
-      load8<MR_BF16>(pre, row * ldpre + col, x[r]);
+  for (int r = 0; r < 4; ++r) {
+    if (row0 + 2 * r >= M || col >= N) continue;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      d[r][k] *= activate_slope<F>(x[r][k]);
+      sums[k] += d[r][k];
     }
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      if (row0 + r >= M) continue;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        d[r][k] *= activate_slope<F>(x[r][k]);
-        sums[k] += d[r][k];
-      }
-      store8<MR_BF16>(dpre, (row0 + r) * ldd + col, d[r]);
-    }
+    store8<MR_BF16>(dpre, (row0 + 2 * r) * ldd + col, d[r]);
   }
   if (!colsum) return;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) part[wave][lane * 8 + k] = sums[k];
+  for (int k = 0; k < 8; ++k) {
+    sums[k] += __shfl_xor(sums[k], 32, 64);
+    if (lane < 32) part[wave][lane * 8 + k] = sums[k];
+  }
   __syncthreads();
-  for (int c = threadIdx.x; c < 512; c += 256)
-    if (static_cast<int>(blockIdx.x) * 512 + c < N)
-      colsum[static_cast<int64_t>(blockIdx.y) * N + blockIdx.x * 512 + c] = part[0][c] + part[1][c] + part[2][c] + part[3][c];
+  const int c = threadIdx.x;
+  if (static_cast<int>(blockIdx.x) * 256 + c < N)
+    colsum[static_cast<int64_t>(blockIdx.y) * N + blockIdx.x * 256 + c] = part[0][c] + part[1][c] + part[2][c] + part[3][c];
 }
 
 // dbias: the column sums of 32 rows each, added up in a fixed order. A block takes
@@ -259,7 +261,7 @@ int mr_act_bwd(int64_t M, int64_t N, const void* dout, int dout_dtype, int64_t l
                   "itself) or each other");
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 g(static_cast<unsigned>((N + 511) / 512), static_cast<unsigned>((M + 31) / 32));
+  const dim3 g(static_cast<unsigned>((N + 255) / 256), static_cast<unsigned>((M + 31) / 32));
   const uint16_t* x = static_cast<const uint16_t*>(pre);
   uint16_t* d = static_cast<uint16_t*>(dpre);
   float* cs = dbias ? partials : nullptr;
