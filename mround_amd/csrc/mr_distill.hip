@@ -135,10 +135,17 @@ __device__ __forceinline__ float exp_t(float d, ExpScale c) {
   return __builtin_amdgcn_exp2f(__builtin_fmaf(d, c.hi, d * c.lo));
 }
 
-// A sum of exponentials about `from`, about `to` >= from. (About minus infinity it
-// is zero, or NaN, and stays.)
-__device__ __forceinline__ float rebase(float s, float from, float to, ExpScale c) {
-  return from == -kInf ? s : s * exp_t(from - to, c);
+// A piece's gradient: its terms as the sum had them, 2^(v hi - b), times g; in fp32
+// to its precision, about `about`.
+template <int DT>
+__device__ __forceinline__ uint4 gradient_piece(uint4 q, float about, float b, float g, ExpScale c) {
+  constexpr int E = kPiece<DT>;
+  float v[E];
+  widen<DT>(q, v);
+#pragma unroll
+  for (int k = 0; k < E; ++k)
+    v[k] = (DT == MR_F32 ? exp_t(v[k] - about, c) : __builtin_amdgcn_exp2f(__builtin_fmaf(v[k], c.hi, b))) * g;
+  return narrow<DT>(v);
 }
 
 ExpScale exp_scale(double temperature) {
@@ -175,6 +182,93 @@ __device__ __forceinline__ T waves_sum(const T* v) {
   for (int off = W / 2; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
   return x;
 }
+
+// A logit at or below this has no part in a sum: masks write the types' lowest
+// values, whose exponents are no floats.
+constexpr float kMasked = -1e37f;
+
+// A running sum of exp(v / T), as s 2^base: base is max hi, so a term is one fused
+// multiply-add and the exponential, 2^(v hi - base). What hi lacks of log2(e) / T
+// comes back at the end, to first order, with the mean of v (from one in E of the terms).
+struct RunningSum {
+  float max = -kInf, base = 0.0f, s = 0.0f, ve = 0.0f, e = 0.0f;
+
+  template <int DT, int U>
+  __device__ __forceinline__ void add(const uint4 (&r)[U], float mx, ExpScale c) {
+    constexpr int E = kPiece<DT>;
+    if (mx > max) {
+      if (mx > kMasked) {
+        const float grown = mx * c.hi, f = max > kMasked ? __builtin_amdgcn_exp2f(base - grown) : 1.0f;
+        base = grown;
+        s *= f;
+        ve *= f;
+        e *= f;
+      }
+      max = mx;
+    }
+    const float b = -base;
+    float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      float v[E];
+      widen<DT>(r[j], v);
+#pragma unroll
+      for (int k = 0; k < E; k += 2) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(v[k], c.hi, b));
+        if (k == 0) {
+          ve = __builtin_fmaf(fmaxf(v[0], -1e30f), x, ve);
+          e += x;
+        }
+        s0 += x;
+        s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(v[k + 1], c.hi, b));
+      }
+    }
+    s += s0 + s1;
+  }
+
+  template <int W>
+  struct Shared {
+    float max[W], base[W], s[W], ve[W], e[W];
+  };
+  // The wave's into the block's, before a barrier.
+  template <int W>
+  __device__ __forceinline__ void publish(Shared<W>& sh) {
+    const float about = wave_max(max > kMasked ? base : -kInf), f = max > kMasked ? __builtin_amdgcn_exp2f(base - about) : 1.0f;
+    max = wave_max(max);
+    s = wave_sum(s * f);
+    ve = wave_sum(ve * f);
+    e = wave_sum(e * f);
+    if ((threadIdx.x & 63) == 0) {
+      const int w = threadIdx.x >> 6;
+      sh.max[w] = max;
+      sh.base[w] = about;
+      sh.s[w] = s;
+      sh.ve[w] = ve;
+      sh.e[w] = e;
+    }
+  }
+};
+
+// The block's sum: sum 2^exponent, and the maximum, on every thread.
+template <int W>
+struct BlockSum {
+  double sum, exponent;
+  float max;
+  __device__ __forceinline__ BlockSum(const RunningSum::Shared<W>& sh, ExpScale c) {
+    const int w = threadIdx.x % W;
+    max = waves_max<W>(sh.max);
+    const float about = waves_max<W>(sh.base), f = sh.base[w] == -kInf ? 1.0f : __builtin_amdgcn_exp2f(sh.base[w] - about);
+    sum = static_cast<double>(sh.s[w] * f);
+    float v = sh.ve[w] * f, n = sh.e[w] * f;
+    for (int off = W / 2; off > 0; off >>= 1) {
+      sum += __shfl_xor(sum, off, 64);
+      v += __shfl_xor(v, off, 64);
+      n += __shfl_xor(n, off, 64);
+    }
+    const float mean = n > 0.0f && v < kInf && v > -kInf ? v / n : max;
+    exponent = about == -kInf ? 0.0 : static_cast<double>(about) + static_cast<double>(c.lo) * mean;
+  }
+};
 
 // ------------------------------------------------------------------ top logits --
 
@@ -214,7 +308,7 @@ __global__ __launch_bounds__(THREADS, 8) void top_rows(TopParams p) {
   constexpr int E = kPiece<DT>, ES = 16 / E, W = THREADS / 64, U = 4;
   __shared__ unsigned long long list[kCandidates];
   __shared__ int owners[2 * THREADS];
-  __shared__ float s_m[W], s_b[W], s_s[W], s_v[W], s_n[W];
+  __shared__ RunningSum::Shared<W> s_sum;
   __shared__ int counts[2][4][W];
   __shared__ int n_owners, n_list;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -223,9 +317,10 @@ __global__ __launch_bounds__(THREADS, 8) void top_rows(TopParams p) {
   const int64_t pieces = (V + E - 1) / E;
   if (tid == 0) n_owners = n_list = 0;
 
-  float top[2] = {-kInf, -kInf}, m = -kInf, base = 0.0f, s = 0.0f, dv = 0.0f, dn = 0.0f;
+  float top[2] = {-kInf, -kInf};
   const bool has[2] = {tid < pieces, tid + THREADS < pieces};
-  auto add_up = [&](uint4(&r)[U]) __attribute__((always_inline)) {
+  RunningSum running;
+  auto add_up = [&](const uint4(&r)[U]) __attribute__((always_inline)) {
     float mx[2] = {-kInf, -kInf};
 #pragma unroll
     for (int j = 0; j < U; ++j) {
@@ -236,35 +331,7 @@ __global__ __launch_bounds__(THREADS, 8) void top_rows(TopParams p) {
     }
     top[0] = fmaxf(top[0], mx[0]);
     top[1] = fmaxf(top[1], mx[1]);
-    const float mn = fmaxf(m, fmaxf(mx[0], mx[1]));
-    if (mn > m) {
-      const float grown = mn * p.c.hi, f = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(base - grown);
-      base = grown;
-      s *= f;
-      dv *= f;
-      dn *= f;
-    }
-    m = mn;
-    // exp(v / T) about 2^base: one fused multiply-add and the exponential. What hi
-    // lacks of log2(e) / T comes back with the mean of v, from one in E of the terms.
-    const float b = -base;
-    float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      float v[E];
-      widen<DT>(r[j], v);
-#pragma unroll
-      for (int k = 0; k < E; k += 2) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(v[k], p.c.hi, b));
-        if (k == 0) {
-          dv = __builtin_fmaf(fmaxf(v[0], -1e30f), e, dv);
-          dn += e;
-        }
-        s0 += e;
-        s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(v[k + 1], p.c.hi, b));
-      }
-    }
-    s += s0 + s1;
+    running.add<DT, U>(r, fmaxf(mx[0], mx[1]), p.c);
   };
   if (V >= E) {
     for (int64_t i0 = tid; i0 < pieces; i0 += U * THREADS) {
@@ -283,45 +350,20 @@ __global__ __launch_bounds__(THREADS, 8) void top_rows(TopParams p) {
     r[0] = short_row<DT>(x, V);
     add_up(r);
   }
-  {
-    const float about = wave_max(m == -kInf ? -kInf : base);
-    const float f = m == -kInf ? 1.0f : __builtin_amdgcn_exp2f(base - about);
-    m = wave_max(m);
-    s = wave_sum(s * f);
-    dv = wave_sum(dv * f);
-    dn = wave_sum(dn * f);
-    if (lane == 0) {
-      s_m[wave] = m;
-      s_b[wave] = about;
-      s_s[wave] = s;
-      s_v[wave] = dv;
-      s_n[wave] = dn;
-    }
-  }
+  running.publish<W>(s_sum);
   __syncthreads();
-  m = waves_max<W>(s_m);
-  bool odd;  // a NaN, an infinity, minus infinity throughout, or a maximum whose exponent is no float32
+  bool odd;  // a NaN, an infinity, or no logit above the masks' values
   {
-    const float about = waves_max<W>(s_b), own = s_b[tid % W];
-    const float f = own == -kInf ? 1.0f : __builtin_amdgcn_exp2f(own - about);
-    double sum = static_cast<double>(s_s[tid % W] * f);
-    float v = s_v[tid % W] * f, n = s_n[tid % W] * f;
-    for (int off = W / 2; off > 0; off >>= 1) {
-      sum += __shfl_xor(sum, off, 64);
-      v += __shfl_xor(v, off, 64);
-      n += __shfl_xor(n, off, 64);
-    }
-    odd = !(sum > 0.0 && sum < static_cast<double>(kInf) && m < kInf);
-    if (tid == 0 && p.lse) {
-      const float mean = n > 0.0f && v < kInf && v > -kInf ? v / n : m;
-      const double l = 0.69314718055994530942 * (static_cast<double>(about) + static_cast<double>(p.c.lo) * mean) + log(sum);
-      // (odd: the maximum alone, an infinity or past what its terms reach; a NaN is
-      // the list's first entry, which tells)
-      p.lse[row] = static_cast<float>(odd ? m / p.temperature : l);
-    }
+    const BlockSum<W> all(s_sum, p.c);
+    odd = !(all.sum > 0.0 && all.sum < static_cast<double>(kInf) && all.max < kInf);
+    // (odd: the maximum alone; a NaN is the list's first entry, which tells)
+    if (tid == 0 && p.lse)
+      p.lse[row] = static_cast<float>(odd ? all.max / p.temperature : 0.69314718055994530942 * all.exponent + log(all.sum));
   }
 
-  // The largest 16-bit key that k of the maxima reach, two bits at a time.
+  // The largest 16-bit key that k of the maxima reach, two bits at a time. (Four bits
+  // a time are fewer barriers and more ballots: 2044 rows of 151936 4 us slower. One
+  // maximum a thread for short lists: twice the pieces to read again, 8 us slower.)
   uint32_t tau = 0;
   {
     const uint32_t k0 = has[0] ? order_key(top[0]) >> 16 : 0, k1 = has[1] ? order_key(top[1]) >> 16 : 0;
@@ -345,8 +387,8 @@ __global__ __launch_bounds__(THREADS, 8) void top_rows(TopParams p) {
       tau |= best << shift;
     }
     if (!odd) {
-      if (k0 >= tau && has[0]) owners[atomicAdd(&n_owners, 1)] = 2 * tid;
-      if (k1 >= tau && has[1]) owners[atomicAdd(&n_owners, 1)] = 2 * tid + 1;
+      if (has[0] && k0 >= tau) owners[atomicAdd(&n_owners, 1)] = 2 * tid;
+      if (has[1] && k1 >= tau) owners[atomicAdd(&n_owners, 1)] = 2 * tid + 1;
     }
   }
   __syncthreads();
@@ -475,8 +517,11 @@ __global__ __launch_bounds__(THREADS, 8) void top_rows(TopParams p) {
   while (size < n) size *= 2;
   for (int i = n + tid; i < size; i += THREADS) list[i] = 0;
   __syncthreads();
+  // (a wave's 64 pairs of strides up to 64 lie in 128 entries of its own, which its
+  // LDS accesses, in order as they are, leave as the next stride needs them)
   for (int width = 2; width <= size; width *= 2)
     for (int stride = width / 2; stride > 0; stride /= 2) {
+      if (stride > 64 || (stride == 64 && width > 128)) __syncthreads();
       for (int q = tid; q < size / 2; q += THREADS) {
         const int i = ((q & ~(stride - 1)) << 1) | (q & (stride - 1)), j = i + stride;
         const unsigned long long a = list[i], b = list[j];
@@ -486,8 +531,10 @@ __global__ __launch_bounds__(THREADS, 8) void top_rows(TopParams p) {
           list[j] = a;
         }
       }
-      __syncthreads();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_wave_barrier();
     }
+  __syncthreads();
   for (int i = tid; i < k_out; i += THREADS) emit(i, list[i]);
 }
 
@@ -729,7 +776,9 @@ __device__ __forceinline__ void store_piece(uint8_t* row, int i, int V, uint4 o)
 // only a sum outside 2^-64 .. 2^64 is formed again about the maximum itself.
 // exp(v / T) is 2^(v hi - b), one fused multiply-add: b is any number, and what
 // hi lacks of log2(e) / T is made up in the sum's base, to first order, by the
-// mean of v (over one in E of the terms).
+// mean of v (over one in E of the terms). The gradient takes the same terms times
+// one factor (in the exponent it would save that multiplication, and be off by
+// 2^-24 of the largest logit).
 template <int DT, int THREADS, int N>
 __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   constexpr int E = kPiece<DT>, ES = 16 / E, W = THREADS / 64;
@@ -737,7 +786,6 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   __shared__ typename List<DT, THREADS>::Shared s;
   __shared__ float s_first[W], s_ve[W], s_e[W];
   __shared__ float s_g;
-  __shared__ uint32_t s_sign;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int64_t row = blockIdx.x;
   const int V = p.V, pieces = (V + E - 1) / E;
@@ -835,6 +883,7 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
     if (lane == 0) s_first[wave] = mx;
     __syncthreads();
     about = waves_max<W>(s_first);
+    if (about <= kMasked) about = 0.0f;  // (every term is then zero)
     fresh();
     add_up(std::false_type{});
     const double r64 = wave_sum(static_cast<double>(sum));
@@ -856,30 +905,18 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
     if (wave == 0) {
       const RowSums x = row_sums();
       const double g = l.n < 0 ? __builtin_nan("") : x.rest_gradient(p);
-      if (lane == 0) {
-        // f32: term and gradient to its precision, (v - about) log2(e) / T in two
-        // parts; else the factor goes into the exponent, its sign onto the pairs
-        s_g = static_cast<float>(DT == MR_F32 ? g * exp2(about * (static_cast<double>(p.c.hi) + p.c.lo) - x.base)
-                                              : log2(fabs(g)) - x.base);
-        s_sign = g < 0.0 ? 0x80008000u : 0u;
-      }
+      if (lane == 0)
+        s_g = static_cast<float>(DT == MR_F32 ? g * exp2(about * (static_cast<double>(p.c.hi) + p.c.lo) - x.base) : g);
     }
     __syncthreads();
-    const float g = s_g;
-    const uint32_t sign = s_sign;
+    const float g = s_g, b = -about * p.c.hi;
     const int t = anew();
     fresh();
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const int i = j * THREADS + t;
       if (i >= pieces) continue;
-      float v[E];
-      widen<DT>(r[j], v);
-#pragma unroll
-      for (int k = 0; k < E; ++k)
-        v[k] = DT == MR_F32 ? exp_t(v[k] - about, p.c) * g : __builtin_amdgcn_exp2f(__builtin_fmaf(v[k], p.c.hi, g));
-      uint4 o = narrow<DT>(v);
-      if constexpr (DT != MR_F32) o = make_uint4(o.x ^ sign, o.y ^ sign, o.z ^ sign, o.w ^ sign);
+      uint4 o = gradient_piece<DT>(r[j], about, b, g, p.c);
       if (none) o = make_uint4(0, 0, 0, 0);
       store_piece<DT>(dz, i, V, o);
     }
@@ -890,15 +927,17 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   if (p.dz && l.n > 0) x.list_gradients(p, l, dz);
 }
 
-// Longer rows (and those shorter than a piece), read twice: the sum about a running maximum, then the gradient.
+// Long rows whose gradient is not asked for, those too long to hold, which are read
+// twice, and those shorter than a piece. Nothing is held, so a CU works on two rows
+// (the loss alone of 2044 rows of 151936: 135 us, 200 held; of 32000 68 and 45).
 template <int DT>
-__global__ __launch_bounds__(1024) void distill_twice(DistillParams p) {
+__global__ __launch_bounds__(1024, 8) void distill_stream(DistillParams p) {
   constexpr int THREADS = 1024, U = 4;
   constexpr int E = kPiece<DT>, ES = 16 / E, W = THREADS / 64;
   extern __shared__ uint32_t bitmap[];
   __shared__ typename List<DT, THREADS>::Shared s;
-  __shared__ float s_max[W];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  __shared__ RunningSum::Shared<W> s_sum;
+  const int tid = threadIdx.x;
   const int64_t row = blockIdx.x;
   const int V = p.V, pieces = (V + E - 1) / E;
   const uint8_t* z = static_cast<const uint8_t*>(p.z) + row * p.ldz * ES;
@@ -906,9 +945,9 @@ __global__ __launch_bounds__(1024) void distill_twice(DistillParams p) {
   List<DT, THREADS> l(bitmap + (V + 31) / 32 + 1, p.k);
   const typename List<DT, THREADS>::Entries entries = l.load(p, row);
   for (int i = tid; i <= (V + 31) / 32; i += THREADS) bitmap[i] = 0;
-  __syncthreads();
+  lds_barrier();
   l.mark(p, entries, z, bitmap, s);
-  __syncthreads();
+  lds_barrier();
   auto get = [&](int i) __attribute__((always_inline)) { return V >= E ? piece_bytes<DT>(z, i, V) : short_row<DT>(z, V); };
   // the listed elements of a piece and those that are not its own
   auto left_out = [&](int i) __attribute__((always_inline)) {
@@ -916,45 +955,37 @@ __global__ __launch_bounds__(1024) void distill_twice(DistillParams p) {
     const int at = min(i * E, V - E);
     return (__builtin_amdgcn_alignbit(bitmap[(at >> 5) + 1], bitmap[at >> 5], at & 31) | piece_drop<DT>(i, V)) & ((1u << E) - 1);
   };
-  float mx = -kInf, sum = 0.0f;
+  RunningSum running;
   for (int i0 = tid; i0 < pieces; i0 += U * THREADS) {
     uint4 q[U];
 #pragma unroll
     for (int j = 0; j < U; ++j) q[j] = get(i0 + j * THREADS);
-    float v[U][E];
-    float m = mx;
+    float mx = -kInf;
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       if (const uint32_t bits = left_out(i0 + j * THREADS)) take_out<DT>(q[j], bits);
-      widen<DT>(q[j], v[j]);
+      float v[E];
+      widen<DT>(q[j], v);
 #pragma unroll
-      for (int k = 0; k < E; ++k) m = fmaxf(m, v[j][k]);
+      for (int k = 0; k < E; ++k) mx = fmaxf(mx, v[k]);
     }
-    const float about = m == -kInf ? 0.0f : m;
-    if (m > mx) sum = rebase(sum, mx, about, p.c);
-    mx = m;
-#pragma unroll
-    for (int j = 0; j < U; ++j)
-#pragma unroll
-      for (int k = 0; k < E; ++k) sum += exp_t(v[j][k] - about, p.c);
+    running.add<DT, U>(q, mx, p.c);
   }
-  const float m = wave_max(mx);
-  if (lane == 0) s_max[wave] = m;
+  running.publish<W>(s_sum);
   l.publish(p, s);
   __syncthreads();
   l.collect(s);
-  float about = waves_max<W>(s_max);
-  sum = rebase(sum, mx, about, p.c);
-  if (about == -kInf) about = 0.0f;
-  l.sums(p, sum, s);
+  l.sums(p, 0.0f, s);
   __syncthreads();  // (and the list's reads of the row are done)
   l.finish(s);
-  const double base = static_cast<double>(about) * (static_cast<double>(p.c.hi) + p.c.lo);
-  const RowSums x(p, l, waves_sum<W>(s.rest), base);
+  const BlockSum<W> rest(s_sum, p.c);
+  const RowSums x(p, l, rest.sum, rest.exponent);
   if (tid == 0) p.row_loss[row] = x.loss(p, l);
   if (!p.dz) return;
   const bool none = l.n == 0;
-  const float g = l.n < 0 ? __builtin_nanf("") : static_cast<float>(x.rest_gradient(p));
+  const double g64 = l.n < 0 ? __builtin_nan("") : x.rest_gradient(p);
+  const float about = rest.max > kMasked ? rest.max : 0.0f, base = -about * p.c.hi;
+  const float g = static_cast<float>(DT == MR_F32 ? g64 * exp2(about * (static_cast<double>(p.c.hi) + p.c.lo) - x.base) : g64);
   for (int i0 = tid; i0 < pieces; i0 += U * THREADS) {
     uint4 q[U];
 #pragma unroll
@@ -964,11 +995,9 @@ __global__ __launch_bounds__(1024) void distill_twice(DistillParams p) {
       const int i = i0 + j * THREADS;
       if (i >= pieces) continue;
       if (const uint32_t bits = left_out(i)) take_out<DT>(q[j], bits);
-      float v[E];
-      widen<DT>(q[j], v);
-#pragma unroll
-      for (int k = 0; k < E; ++k) v[k] = none ? 0.0f : exp_t(v[k] - about, p.c) * g;
-      store_piece<DT>(dz, i, V, narrow<DT>(v));
+      uint4 o = gradient_piece<DT>(q[j], about, base, g, p.c);
+      if (none) o = make_uint4(0, 0, 0, 0);
+      store_piece<DT>(dz, i, V, o);
     }
   }
   __syncthreads();  // the rest's stores are done where the list's follow
@@ -1025,7 +1054,13 @@ int mr_top_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t 
   TopParams p{logits, ld, V, k, exp_scale(temperature), temperature, values, ids, lse};
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 g(static_cast<unsigned>(T));
-#define MR_TOP(DT) hipLaunchKernelGGL((top_rows<DT, 1024>), g, dim3(1024), 0, s, p)
+  // short rows by blocks of 256 threads, eight to a CU, where these have maxima
+  // enough for lists of k
+#define MR_TOP(DT)                                                                                          \
+  do {                                                                                                      \
+    if (V <= 16384 && k <= 256) hipLaunchKernelGGL((top_rows<DT, 256>), g, dim3(256), 0, s, p);              \
+    else hipLaunchKernelGGL((top_rows<DT, 1024>), g, dim3(1024), 0, s, p);                                   \
+  } while (0)
   if (dtype == MR_BF16) MR_TOP(MR_BF16);
   else if (dtype == MR_F16) MR_TOP(MR_F16);
   else MR_TOP(MR_F32);
@@ -1085,14 +1120,14 @@ int mr_distill(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, 
     // the fewest threads that hold the row in at most 8 pieces each, then more pieces
 #define MR_DISTILL_D(DT)                                                                   \
   do {                                                                                     \
-    if (V * es < 16) hipLaunchKernelGGL((distill_twice<DT>), g, dim3(1024), lds, s, p);     \
+    if (V * es < 16 || (!dlogits && pieces > 512 * 8)) hipLaunchKernelGGL((distill_stream<DT>), g, dim3(1024), lds, s, p); \
     else if (pieces <= 256 * 4) MR_DISTILL(DT, 256, 4);                                    \
     else if (pieces <= 256 * 8) MR_DISTILL(DT, 256, 8);                                    \
     else if (pieces <= 512 * 8) MR_DISTILL(DT, 512, 8);                                    \
     else if (pieces <= 1024 * 8) MR_DISTILL(DT, 1024, 8);                                  \
     else if (pieces <= 1024 * 14) MR_DISTILL(DT, 1024, 14);                                \
     else if (pieces <= 1024 * 20) MR_DISTILL(DT, 1024, 20);                                \
-    else hipLaunchKernelGGL((distill_twice<DT>), g, dim3(1024), lds, s, p);                \
+    else hipLaunchKernelGGL((distill_stream<DT>), g, dim3(1024), lds, s, p);                \
   } while (0)
     if (dtype == MR_BF16) MR_DISTILL_D(MR_BF16);
     else if (dtype == MR_F16) MR_DISTILL_D(MR_F16);

@@ -159,9 +159,9 @@ def reference(z, values, ids, *, scale, lse=None, temperature=1.0, upcast=torch.
         if q_rest > 0:
             loss[r] += q_rest * (math.log(q_rest) - log_rest)
         total = float(q.sum()) + q_rest
-        factor = total - (q_rest / math.exp(log_rest) if q_rest > 0 else 0.0)
-        grad[r] = p[r] * factor
-        size[r] = p[r] * (total + (q_rest / math.exp(log_rest) if q_rest > 0 else 0.0))
+        share = torch.exp(log_p[r] - log_rest) if q_rest > 0 else torch.zeros_like(p[r])  # of the rest
+        grad[r] = p[r] * total - q_rest * share
+        size[r] = p[r] * total + q_rest * share
         grad[r][i] = p[r][i] * total - q
         size[r][i] = p[r][i] * total + q
         weight[r] = total
@@ -205,10 +205,11 @@ def check(z, values, ids, *, scale, lse=None, temperature=1.0):
         + 2.0 ** -120 * scale
     gerr = (d.cpu().double() - grad).abs()
     assert bool((gerr <= gtol).all()), f"gradient: worst {float((gerr / gtol).max())} of its bound"
-    # the gradient over the logits, and no gradient: the same bits
+    # the gradient over the logits: the same bits; no gradient: within the same bound
     row2, _, d2 = run(z, values, ids, scale=scale, lse=lse, temperature=temperature, in_place=True)
     row3, _, _ = run(z, values, ids, scale=scale, lse=lse, temperature=temperature, grad=False)
-    assert torch.equal(row, row2) and torch.equal(row, row3) and torch.equal(d, d2)
+    assert torch.equal(row, row2) and torch.equal(d, d2)
+    assert bool(((row3.cpu().double() - want).abs() <= tol).all())
 
 
 # rows, V, k: a piece, odd widths, each block size and registers a thread, rows read twice
@@ -297,6 +298,39 @@ def test_rows_that_leave_nothing(tail, V):
     assert bool((gerr <= 2 * size * (unit(V) + 4 * far * 2.0 ** -24) + 2.0 ** -24 * grad.abs() + 2.0 ** -120).all())
     assert bool((d[3][torch.isinf(z[3])] == 0).all())
     assert math.isnan(float(loss))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("V", [300, 100003])
+def test_masks_of_the_lowest_value(V, dtype):
+    """A mask of the type's lowest value takes logits out as minus infinity does, of most of the row and of all of
+    it but the list, whatever stands in the row's first pieces; far rows keep their sums."""
+    T, k = 4, 5
+    low = torch.finfo(DT[dtype]).min
+    z, values, ids, teacher = make(T, V, k, dtype, seed=8)
+    z[0, V // 4:] = low
+    z[1, : V - 3] = low
+    z[1, V - 3:] = 0.5
+    keep = torch.zeros(V, dtype=torch.bool)
+    keep[ids[2].long()] = True
+    z[2, ~keep] = low
+    z[3] = (z[3].float() - 30000).to(z.dtype)  # far from zero, and in one binade
+    lse = torch.logsumexp(teacher.double(), 1).float()
+    # the list and the row's far part alone above the mask: what the formulas say of minus infinity
+    as_inf = torch.where(z == low, torch.full_like(z, -math.inf), z) if dtype != "f16" else z
+    for tail in (lse, None):
+        want, grad, size, weight, far = reference(as_inf, values, ids, scale=64.0, lse=tail)
+        row, _, d = run(z, values, ids, scale=64.0, lse=tail)
+        row2, _, _ = run(z, values, ids, scale=64.0, lse=tail, grad=False)
+        tol = 2 * weight * unit(V) + 2.0 ** -24 * want.abs() + 1e-12
+        for r in (row, row2):
+            err = (r.cpu().double() - want).abs()
+            ok = (err <= tol) | (torch.isinf(want) & (r.cpu().double() == want))
+            assert bool(ok.all()), (tail is None, r, want)
+        gtol = 2 * size * (unit(V) + 4 * far * 2.0 ** -24) + torch.finfo(z.dtype).eps / 2 * grad.abs() \
+            + 2.0 ** -25 * (dtype == "f16") + 2.0 ** -100
+        assert bool(((d.cpu().double() - grad).abs() <= gtol).all())
 
 
 @pytest.mark.gpu
