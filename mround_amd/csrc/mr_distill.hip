@@ -779,13 +779,20 @@ __device__ __forceinline__ void store_piece(uint8_t* row, int i, int V, uint4 o)
 // mean of v (over one in E of the terms). The gradient takes the same terms times
 // one factor (in the exponent it would save that multiplication, and be off by
 // 2^-24 of the largest logit).
-template <int DT, int THREADS, int N>
+//
+// Two rows to a CU hide one another's waits: 2044 16-bit rows of 65536 logits take
+// 181 us by one block of 1024 threads a CU and 121 by two of 512, and 1022 float32
+// rows of 49152 108 and 88. So M further pieces of a thread lie in LDS, where rows
+// somewhat past the registers of half a CU still come in twos. Longer ones (the 2044
+// of 151936: 326 us, of which the loads alone are 135) have the CU to themselves.
+template <int DT, int THREADS, int N, int M>
 __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   constexpr int E = kPiece<DT>, ES = 16 / E, W = THREADS / 64;
   extern __shared__ uint32_t bitmap[];  // a bit per logit, a word more, and the list
   __shared__ typename List<DT, THREADS>::Shared s;
   __shared__ float s_first[W], s_ve[W], s_e[W];
   __shared__ float s_g;
+  __shared__ uint4 beside[M ? M * THREADS : 1];  // pieces N .. N + M - 1
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int64_t row = blockIdx.x;
   const int V = p.V, pieces = (V + E - 1) / E;
@@ -803,6 +810,9 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
     asm volatile("" : "+v"(t));
     return t;
   };
+  uint4 early[M ? M : 1];  // on their way to LDS
+#pragma unroll
+  for (int j = 0; j < M; ++j) early[j] = ld16(z + static_cast<uint32_t>(first(tid, N + j) * ES));
 #pragma unroll
   for (int j = 0; j < N; ++j) r[j] = ld16(z + static_cast<uint32_t>(first(tid, j) * ES));
   for (int i = tid; i <= (V + 31) / 32; i += THREADS) bitmap[i] = 0;
@@ -810,7 +820,7 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   l.mark(p, entries, z, bitmap, s);
   {
     float v[E], mx = -kInf;
-    widen<DT>(r[0], v);
+    widen<DT>(M ? early[0] : r[0], v);
 #pragma unroll
     for (int k = 0; k < E; ++k) mx = fmaxf(mx, v[k]);
     mx = wave_max(mx);
@@ -830,15 +840,14 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
     const int t = anew();
     float s0 = 0.0f, s1 = 0.0f;
     ve = se = 0.0f;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
+    auto one = [&](int j, uint4& q) __attribute__((always_inline)) {
       if constexpr (decltype(takes)::value) {
         const int at = first(t, j), drop = min((j * THREADS + t) * E - at, E);
         const uint32_t bits = __builtin_amdgcn_alignbit(bitmap[(at >> 5) + 1], bitmap[at >> 5], at & 31) | ((1u << drop) - 1);
-        if (bits & ((1u << E) - 1)) take_out<DT>(r[j], bits);
+        if (bits & ((1u << E) - 1)) take_out<DT>(q, bits);
       }
       float v[E];
-      widen<DT>(r[j], v);
+      widen<DT>(q, v);
 #pragma unroll
       for (int k = 0; k < E; k += 2) {
         const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(v[k], p.c.hi, b));
@@ -851,9 +860,25 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
       }
       // Here, as the pieces arrive: left alone the sums move behind the next barrier,
       // and the bitmap's words of every piece are read ahead (40 registers).
-      asm volatile("" : "+v"(s0), "+v"(s1), "+v"(ve), "+v"(se));
+      // (And of float32 pieces, copies from before the listed were taken out are kept.)
+      if constexpr (DT == MR_F32)
+        asm volatile("" : "+v"(s0), "+v"(s1), "+v"(ve), "+v"(se), "+v"(q.x), "+v"(q.y), "+v"(q.z), "+v"(q.w));
+      else
+        asm volatile("" : "+v"(s0), "+v"(s1), "+v"(ve), "+v"(se));
       if (j & 1) __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (int j = 0; j < M; ++j) {
+      if constexpr (decltype(takes)::value) {
+        one(N + j, early[j]);
+        beside[j * THREADS + tid] = early[j];
+      } else {
+        uint4 q = beside[j * THREADS + tid];
+        one(N + j, q);
+      }
     }
+#pragma unroll
+    for (int j = 0; j < N; ++j) one(j, r[j]);
     sum = s0 + s1;
     ve = wave_sum(ve);
     se = wave_sum(se);
@@ -872,13 +897,16 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   if (!(rest0 > 0x1p-64 && rest0 < 0x1p64)) {  // (or a NaN)
     fresh();
     float mx = -kInf;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
+    auto most = [&](uint4 q) __attribute__((always_inline)) {
       float v[E];
-      widen<DT>(r[j], v);
+      widen<DT>(q, v);
 #pragma unroll
       for (int k = 0; k < E; ++k) mx = fmaxf(mx, v[k]);
-    }
+    };
+#pragma unroll
+    for (int j = 0; j < N; ++j) most(r[j]);
+#pragma unroll
+    for (int j = 0; j < M; ++j) most(beside[j * THREADS + tid]);
     mx = wave_max(mx);
     if (lane == 0) s_first[wave] = mx;
     __syncthreads();
@@ -912,14 +940,18 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
     const float g = s_g, b = -about * p.c.hi;
     const int t = anew();
     fresh();
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
+    auto put = [&](int j, uint4 q) __attribute__((always_inline)) {
       const int i = j * THREADS + t;
-      if (i >= pieces) continue;
-      uint4 o = gradient_piece<DT>(r[j], about, b, g, p.c);
+      if (i >= pieces) return;
+      uint4 o = gradient_piece<DT>(q, about, b, g, p.c);
       if (none) o = make_uint4(0, 0, 0, 0);
       store_piece<DT>(dz, i, V, o);
-    }
+      if (DT == MR_F32) __builtin_amdgcn_sched_barrier(0);  // (else pieces in float32 are worked on together, and spill)
+    };
+#pragma unroll
+    for (int j = 0; j < N; ++j) put(j, r[j]);
+#pragma unroll
+    for (int j = 0; j < M; ++j) put(N + j, beside[j * THREADS + tid]);
     __syncthreads();  // the rest's stores are done where the list's follow
   }
   const RowSums x = row_sums();
@@ -1116,18 +1148,21 @@ int mr_distill(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, 
     const dim3 g(static_cast<unsigned>(T));
     const size_t lds = static_cast<size_t>((V + 31) / 32 + 1) * 4 + static_cast<size_t>(k) * 8;
     const int64_t pieces = (V * es + 15) / 16;
-#define MR_DISTILL(DT, THREADS, N) hipLaunchKernelGGL((distill_held<DT, THREADS, N>), g, dim3(THREADS), lds, s, p)
-    // the fewest threads that hold the row in at most 8 pieces each, then more pieces
-#define MR_DISTILL_D(DT)                                                                   \
-  do {                                                                                     \
-    if (V * es < 16 || (!dlogits && pieces > 512 * 8)) hipLaunchKernelGGL((distill_stream<DT>), g, dim3(1024), lds, s, p); \
-    else if (pieces <= 256 * 4) MR_DISTILL(DT, 256, 4);                                    \
-    else if (pieces <= 256 * 8) MR_DISTILL(DT, 256, 8);                                    \
-    else if (pieces <= 512 * 8) MR_DISTILL(DT, 512, 8);                                    \
-    else if (pieces <= 1024 * 8) MR_DISTILL(DT, 1024, 8);                                  \
-    else if (pieces <= 1024 * 14) MR_DISTILL(DT, 1024, 14);                                \
-    else if (pieces <= 1024 * 20) MR_DISTILL(DT, 1024, 20);                                \
-    else hipLaunchKernelGGL((distill_stream<DT>), g, dim3(1024), lds, s, p);                \
+#define MR_DISTILL(DT, THREADS, N, M) hipLaunchKernelGGL((distill_held<DT, THREADS, N, M>), g, dim3(THREADS), lds, s, p)
+    // the fewest threads that hold the row in at most 8 pieces each, then more
+    // pieces, as long as two rows fit a CU; then one row
+#define MR_DISTILL_D(DT)                                                                                 \
+  do {                                                                                                   \
+    if (V * es < 16 || (!dlogits && pieces > 512 * 8))                                                   \
+      hipLaunchKernelGGL((distill_stream<DT>), g, dim3(1024), lds, s, p);                                \
+    else if (pieces <= 256 * 4) MR_DISTILL(DT, 256, 4, 0);                                               \
+    else if (pieces <= 256 * 8) MR_DISTILL(DT, 256, 8, 0);                                               \
+    else if (pieces <= 512 * 8) MR_DISTILL(DT, 512, 8, 0);                                               \
+    else if (pieces <= 512 * 16) MR_DISTILL(DT, 512, 16, 0);                                             \
+    else if (pieces <= 512 * 20) MR_DISTILL(DT, 512, 20, 0);                                             \
+    else if (pieces <= 512 * 24) MR_DISTILL(DT, 512, 17, 7);                                             \
+    else if (pieces <= 1024 * 20) MR_DISTILL(DT, 1024, 20, 0);                                           \
+    else hipLaunchKernelGGL((distill_stream<DT>), g, dim3(1024), lds, s, p);                             \
   } while (0)
     if (dtype == MR_BF16) MR_DISTILL_D(MR_BF16);
     else if (dtype == MR_F16) MR_DISTILL_D(MR_F16);

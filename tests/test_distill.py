@@ -214,7 +214,8 @@ def check(z, values, ids, *, scale, lse=None, temperature=1.0):
 
 # rows, V, k: a piece, odd widths, each block size and registers a thread, rows read twice
 DISTILL_CASES = [(1, 1, 1), (3, 5, 2), (4, 100, 100), (5, 1001, 17), (2, 5000, 1024), (3, 8193, 64), (3, 16385, 300),
-                 (2, 40001, 33), (2, 90000, 8), (2, 151936, 64), (2, 151935, 64), (2, 200001, 100)]
+                 (2, 40001, 33), (2, 52001, 33), (2, 75001, 12), (2, 90000, 8), (2, 106001, 40), (2, 151936, 64),
+                 (2, 151935, 64), (2, 200001, 100), (1, 1 << 20, 1024)]
 
 
 @pytest.mark.gpu
