@@ -272,8 +272,8 @@ def _scoring_tokens(calibration, vocab: int, samples: int, sequence: int, *, see
 def _plan_mixed(model: DecoderModel, base: QuantScheme, average_bits: float, candidate_bits, calibration,
                 *, gradient_source: str = "auto", remainder_bits: int | None = None,
                 scoring_samples: int | None = None, scoring_seq_len: int | None = None,
-                scoring_batch: int | None = None, seed: int = 0, device="cuda",
-                progress=None) -> tuple[dict[str, QuantScheme], dict[str, Any]]:
+                scoring_batch: int | None = None, seed: int = 0, device="cuda", progress=None,
+                objective: str = "labels") -> tuple[dict[str, QuantScheme], dict[str, Any]]:
     """Score, allocate, and return per-layer schemes plus what was decided
     (mround/api.py:1471-1695)."""
     from mround_amd.pipeline.scoring import eligible_block_layers, score_widths
@@ -299,7 +299,8 @@ def _plan_mixed(model: DecoderModel, base: QuantScheme, average_bits: float, can
     tokens = _scoring_tokens(calibration, int(model.config["vocab_size"]), samples, sequence, seed=seed,
                              device=device)
     batches = [tokens[i:i + batch] for i in range(0, samples, batch)]
-    scored = score_widths(model, batches, widths, base, gradient_source=gradient_source, progress=progress)
+    scored = score_widths(model, batches, widths, base, gradient_source=gradient_source, progress=progress,
+                          objective=objective)
     dtype_bits = _dtype_bits(model)
     options = score_layer_options(scored.scores, scored.shapes, base, dtype_bits=dtype_bits)
     budget = mixed_budget_bits(scored.shapes, average_bits, base.group_size, dtype_bits=dtype_bits)
@@ -311,7 +312,7 @@ def _plan_mixed(model: DecoderModel, base: QuantScheme, average_bits: float, can
     info.update(
         source="scored", predicted_loss=allocation.predicted_loss, scoring_seconds=round(scored.seconds, 1),
         scoring_samples=samples, scoring_seq_len=sequence, scoring_batch_size=batch,
-        gradient_source=gradient_source, gradient_source_requested=requested,
+        gradient_source=gradient_source, gradient_source_requested=requested, objective=objective,
         scored_weights=scored_weights,
         describe=(f"planned {summary}; {info['achieved_code_bits']:.3f} code bits per weight against a "
                   f"target of {average_bits:g}, remainder at {remainder} bits, scored {samples}x{sequence} "
@@ -522,6 +523,11 @@ def predict_time(model: str | Path, *, bits: int = 4, group_size: int = 64,
                             scoring_seq_len=scoring_seq_len, gradient_source=sensitivity_gradients)
 
 
+def _check_objective(objective: str) -> None:
+    if objective not in ("labels", "teacher"):
+        raise SchemeError(f"sensitivity_objective must be 'labels' or 'teacher', got {objective!r}")
+
+
 def _check_calibration_sizes(tuning: TuningConfig) -> None:
     """mround/pipeline/calibration.py:442-447, before anything is predicted or loaded."""
     if tuning.n_samples < 1 or tuning.seq_len < 1 or tuning.batch_size < 1:
@@ -557,7 +563,8 @@ def quantize(model: str | Path, *, output_dir: str | Path, bits: int = 4, group_
              scale_init: ScaleInit | str | None = None, seed: int | None = None,
              memory_budget: int | None = None, memory_check: bool = True,
              min_block_coverage: float = MIN_BLOCK_COVERAGE, split_precision: bool | None = None,
-             device: str = "cuda", progress=None, scoring_progress=None) -> QuantizeResult:
+             device: str = "cuda", progress=None, scoring_progress=None,
+             sensitivity_objective: str = "labels") -> QuantizeResult:
     """Quantize the local checkpoint ``model`` into ``output_dir``.
 
     ``calibration`` is ``"random"`` (``"auto"`` is the same here: token ids
@@ -567,6 +574,9 @@ def quantize(model: str | Path, *, output_dir: str | Path, bits: int = 4, group_
     and an exact allocation (or, with ``plan``, the given per-layer widths),
     the block layers tuned at their assigned widths and the remainder at
     ``remainder_bits`` (default: the width nearest the average, ties up).
+    The scoring pass takes its gradients from the cross-entropy of the
+    calibration tokens, or with ``sensitivity_objective`` "teacher" from the
+    divergence between the quantized model's predictions and the model's own.
     The run's device memory is predicted from ``config.json`` before anything
     is loaded (``predict_memory``) and a run past ``memory_budget`` (default
     90 % of the device's memory) is refused with ``MemoryBudgetError`` unless
@@ -592,6 +602,7 @@ def quantize(model: str | Path, *, output_dir: str | Path, bits: int = 4, group_
         raise UnsupportedSchemeError(f"export format {export_format!r} is not supported; only 'mlx'")
     if holdout_batches < 0:
         raise CalibrationError(f"holdout_batches must be zero or more, got {holdout_batches}")
+    _check_objective(sensitivity_objective)
     _refuse_unusable_plan(plan, average_bits, candidate_bits)
     resolved, widths = _resolve_scheme(bits=bits, group_size=group_size, symmetry=symmetry,
                                        average_bits=average_bits, candidate_bits=candidate_bits,
@@ -651,7 +662,8 @@ def quantize(model: str | Path, *, output_dir: str | Path, bits: int = 4, group_
                 m, resolved, average_bits, candidate_bits, calibration,
                 gradient_source=sensitivity_gradients, remainder_bits=remainder_bits,
                 scoring_samples=scoring_samples, scoring_seq_len=scoring_seq_len,
-                scoring_batch=scoring_batch_size, seed=seed, device=device, progress=scoring_progress)
+                scoring_batch=scoring_batch_size, seed=seed, device=device, progress=scoring_progress,
+                objective=sensitivity_objective)
         remainder_scheme = resolved.with_bits(int(mixed["remainder_bits"]))
         plan_s = time.perf_counter() - tp
         if requested_split is None:  # the plan decides which widths are tuned
@@ -770,10 +782,13 @@ def plan_mixed_precision(model: str | Path, average_bits: float, candidate_bits:
                          calibration: str | torch.Tensor = "random", sensitivity_gradients: str = "auto",
                          remainder_bits: int | None = None, scoring_samples: int | None = None,
                          scoring_seq_len: int | None = None, scoring_batch_size: int | None = None,
-                         seed: int | None = None, device: str = "cuda", progress=None) -> dict[str, Any]:
+                         seed: int | None = None, device: str = "cuda", progress=None,
+                         sensitivity_objective: str = "labels") -> dict[str, Any]:
     """Score and allocate, and stop there: nothing is tuned or written
     (mround/api.py:943-1085). Returns the plan summary, whose
-    ``assignments`` map each block layer path to its width."""
+    ``assignments`` map each block layer path to its width.
+    ``sensitivity_objective`` as :func:`quantize`'s."""
+    _check_objective(sensitivity_objective)
     resolved, widths = _resolve_scheme(bits=bits, group_size=group_size, symmetry=symmetry,
                                        average_bits=average_bits, candidate_bits=candidate_bits,
                                        remainder_bits=remainder_bits, scheme=scheme, scale_init=scale_init)
@@ -787,5 +802,5 @@ def plan_mixed_precision(model: str | Path, average_bits: float, candidate_bits:
                           gradient_source=sensitivity_gradients, remainder_bits=remainder_bits,
                           scoring_samples=scoring_samples, scoring_seq_len=scoring_seq_len,
                           scoring_batch=scoring_batch_size, seed=0 if seed is None else int(seed),
-                          device=device, progress=progress)
+                          device=device, progress=progress, objective=sensitivity_objective)
     return info

@@ -74,6 +74,9 @@ def _parser() -> argparse.ArgumentParser:
     pl.add_argument("--asym", action="store_true")
     pl.add_argument("--remainder-bits", type=int, default=None)
     pl.add_argument("--gradients", default="auto", help="auto, own_width or widest")
+    pl.add_argument("--objective", default="labels", choices=("labels", "teacher"),
+                    help="score with the cross-entropy of the tokens, or with the divergence from the "
+                         "unquantized model's own predictions")
     pl.add_argument("--scoring-samples", type=int, default=None)
     pl.add_argument("--scoring-seq-len", type=int, default=None)
     pl.add_argument("--scoring-batch-size", type=int, default=None)
@@ -129,7 +132,8 @@ def main(argv=None) -> int:
             info = api.plan_mixed_precision(
                 args.model, args.average_bits, _widths(args.options), bits=args.bits,
                 group_size=args.group_size, symmetry=Symmetry.ASYMMETRIC if args.asym else Symmetry.SYMMETRIC,
-                sensitivity_gradients=args.gradients, remainder_bits=args.remainder_bits,
+                sensitivity_gradients=args.gradients, sensitivity_objective=args.objective,
+                remainder_bits=args.remainder_bits,
                 scoring_samples=args.scoring_samples, scoring_seq_len=args.scoring_seq_len,
                 scoring_batch_size=args.scoring_batch_size, seed=args.seed,
                 progress=lambda step: print(step.describe(), flush=True))

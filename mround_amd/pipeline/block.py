@@ -67,6 +67,10 @@ class BlockShape:
     # RoPE frequency scaling as sorted (key, value) pairs of the config's
     # rope_scaling ("rope_type" plus its parameters); empty: none.
     rope_scaling: tuple = ()
+    # the rotated part of a head (0: all of it), and whether its pairs are
+    # neighbours (mlx's rope_traditional) rather than halves
+    rotary_dim: int = 0
+    rope_interleaved: bool = False
 
     @property
     def qkv_rows(self) -> int:
@@ -96,6 +100,8 @@ class BlockShape:
             problems.append("hidden and n_heads * head_dim must be multiples of 64")
         if self.intermediate % 64:
             problems.append(f"intermediate size {self.intermediate} is not a multiple of 64")
+        if self.rotary_dim % 2 or not 0 <= self.rotary_dim <= self.head_dim:
+            problems.append(f"the rotated part {self.rotary_dim} of a head is not an even size up to {self.head_dim}")
         if seq_len is not None and seq_len % 128:
             problems.append(f"sequence length {seq_len} is not a multiple of 128")
         if problems:
@@ -210,18 +216,22 @@ def workspace_bytes(shape: BlockShape, batch: int, seq_len: int,
     return gemm, attn
 
 
-ROPE_TYPES = ("default", "linear", "llama3")
+ROPE_TYPES = ("default", "linear", "llama3", "yarn")
 
 
 def rope_frequencies(head_dim: int, theta: float, scaling: tuple = ()) -> torch.Tensor:
-    """The rotary frequencies ``theta^(-2i/d)`` (float64), rescaled as the
-    config's ``rope_scaling`` asks: "linear" divides every frequency by
-    ``factor``; "llama3" (Meta's Llama 3.1 rule) keeps the frequencies whose
-    wavelength is under ``original_max_position_embeddings / high_freq_factor``,
-    divides those over ``original_max_position_embeddings / low_freq_factor``
-    by ``factor``, and blends the two linearly in between, by where
+    """The rotary frequencies ``theta^(-2i/d)`` (float64; ``head_dim``: the
+    rotated part), rescaled as the config's ``rope_scaling`` asks: "linear"
+    divides every frequency by ``factor``; "llama3" (Meta's Llama 3.1 rule)
+    keeps the frequencies whose wavelength is under
+    ``original_max_position_embeddings / high_freq_factor``, divides those over
+    ``original_max_position_embeddings / low_freq_factor`` by ``factor``, and
+    blends the two linearly in between, by where
     ``original_max_position_embeddings / wavelength`` falls between the two
-    factors."""
+    factors; "yarn" (Peng et al., 2023) keeps the pairs that turn
+    ``beta_fast`` times and more over ``original_max_position_embeddings``,
+    divides those of ``beta_slow`` turns and less by ``factor`` and blends in
+    between, linearly in the pair's index (:func:`rope_magnitude` goes with it)."""
     inv = theta ** (-torch.arange(0, head_dim, 2, dtype=torch.float64) / head_dim)
     params = dict(scaling)
     kind = params.get("rope_type", "default")
@@ -238,7 +248,38 @@ def rope_frequencies(head_dim: int, theta: float, scaling: tuple = ()) -> torch.
         scaled = (1 - blend) * inv / factor + blend * inv
         return torch.where(wavelength < context / high, inv,
                            torch.where(wavelength > context / low, inv / factor, scaled))
+    if kind == "yarn":
+        context = float(params["original_max_position_embeddings"])
+
+        def pair_of(turns: float) -> float:  # the pair (not whole) that turns so often over the context
+            return head_dim * math.log(context / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+        first, last = pair_of(float(params.get("beta_fast", 32.0))), pair_of(float(params.get("beta_slow", 1.0)))
+        if params.get("truncate", True):
+            first, last = math.floor(first), math.ceil(last)
+        first, last = max(first, 0), min(last, head_dim - 1)
+        width = last - first if last != first else 1e-3
+        slow = ((torch.arange(head_dim // 2, dtype=torch.float64) - first) / width).clamp(0.0, 1.0)
+        return inv / factor * slow + inv * (1 - slow)
     raise ArchitectureError(f"rope_scaling type {kind!r} is not supported (supported: {', '.join(ROPE_TYPES)})")
+
+
+def rope_magnitude(scaling: tuple = ()) -> float:
+    """What the rotated part of queries and keys is multiplied by: 1, or with
+    "yarn" the config's ``attention_factor``, the ratio of its ``mscale`` and
+    ``mscale_all_dim`` corrections, or ``0.1 ln(factor) + 1``."""
+    params = dict(scaling)
+    if params.get("rope_type") != "yarn":
+        return 1.0
+    if params.get("attention_factor") is not None:
+        return float(params["attention_factor"])
+
+    def grown(m: float) -> float:
+        return 0.1 * m * math.log(params["factor"]) + 1.0 if params["factor"] > 1 else 1.0
+
+    if params.get("mscale") and params.get("mscale_all_dim"):
+        return grown(params["mscale"]) / grown(params["mscale_all_dim"])
+    return grown(1.0)
 
 
 def rope_table(seq_len: int, head_dim: int, theta: float, device, scaling: tuple = ()) -> torch.Tensor:
@@ -313,7 +354,17 @@ class BlockEngine:
             self.acts = e(T, 3 * mlp)
             self.qkv32, self.qkv_lo = e(T, shape.qkv_rows, dt=f32), e(T, shape.qkv_rows)
             self.attns = e(T, 3 * hq_d)
-        self.cos_sin = rope_table(seq_len, shape.head_dim, shape.rope_theta, self.device, shape.rope_scaling)
+        # The rotation of halves of whole heads reads a table; any other one
+        # (rope_positions) computes its angles from positions and frequencies.
+        self.rope_scale = rope_magnitude(shape.rope_scaling)
+        rotary = shape.rotary_dim or shape.head_dim
+        self.table_rope = rotary == shape.head_dim and not shape.rope_interleaved and self.rope_scale == 1.0
+        self.cos_sin = self.positions = self.rope_freq = None
+        if self.table_rope:
+            self.cos_sin = rope_table(seq_len, shape.head_dim, shape.rope_theta, self.device, shape.rope_scaling)
+        else:
+            self.positions = torch.arange(seq_len, dtype=torch.int32, device=self.device).repeat(batch)
+            self.rope_freq = rope_frequencies(rotary, shape.rope_theta, shape.rope_scaling).to(self.device)
         self.scale = 1.0 / math.sqrt(shape.head_dim)
         self.place = placements(shape)
         self.loss_ws = K.loss_workspace(self.device, T * h)
@@ -338,6 +389,17 @@ class BlockEngine:
                  "grad_out16", "dgu", "dx2", "dh2", "dattn", "dqkv")
     PER_SEQUENCE = ("lse", "dsum")
     SPLIT_PER_TOKEN = ("x1s", "x2s", "acts", "qkv32", "qkv_lo", "attns")
+
+    def _rotate(self, x: torch.Tensor, *, backward: bool = False) -> None:
+        """Rotate the query and key heads of q/k/v rows ``x`` in place."""
+        s = self.shape
+        if self.table_rope:
+            K.rope(x, seq_len=self.seq_len, n_heads=s.n_heads + s.n_kv_heads, head_dim=s.head_dim,
+                   cos_sin=self.cos_sin, backward=backward)
+        else:
+            K.rope_positions(x, self.positions[:self.tokens], self.rope_freq, n_heads=s.n_heads + s.n_kv_heads,
+                             head_dim=s.head_dim, pairing="interleaved" if s.rope_interleaved else "half",
+                             scale=self.rope_scale, backward=backward)
 
     def set_sequences(self, n: int) -> None:
         """Run the next passes over ``n`` sequences (at most the capacity the
@@ -455,8 +517,7 @@ class BlockEngine:
         K.rmsnorm_fwd(x, self.norm_in, s.norm_eps, self.x1, self.rstd1)
         self._run("gemm_qkv", lambda: K.gemm("nt", self.x1, self.wq["qkv"], self.qkv, M=T, N=s.qkv_rows,
                                              K=h, bias=self.bias_qkv, workspace=ws))
-        K.rope(self.qkv, seq_len=self.seq_len, n_heads=s.n_heads + s.n_kv_heads, head_dim=s.head_dim,
-               cos_sin=self.cos_sin)
+        self._rotate(self.qkv)
         self._run("attn_fwd", lambda: K.attn_fwd(
             self.qkv, batch=self.batch, seq_len=self.seq_len, n_heads=s.n_heads,
             n_kv_heads=s.n_kv_heads, head_dim=s.head_dim, scale=self.scale, out=self.attn, lse=self.lse))
@@ -487,8 +548,11 @@ class BlockEngine:
         self._run("gemm_qkv", lambda: K.gemm("nt", self.x1s, self.wqs["qkv"], self.qkv32, M=T, N=s.qkv_rows,
                                              K=3 * h, bias=self.bias_qkv, workspace=ws))
         # rotated in fp32, then hi (the backward's q/k/v) and lo halves
+        if not self.table_rope:
+            self._rotate(self.qkv32)
         K.rope_split(self.qkv32, self.qkv, self.qkv_lo, seq_len=self.seq_len,
-                     n_rope_heads=s.n_heads + s.n_kv_heads, head_dim=s.head_dim, cos_sin=self.cos_sin)
+                     n_rope_heads=s.n_heads + s.n_kv_heads if self.table_rope else 0, head_dim=s.head_dim,
+                     cos_sin=self.cos_sin if self.table_rope else self.norm_in)  # (no head left to rotate: not read)
         self._run("attn_fwd", lambda: K.attn_fwd_split(
             self.qkv, self.qkv_lo, batch=self.batch, seq_len=self.seq_len, n_heads=s.n_heads,
             n_kv_heads=s.n_kv_heads, head_dim=s.head_dim, scale=self.scale, out=self.attn,
@@ -583,8 +647,7 @@ class BlockEngine:
             self.qkv, self.attn, self.dattn, self.lse, self.dsum, batch=self.batch,
             seq_len=self.seq_len, n_heads=s.n_heads, n_kv_heads=s.n_kv_heads, head_dim=s.head_dim,
             scale=self.scale, dqkv=self.dqkv, workspace=self.attn_ws))
-        K.rope(self.dqkv, seq_len=self.seq_len, n_heads=s.n_heads + s.n_kv_heads,
-               head_dim=s.head_dim, cos_sin=self.cos_sin, backward=True)
+        self._rotate(self.dqkv, backward=True)
         self._run("gemm_dw_qkv", lambda: K.gemm("tn", self.dqkv, self.x1, self.dw["qkv"], M=s.qkv_rows,
                                                 N=h, K=T, resid=acc("qkv"), workspace=ws))
         if dx_out is None:

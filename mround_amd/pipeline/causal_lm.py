@@ -11,6 +11,7 @@ block kernels:
     x_{i+1} = block_i(x_i)                            BlockEngine.forward
     logits = rmsnorm(x_L) head^T  (bf16)              mr_rmsnorm_fwd, mr_gemm nt
     loss = mean_t CE(logits_t, label_t)               mr_cross_entropy
+           (or the divergence from a teacher's top logits, mr_distill)
     dlogits -> dx_L -> block backward i = L-1 .. 0    mr_gemm nn, mr_rmsnorm_bwd,
                                                       BlockEngine.backward(dx_out)
 
@@ -40,6 +41,7 @@ Layout in HBM, allocated once:
 
 from __future__ import annotations
 
+import dataclasses
 from collections.abc import Callable, Mapping
 
 import torch
@@ -54,6 +56,19 @@ from mround_amd.schemes import DEFAULT_EPS_FP32, QuantScheme
 def padded_length(seq_len: int) -> int:
     """Positions the engine runs for sequences of ``seq_len`` tokens."""
     return aligned_length(seq_len - 1)
+
+
+@dataclasses.dataclass(frozen=True)
+class TeacherList:
+    """A model's likeliest tokens at every row of a batch (``CausalLM.teacher_list``):
+    float32 logits and int32 ids ``[T, top]`` (ids -1 at rows that are padding), the
+    rows' log-sum-exp ``[T]`` at ``temperature``, and the tokens they belong to."""
+
+    values: torch.Tensor
+    ids: torch.Tensor
+    lse: torch.Tensor
+    temperature: float
+    tokens: torch.Tensor
 
 
 class CausalLM:
@@ -153,12 +168,9 @@ class CausalLM:
         eng.bias_qkv, eng.norm_in, eng.norm_post = self.params[b]
 
     # ---------------------------------------------------------------- pass --
-    def run(self, tokens: torch.Tensor,
-            on_block: Callable[[int, dict[str, torch.Tensor]], None] | None = None) -> torch.Tensor:
-        """Forward and backward for one batch of token ids ``[n, seq_len]``
-        (n <= batch). ``on_block(i, dw)`` receives block i's dL/dW' (fused
-        layout, valid until the next block's backward) from the last block to
-        the first. Returns the mean loss as a device scalar."""
+    def _logits(self, tokens: torch.Tensor, keep: bool) -> int:
+        """The batch's logits (with ``keep``, every block's activations too);
+        returns its sequences."""
         if tokens.dim() != 2 or tokens.shape[1] != self.seq_len or not 1 <= tokens.shape[0] <= self.batch:
             raise CalibrationError(f"a scoring batch is [<= {self.batch}, {self.seq_len}] token ids, "
                                    f"got {tuple(tokens.shape)}")
@@ -171,19 +183,54 @@ class CausalLM:
         eng, s, L = self.eng, self.shape, len(self.model.blocks)
         T, h = self.tokens, s.hidden
         K.embed_rows(self.model.embed, self.ids.view(-1), self.stream[0])
-        keep = self.acts is not None
         for b in range(L):
             self._bind_block(b)
             if keep:
                 eng.bind(self.acts[b])
             eng.forward(self.stream[b], self.stream[b + 1], save=keep)
-        # head and loss
-        V = self.vocab
         K.rmsnorm_fwd(self.stream[L], self.final_norm, s.norm_eps, self.xn, self.rstd)
         K.gemm("nt", self.xn, self.head, self.logits, M=T, N=self.logits.shape[1], K=h,
                workspace=eng.gemm_ws)
-        K.cross_entropy(self.logits, self.labels.view(-1), V=V, scale=1.0 / (n * self.n_in),
-                        row_loss=self.row_loss, loss_out=self.loss, dlogits=self.logits)
+        return n
+
+    def teacher_list(self, tokens: torch.Tensor, top: int = 64, temperature: float = 1.0) -> TeacherList:
+        """The ``top`` likeliest tokens at every position of a batch under the
+        current weights (``set_weights({})`` gives the model's own), for ``run``
+        under other weights."""
+        if not 1 <= top <= 1024:
+            raise CalibrationError(f"a teacher's list holds 1 to 1024 tokens, got {top}")
+        self._logits(tokens, False)
+        T, top = self.tokens, min(top, self.vocab)
+        values = torch.empty(T, top, dtype=torch.float32, device=self.device)
+        ids = torch.empty(T, top, dtype=torch.int32, device=self.device)
+        lse = torch.empty(T, dtype=torch.float32, device=self.device)
+        K.top_logits(self.logits, V=self.vocab, values=values, ids=ids, lse=lse, temperature=temperature)
+        ids.masked_fill_(self.labels.view(-1, 1) < 0, -1)
+        return TeacherList(values, ids, lse, float(temperature), tokens)
+
+    def run(self, tokens: torch.Tensor,
+            on_block: Callable[[int, dict[str, torch.Tensor]], None] | None = None,
+            teacher: TeacherList | None = None) -> torch.Tensor:
+        """Forward and backward for one batch of token ids ``[n, seq_len]``
+        (n <= batch). ``on_block(i, dw)`` receives block i's dL/dW' (fused
+        layout, valid until the next block's backward) from the last block to
+        the first. Returns the mean loss as a device scalar: the cross-entropy
+        of the next tokens, or with ``teacher`` (the list of the same batch) the
+        divergence from the teacher's distribution, its tokens off the list one
+        outcome."""
+        if teacher is not None and (teacher.ids.shape[0] != self.tokens or teacher.tokens.shape != tokens.shape):
+            raise CalibrationError("the teacher's list belongs to another batch")
+        keep = self.acts is not None
+        n = self._logits(tokens, keep)
+        eng, s, L = self.eng, self.shape, len(self.model.blocks)
+        T, h, V = self.tokens, s.hidden, self.vocab
+        scale = 1.0 / (n * self.n_in)
+        if teacher is None:
+            K.cross_entropy(self.logits, self.labels.view(-1), V=V, scale=scale, row_loss=self.row_loss,
+                            loss_out=self.loss, dlogits=self.logits)
+        else:
+            K.distill_loss(self.logits, teacher.values, teacher.ids, V=V, scale=scale, row_loss=self.row_loss,
+                           lse=teacher.lse, temperature=teacher.temperature, loss_out=self.loss, dlogits=self.logits)
         K.gemm("nn", self.logits, self.head, self.dxn, M=T, N=h, K=self.logits.shape[1],
                workspace=eng.gemm_ws)
         cur, nxt = self.grads

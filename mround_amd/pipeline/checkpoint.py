@@ -56,11 +56,32 @@ def rope_scaling(config: dict[str, Any]) -> tuple:
     if kind == "default":
         return ()
     need = {"linear": ("factor",),
-            "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings")}[kind]
+            "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"),
+            "yarn": ("factor", "original_max_position_embeddings")}[kind]
     missing = [k for k in need if k not in raw]
     if missing:
         raise ArchitectureError(f"rope_scaling of type {kind!r} lacks {', '.join(missing)}")
-    return tuple(sorted([("rope_type", kind)] + [(k, float(raw[k])) for k in need]))
+    pairs = [("rope_type", kind)] + [(k, float(raw[k])) for k in need]
+    if kind == "yarn":
+        pairs += [(k, float(raw[k])) for k in ("beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim")
+                  if raw.get(k) is not None]
+        if not raw.get("truncate", True):
+            pairs.append(("truncate", 0.0))
+    return tuple(sorted(pairs))
+
+
+def rotary_dim(config: dict[str, Any], head_dim: int) -> int:
+    """The rotated part of a head: ``partial_rotary_factor`` of it (top-level or
+    inside ``rope_parameters``), 0 for all of it."""
+    part = config.get("partial_rotary_factor")
+    if part is None:
+        part = (config.get("rope_parameters") or {}).get("partial_rotary_factor")
+    if part is None or float(part) == 1.0:
+        return 0
+    r = int(head_dim * float(part))
+    if r <= 0 or r % 2 or r > head_dim:
+        raise ArchitectureError(f"partial_rotary_factor {part} of a head of {head_dim} is not an even part of it")
+    return r
 
 
 def rope_theta(config: dict[str, Any]) -> float:
@@ -86,7 +107,9 @@ def block_shape(config: dict[str, Any]) -> BlockShape:
                       n_kv_heads=int(config.get("num_key_value_heads") or heads), head_dim=head_dim,
                       intermediate=int(config["intermediate_size"]),
                       norm_eps=float(config.get("rms_norm_eps", 1e-6)),
-                      rope_theta=rope_theta(config), attn_bias=bias, rope_scaling=rope_scaling(config))
+                      rope_theta=rope_theta(config), attn_bias=bias, rope_scaling=rope_scaling(config),
+                      rotary_dim=rotary_dim(config, head_dim),
+                      rope_interleaved=bool(config.get("rope_traditional", False)))
 
 
 def _read_tensors(path: Path, device) -> dict[str, torch.Tensor]:

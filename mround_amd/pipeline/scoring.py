@@ -11,6 +11,10 @@ importance, scoring.py:196-211). Two schedules, as the reference's:
 * ``"widest"`` (scoring.py:318-365): the model at the widest width, one
   backward per batch, every width's perturbation against it.
 
+Beside the reference's objective ("labels") stands one that needs no text
+("teacher"): the divergence of the quantized model's predictions from the
+model's own at its full weights, kept as every position's likeliest tokens.
+
 Each block's gradients are reduced as its backward ends, by
 ``mr_delta_loss_mapped`` reading the fused gradient operand in place (every
 width in one pass, terms in fp32, sums in fp64), so no model-sized gradient or
@@ -35,6 +39,7 @@ from mround_amd.schemes import DEFAULT_EPS_FP32, QuantScheme, ScaleInit
 __all__ = ["ScoringProgress", "SensitivityScores", "eligible_block_layers", "score_widths"]
 
 GRADIENT_SCHEDULES = ("own_width", "widest")
+OBJECTIVES = ("labels", "teacher")
 
 
 @dataclasses.dataclass
@@ -127,19 +132,25 @@ def _grids(eligible, scheme: QuantScheme) -> dict[str, torch.Tensor]:
 def score_widths(model, batches: Sequence[torch.Tensor], widths: Sequence[int], base_scheme: QuantScheme,
                  *, eps: float = DEFAULT_EPS_FP32, gradient_source: str = "own_width",
                  progress: Callable[[ScoringProgress], None] | None = None,
-                 keep_activations: bool | None = None) -> SensitivityScores:
+                 keep_activations: bool | None = None, objective: str = "labels", teacher_top: int = 64,
+                 temperature: float = 1.0) -> SensitivityScores:
     """Score every block layer at every candidate width
     (mround/pipeline/scoring.py:425-583).
 
     ``batches`` are ``[n, seq_len]`` token-id tensors (one ``seq_len``; the
     first batch's sequence count sizes the engine and a later batch may hold
-    fewer). Raises ``ValueError`` for no widths, no batches, an unknown
-    ``gradient_source`` or when every layer is skipped.
+    fewer). ``objective`` "teacher" scores with the gradient of the divergence
+    from the model's own ``teacher_top`` likeliest tokens (and the rest as one)
+    at ``temperature``, in place of the cross-entropy of the batches' tokens.
+    Raises ``ValueError`` for no widths, no batches, an unknown
+    ``gradient_source`` or ``objective``, or when every layer is skipped.
     """
     if not widths:
         raise ValueError("no candidate widths to score")
     if gradient_source not in GRADIENT_SCHEDULES:
         raise ValueError(f"gradient_source must be 'own_width' or 'widest', got {gradient_source!r}")
+    if objective not in OBJECTIVES:
+        raise ValueError(f"objective must be 'labels' or 'teacher', got {objective!r}")
     if not batches:
         raise ValueError("no calibration batches to score on")
     started = time.perf_counter()
@@ -151,6 +162,10 @@ def score_widths(model, batches: Sequence[torch.Tensor], widths: Sequence[int], 
     batch = max(int(t.shape[0]) for t in batches)
     seq_len = int(batches[0].shape[1])
     lm = CausalLM(model, batch=batch, seq_len=seq_len, device=dev, keep_activations=keep_activations)
+    teachers = [None] * len(batches)
+    if objective == "teacher":
+        lm.set_weights({})
+        teachers = [lm.teacher_list(t, teacher_top, temperature) for t in batches]
     place = placements(lm.shape)
     names = {f"{blk.name}.{n}": n for blk in model.blocks for n in LAYERS}
 
@@ -201,8 +216,8 @@ def score_widths(model, batches: Sequence[torch.Tensor], widths: Sequence[int], 
             report("width", built, len(order))
             acc = {p: torch.zeros(1, dtype=torch.float64, device=dev) for p in eligible}
             on_block = accumulate([width], [grids], acc)
-            for tokens in batches:
-                lm.run(tokens, on_block)
+            for tokens, teacher in zip(batches, teachers):
+                lm.run(tokens, on_block, teacher)
                 done += 1
                 report("backward", done, passes, len(order) - built)
             for p in eligible:
@@ -214,8 +229,8 @@ def score_widths(model, batches: Sequence[torch.Tensor], widths: Sequence[int], 
         report("perturbations", len(order), len(order))
         acc = {p: torch.zeros(len(order), dtype=torch.float64, device=dev) for p in eligible}
         on_block = accumulate(order, all_grids, acc)
-        for i, tokens in enumerate(batches, start=1):
-            lm.run(tokens, on_block)
+        for i, (tokens, teacher) in enumerate(zip(batches, teachers), start=1):
+            lm.run(tokens, on_block, teacher)
             report("backward", i, len(batches))
         for p in eligible:
             vals = acc[p].cpu().tolist()
