@@ -288,7 +288,9 @@ int mr_top_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t 
  * unlisted logit is above minus infinity the term of the rest is left out.
  * Terms with q_j = 0 count nothing; a listed logit of minus infinity with
  * q_j > 0 makes the loss infinite.
- * Unlisted logits of -1e37 and below, as masks write them, count as minus infinity.
+ * Unlisted logits of -1e37 and below, as masks write them, count as minus infinity;
+ * a row with an unlisted logit so large that logit / temperature in powers of two is no
+ * float has no finite loss. Temperatures lie in [1/1024, 1024], here and above.
  * Beside mr_cross_entropy as the objective the scores are gradients of
  * (mround/pipeline/scoring.py:183-192).
  */

@@ -24,7 +24,7 @@
 namespace mr {
 namespace {
 
-constexpr float kInf = __builtin_inff();
+constexpr float kInf = __builtin_inff(), kMaxFloat = 3.4028234663852886e38f;
 constexpr int kMaxTop = 1024;
 
 __device__ __forceinline__ uint4 ld16(const uint8_t* p) {  // any alignment
@@ -148,6 +148,9 @@ __device__ __forceinline__ uint4 gradient_piece(uint4 q, float about, float b, f
   return narrow<DT>(v);
 }
 
+// Temperatures whose log2(e) / T leaves room for masked logits and for its low part.
+constexpr float kMinTemperature = 1.0f / 1024, kMaxTemperature = 1024.0f;
+
 ExpScale exp_scale(double temperature) {
   // hi from below and lo above zero: minus infinity times either is minus infinity
   const double c = 1.4426950408889634073599 / temperature;
@@ -198,7 +201,8 @@ struct RunningSum {
     constexpr int E = kPiece<DT>;
     if (mx > max) {
       if (mx > kMasked) {
-        const float grown = mx * c.hi, f = max > kMasked ? __builtin_amdgcn_exp2f(base - grown) : 1.0f;
+        // (a product past the floats is their end: an exponential above it overflows, as it should)
+        const float grown = clampf(mx * c.hi, -kMaxFloat, kMaxFloat), f = max > kMasked ? __builtin_amdgcn_exp2f(base - grown) : 1.0f;
         base = grown;
         s *= f;
         ve *= f;
@@ -835,7 +839,7 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   float about = waves_max<W>(s_first);
   float sum, ve, se;
   auto add_up = [&](auto takes) __attribute__((always_inline)) {
-    if (!(about > -kInf && about < kInf)) about = 0.0f;
+    if (!(__builtin_fabsf(about * p.c.hi) < kInf)) about = 0.0f;  // (so a sum past the floats becomes infinite)
     const float b = -about * p.c.hi;
     const int t = anew();
     float s0 = 0.0f, s1 = 0.0f;
@@ -1068,8 +1072,8 @@ int mr_top_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t 
   if (!valid_dtype(dtype)) return fail(MR_EINVAL, "mr_top_logits: bad dtype %d", dtype);
   if (k < 1 || k > kMaxTop || k > V)
     return fail(MR_EINVAL, "mr_top_logits: k=%d must lie in [1, %d] and not pass V", k, kMaxTop);
-  if (!(temperature > 0.0f && temperature < __builtin_inff()))
-    return fail(MR_EINVAL, "mr_top_logits: the temperature must be positive and finite");
+  if (!(temperature >= kMinTemperature && temperature <= kMaxTemperature))
+    return fail(MR_EINVAL, "mr_top_logits: the temperature must lie in [1/1024, 1024]");
   if (T == 0) return MR_OK;
   if (!logits || !values || !ids) return fail(MR_EINVAL, "mr_top_logits: null pointer");
   if (ld < V) return fail(MR_EINVAL, "mr_top_logits: the leading dimension is smaller than V");
@@ -1111,8 +1115,8 @@ int mr_distill(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, 
   if (V > kBitmapMaxV) return fail(MR_EINVAL, "mr_distill: vocabularies of more than %d", kBitmapMaxV);
   if (!valid_dtype(dtype)) return fail(MR_EINVAL, "mr_distill: bad dtype %d", dtype);
   if (k < 1 || k > kMaxTop) return fail(MR_EINVAL, "mr_distill: k=%d must lie in [1, %d]", k, kMaxTop);
-  if (!(temperature > 0.0f && temperature < __builtin_inff()))
-    return fail(MR_EINVAL, "mr_distill: the temperature must be positive and finite");
+  if (!(temperature >= kMinTemperature && temperature <= kMaxTemperature))
+    return fail(MR_EINVAL, "mr_distill: the temperature must lie in [1/1024, 1024]");
   if (!row_loss || (T > 0 && (!logits || !top_values || !top_ids))) return fail(MR_EINVAL, "mr_distill: null pointer");
   if (ld < V || (dlogits && ldd < V)) return fail(MR_EINVAL, "mr_distill: a leading dimension is smaller than V");
   if (T > 0x7fffffff) return fail(MR_EINVAL, "mr_distill: too many rows");

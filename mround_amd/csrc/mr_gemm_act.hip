@@ -23,7 +23,7 @@ int act_forward(const GemmParams& p, bool bf16, hipStream_t s) {
 // rows' column sums. Bound by memory; blocks of 512 columns left 4 waves a CU at
 // 4005 x 896.
 template <int F, int DT>
-__global__ __launch_bounds__(256) void act_bwd_rows(const void* __restrict__ dout, int64_t ldo, const uint16_t* pre,
+__global__ __launch_bounds__(256) void act_bwd_rows(const void* dout, int64_t ldo, const uint16_t* pre,
                                                     int64_t ldpre, uint16_t* dpre, int64_t ldd, int64_t M, int N,
                                                     float* colsum) {
   __shared__ float part[4][256];

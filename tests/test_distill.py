@@ -473,3 +473,49 @@ def test_bindings_refuse_on_the_host():
         K.distill_loss(z, v, i, lse=torch.zeros(3), **kw)
     with pytest.raises(KernelError, match="ROCm device"):
         K.distill_loss(z, v, i, **kw)
+
+
+# ------------------------------------------------------- the ends of the range --
+
+def test_temperatures_out_of_range_are_refused():
+    lib, P, f = K.lib(), ctypes.c_void_p, ctypes.c_float
+    for temp in (1e-4, 2e3):
+        assert lib.mr_top_logits(P(1 << 20), 1, 1000, 4, 1000, 8, f(temp), P(1 << 24), P(1 << 25), None, None) == -22
+        assert b"temperature" in lib.mr_last_error()
+        assert lib.mr_distill(P(1 << 20), 0, 1000, 4, 1000, P(1 << 22), P(1 << 23), 8, None, f(temp), f(1.0), P(1 << 25), None,
+                              None, 1000, None) == -22
+        assert b"temperature" in lib.mr_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [300, 40000, 200003])
+@pytest.mark.parametrize("temperature", [2.0 ** -10, 2.0 ** 10])
+def test_temperatures_at_the_ends(V, temperature):
+    # (logits of the temperature's own size, so that rows are no one-hot)
+    T, k = 3, 8
+    z, values, ids, teacher = make(T, V, k, "f32", seed=12)
+    z, values, teacher = z * temperature, values * temperature, teacher * temperature
+    lse = torch.logsumexp(teacher.double() / temperature, 1).float()
+    check(z, values, ids, scale=temperature, lse=lse, temperature=temperature)
+    check_top(z, k, temperature=temperature)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [300, 40000, 100003, 200003])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_logits_whose_exponents_are_no_floats(V, dtype):
+    """A logit of 3e38: the largest of the list, its log-sum-exp the logit over the temperature; off a list no
+    finite loss, as an infinity there."""
+    z = torch.randn(4, V, generator=torch.Generator().manual_seed(3)).to(DT[dtype])
+    z[1, V - 3] = z[2, 7] = 3e38
+    z[3] = -3e38
+    z[3, 5] = 0.0
+    values, ids, lse = run_top(z.to(dev()), V, 8, 0.75)
+    big = float(z[1, V - 3])
+    assert ids[1, 0] == V - 3 and ids[2, 0] == 7 and ids[3, 0] == 5 and float(values[1, 0]) == big
+    assert bool(torch.isinf(lse[1:3]).all()) and float(lse[3]) == 0.0
+    lists, t = torch.arange(10, 18).repeat(4, 1).int(), torch.zeros(4, 8)
+    for tail in (torch.full((4,), 2.5), None):
+        for grad in (True, False):
+            row, _, _ = run(z, t, lists, scale=1.0, lse=tail, temperature=0.75, grad=grad)
+            assert bool(torch.isfinite(row[0])) and not bool(torch.isfinite(row[1:3]).any()), (tail, grad)
