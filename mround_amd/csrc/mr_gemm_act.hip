@@ -8,6 +8,11 @@
 // the epilogues are mr_gemm_tiles.h's: what f costs is the epilogue's time, in the
 // product's last microseconds, where an output in fp32 and a pass of its own would
 // write and read it again.
+//
+// Bound by the matrix cores: silu of 16384 x 18944 x 3584 with the pre-activation
+// saved takes 1758 us (1265 TFLOP/s). At 4096 x 11008 x 2048, where the products
+// alone take 163 us forward and 147 backward, the epilogues come to 163 (relu) to
+// 179 us and 155 to 181 us (erf gelu), and a bias gradient to 6 us more.
 #include "mr_gemm_tiles.h"
 
 namespace mr {
