@@ -27,10 +27,16 @@ namespace {
 constexpr float kInf = __builtin_inff(), kMaxFloat = 3.4028234663852886e38f;
 constexpr int kMaxTop = 1024;
 
-__device__ __forceinline__ uint4 ld16(const uint8_t* p) {  // any alignment
+// 16 bytes at any element; nt: past the caches, of what is read once.
+typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ uint4 ld16(const uint8_t* p) {
   uint4 v;
   __builtin_memcpy(&v, p, 16);
   return v;
+}
+__device__ __forceinline__ uint4 ld16nt(const uint8_t* p) {
+  const u32x4u v = __builtin_nontemporal_load(reinterpret_cast<const u32x4u*>(p));
+  return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
 // Elements of a 16-byte piece of type DT, widened.
@@ -94,10 +100,11 @@ __device__ __forceinline__ void take_out(uint4& q, uint32_t bits) {
 // bytes that start at its first element or end the row, whichever is sooner; the
 // rest is minus infinity. The load is whole and without a branch (a branch around
 // a load makes each wait for the last).
-template <int DT>
+template <int DT, bool NT = false>
 __device__ __forceinline__ uint4 piece_bytes(const uint8_t* row, int64_t i, int64_t V) {
   constexpr int E = kPiece<DT>, ES = 16 / E;
-  return ld16(row + min(i * E, V - E) * ES);
+  const uint8_t* at = row + min(i * E, V - E) * ES;
+  return NT ? ld16nt(at) : ld16(at);
 }
 template <int DT>
 __device__ __forceinline__ uint32_t piece_drop(int64_t i, int64_t V) {  // bits of the elements that are not the piece's
@@ -748,12 +755,14 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// Piece i of a gradient row, laid out as piece_bytes reads it.
+// Piece i of a gradient row, laid out as piece_bytes reads it. The gradient passes by
+// the caches: 2044 rows of 151936 286 us by plain stores and loads, 254 by these
+// stores, 241 by such loads too of the pieces that are read once.
 template <int DT>
 __device__ __forceinline__ void store_piece(uint8_t* row, int i, int V, uint4 o) {
   constexpr int E = kPiece<DT>, ES = 16 / E;
   if ((i + 1) * E <= V) {
-    __builtin_memcpy(row + static_cast<uint32_t>(i * 16), &o, 16);
+    __builtin_nontemporal_store(u32x4u{o.x, o.y, o.z, o.w}, reinterpret_cast<u32x4u*>(row + static_cast<uint32_t>(i * 16)));
     return;
   }
   const uint32_t w[4] = {o.x, o.y, o.z, o.w};
@@ -784,12 +793,14 @@ __device__ __forceinline__ void store_piece(uint8_t* row, int i, int V, uint4 o)
 // one factor (in the exponent it would save that multiplication, and be off by
 // 2^-24 of the largest logit).
 //
-// Two rows to a CU hide one another's waits: 2044 16-bit rows of 65536 logits take
+// Two rows to a CU hide one another's waits: 2044 16-bit rows of 65536 logits took
 // 181 us by one block of 1024 threads a CU and 121 by two of 512, and 1022 float32
-// rows of 49152 108 and 88. So M further pieces of a thread lie in LDS, where rows
-// somewhat past the registers of half a CU still come in twos. Longer ones (the 2044
-// of 151936: 326 us, of which the loads alone are 135) have the CU to themselves.
-template <int DT, int THREADS, int N, int M>
+// rows of 49152 108 and 88. So M further pieces of a thread lie in LDS, and R more,
+// of rows past both, are read twice, for the sum through the registers of the held
+// ones before these come and for the gradient as they leave: 2044 rows of 151936
+// took 326 us by a CU a row, all held, and 305 so. What else the two rows took from
+// one another were their ways through the caches (store_piece): 241 us now, 5.2 TB/s.
+template <int DT, int THREADS, int N, int M, int R>
 __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   constexpr int E = kPiece<DT>, ES = 16 / E, W = THREADS / 64;
   extern __shared__ uint32_t bitmap[];  // a bit per logit, a word more, and the list
@@ -797,6 +808,7 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   __shared__ float s_first[W], s_ve[W], s_e[W];
   __shared__ float s_g;
   __shared__ uint4 beside[M ? M * THREADS : 1];  // pieces N .. N + M - 1
+  static_assert(R <= N, "the pieces that are read again pass through the held ones' registers");
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int64_t row = blockIdx.x;
   const int V = p.V, pieces = (V + E - 1) / E;
@@ -816,12 +828,20 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   };
   uint4 early[M ? M : 1];  // on their way to LDS
 #pragma unroll
-  for (int j = 0; j < M; ++j) early[j] = ld16(z + static_cast<uint32_t>(first(tid, N + j) * ES));
+  for (int j = 0; j < M; ++j) early[j] = ld16nt(z + static_cast<uint32_t>(first(tid, N + j) * ES));
+  constexpr int AHEAD = R > 8 ? 8 : N;
 #pragma unroll
-  for (int j = 0; j < N; ++j) r[j] = ld16(z + static_cast<uint32_t>(first(tid, j) * ES));
+  for (int j = 0; j < AHEAD; ++j)
+    r[j] = j < R ? ld16(z + static_cast<uint32_t>(first(tid, N + M + j) * ES)) : ld16nt(z + static_cast<uint32_t>(first(tid, j) * ES));
   for (int i = tid; i <= (V + 31) / 32; i += THREADS) bitmap[i] = 0;
   lds_barrier();
   l.mark(p, entries, z, bitmap, s);
+#pragma unroll
+  for (int j = AHEAD; j < N; ++j) {  // (the list's registers before these)
+    int at = first(tid, j < R ? N + M + j : j) * ES;
+    asm volatile("" : "+v"(at));
+    r[j] = ld16(z + static_cast<uint32_t>(at));
+  }
   {
     float v[E], mx = -kInf;
     widen<DT>(M ? early[0] : r[0], v);
@@ -844,7 +864,7 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
     const int t = anew();
     float s0 = 0.0f, s1 = 0.0f;
     ve = se = 0.0f;
-    auto one = [&](int j, uint4& q) __attribute__((always_inline)) {
+    auto one = [&](int j, uint4& q, auto takes) __attribute__((always_inline)) {
       if constexpr (decltype(takes)::value) {
         const int at = first(t, j), drop = min((j * THREADS + t) * E - at, E);
         const uint32_t bits = __builtin_amdgcn_alignbit(bitmap[(at >> 5) + 1], bitmap[at >> 5], at & 31) | ((1u << drop) - 1);
@@ -874,15 +894,30 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
 #pragma unroll
     for (int j = 0; j < M; ++j) {
       if constexpr (decltype(takes)::value) {
-        one(N + j, early[j]);
+        one(N + j, early[j], takes);
         beside[j * THREADS + tid] = early[j];
       } else {
         uint4 q = beside[j * THREADS + tid];
-        one(N + j, q);
+        one(N + j, q, takes);
+      }
+    }
+    if constexpr (decltype(takes)::value) {
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        one(N + M + j, r[j], takes);
+        int at = first(t, j) * ES;
+        asm volatile("" : "+v"(at));  // (behind the sum, whose piece's registers it takes)
+        r[j] = ld16nt(z + static_cast<uint32_t>(at));
+      }
+    } else {
+#pragma unroll 1
+      for (int j = 0; j < R; ++j) {
+        uint4 q = ld16(z + static_cast<uint32_t>(first(t, N + M + j) * ES));
+        one(N + M + j, q, std::true_type{});
       }
     }
 #pragma unroll
-    for (int j = 0; j < N; ++j) one(j, r[j]);
+    for (int j = 0; j < N; ++j) one(j, r[j], takes);
     sum = s0 + s1;
     ve = wave_sum(ve);
     se = wave_sum(se);
@@ -911,6 +946,14 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
     for (int j = 0; j < N; ++j) most(r[j]);
 #pragma unroll
     for (int j = 0; j < M; ++j) most(beside[j * THREADS + tid]);
+#pragma unroll 1
+    for (int j = 0; j < R; ++j) {
+      const int at = first(tid, N + M + j), drop = min(((N + M + j) * THREADS + tid) * E - at, E);
+      uint4 q = ld16(z + static_cast<uint32_t>(at * ES));
+      const uint32_t bits = __builtin_amdgcn_alignbit(bitmap[(at >> 5) + 1], bitmap[at >> 5], at & 31) | ((1u << drop) - 1);
+      take_out<DT>(q, bits);
+      most(q);
+    }
     mx = wave_max(mx);
     if (lane == 0) s_first[wave] = mx;
     __syncthreads();
@@ -953,9 +996,14 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
       if (DT == MR_F32) __builtin_amdgcn_sched_barrier(0);  // (else pieces in float32 are worked on together, and spill)
     };
 #pragma unroll
-    for (int j = 0; j < N; ++j) put(j, r[j]);
+    for (int j = 0; j < N; ++j) {
+      put(j, r[j]);
+      if (j < R) r[j] = ld16nt(z + static_cast<uint32_t>(first(t, N + M + j) * ES));
+    }
 #pragma unroll
     for (int j = 0; j < M; ++j) put(N + j, beside[j * THREADS + tid]);
+#pragma unroll
+    for (int j = 0; j < R; ++j) put(N + M + j, r[j]);
     __syncthreads();  // the rest's stores are done where the list's follow
   }
   const RowSums x = row_sums();
@@ -984,7 +1032,7 @@ __global__ __launch_bounds__(1024, 8) void distill_stream(DistillParams p) {
   lds_barrier();
   l.mark(p, entries, z, bitmap, s);
   lds_barrier();
-  auto get = [&](int i) __attribute__((always_inline)) { return V >= E ? piece_bytes<DT>(z, i, V) : short_row<DT>(z, V); };
+  auto get = [&](int i) __attribute__((always_inline)) { return V >= E ? piece_bytes<DT, true>(z, i, V) : short_row<DT>(z, V); };
   // the listed elements of a piece and those that are not its own
   auto left_out = [&](int i) __attribute__((always_inline)) {
     if (V < E) return i ? 0xffu : bitmap[0] & 0xffu;
@@ -1152,20 +1200,24 @@ int mr_distill(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, 
     const dim3 g(static_cast<unsigned>(T));
     const size_t lds = static_cast<size_t>((V + 31) / 32 + 1) * 4 + static_cast<size_t>(k) * 8;
     const int64_t pieces = (V * es + 15) / 16;
-#define MR_DISTILL(DT, THREADS, N, M) hipLaunchKernelGGL((distill_held<DT, THREADS, N, M>), g, dim3(THREADS), lds, s, p)
+    // what 7 pieces a thread and the block's sums leave of half a CU's LDS
+    constexpr size_t kTwoRows = 81920 - 512 * 7 * 16 - 2048;
+#define MR_DISTILL(DT, THREADS, N, M, R) hipLaunchKernelGGL((distill_held<DT, THREADS, N, M, R>), g, dim3(THREADS), lds, s, p)
     // the fewest threads that hold the row in at most 8 pieces each, then more
     // pieces, as long as two rows fit a CU; then one row
 #define MR_DISTILL_D(DT)                                                                                 \
   do {                                                                                                   \
     if (V * es < 16 || (!dlogits && pieces > 512 * 8))                                                   \
       hipLaunchKernelGGL((distill_stream<DT>), g, dim3(1024), lds, s, p);                                \
-    else if (pieces <= 256 * 4) MR_DISTILL(DT, 256, 4, 0);                                               \
-    else if (pieces <= 256 * 8) MR_DISTILL(DT, 256, 8, 0);                                               \
-    else if (pieces <= 512 * 8) MR_DISTILL(DT, 512, 8, 0);                                               \
-    else if (pieces <= 512 * 16) MR_DISTILL(DT, 512, 16, 0);                                             \
-    else if (pieces <= 512 * 20) MR_DISTILL(DT, 512, 20, 0);                                             \
-    else if (pieces <= 512 * 24) MR_DISTILL(DT, 512, 17, 7);                                             \
-    else if (pieces <= 1024 * 20) MR_DISTILL(DT, 1024, 20, 0);                                           \
+    else if (pieces <= 256 * 4) MR_DISTILL(DT, 256, 4, 0, 0);                                               \
+    else if (pieces <= 256 * 8) MR_DISTILL(DT, 256, 8, 0, 0);                                               \
+    else if (pieces <= 512 * 8) MR_DISTILL(DT, 512, 8, 0, 0);                                               \
+    else if (pieces <= 512 * 16) MR_DISTILL(DT, 512, 16, 0, 0);                                             \
+    else if (pieces <= 512 * 20) MR_DISTILL(DT, 512, 20, 0, 0);                                             \
+    else if (pieces <= 512 * 24) MR_DISTILL(DT, 512, 17, 7, 0);                                             \
+    else if (pieces <= 512 * 31) MR_DISTILL(DT, 512, 17, 6, 8);                                          \
+    else if (pieces <= 512 * 39 && lds <= kTwoRows) MR_DISTILL(DT, 512, 16, 7, 16);                      \
+    else if (pieces <= 512 * 40) MR_DISTILL(DT, 512, 17, 6, 17);                                           \
     else hipLaunchKernelGGL((distill_stream<DT>), g, dim3(1024), lds, s, p);                             \
   } while (0)
     if (dtype == MR_BF16) MR_DISTILL_D(MR_BF16);

@@ -53,6 +53,16 @@ __device__ __forceinline__ uint4 ld16(const uint8_t* p) {
 }
 __device__ __forceinline__ void st16(uint8_t* p, uint4 v) { __builtin_memcpy(p, &v, 16); }
 
+// The same of 16-byte places.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint4 ld16s(const uint8_t* p) {
+  const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void st16s(uint8_t* p, uint4 v) {
+  __builtin_nontemporal_store(u32x4{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4*>(p));
+}
+
 // E consecutive elements of a 16-byte register, widened, and back.
 template <int DT, int E>
 __device__ __forceinline__ void widen(uint4 r, float (&v)[E]) {
@@ -130,8 +140,8 @@ __global__ __launch_bounds__(kRopeBlock) void rope_any(RopeParams p) {
     const uint8_t* row = xb + static_cast<int64_t>(u.tok) * p.ldx * ES;
     Unit v{};
     if (VEC && u.na == E && u.nb == E) {
-      v.a = *reinterpret_cast<const uint4*>(row + u.a * ES);
-      v.b = *reinterpret_cast<const uint4*>(row + u.b * ES);
+      v.a = ld16s(row + u.a * ES);
+      v.b = ld16s(row + u.b * ES);
     } else if (u.na == E && u.nb == E) {
       v.a = ld16(row + u.a * ES);
       v.b = ld16(row + u.b * ES);
@@ -150,8 +160,8 @@ __global__ __launch_bounds__(kRopeBlock) void rope_any(RopeParams p) {
   auto store = [&](const At& u, const Unit& v) __attribute__((always_inline)) {
     uint8_t* row = ob + static_cast<int64_t>(u.tok) * p.ldo * ES;
     if (VEC && u.na == E && u.nb == E) {
-      *reinterpret_cast<uint4*>(row + u.a * ES) = v.a;
-      *reinterpret_cast<uint4*>(row + u.b * ES) = v.b;
+      st16s(row + u.a * ES, v.a);
+      st16s(row + u.b * ES, v.b);
     } else if (u.na == E && u.nb == E) {
       st16(row + u.a * ES, v.a);
       st16(row + u.b * ES, v.b);

@@ -519,3 +519,38 @@ def test_logits_whose_exponents_are_no_floats(V, dtype):
         for grad in (True, False):
             row, _, _ = run(z, t, lists, scale=1.0, lse=tail, temperature=0.75, grad=grad)
             assert bool(torch.isfinite(row[0])) and not bool(torch.isfinite(row[1:3]).any()), (tail, grad)
+
+
+# the last row of each size of block, the first of the next, and lists that leave room for fewer pieces beside them
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("case", [(2, 126976, 8), (2, 126977, 9), (2, 151936, 1024), (2, 159744, 16), (2, 159745, 16),
+                                  (1, 163840, 1000), (1, 163841, 5), (2, 63488, 7), (2, 63489, 7), (2, 76000, 1024),
+                                  (1, 79873, 5), (1, 81920, 700), (1, 81921, 3)], ids=lambda c: "x".join(map(str, c)))
+def test_rows_read_twice(case, dtype):
+    test_distill(case, True, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [70001, 120001, 151936])
+def test_odd_rows_that_are_read_twice(V):
+    for tail in (True, False):
+        test_rows_that_leave_nothing(tail, V)
+    for dtype in ("bf16", "f32"):
+        test_masks_of_the_lowest_value(V, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [70000, 120000, 151936])
+def test_a_peak_anywhere(V, dtype):
+    """A logit of 300, off the list, at places all over the row: the sum about the first pieces' maximum has no room
+    for it and is formed anew."""
+    T, k = 40, 8
+    z, values, ids, teacher = make(T, V, k, dtype, seed=V + 1)
+    for r in range(T):
+        c = (r * V) // T + r
+        while c in ids[r].tolist():
+            c += 1
+        z[r, c] = 300.0
+    check(z, values, ids, scale=1.0, lse=torch.logsumexp(teacher.double(), 1).float())
