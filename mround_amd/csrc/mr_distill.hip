@@ -1011,12 +1011,16 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   if (p.dz && l.n > 0) x.list_gradients(p, l, dz);
 }
 
-// Long rows whose gradient is not asked for, those too long to hold, which are read
-// twice, and those shorter than a piece. Nothing is held, so a CU works on two rows
-// (the loss alone of 2044 rows of 151936: 135 us, 200 held; of 32000 68 and 45).
-template <int DT>
-__global__ __launch_bounds__(1024, 8) void distill_stream(DistillParams p) {
-  constexpr int THREADS = 1024, U = 4;
+// Rows whose gradient is not asked for, where they are longer than 2048 pieces, those
+// too long to hold, which are read twice, and those shorter than a piece. Nothing is
+// held, so a CU works on two rows by 1024 threads, on four by 512 and on eight by 256,
+// which hide one another's waits: the loss alone of 2044 rows of 151936 bf16 logits 132,
+// 115 and 108 us (5.7 TB/s), of 50304 80, 52 and 49; but 64 rows of 151936 23, 23 and 28.
+// With the gradient the few rows at a time find more of themselves in the caches on
+// the second reading: 2044 of 200000 374, 379 and 415.
+template <int DT, int THREADS, bool GRAD>
+__global__ __launch_bounds__(THREADS, 8) void distill_stream(DistillParams p) {
+  constexpr int U = 4;
   constexpr int E = kPiece<DT>, ES = 16 / E, W = THREADS / 64;
   extern __shared__ uint32_t bitmap[];
   __shared__ typename List<DT, THREADS>::Shared s;
@@ -1032,7 +1036,9 @@ __global__ __launch_bounds__(1024, 8) void distill_stream(DistillParams p) {
   lds_barrier();
   l.mark(p, entries, z, bitmap, s);
   lds_barrier();
-  auto get = [&](int i) __attribute__((always_inline)) { return V >= E ? piece_bytes<DT, true>(z, i, V) : short_row<DT>(z, V); };
+  auto get = [&](int i, auto last) __attribute__((always_inline)) {
+    return V >= E ? piece_bytes<DT, decltype(last)::value>(z, i, V) : short_row<DT>(z, V);
+  };
   // the listed elements of a piece and those that are not its own
   auto left_out = [&](int i) __attribute__((always_inline)) {
     if (V < E) return i ? 0xffu : bitmap[0] & 0xffu;
@@ -1043,7 +1049,7 @@ __global__ __launch_bounds__(1024, 8) void distill_stream(DistillParams p) {
   for (int i0 = tid; i0 < pieces; i0 += U * THREADS) {
     uint4 q[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) q[j] = get(i0 + j * THREADS);
+    for (int j = 0; j < U; ++j) q[j] = get(i0 + j * THREADS, std::bool_constant<!GRAD>{});
     float mx = -kInf;
 #pragma unroll
     for (int j = 0; j < U; ++j) {
@@ -1065,7 +1071,7 @@ __global__ __launch_bounds__(1024, 8) void distill_stream(DistillParams p) {
   const BlockSum<W> rest(s_sum, p.c);
   const RowSums x(p, l, rest.sum, rest.exponent);
   if (tid == 0) p.row_loss[row] = x.loss(p, l);
-  if (!p.dz) return;
+  if constexpr (!GRAD) return;
   const bool none = l.n == 0;
   const double g64 = l.n < 0 ? __builtin_nan("") : x.rest_gradient(p);
   const float about = rest.max > kMasked ? rest.max : 0.0f, base = -about * p.c.hi;
@@ -1073,7 +1079,7 @@ __global__ __launch_bounds__(1024, 8) void distill_stream(DistillParams p) {
   for (int i0 = tid; i0 < pieces; i0 += U * THREADS) {
     uint4 q[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) q[j] = get(i0 + j * THREADS);
+    for (int j = 0; j < U; ++j) q[j] = get(i0 + j * THREADS, std::true_type{});
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const int i = i0 + j * THREADS;
@@ -1138,11 +1144,13 @@ int mr_top_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t 
   TopParams p{logits, ld, V, k, exp_scale(temperature), temperature, values, ids, lse};
   hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 g(static_cast<unsigned>(T));
-  // short rows by blocks of 256 threads, eight to a CU, where these have maxima
-  // enough for lists of k
+  // Short rows by blocks of 256 threads, eight to a CU, longer ones by four of 512,
+  // where these have maxima enough for lists of k: 2044 rows of 20000 bf16 logits 67 us
+  // by 1024 threads, 38 by 512, 32 by 256; of 50304 78, 51, 57; of 151936 144, 138, 163.
 #define MR_TOP(DT)                                                                                          \
   do {                                                                                                      \
-    if (V <= 16384 && k <= 256) hipLaunchKernelGGL((top_rows<DT, 256>), g, dim3(256), 0, s, p);              \
+    if (V <= 24576 && k <= 256) hipLaunchKernelGGL((top_rows<DT, 256>), g, dim3(256), 0, s, p);              \
+    else if (k <= 512) hipLaunchKernelGGL((top_rows<DT, 512>), g, dim3(512), 0, s, p);                       \
     else hipLaunchKernelGGL((top_rows<DT, 1024>), g, dim3(1024), 0, s, p);                                   \
   } while (0)
   if (dtype == MR_BF16) MR_TOP(MR_BF16);
@@ -1203,13 +1211,20 @@ int mr_distill(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, 
     // what 7 pieces a thread and the block's sums leave of half a CU's LDS
     constexpr size_t kTwoRows = 81920 - 512 * 7 * 16 - 2048;
 #define MR_DISTILL(DT, THREADS, N, M, R) hipLaunchKernelGGL((distill_held<DT, THREADS, N, M, R>), g, dim3(THREADS), lds, s, p)
-    // the fewest threads that hold the row in at most 8 pieces each, then more
-    // pieces, as long as two rows fit a CU; then one row
+    // The fewest threads that hold the row in at most 8 pieces each, then more pieces,
+    // some of them in LDS, then some read twice, as long as two rows fit a CU;
+    // the loss alone by small blocks where there are rows for eight of them a CU and
+    // room for their bitmaps; a row that is read twice by the whole of half a CU
+#define MR_STREAM(DT, THREADS, GRAD) \
+  hipLaunchKernelGGL((distill_stream<DT, THREADS, GRAD>), g, dim3(THREADS), lds, s, p)
 #define MR_DISTILL_D(DT)                                                                                 \
   do {                                                                                                   \
-    if (V * es < 16 || (!dlogits && pieces > 512 * 8))                                                   \
-      hipLaunchKernelGGL((distill_stream<DT>), g, dim3(1024), lds, s, p);                                \
-    else if (pieces <= 256 * 4) MR_DISTILL(DT, 256, 4, 0, 0);                                               \
+    if (V * es < 16 || (!dlogits && pieces > 256 * 8)) {                                                   \
+      if (dlogits) MR_STREAM(DT, 1024, true);                                                              \
+      else if (T >= 1024 && lds <= 20480) MR_STREAM(DT, 256, false);                                       \
+      else if (lds <= 40960) MR_STREAM(DT, 512, false);                                                    \
+      else MR_STREAM(DT, 1024, false);                                                                     \
+    } else if (pieces <= 256 * 4) MR_DISTILL(DT, 256, 4, 0, 0);                                               \
     else if (pieces <= 256 * 8) MR_DISTILL(DT, 256, 8, 0, 0);                                               \
     else if (pieces <= 512 * 8) MR_DISTILL(DT, 512, 8, 0, 0);                                               \
     else if (pieces <= 512 * 16) MR_DISTILL(DT, 512, 16, 0, 0);                                             \
@@ -1218,12 +1233,13 @@ int mr_distill(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, 
     else if (pieces <= 512 * 31) MR_DISTILL(DT, 512, 17, 6, 8);                                          \
     else if (pieces <= 512 * 39 && lds <= kTwoRows) MR_DISTILL(DT, 512, 16, 7, 16);                      \
     else if (pieces <= 512 * 40) MR_DISTILL(DT, 512, 17, 6, 17);                                           \
-    else hipLaunchKernelGGL((distill_stream<DT>), g, dim3(1024), lds, s, p);                             \
+    else MR_STREAM(DT, 1024, true);                             \
   } while (0)
     if (dtype == MR_BF16) MR_DISTILL_D(MR_BF16);
     else if (dtype == MR_F16) MR_DISTILL_D(MR_F16);
     else MR_DISTILL_D(MR_F32);
 #undef MR_DISTILL_D
+#undef MR_STREAM
 #undef MR_DISTILL
     MR_LAUNCH_CHECK("mr_distill");
   }

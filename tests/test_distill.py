@@ -554,3 +554,27 @@ def test_a_peak_anywhere(V, dtype):
             c += 1
         z[r, c] = 300.0
     check(z, values, ids, scale=1.0, lse=torch.logsumexp(teacher.double(), 1).float())
+
+
+# rows enough for small blocks of the loss alone, a row or two of each bound on a block's size
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [(1100, 20000, 16), (1030, 17001, 700), (3, 17001, 16), (2, 320000, 16), (2, 400000, 900),
+                                  (2, 16384, 5), (2, 16385, 5)], ids=lambda c: "x".join(map(str, c)))
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_loss_alone_is_the_loss(case, dtype):
+    T, V, k = case
+    z, values, ids, teacher = make(T, V, k, dtype, seed=V, ragged=True)
+    lse = torch.logsumexp(teacher.double(), 1).float()
+    want, *_, weight, _ = reference(z, values, ids, scale=1.0, lse=lse)
+    row, loss, _ = run(z, values, ids, scale=1.0, lse=lse, grad=False)
+    tol = 2 * weight * unit(V) + 2.0 ** -24 * want.abs() + 1e-12
+    assert bool(((row.cpu().double() - want).abs() <= tol).all())
+    assert abs(float(loss) - float(row.double().sum())) <= 2.0 ** -23 * float(row.double().abs().sum())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [(2, 24576, 256), (2, 24577, 256), (2, 24000, 257), (2, 30000, 512), (2, 30000, 513),
+                                  (2, 700, 512), (2, 700, 513), (2, 4096, 512)], ids=lambda c: "x".join(map(str, c)))
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_top_logits_by_each_block(case, dtype):
+    test_top_logits(case, dtype)
