@@ -15,11 +15,10 @@
 // there: no table of positions is read or kept, at any length.
 //
 // Bound by memory: an element is read and written once. 16384 tokens of 32 bf16
-// heads of 128 take 50 us (268 MB, 5.4 TB/s; 57 us through the caches, where a plain copy reaches
-// 5.0 TB/s), 4000 of 16
-// float16 heads, 32 of 64 elements rotated, 6 us, and 8 tokens 3 us, where a call's
-// own 8 us on the host are what counts. A thread has 4 x 32 bytes on their way while
-// the angles are worked out.
+// heads of 128 take 50 us (268 MB, 5.4 TB/s; 57 us through the caches), 4000 of 16
+// float16 heads, 32 of 64 elements rotated, 6 us, and 8 tokens 3 us, where a call's own
+// 8 us on the host are what counts. A thread has 4 x 32 bytes on their way while the
+// angles are worked out.
 #include "mr_common.h"
 
 namespace mr {

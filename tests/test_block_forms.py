@@ -353,3 +353,27 @@ def test_a_list_of_another_batch_is_refused():
         lm.run(tokens[:1], teacher=teacher)
     with pytest.raises(CalibrationError, match="1 to 1024"):
         lm.teacher_list(tokens, top=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", [dict(partial_rotary_factor=0.5),
+                                  dict(rope_traditional=True, rope_scaling={"rope_type": "yarn", "factor": 4.0,
+                                                                            "original_max_position_embeddings": 64})],
+                         ids=["partial", "interleaved-yarn"])
+def test_quantize_blocks_of_other_forms(tmp_path, form):
+    """The whole run: scores by the teacher, tuning (steps recorded and replayed), holdout, export."""
+    from mround_amd.schemes import TuningConfig
+
+    cfg = dict(BASE, hidden_size=128, num_attention_heads=2, num_key_value_heads=1, head_dim=64, intermediate_size=256,
+               num_hidden_layers=2, vocab_size=200, rms_norm_eps=1e-6, tie_word_embeddings=True, torch_dtype="bfloat16", **form)
+    src = write_random_checkpoint(tmp_path / "m", cfg, seed=2, std=0.05)
+    tuning = TuningConfig(iters=24, batch_size=2, n_samples=8, seq_len=100)
+    kw = dict(symmetry=Symmetry.ASYMMETRIC, tuning=tuning, seed=5, average_bits=3.0, candidate_bits=(2, 4),
+              sensitivity_objective="teacher")
+    res = api.quantize(src, output_dir=tmp_path / "q", **kw)
+    again = api.quantize(src, output_dir=tmp_path / "q2", **kw)
+    assert len(res.summary.blocks) == 2
+    for a, b in zip(res.summary.blocks, again.summary.blocks):
+        assert math.isfinite(a.initial_loss) and a.final_loss <= a.initial_loss
+        assert (a.initial_loss, a.final_loss) == (b.initial_loss, b.final_loss)
+    assert (tmp_path / "q" / "model.safetensors").read_bytes() == (tmp_path / "q2" / "model.safetensors").read_bytes()
