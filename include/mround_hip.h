@@ -267,7 +267,7 @@ int mr_cross_entropy(const void* logits, int64_t ld, int64_t T, int64_t V, const
  * int32 ids [T, k], and, if lse is non-NULL, lse[t] = log sum_i exp(logits[t, i]
  * / temperature).
  */
-int mr_top_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, int k, float temperature,
+int mr_top_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, int k, double temperature,
                   float* values, int32_t* ids, float* lse, void* stream);
 
 /*
@@ -295,7 +295,7 @@ int mr_top_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t 
  * (mround/pipeline/scoring.py:183-192).
  */
 int mr_distill(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, const float* top_values,
-               const int32_t* top_ids, int k, const float* top_lse, float temperature, float scale,
+               const int32_t* top_ids, int k, const float* top_lse, double temperature, float scale,
                float* row_loss, float* loss_out, void* dlogits, int64_t ldd, void* stream);
 
 /*

@@ -156,7 +156,7 @@ __device__ __forceinline__ uint4 gradient_piece(uint4 q, float about, float b, f
 }
 
 // Temperatures whose log2(e) / T leaves room for masked logits and for its low part.
-constexpr float kMinTemperature = 1.0f / 1024, kMaxTemperature = 1024.0f;
+constexpr double kMinTemperature = 1.0 / 1024, kMaxTemperature = 1024.0;
 
 ExpScale exp_scale(double temperature) {
   // hi from below and lo above zero: minus infinity times either is minus infinity
@@ -1117,7 +1117,7 @@ bool element_aligned(const void* p, int es) { return reinterpret_cast<uintptr_t>
 
 extern "C" {
 
-int mr_top_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, int k, float temperature,
+int mr_top_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, int k, double temperature,
                   float* values, int32_t* ids, float* lse, void* stream) {
   using namespace mr;
   clear_error();
@@ -1162,7 +1162,7 @@ int mr_top_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t 
 }
 
 int mr_distill(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, const float* top_values,
-               const int32_t* top_ids, int k, const float* top_lse, float temperature, float scale, float* row_loss,
+               const int32_t* top_ids, int k, const float* top_lse, double temperature, float scale, float* row_loss,
                float* loss_out, void* dlogits, int64_t ldd, void* stream) {
   using namespace mr;
   clear_error();
@@ -1204,7 +1204,7 @@ int mr_distill(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, 
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (T > 0) {
     DistillParams p{logits, ld, static_cast<int>(V), k, top_values, top_ids, top_lse, exp_scale(temperature),
-                    1.0 / static_cast<double>(temperature), scale, row_loss, dlogits, ldd};
+                    1.0 / temperature, scale, row_loss, dlogits, ldd};
     const dim3 g(static_cast<unsigned>(T));
     const size_t lds = static_cast<size_t>((V + 31) / 32 + 1) * 4 + static_cast<size_t>(k) * 8;
     const int64_t pieces = (V * es + 15) / 16;

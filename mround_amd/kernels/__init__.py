@@ -127,8 +127,8 @@ _SIGNATURES = {
     "mr_delta_loss_mapped": (_I, [_P, _I, _P, _L, _L, _I, _P, _I, _I, _F, _P, _L, _L, _L, _P, _P,
                                   _P]),
     "mr_cross_entropy": (_I, [_P, _L, _L, _L, _P, _F, _P, _P, _P, _L, _P]),
-    "mr_top_logits": (_I, [_P, _I, _L, _L, _L, _I, _F, _P, _P, _P, _P]),
-    "mr_distill": (_I, [_P, _I, _L, _L, _L, _P, _P, _I, _P, _F, _F, _P, _P, _P, _L, _P]),
+    "mr_top_logits": (_I, [_P, _I, _L, _L, _L, _I, _D, _P, _P, _P, _P]),
+    "mr_distill": (_I, [_P, _I, _L, _L, _L, _P, _P, _I, _P, _D, _F, _P, _P, _P, _L, _P]),
     "mr_embed_rows": (_I, [_P, _I, _L, _L, _L, _P, _L, _P, _L, _P]),
 }
 

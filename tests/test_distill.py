@@ -424,7 +424,7 @@ def test_top_logits_refusals_before_launch():
     lib, P, f = K.lib(), ctypes.c_void_p, ctypes.c_float
 
     def call(x=P(1 << 20), dt=1, ld=1000, T=4, V=1000, k=8, temp=1.0, values=P(1 << 24), ids=P(1 << 25), lse=P(1 << 26)):
-        return lib.mr_top_logits(x, dt, ld, T, V, k, f(temp), values, ids, lse, None)
+        return lib.mr_top_logits(x, dt, ld, T, V, k, ctypes.c_double(temp), values, ids, lse, None)
 
     for bad, word in ((dict(x=None), b"null"), (dict(values=None), b"null"), (dict(ids=None), b"null"),
                       (dict(dt=5), b"dtype"), (dict(T=-1), b"sizes"), (dict(V=0), b"sizes"), (dict(k=0), b"k=0"),
@@ -442,7 +442,7 @@ def test_distill_refusals_before_launch():
 
     def call(z=P(1 << 20), dt=0, ld=1000, T=4, V=1000, t=P(1 << 22), ids=P(1 << 23), k=8, lse=P(1 << 24), temp=1.0,
              row=P(1 << 25), loss=P(1 << 26), d=P(1 << 27), ldd=1000):
-        return lib.mr_distill(z, dt, ld, T, V, t, ids, k, lse, f(temp), f(1.0), row, loss, d, ldd, None)
+        return lib.mr_distill(z, dt, ld, T, V, t, ids, k, lse, ctypes.c_double(temp), f(1.0), row, loss, d, ldd, None)
 
     for bad, word in ((dict(z=None), b"null"), (dict(t=None), b"null"), (dict(ids=None), b"null"), (dict(row=None), b"null"),
                       (dict(dt=-1), b"dtype"), (dict(T=-2), b"sizes"), (dict(V=0), b"sizes"),
@@ -480,9 +480,9 @@ def test_bindings_refuse_on_the_host():
 def test_temperatures_out_of_range_are_refused():
     lib, P, f = K.lib(), ctypes.c_void_p, ctypes.c_float
     for temp in (1e-4, 2e3):
-        assert lib.mr_top_logits(P(1 << 20), 1, 1000, 4, 1000, 8, f(temp), P(1 << 24), P(1 << 25), None, None) == -22
+        assert lib.mr_top_logits(P(1 << 20), 1, 1000, 4, 1000, 8, ctypes.c_double(temp), P(1 << 24), P(1 << 25), None, None) == -22
         assert b"temperature" in lib.mr_last_error()
-        assert lib.mr_distill(P(1 << 20), 0, 1000, 4, 1000, P(1 << 22), P(1 << 23), 8, None, f(temp), f(1.0), P(1 << 25), None,
+        assert lib.mr_distill(P(1 << 20), 0, 1000, 4, 1000, P(1 << 22), P(1 << 23), 8, None, ctypes.c_double(temp), f(1.0), P(1 << 25), None,
                               None, 1000, None) == -22
         assert b"temperature" in lib.mr_last_error()
 
@@ -578,3 +578,14 @@ def test_loss_alone_is_the_loss(case, dtype):
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_top_logits_by_each_block(case, dtype):
     test_top_logits(case, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("temperature", [0.7, 1.354, 2.3])
+def test_temperatures_that_are_no_floats(temperature):
+    """The temperature is a double: in float32 2^-25 of a logit would be missing between the list and its log-sum-exp,
+    3e-7 of every probability at logits of 10."""
+    T, V, k = 8, 4363, 78
+    z, values, ids, teacher = make(T, V, k, "bf16", seed=31, noise=0.1)
+    check(z, values, ids, scale=1.0, lse=torch.logsumexp(teacher.double() / temperature, 1).float(), temperature=temperature)
+    check_top(z, k, temperature=temperature)
