@@ -856,7 +856,10 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
 #pragma unroll
     for (int j = 0; j < N; ++j) asm volatile("" : "+v"(r[j].x), "+v"(r[j].y), "+v"(r[j].z), "+v"(r[j].w));
   };
+  // (A mask is no maximum: about itself its terms would be one where its product with log2(e) / T is exact. About
+  // zero each is zero.)
   float about = waves_max<W>(s_first);
+  if (about <= kMasked) about = 0.0f;
   float sum, ve, se;
   auto add_up = [&](auto takes) __attribute__((always_inline)) {
     if (!(__builtin_fabsf(about * p.c.hi) < kInf)) about = 0.0f;  // (so a sum past the floats becomes infinite)

@@ -589,3 +589,36 @@ def test_temperatures_that_are_no_floats(temperature):
     z, values, ids, teacher = make(T, V, k, "bf16", seed=31, noise=0.1)
     check(z, values, ids, scale=1.0, lse=torch.logsumexp(teacher.double() / temperature, 1).float(), temperature=temperature)
     check_top(z, k, temperature=temperature)
+
+
+# ------------------------------------------------------------ masks and far logits --
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [300, 16385, 40001, 100003, 151936])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("temperature", [0.75, 1.0, 1.5, 2.0, 2.034, 2.158, 2.5, 3.679, 4.0, 300.0])
+def test_masks_at_any_temperature(temperature, dtype, V):
+    """Every unlisted logit at a mask's value, one that is exact in powers of two over the temperature among them:
+    no such outcome, with the gradient as without it, and no gradient on what is masked. In the other rows a few
+    logits lie off the list and off the mask, first and last in the row."""
+    T, k = 6, 5
+    z, values, ids, teacher = make(T, V, k, dtype, seed=18)
+    ids = torch.argsort(torch.rand(T, V - 40, generator=torch.Generator().manual_seed(V)), 1)[:, :k].int() + 20
+    values = teacher.gather(1, ids.long())
+    listed = torch.zeros(T, V, dtype=torch.bool).scatter_(1, ids.long(), True)
+    lows = torch.tensor([torch.finfo(DT[dtype]).min, -2.0 ** 125, -2.0 ** 126]).to(z.dtype).repeat(2)[:, None]
+    free = listed.clone()
+    free[3, :3] = free[4, V - 3:] = free[5, V // 2] = True
+    z = torch.where(free, z, lows.expand(T, V))
+    as_inf = torch.where(free, z, torch.full_like(z, -math.inf))
+    lse = torch.logsumexp(teacher.double() / temperature, 1).float()
+    for tail in (lse, None):
+        want, grad, size, weight, far = reference(as_inf, values, ids, scale=64.0, lse=tail, temperature=temperature)
+        row, _, d = run(z, values, ids, scale=64.0, lse=tail, temperature=temperature)
+        alone, _, _ = run(z, values, ids, scale=64.0, lse=tail, temperature=temperature, grad=False)
+        tol = 2 * weight * unit(V) + 2.0 ** -24 * want.abs() + 1e-12
+        for r in (row, alone):
+            assert bool(((r.cpu().double() - want).abs() <= tol).all()), (tail is None, r, want)
+        gtol = 2 * size * (unit(V) + 4 * far * 2.0 ** -24) + torch.finfo(z.dtype).eps / 2 * grad.abs() + 2.0 ** -100
+        assert bool(((d.cpu().double() - grad).abs() <= gtol).all())
+        assert bool((d.cpu()[~free] == 0).all())
