@@ -142,6 +142,33 @@ __device__ __forceinline__ float exp_t(float d, ExpScale c) {
   return __builtin_amdgcn_exp2f(__builtin_fmaf(d, c.hi, d * c.lo));
 }
 
+// A value that all lanes share, in a scalar register.
+__device__ __forceinline__ float uniform(float x) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
+}
+
+// Past 2^24 powers of two a float's step is one power or more, and v hi - base (base: max hi, rounded) is off
+// zero at the maximum itself by as much: exponentials of a few hundred past 2^30. There, far from zero, terms are
+// formed of differences (exp_t), or, of 16-bit logits, whose steps are then 2^13 powers and leave of all terms
+// those at the maximum, with a log2(e) / T of 12 bits, whose product with it is exact.
+constexpr float kFar = 0x1p24f;
+__device__ __forceinline__ bool is_far(float about, ExpScale c) {
+  const float x = __builtin_fabsf(about * c.hi);
+  return x > kFar && x < kInf;
+}
+template <int DT>
+__device__ __forceinline__ ExpScale scale_at(float about, ExpScale c) {
+  if constexpr (DT != MR_F32) {
+    const uint32_t hi = __float_as_uint(c.hi);
+    c.hi = uniform(__uint_as_float(is_far(about, c) ? hi & 0xfffff000u : hi));
+  }
+  return c;
+}
+// The base of a sum about a far maximum, in powers of two.
+__device__ __forceinline__ double far_base(float about, ExpScale c) {
+  return static_cast<double>(about) * (static_cast<double>(c.hi) + c.lo);
+}
+
 // A piece's gradient: its terms as the sum had them, 2^(v hi - b), times g; in fp32
 // to its precision, about `about`.
 template <int DT>
@@ -786,7 +813,8 @@ __device__ __forceinline__ void store_piece(uint8_t* row, int i, int V, uint4 o)
 // itself, and 2 exponentials a logit (4 issue slots each) take as long as the
 // row's loads. So the sum does not wait for the row's maximum: it runs about the
 // maximum of the first pieces to arrive, piece by piece as the others do, and
-// only a sum outside 2^-64 .. 2^64 is formed again about the maximum itself.
+// only a sum outside 2^-64 .. 2^64, or far from zero, is formed again about the
+// maximum itself.
 // exp(v / T) is 2^(v hi - b), one fused multiply-add: b is any number, and what
 // hi lacks of log2(e) / T is made up in the sum's base, to first order, by the
 // mean of v (over one in E of the terms). The gradient takes the same terms times
@@ -863,7 +891,19 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   float sum, ve, se;
   auto add_up = [&](auto takes) __attribute__((always_inline)) {
     if (!(__builtin_fabsf(about * p.c.hi) < kInf)) about = 0.0f;  // (so a sum past the floats becomes infinite)
-    const float b = -about * p.c.hi;
+    // (far from zero the first sum is only one to be formed again)
+    constexpr bool again = !decltype(takes)::value;
+    const ExpScale c = again ? scale_at<DT>(about, p.c) : p.c;
+    const bool apart = again && DT == MR_F32 && is_far(about, p.c);
+    const float b = -about * c.hi;
+    auto term = [&](float v) __attribute__((always_inline)) {
+      float x = __builtin_fmaf(v, c.hi, b);
+      if (apart) {
+        const float d = v - about;
+        x = __builtin_fmaf(d, c.hi, d * c.lo);
+      }
+      return __builtin_amdgcn_exp2f(x);
+    };
     const int t = anew();
     float s0 = 0.0f, s1 = 0.0f;
     ve = se = 0.0f;
@@ -877,13 +917,13 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
       widen<DT>(q, v);
 #pragma unroll
       for (int k = 0; k < E; k += 2) {
-        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(v[k], p.c.hi, b));
+        const float e0 = term(v[k]);
         if (k == 0) {
           ve = __builtin_fmaf(fmaxf(v[0], -1e30f), e0, ve);
           se += e0;
         }
         s0 += e0;
-        s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(v[k + 1], p.c.hi, b));
+        s1 += term(v[k + 1]);
       }
       // Here, as the pieces arrive: left alone the sums move behind the next barrier,
       // and the bitmap's words of every piece are read ahead (40 registers).
@@ -936,7 +976,9 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   l.sums(p, sum, s);
   __syncthreads();  // (and every read of the row is done)
   const double rest0 = waves_sum<W>(s.rest);
-  if (!(rest0 > 0x1p-64 && rest0 < 0x1p64)) {  // (or a NaN)
+  // (the row's values, one for all lanes: what a branch of a wave keeps of both sides spilled)
+  const bool anew_about = !(rest0 > 0x1p-64 && rest0 < 0x1p64) || is_far(about, p.c);  // (or a NaN)
+  if (__builtin_amdgcn_readfirstlane(anew_about)) {
     fresh();
     float mx = -kInf;
     auto most = [&](uint4 q) __attribute__((always_inline)) {
@@ -974,7 +1016,8 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
     const float v = waves_sum<W>(s_ve), e = waves_sum<W>(s_e);
     l.finish(s);
     return RowSums(p, l, waves_sum<W>(s.rest),
-                   static_cast<double>(about * p.c.hi) + lo * (e > 0.0f ? static_cast<double>(v / e) : about));
+                   is_far(about, p.c) ? far_base(about, p.c)
+                                      : static_cast<double>(about * p.c.hi) + lo * (e > 0.0f ? static_cast<double>(v / e) : about));
   };
   const bool none = l.n == 0;
   if (p.dz) {
@@ -987,13 +1030,14 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
         s_g = static_cast<float>(DT == MR_F32 ? g * exp2(about * (static_cast<double>(p.c.hi) + p.c.lo) - x.base) : g);
     }
     __syncthreads();
-    const float g = s_g, b = -about * p.c.hi;
+    const ExpScale c = scale_at<DT>(about, p.c);
+    const float g = uniform(s_g), b = -about * c.hi;
     const int t = anew();
     fresh();
     auto put = [&](int j, uint4 q) __attribute__((always_inline)) {
       const int i = j * THREADS + t;
       if (i >= pieces) return;
-      uint4 o = gradient_piece<DT>(q, about, b, g, p.c);
+      uint4 o = gradient_piece<DT>(q, about, b, g, c);
       if (none) o = make_uint4(0, 0, 0, 0);
       store_piece<DT>(dz, i, V, o);
       if (DT == MR_F32) __builtin_amdgcn_sched_barrier(0);  // (else pieces in float32 are worked on together, and spill)
@@ -1071,13 +1115,31 @@ __global__ __launch_bounds__(THREADS, 8) void distill_stream(DistillParams p) {
   l.sums(p, 0.0f, s);
   __syncthreads();  // (and the list's reads of the row are done)
   l.finish(s);
-  const BlockSum<W> rest(s_sum, p.c);
+  BlockSum<W> rest(s_sum, p.c);
+  const float about = rest.max > kMasked ? rest.max : 0.0f;
+  if (is_far(about, p.c)) {
+    float sum = 0.0f;
+    for (int i = tid; i < pieces; i += THREADS) {
+      uint4 q = get(i, std::false_type{});
+      take_out<DT>(q, left_out(i));
+      float v[E];
+      widen<DT>(q, v);
+#pragma unroll
+      for (int k = 0; k < E; ++k) sum += exp_t(v[k] - about, p.c);
+    }
+    const double r64 = wave_sum(static_cast<double>(sum));
+    if ((tid & 63) == 0) s.rest[tid >> 6] = r64;
+    __syncthreads();
+    rest.sum = waves_sum<W>(s.rest);
+    rest.exponent = far_base(about, p.c);
+  }
   const RowSums x(p, l, rest.sum, rest.exponent);
   if (tid == 0) p.row_loss[row] = x.loss(p, l);
   if constexpr (!GRAD) return;
   const bool none = l.n == 0;
   const double g64 = l.n < 0 ? __builtin_nan("") : x.rest_gradient(p);
-  const float about = rest.max > kMasked ? rest.max : 0.0f, base = -about * p.c.hi;
+  const ExpScale c = scale_at<DT>(about, p.c);
+  const float base = -about * c.hi;
   const float g = static_cast<float>(DT == MR_F32 ? g64 * exp2(about * (static_cast<double>(p.c.hi) + p.c.lo) - x.base) : g64);
   for (int i0 = tid; i0 < pieces; i0 += U * THREADS) {
     uint4 q[U];
@@ -1088,7 +1150,7 @@ __global__ __launch_bounds__(THREADS, 8) void distill_stream(DistillParams p) {
       const int i = i0 + j * THREADS;
       if (i >= pieces) continue;
       if (const uint32_t bits = left_out(i)) take_out<DT>(q[j], bits);
-      uint4 o = gradient_piece<DT>(q[j], about, base, g, p.c);
+      uint4 o = gradient_piece<DT>(q[j], about, base, g, c);
       if (none) o = make_uint4(0, 0, 0, 0);
       store_piece<DT>(dz, i, V, o);
     }

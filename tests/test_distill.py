@@ -622,3 +622,66 @@ def test_masks_at_any_temperature(temperature, dtype, V):
         gtol = 2 * size * (unit(V) + 4 * far * 2.0 ** -24) + torch.finfo(z.dtype).eps / 2 * grad.abs() + 2.0 ** -100
         assert bool(((d.cpu().double() - grad).abs() <= gtol).all())
         assert bool((d.cpu()[~free] == 0).all())
+
+
+def far_reference(z, values, ids, *, scale, lse, temperature):
+    """``reference`` for rows whose unlisted logits lie far from the listed: the rest's shares as a softmax of its own
+    (as a difference of log-probabilities of 1e10 they would keep no digit in float64 either), and of each exponent
+    the distance from the largest of its kind, where that leaves anything."""
+    want, _, _, weight, _ = reference(z, values, ids, scale=scale, lse=lse, temperature=temperature)
+    u, t = z.double() / temperature, values.double() / temperature
+    listed = torch.zeros(z.shape, dtype=torch.bool).scatter_(1, ids.long(), True)
+    q = torch.exp(t - lse.double()[:, None]) if lse is not None else torch.softmax(t, 1)
+    q_rest = (1 - q.sum(1, keepdim=True)).clamp_min(0) if lse is not None else torch.zeros(z.shape[0], 1).double()
+    p = torch.log_softmax(u, 1).exp() * (q.sum(1, keepdim=True) + q_rest)
+    target = (q_rest * torch.softmax(u.masked_fill(listed, -math.inf), 1)).scatter(1, ids.long(), q)
+    away = torch.where(listed, u - u.amax(1, keepdim=True), u - u.masked_fill(listed, -math.inf).amax(1, keepdim=True)).abs()
+    away = torch.where(away < 200, away, torch.zeros_like(away))
+    gs = scale / temperature
+    return want, (p - target) * gs, (p + target) * gs, weight, away, u.abs().amax(1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [3, 7, 300, 16385, 40001, 100003, 151936, 200003])
+@pytest.mark.parametrize("size,dtype", [(s, t) for t in ("bf16", "f32") for s in (-3e7, -1e9, -1e10, -7e11, -1e20, -1e33, 1e10, 1e20)]
+                         + [(-3e4, "f16"), (3e4, "f16")])
+def test_unlisted_logits_far_from_zero(size, dtype, V):
+    """Unlisted logits where a float's step is many powers of two: equal, steps of the type apart, or one far above
+    the rest; the first half of a row holds the largest or none of it.
+
+    The loss carries 2^-47 of |z / T| for each of its two logarithms (log2(e) / T is two floats), the gradient the
+    errors of exponents a few steps from their largest."""
+    T, k = 5, min(3, V - 2)
+    for temperature in (2.0 ** -10, 0.7, 1.0, 2.0, 100.0):
+        g = torch.Generator().manual_seed(V)
+        z, _, _, teacher = make(T, V, k, dtype, seed=28)
+        ids = torch.argsort(torch.rand(T, V, generator=g), 1)[:, :k].int()
+        values = teacher.gather(1, ids.long())
+        listed = torch.zeros(T, V, dtype=torch.bool).scatter_(1, ids.long(), True)
+        step = 2.0 ** (math.floor(math.log2(abs(size))) - {"bf16": 7, "f16": 10, "f32": 23}[dtype])
+        far = torch.full((T, V), size, dtype=torch.float64)
+        far[1] -= step * torch.randint(0, 4, (V,), generator=g)
+        far[2, : V // 2] *= 2 if size < 0 else 0.5
+        far[3, V // 2:] *= 2 if size < 0 else 0.5
+        if size > 0:
+            far[4] = 0.0
+        far[4, :-1] -= 64 * step * (torch.arange(V - 1) % 3)
+        far[4, -1] = size
+        z = torch.where(listed, z.double(), far).to(z.dtype)
+        # a rest of a fifth and more
+        lse = (torch.logsumexp(values.double() / temperature, 1) + 0.25).float()
+        for tail in (lse, None):
+            kw = dict(scale=0.37, lse=tail, temperature=temperature)
+            want, grad, size_, weight, away, u_max = far_reference(z, values, ids, **kw)
+            row, _, d = run(z, values, ids, **kw)
+            row2, _, d2 = run(z, values, ids, in_place=True, **kw)
+            alone, _, _ = run(z, values, ids, grad=False, **kw)
+            tol = 2 * weight * unit(V) + 2.0 ** -24 * want.abs() + 2.0 ** -46 * weight * u_max + 1e-12
+            for r in (row, alone):
+                err = (r.cpu().double() - want).abs()
+                assert bool((err <= tol).all()), (temperature, tail is None, r, want)
+            assert torch.equal(row, row2) and torch.equal(d, d2)
+            gtol = 2 * size_ * (unit(V) + 4 * away * 2.0 ** -24) + torch.finfo(z.dtype).eps / 2 * grad.abs() \
+                + 2.0 ** -25 * (dtype == "f16") + 2.0 ** -120
+            err = (d.cpu().double() - grad).abs()
+            assert bool((err <= gtol).all()), (temperature, tail is None, float((err / gtol).max()))
