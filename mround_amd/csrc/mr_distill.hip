@@ -303,7 +303,8 @@ struct BlockSum {
       v += __shfl_xor(v, off, 64);
       n += __shfl_xor(n, off, 64);
     }
-    const float mean = n > 0.0f && v < kInf && v > -kInf ? v / n : max;
+    // (far from zero the mean of v, which ends at -1e30, is the maximum to a few steps of 2^-24)
+    const float mean = n > 0.0f && v < kInf && v > -kInf && !is_far(max, c) ? v / n : max;
     exponent = about == -kInf ? 0.0 : static_cast<double>(about) + static_cast<double>(c.lo) * mean;
   }
 };

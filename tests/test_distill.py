@@ -685,3 +685,29 @@ def test_unlisted_logits_far_from_zero(size, dtype, V):
                 + 2.0 ** -25 * (dtype == "f16") + 2.0 ** -120
             err = (d.cpu().double() - grad).abs()
             assert bool((err <= gtol).all()), (temperature, tail is None, float((err / gtol).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [30, 2048, 9000, 60001])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("size", [-3e7, -1e9, 2.0 ** 31, -7e11, -2.0 ** 102, -2.0 ** 110, -2.0 ** 122, 1e20, 1e30])
+def test_top_logits_far_from_zero(size, dtype, V):
+    """Log-sum-exps of logits where a float's step is many powers of two, masks of other code's making among them:
+    equal, steps of the type apart, halves of a row far from one another."""
+    T, k = 4, min(V, 257)
+    g = torch.Generator().manual_seed(V)
+    step = 2.0 ** (math.floor(math.log2(abs(size))) - (7 if dtype == "bf16" else 23))
+    z = torch.full((T, V), size, dtype=torch.float64)
+    z[1] -= step * torch.randint(0, 4, (V,), generator=g)
+    z[2, : V // 2] *= 2 if size < 0 else 0.5
+    z[3, :-1] -= 64 * step * (torch.arange(V - 1) % 3)
+    z = z.to(DT[dtype])
+    for temperature in (2.0 ** -10, 0.7, 1.0, 2.0, 3.1, 100.0):
+        ref = torch.logsumexp(z.double() / temperature, 1)
+        over = ref.abs() >= 2.0 ** 128  # (as a float32 an infinity)
+        if bool(over.any()):
+            _, ids, lse = run_top(z[over].to(dev()), V, k, temperature)
+            assert np.array_equal(ids.cpu().numpy(), ordered(z[over].double().numpy(), k))
+            assert torch.equal(lse.cpu(), ref[over].float())
+        if not bool(over.all()):
+            check_top(z[~over], k, temperature)
