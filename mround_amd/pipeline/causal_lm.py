@@ -62,13 +62,29 @@ def padded_length(seq_len: int) -> int:
 class TeacherList:
     """A model's likeliest tokens at every row of a batch (``CausalLM.teacher_list``):
     float32 logits and int32 ids ``[T, top]`` (ids -1 at rows that are padding), the
-    rows' log-sum-exp ``[T]`` at ``temperature``, and the tokens they belong to."""
+    rows' log-sum-exp ``[T]`` at ``temperature``, the tokens they belong to, and an
+    int32 copy of these with the version they had (in-place writes raise it)."""
 
     values: torch.Tensor
     ids: torch.Tensor
     lse: torch.Tensor
     temperature: float
     tokens: torch.Tensor
+    batch: torch.Tensor
+    version: int | None
+
+    def belongs_to(self, tokens: torch.Tensor) -> bool:
+        """Whether ``tokens`` are the list's batch. The tensor that the list was
+        made from, not written since, is; another one is compared with the
+        copy, for which the device is waited for."""
+        if tokens is self.tokens and self.version is not None and self.version == _version(tokens):
+            return True
+        return tokens.shape == self.batch.shape and torch.equal(
+            tokens.to(device=self.batch.device, dtype=torch.int32), self.batch)
+
+
+def _version(t: torch.Tensor) -> int | None:
+    return None if t.is_inference() else t._version
 
 
 class CausalLM:
@@ -206,7 +222,8 @@ class CausalLM:
         lse = torch.empty(T, dtype=torch.float32, device=self.device)
         K.top_logits(self.logits, V=self.vocab, values=values, ids=ids, lse=lse, temperature=temperature)
         ids.masked_fill_(self.labels.view(-1, 1) < 0, -1)
-        return TeacherList(values, ids, lse, float(temperature), tokens)
+        return TeacherList(values, ids, lse, float(temperature), tokens,
+                           tokens.to(device=self.device, dtype=torch.int32, copy=True), _version(tokens))
 
     def run(self, tokens: torch.Tensor,
             on_block: Callable[[int, dict[str, torch.Tensor]], None] | None = None,
@@ -218,7 +235,7 @@ class CausalLM:
         of the next tokens, or with ``teacher`` (the list of the same batch) the
         divergence from the teacher's distribution, its tokens off the list one
         outcome."""
-        if teacher is not None and (teacher.ids.shape[0] != self.tokens or teacher.tokens.shape != tokens.shape):
+        if teacher is not None and (teacher.ids.shape[0] != self.tokens or not teacher.belongs_to(tokens)):
             raise CalibrationError("the teacher's list belongs to another batch")
         keep = self.acts is not None
         n = self._logits(tokens, keep)

@@ -377,3 +377,49 @@ def test_quantize_blocks_of_other_forms(tmp_path, form):
         assert math.isfinite(a.initial_loss) and a.final_loss <= a.initial_loss
         assert (a.initial_loss, a.final_loss) == (b.initial_loss, b.final_loss)
     assert (tmp_path / "q" / "model.safetensors").read_bytes() == (tmp_path / "q2" / "model.safetensors").read_bytes()
+
+
+def test_a_list_knows_its_batch():
+    from mround_amd.pipeline.causal_lm import TeacherList
+
+    def made_from(t):
+        e = torch.empty(0)
+        return TeacherList(e, e, e, 1.0, t, t.to(torch.int32, copy=True), None if t.is_inference() else t._version)
+
+    tokens = torch.randint(0, 300, (2, 65))
+    teacher = made_from(tokens)
+    other = tokens.clone()
+    other[1, 7] += 1
+    assert teacher.belongs_to(tokens) and teacher.belongs_to(tokens.clone()) and teacher.belongs_to(tokens.int())
+    assert not teacher.belongs_to(other) and not teacher.belongs_to(tokens[:1]) and not teacher.belongs_to(tokens[:, :64])
+    tokens[0, 3] += 1  # the same tensor with other tokens, and as it was
+    assert not teacher.belongs_to(tokens)
+    tokens[0, 3] -= 1
+    assert teacher.belongs_to(tokens)
+    with torch.inference_mode():
+        inside = torch.randint(0, 300, (2, 65))
+        teacher = made_from(inside)
+        assert teacher.belongs_to(inside)
+        inside[0, 0] += 1
+        assert not teacher.belongs_to(inside)
+
+
+@pytest.mark.gpu
+def test_a_list_of_other_tokens_is_refused():
+    """Lists of batches of one shape, taken before either is run, as a scoring pass takes them."""
+    from mround_amd.pipeline.causal_lm import CausalLM
+
+    model, _ = tiny_model({})
+    lm = CausalLM(model, batch=2, seq_len=65, device=dev())
+    lm.set_weights({})
+    first, second = torch.randint(0, 300, (2, 65)), torch.randint(0, 300, (2, 65), device=dev())
+    lists = lm.teacher_list(first), lm.teacher_list(second)
+    with pytest.raises(CalibrationError, match="another batch"):
+        lm.run(first, teacher=lists[1])
+    with pytest.raises(CalibrationError, match="another batch"):
+        lm.run(second, teacher=lists[0])
+    assert abs(float(lm.run(first, teacher=lists[0]))) < 1e-5
+    assert abs(float(lm.run(second.clone(), teacher=lists[1]))) < 1e-5
+    second[0, 0] = (second[0, 0] + 1) % 300
+    with pytest.raises(CalibrationError, match="another batch"):
+        lm.run(second, teacher=lists[1])
