@@ -523,9 +523,13 @@ def predict_time(model: str | Path, *, bits: int = 4, group_size: int = 64,
                             scoring_seq_len=scoring_seq_len, gradient_source=sensitivity_gradients)
 
 
-def _check_objective(objective: str) -> None:
+def _check_objective(objective: str, *, scored: bool) -> None:
+    """``scored``: whether the run has a scoring pass, the only place of an objective."""
     if objective not in ("labels", "teacher"):
         raise SchemeError(f"sensitivity_objective must be 'labels' or 'teacher', got {objective!r}")
+    if objective != "labels" and not scored:
+        raise SchemeError(f"sensitivity_objective={objective!r} is the objective of a scoring pass, which a run "
+                          "without average_bits, or with a given plan, does not make")
 
 
 def _check_calibration_sizes(tuning: TuningConfig) -> None:
@@ -576,7 +580,9 @@ def quantize(model: str | Path, *, output_dir: str | Path, bits: int = 4, group_
     ``remainder_bits`` (default: the width nearest the average, ties up).
     The scoring pass takes its gradients from the cross-entropy of the
     calibration tokens, or with ``sensitivity_objective`` "teacher" from the
-    divergence between the quantized model's predictions and the model's own.
+    divergence between the quantized model's predictions and the model's own
+    (refused where there is no scoring pass: no ``average_bits``, or a given
+    ``plan``).
     The run's device memory is predicted from ``config.json`` before anything
     is loaded (``predict_memory``) and a run past ``memory_budget`` (default
     90 % of the device's memory) is refused with ``MemoryBudgetError`` unless
@@ -602,7 +608,7 @@ def quantize(model: str | Path, *, output_dir: str | Path, bits: int = 4, group_
         raise UnsupportedSchemeError(f"export format {export_format!r} is not supported; only 'mlx'")
     if holdout_batches < 0:
         raise CalibrationError(f"holdout_batches must be zero or more, got {holdout_batches}")
-    _check_objective(sensitivity_objective)
+    _check_objective(sensitivity_objective, scored=average_bits is not None and plan is None)
     _refuse_unusable_plan(plan, average_bits, candidate_bits)
     resolved, widths = _resolve_scheme(bits=bits, group_size=group_size, symmetry=symmetry,
                                        average_bits=average_bits, candidate_bits=candidate_bits,
@@ -788,7 +794,7 @@ def plan_mixed_precision(model: str | Path, average_bits: float, candidate_bits:
     (mround/api.py:943-1085). Returns the plan summary, whose
     ``assignments`` map each block layer path to its width.
     ``sensitivity_objective`` as :func:`quantize`'s."""
-    _check_objective(sensitivity_objective)
+    _check_objective(sensitivity_objective, scored=True)
     resolved, widths = _resolve_scheme(bits=bits, group_size=group_size, symmetry=symmetry,
                                        average_bits=average_bits, candidate_bits=candidate_bits,
                                        remainder_bits=remainder_bits, scheme=scheme, scale_init=scale_init)

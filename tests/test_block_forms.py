@@ -423,3 +423,18 @@ def test_a_list_of_other_tokens_is_refused():
     second[0, 0] = (second[0, 0] + 1) % 300
     with pytest.raises(CalibrationError, match="another batch"):
         lm.run(second, teacher=lists[1])
+
+
+def test_an_objective_without_a_scoring_pass_is_refused(tmp_path):
+    from mround_amd.exceptions import SchemeError
+
+    cfg = dict(BASE, hidden_size=128, num_attention_heads=2, num_key_value_heads=1, head_dim=64, intermediate_size=256,
+               num_hidden_layers=1, vocab_size=200, rms_norm_eps=1e-6, tie_word_embeddings=True, torch_dtype="bfloat16")
+    src = write_random_checkpoint(tmp_path / "m", cfg, seed=2)
+    plan = {f"model.layers.0.{n}": 2 for n in LAYERS}
+    for kw in (dict(), dict(average_bits=2.0, candidate_bits=(2, 4), plan=plan)):
+        with pytest.raises(SchemeError, match="scoring pass"):
+            api.quantize(src, output_dir=tmp_path / "q", device="cpu", sensitivity_objective="teacher", **kw)
+    with pytest.raises(SchemeError, match="must be 'labels' or 'teacher'"):
+        api.quantize(src, output_dir=tmp_path / "q", device="cpu", sensitivity_objective="text")
+    assert not (tmp_path / "q").exists()
