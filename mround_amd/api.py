@@ -40,9 +40,9 @@ from mround_amd import kernels as K
 from mround_amd.planner import memory as M
 from mround_amd.planner.allocator import allocate_bits
 from mround_amd.planner.timing import predict_run_time
-from mround_amd.planner.sensitivity import (SENSITIVITY_SAMPLES, SENSITIVITY_SEQ_LEN, gradient_source_for,
-                                            mixed_budget_bits, score_layer_options, scoring_batch_size,
-                                            storage_bits)
+from mround_amd.planner.sensitivity import (SENSITIVITY_SAMPLES, SENSITIVITY_SEQ_LEN, SENSITIVITY_TEACHER_TOP,
+                                            gradient_source_for, mixed_budget_bits, score_layer_options,
+                                            scoring_batch_size, storage_bits)
 from mround_amd.schemes import (LOW_BIT_THRESHOLD, QuantScheme, ScaleInit, Symmetry,
                                 TuningConfig)
 
@@ -407,7 +407,8 @@ def _read_config(model: str | Path) -> dict[str, Any]:
 
 def _run_shape(config, resolved: QuantScheme, tuning: TuningConfig, *, average_bits, plan, widths,
                gradient_source, scoring_samples, scoring_seq_len, scoring_batch, dense_remainder,
-               quantized_inputs, holdout_batches=0, split_precision=False) -> tuple[M.ModelShape, M.RunShape]:
+               quantized_inputs, holdout_batches=0, split_precision=False,
+               objective="labels") -> tuple[M.ModelShape, M.RunShape]:
     shape = M.ModelShape.from_config(config)
     mixed = average_bits is not None and plan is None
     samples = SENSITIVITY_SAMPLES if scoring_samples is None else int(scoring_samples)
@@ -419,7 +420,8 @@ def _run_shape(config, resolved: QuantScheme, tuning: TuningConfig, *, average_b
                      group_size=resolved.group_size, searched=resolved.scale_init is ScaleInit.SEARCHED,
                      quantized_inputs=quantized_inputs, mixed=mixed, widths=len(widths),
                      gradient_source=source, scoring_samples=samples, scoring_seq_len=sequence,
-                     scoring_batch=batch, dense_remainder=dense_remainder, holdout_batches=holdout_batches,
+                     scoring_batch=batch, teacher_top=SENSITIVITY_TEACHER_TOP if mixed and objective == "teacher" else 0,
+                     dense_remainder=dense_remainder, holdout_batches=holdout_batches,
                      micro_batches=tuning.micro_batches, half=str(config.get("torch_dtype")) == "float16",
                      split=bool(split_precision))
     return shape, run
@@ -468,11 +470,14 @@ def predict_memory(model: str | Path, *, bits: int = 4, group_size: int = 64,
                    tuning: TuningConfig | None = None, scale_init: ScaleInit | str | None = None,
                    quantized_inputs: bool = True, holdout_batches: int = 0,
                    memory_budget: int | None = None, device: str = "cuda",
-                   split_precision: bool | None = None) -> M.MemoryCheck:
+                   split_precision: bool | None = None,
+                   sensitivity_objective: str = "labels") -> M.MemoryCheck:
     """Predict the device memory of the run :func:`quantize` would make, and
     stop (mround/api.py:1088-1192). Reads ``config.json`` and nothing else.
     ``memory_budget`` defaults to 90 % of the device's memory;
-    ``split_precision`` follows :func:`quantize`'s rule."""
+    ``split_precision`` and ``sensitivity_objective`` follow :func:`quantize`'s
+    rules."""
+    _check_objective(sensitivity_objective, scored=average_bits is not None)
     config = _read_config(model)
     resolved, widths = _resolve_scheme(bits=bits, group_size=group_size, symmetry=symmetry,
                                        average_bits=average_bits, candidate_bits=candidate_bits,
@@ -486,7 +491,8 @@ def predict_memory(model: str | Path, *, bits: int = 4, group_size: int = 64,
                             gradient_source=sensitivity_gradients, scoring_samples=scoring_samples,
                             scoring_seq_len=scoring_seq_len, scoring_batch=scoring_batch_size,
                             dense_remainder=dense_remainder, quantized_inputs=quantized_inputs,
-                            holdout_batches=holdout_batches, split_precision=split_precision)
+                            holdout_batches=holdout_batches, split_precision=split_precision,
+                            objective=sensitivity_objective)
     budget = M.default_budget(device) if memory_budget is None else memory_budget
     return M.check_memory(shape, run, budget=budget)
 
@@ -498,11 +504,12 @@ def predict_time(model: str | Path, *, bits: int = 4, group_size: int = 64,
                  scoring_seq_len: int | None = None, scheme: QuantScheme | None = None,
                  tuning: TuningConfig | None = None, scale_init: ScaleInit | str | None = None,
                  per_layer_recipe: bool = False, holdout_batches: int = 0,
-                 split_precision: bool | None = None):
+                 split_precision: bool | None = None, sensitivity_objective: str = "labels"):
     """Predict the seconds the run :func:`quantize` would make takes on one
     MI355X (``mround_amd.planner.timing``), from ``config.json`` alone
-    (mround/cli/main.py:590-624); ``split_precision`` follows
-    :func:`quantize`'s rule."""
+    (mround/cli/main.py:590-624); ``split_precision`` and
+    ``sensitivity_objective`` follow :func:`quantize`'s rules."""
+    _check_objective(sensitivity_objective, scored=average_bits is not None)
     config = _read_config(model)
     resolved, widths = _resolve_scheme(bits=bits, group_size=group_size, symmetry=symmetry,
                                        average_bits=average_bits, candidate_bits=candidate_bits,
@@ -516,7 +523,7 @@ def predict_time(model: str | Path, *, bits: int = 4, group_size: int = 64,
                             gradient_source=sensitivity_gradients, scoring_samples=scoring_samples,
                             scoring_seq_len=scoring_seq_len, scoring_batch=None, dense_remainder=False,
                             quantized_inputs=True, holdout_batches=holdout_batches,
-                            split_precision=split_precision)
+                            split_precision=split_precision, objective=sensitivity_objective)
     return predict_run_time(shape, run, tuning, resolved.bits,
                             candidate_bits=candidate_bits if average_bits is not None else (),
                             per_layer_recipe=per_layer_recipe, scoring_samples=scoring_samples,
@@ -626,7 +633,8 @@ def quantize(model: str | Path, *, output_dir: str | Path, bits: int = 4, group_
                                 gradient_source=sensitivity_gradients, scoring_samples=scoring_samples,
                                 scoring_seq_len=scoring_seq_len, scoring_batch=scoring_batch_size,
                                 dense_remainder=dense_remainder, quantized_inputs=quantized_inputs,
-                                holdout_batches=holdout_batches, split_precision=split_precision)
+                                holdout_batches=holdout_batches, split_precision=split_precision,
+                                objective=sensitivity_objective)
     budget = M.default_budget(device) if memory_budget is None else memory_budget
     memory = M.check_memory(mshape, rshape, budget=budget)
     if memory_check:

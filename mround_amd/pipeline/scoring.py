@@ -34,6 +34,7 @@ from mround_amd.core.quantizer import mode_of
 from mround_amd.core.scale_search import search_scales
 from mround_amd.pipeline.block import LAYERS, placements
 from mround_amd.pipeline.causal_lm import CausalLM
+from mround_amd.planner.sensitivity import SENSITIVITY_TEACHER_TOP
 from mround_amd.schemes import DEFAULT_EPS_FP32, QuantScheme, ScaleInit
 
 __all__ = ["ScoringProgress", "SensitivityScores", "eligible_block_layers", "score_widths"]
@@ -132,7 +133,7 @@ def _grids(eligible, scheme: QuantScheme) -> dict[str, torch.Tensor]:
 def score_widths(model, batches: Sequence[torch.Tensor], widths: Sequence[int], base_scheme: QuantScheme,
                  *, eps: float = DEFAULT_EPS_FP32, gradient_source: str = "own_width",
                  progress: Callable[[ScoringProgress], None] | None = None,
-                 keep_activations: bool | None = None, objective: str = "labels", teacher_top: int = 64,
+                 keep_activations: bool | None = None, objective: str = "labels", teacher_top: int = SENSITIVITY_TEACHER_TOP,
                  temperature: float = 1.0) -> SensitivityScores:
     """Score every block layer at every candidate width
     (mround/pipeline/scoring.py:425-583).

@@ -168,6 +168,7 @@ class RunShape:
     scoring_samples: int = 128
     scoring_seq_len: int = 1024
     scoring_batch: int = 2
+    teacher_top: int = 0  # tokens of a teacher's lists, kept for every scoring batch (0: no teacher)
     dense_remainder: bool = False
     holdout_batches: int = 0
     micro_batches: int = 1
@@ -232,6 +233,10 @@ def predict_memory(m: ModelShape, run: RunShape) -> MemoryPrediction:
             per_width = L * _groups(m, run.group_size) * 4
             grids = per_width * (run.widths if run.gradient_source == "widest" else 1)
         tokens = run.scoring_samples * run.scoring_seq_len * 8
+        if run.teacher_top:  # logits, ids and a log-sum-exp a row, and a copy of the tokens
+            batches = -(-run.scoring_samples // run.scoring_batch)
+            lm += (batches * T * (min(run.teacher_top, m.vocab) * 8 + 4)
+                   + run.scoring_samples * run.scoring_seq_len * 4)
         stages["scoring"] = base + lm + grids + tokens + run.n_samples * run.seq_len * 8
     S = aligned_rows(run.seq_len)  # rows per sequence in the streams and the engine
     T = run.batch_size * S

@@ -32,7 +32,8 @@ targets pass is one more forward over the calibration batches. **A mixed
 run's scoring pass** is a fixed part, a part per block and per block weight,
 and the head (vocabulary x hidden, twice if untied), times 2.74 with a
 backward at each width (``own_width``); it scales with the scoring tokens
-(measured at 128 x 1024).
+(measured at 128 x 1024). A teacher's lists are one more forward over them,
+whatever the widths.
 
 Every run records the prediction beside what it measured.
 
@@ -69,6 +70,9 @@ _SEARCH = (1.433e-02, 4.461e-10)                 # per block: fixed, per block w
 _COMMIT = 5.0e-4                                # per block
 _SCORING = (9.884e-02, 3.352e-02, 8.995e-10, 1.236e-10)  # fixed, per block, per block weight, per head weight
 _OWN_WIDTH = 2.76
+# A teacher's lists, of the pass with one backward a batch: 0.24, 0.28 and 0.26 of
+# it at the 135M, 0.5B and 3B shapes (0.74, 1.00 and 3.56 s without them).
+_TEACHER = 0.26
 _SCORING_TOKENS = SENSITIVITY_SAMPLES * SENSITIVITY_SEQ_LEN
 
 def _duration(seconds: float) -> str:
@@ -185,7 +189,8 @@ def predict_time(model: ModelShape, run: RunShape, *, iters: int, outlier_rule: 
         head = model.vocab * model.hidden * (1 if model.tied else 2)
         seconds = (_SCORING[0] + _SCORING[1] * model.layers + _SCORING[2] * model.layers * model.block_weights
                    + _SCORING[3] * head) * tokens / _SCORING_TOKENS
-        stages["scoring"] = seconds * (_OWN_WIDTH if source == "own_width" else 1.0)
+        stages["scoring"] = seconds * ((_OWN_WIDTH if source == "own_width" else 1.0)
+                                       + (_TEACHER if run.teacher_top else 0.0))
     stages["blocks"] = block * model.layers
     stages["between_blocks"] = batches * forward * model.layers
     return TimePrediction(stages=stages, block=block, blocks=model.layers, iters=iters, outlier_rule=outlier_rule,

@@ -43,3 +43,17 @@ def test_prediction_bounds_the_measured_peak(tmp_path, mixed, quantized_inputs, 
           file=sys.stderr)
     assert rec["peak_stage"] == ("scoring" if mixed else "blocks")
     assert 0.85 * predicted <= measured <= 1.05 * predicted
+
+
+def test_prediction_bounds_a_pass_by_the_teacher(tmp_path):
+    """The lists of 65 scoring batches, the last one not full, beside the small model's engine."""
+    print("case memory teacher", flush=True, file=sys.stderr)
+    src = write_random_checkpoint(tmp_path / "m", SMALL, seed=1)
+    res = api.quantize(src, output_dir=tmp_path / "q", bits=4, symmetry=Symmetry.ASYMMETRIC, seed=2, average_bits=3.0,
+                       candidate_bits=(2, 4), tuning=TuningConfig(iters=2, batch_size=4, n_samples=8, seq_len=256),
+                       scoring_samples=129, scoring_seq_len=1025, scoring_batch_size=2, sensitivity_objective="teacher")
+    rec = json.loads(res.config_path.read_text())
+    memory, predicted = rec["memory"], rec["memory"]["peak"]
+    print(f"  predicted {predicted} measured {memory['peak_allocated']}", file=sys.stderr)
+    assert rec["mixed"]["objective"] == "teacher" and memory["peak_stage"] == "scoring"
+    assert 0.85 * predicted <= memory["peak_allocated"] <= 1.05 * predicted

@@ -227,3 +227,34 @@ def test_split_precision_follows_the_tuned_widths(tmp_path):
     assert api._tuned_widths(scheme, None, (2, 3, 4), None) == (4,)
     assert api._tuned_widths(scheme, 3.0, (2, 3, 4), None) == (2, 3, 4)
     assert api._tuned_widths(scheme, 3.0, (2, 3, 4, 8), {"a": 2, "b": 8}) == (2, 8)
+
+
+def test_a_teachers_lists_are_counted(tmp_path):
+    """Every scoring batch's list (rows of the engine, a batch that is not full too) and the copies of the tokens
+    are on the device through the pass."""
+    write_random_checkpoint(tmp_path / "m", TINY)
+    model = load_model(tmp_path / "m", device="cpu")
+    lm = CausalLM(model, batch=2, seq_len=200, device="cpu", keep_activations=True)
+    m = M.ModelShape.from_config(TINY)
+    kw = dict(n_samples=2, seq_len=128, batch_size=2, group_size=64, mixed=True, widths=2, scoring_samples=5,
+              scoring_seq_len=200, scoring_batch=2)
+    for top, k in ((64, 64), (1000, 250)):
+        extra = (M.predict_memory(m, M.RunShape(**kw, teacher_top=top)).stages["scoring"]
+                 - M.predict_memory(m, M.RunShape(**kw)).stages["scoring"])
+        assert extra == 3 * lm.tokens * (k * 4 + k * 4 + 4) + 5 * 200 * 4
+
+
+def test_predictions_follow_the_objective(tmp_path):
+    from mround_amd.exceptions import SchemeError
+
+    write_random_checkpoint(tmp_path / "m", TINY)
+    kw = dict(average_bits=3, candidate_bits=(2, 4))
+    for predict, of in ((lambda **k: api.predict_memory(tmp_path / "m", device="cpu", memory_budget=10 ** 12, **k),
+                         lambda p: p.prediction.stages), (lambda **k: api.predict_time(tmp_path / "m", **k), lambda p: p.stages)):
+        plain, taught = of(predict(**kw)), of(predict(**kw, sensitivity_objective="teacher"))
+        assert taught["scoring"] > plain["scoring"]
+        assert {k: v for k, v in taught.items() if k != "scoring"} == {k: v for k, v in plain.items() if k != "scoring"}
+        with pytest.raises(SchemeError, match="scoring pass"):
+            predict(sensitivity_objective="teacher")
+        with pytest.raises(SchemeError, match="must be"):
+            predict(**kw, sensitivity_objective="text")

@@ -151,3 +151,22 @@ def test_api_reads_the_config_alone(tmp_path):
     assert 28 * 3.9 < p.stages["blocks"] < 28 * 4.5
     mixed = api.predict_time(tmp_path, average_bits=2.5)
     assert mixed.scoring_source == "own_width" and mixed.stages["scoring"] > 0
+
+
+# geometry, seconds of the scoring pass over 64 batches of 2 x 1024 tokens on one MI355X: one backward a batch by
+# the labels and by the teacher, a backward at each of three widths by the labels and by the teacher
+TAUGHT = [("smollm2-135m", 0.735, 0.911, 2.080, 2.253), ("qwen2.5-0.5b", 0.996, 1.280, 2.784, 3.064),
+          ("qwen2.5-3b", 3.555, 4.486, 9.614, 10.563)]
+
+
+@pytest.mark.parametrize("r", TAUGHT, ids=lambda r: r[0])
+def test_a_teachers_lists_are_a_forward_more(r):
+    """What the teacher adds is a share of the pass with one backward, whatever the widths: the rule's share within a
+    twelfth of every measured one."""
+    geo, widest, widest_taught, own, own_taught = r
+    model = _shape(geo)
+    plain, taught = (RunShape(128, 2048, 8, 64, mixed=True, teacher_top=t) for t in (0, 64))
+    for source, had, has in (("widest", widest, widest_taught), ("own_width", own, own_taught)):
+        p = TM.predict_time(model, plain, iters=200, outlier_rule=False, scoring_source=source).stages["scoring"]
+        q = TM.predict_time(model, taught, iters=200, outlier_rule=False, scoring_source=source).stages["scoring"]
+        assert q / p == pytest.approx(has / had, rel=0.04)
