@@ -41,6 +41,9 @@ def _parser() -> argparse.ArgumentParser:
                    help="candidate widths for --average-bits, comma separated (default: 2,3,4)")
     q.add_argument("--remainder-bits", type=int, default=None,
                    help="width for the tensors outside the block stack (default: nearest the average)")
+    q.add_argument("--objective", default="labels", choices=("labels", "teacher"),
+                   help="what --average-bits scores with: the cross-entropy of the tokens, or the divergence from "
+                        "the unquantized model's own predictions")
     q.add_argument("--plan", default=None, help="JSON file mapping layer paths to widths")
     q.add_argument("--format", default="mlx")
     q.add_argument("--iters", type=int, default=None)
@@ -151,14 +154,14 @@ def main(argv=None) -> int:
                 symmetry=Symmetry.ASYMMETRIC if args.asym else Symmetry.SYMMETRIC,
                 average_bits=args.average_bits, candidate_bits=_widths(args.options),
                 remainder_bits=args.remainder_bits, tuning=_tuning(args), memory_budget=budget,
-                split_precision=args.split_precision)
+                split_precision=args.split_precision, sensitivity_objective=args.objective)
             print(f"  {check.explain()}")
             timing = api.predict_time(
                 args.model, bits=args.bits, group_size=args.group_size,
                 symmetry=Symmetry.ASYMMETRIC if args.asym else Symmetry.SYMMETRIC,
                 average_bits=args.average_bits, candidate_bits=_widths(args.options),
                 remainder_bits=args.remainder_bits, tuning=_tuning(args),
-                split_precision=args.split_precision)
+                split_precision=args.split_precision, sensitivity_objective=args.objective)
             print(f"  {timing.describe()}")
             return 0 if check.fits else 1
         plan = None
@@ -171,6 +174,7 @@ def main(argv=None) -> int:
                               average_bits=args.average_bits, candidate_bits=_widths(args.options),
                               remainder_bits=args.remainder_bits, plan=plan, tuning=_tuning(args),
                               calibration=args.calibration, export_format=args.format,
+                              sensitivity_objective=args.objective,
                               min_block_coverage=0.0 if args.allow_dense else api.MIN_BLOCK_COVERAGE,
                               split_precision=args.split_precision, seed=args.seed, memory_budget=budget,
                               memory_check=not args.skip_memory_check,

@@ -438,3 +438,34 @@ def test_an_objective_without_a_scoring_pass_is_refused(tmp_path):
     with pytest.raises(SchemeError, match="must be 'labels' or 'teacher'"):
         api.quantize(src, output_dir=tmp_path / "q", device="cpu", sensitivity_objective="text")
     assert not (tmp_path / "q").exists()
+
+
+def _small(tmp_path, device, **form):
+    cfg = dict(BASE, hidden_size=128, num_attention_heads=2, num_key_value_heads=1, head_dim=64, intermediate_size=256,
+               num_hidden_layers=1, vocab_size=200, rms_norm_eps=1e-6, tie_word_embeddings=True, torch_dtype="bfloat16", **form)
+    return str(write_random_checkpoint(tmp_path / "m", cfg, seed=2, std=0.05, device=device))
+
+
+def test_the_command_asks_for_an_objective(tmp_path, capsys):
+    from mround_amd.cli import main
+
+    src, out = _small(tmp_path, "cpu"), str(tmp_path / "q")
+    dry = ["quantize", src, "-o", out, "--dry-run", "--memory-budget", "100"]
+    said = []
+    for objective in ("labels", "teacher"):
+        assert main([*dry, "--average-bits", "3", "--objective", objective]) == 0
+        said.append(capsys.readouterr().out.split("scoring ")[1].split(" ")[0])
+    assert said[0] != said[1]  # (the teacher's lists)
+    assert main([*dry, "--objective", "teacher"]) == 1
+    assert "scoring pass" in capsys.readouterr().err
+
+
+@pytest.mark.gpu
+def test_the_command_quantizes_by_the_teacher(tmp_path):
+    from mround_amd.cli import main
+
+    src, out = _small(tmp_path, dev()), tmp_path / "q"
+    assert main(["quantize", src, "-o", str(out), "--asym", "--average-bits", "3", "--options", "2,4", "--objective",
+                 "teacher", "--iters", "4", "--samples", "4", "--seq-len", "100", "--batch-size", "2"]) == 0
+    record = json.loads((out / api.RUN_RECORD).read_text())
+    assert record["mixed"]["objective"] == "teacher" and record["mixed"]["source"] == "scored"
