@@ -26,6 +26,8 @@ void clear_error();
   } while (0)
 
 inline bool valid_dtype(int dt) { return dt == MR_F32 || dt == MR_BF16 || dt == MR_F16; }
+// A launch's threads are counted in 32 bits.
+inline bool too_many_blocks(int64_t blocks, int threads) { return blocks > 0xffffffffll / threads; }
 inline int dtype_bytes(int dt) { return dt == MR_F32 ? 4 : 2; }
 
 __device__ __forceinline__ float bf16_to_f32(uint16_t h) {

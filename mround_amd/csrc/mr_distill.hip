@@ -1213,10 +1213,13 @@ int mr_top_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t 
   // Short rows by blocks of 256 threads, eight to a CU, longer ones by four of 512,
   // where these have maxima enough for lists of k: 2044 rows of 20000 bf16 logits 67 us
   // by 1024 threads, 38 by 512, 32 by 256; of 50304 78, 51, 57; of 151936 144, 138, 163.
+  const int threads = V <= 24576 && k <= 256 ? 256 : k <= 512 ? 512 : 1024;
+  if (too_many_blocks(T, threads)) return fail(MR_EINVAL, "mr_top_logits: too large, a launch takes %lld such rows",
+                                               0xffffffffll / threads);
 #define MR_TOP(DT)                                                                                          \
   do {                                                                                                      \
-    if (V <= 24576 && k <= 256) hipLaunchKernelGGL((top_rows<DT, 256>), g, dim3(256), 0, s, p);              \
-    else if (k <= 512) hipLaunchKernelGGL((top_rows<DT, 512>), g, dim3(512), 0, s, p);                       \
+    if (threads == 256) hipLaunchKernelGGL((top_rows<DT, 256>), g, dim3(256), 0, s, p);                      \
+    else if (threads == 512) hipLaunchKernelGGL((top_rows<DT, 512>), g, dim3(512), 0, s, p);                 \
     else hipLaunchKernelGGL((top_rows<DT, 1024>), g, dim3(1024), 0, s, p);                                   \
   } while (0)
   if (dtype == MR_BF16) MR_TOP(MR_BF16);
@@ -1276,13 +1279,18 @@ int mr_distill(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, 
     const int64_t pieces = (V * es + 15) / 16;
     // what 7 pieces a thread and the block's sums leave of half a CU's LDS
     constexpr size_t kTwoRows = 81920 - 512 * 7 * 16 - 2048;
-#define MR_DISTILL(DT, THREADS, N, M, R) hipLaunchKernelGGL((distill_held<DT, THREADS, N, M, R>), g, dim3(THREADS), lds, s, p)
+#define MR_ROWS(KERNEL, THREADS)                                                                              \
+  do {                                                                                                       \
+    if (too_many_blocks(T, THREADS))                                                                         \
+      return fail(MR_EINVAL, "mr_distill: too many rows, a launch takes %lld", 0xffffffffll / (THREADS));     \
+    hipLaunchKernelGGL(KERNEL, g, dim3(THREADS), lds, s, p);                                                  \
+  } while (0)
+#define MR_DISTILL(DT, THREADS, N, M, R) MR_ROWS((distill_held<DT, THREADS, N, M, R>), THREADS)
     // The fewest threads that hold the row in at most 8 pieces each, then more pieces,
     // some of them in LDS, then some read twice, as long as two rows fit a CU;
     // the loss alone by small blocks where there are rows for eight of them a CU and
     // room for their bitmaps; a row that is read twice by the whole of half a CU
-#define MR_STREAM(DT, THREADS, GRAD) \
-  hipLaunchKernelGGL((distill_stream<DT, THREADS, GRAD>), g, dim3(THREADS), lds, s, p)
+#define MR_STREAM(DT, THREADS, GRAD) MR_ROWS((distill_stream<DT, THREADS, GRAD>), THREADS)
 #define MR_DISTILL_D(DT)                                                                                 \
   do {                                                                                                   \
     if (V * es < 16 || (!dlogits && pieces > 256 * 8)) {                                                   \
@@ -1307,6 +1315,7 @@ int mr_distill(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, 
 #undef MR_DISTILL_D
 #undef MR_STREAM
 #undef MR_DISTILL
+#undef MR_ROWS
     MR_LAUNCH_CHECK("mr_distill");
   }
   if (loss_out) {

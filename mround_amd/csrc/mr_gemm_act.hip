@@ -98,6 +98,7 @@ int add_bias_gradient(const char* fn, const float* partials, int64_t M, int64_t 
 // What both backward entry points ask of dbias and its partial sums.
 int check_bias_gradient(const char* fn, int64_t M, int64_t N, const float* dbias, const float* partials, size_t bytes) {
   if (!dbias) return MR_OK;
+  if (too_many_blocks((N + 63) / 64, 1024)) return fail(MR_EINVAL, "%s: too large, N=%lld", fn, static_cast<long long>(N));
   if (!partials || static_cast<int64_t>(bytes) < partial_bytes(M, N))
     return fail(MR_EINVAL, "%s: dbias needs %lld bytes of partials", fn, static_cast<long long>(partial_bytes(M, N)));
   if (!aligned16(partials) || reinterpret_cast<uintptr_t>(dbias) % 4)

@@ -303,6 +303,8 @@ int mr_rope_positions(const void* x, int dtype, int64_t ldx, int64_t T, int n_he
   const int64_t even = T / 1024;
   if (tokens > even) tokens = even > 0 ? even : 1;
   p.tokens = static_cast<int>(tokens);
+  if (too_many_blocks((T + tokens - 1) / tokens, kRopeBlock))
+    return fail(MR_EINVAL, "mr_rope_positions: too many rows, a launch takes %lld", 0xffffffffll / kRopeBlock * tokens);
   const dim3 grid(static_cast<unsigned>((T + tokens - 1) / tokens)), block(kRopeBlock);
   const size_t lds = static_cast<size_t>(tokens) * p.pairs * sizeof(float2);
   hipStream_t s = static_cast<hipStream_t>(stream);

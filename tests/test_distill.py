@@ -711,3 +711,22 @@ def test_top_logits_far_from_zero(size, dtype, V):
             assert torch.equal(lse.cpu(), ref[over].float())
         if not bool(over.all()):
             check_top(z[~over], k, temperature)
+
+
+def test_rows_past_a_launch_are_refused_before_it():
+    """A block a row: blocks times threads is a 32-bit number. Every size of block, at the first row too many."""
+    lib, P, f = K.lib(), ctypes.c_void_p, ctypes.c_float
+    far = lambda n: P(n << 50)
+
+    for V, k, threads in ((8, 2, 256), (24576, 256, 256), (24577, 3, 512), (300, 257, 512), (2000, 513, 1024)):
+        T = (1 << 32) // threads
+        assert lib.mr_top_logits(far(1), 1, V, T, V, k, ctypes.c_double(1.0), far(2), far(3), far(4), None) == -22
+        assert b"too large" in lib.mr_last_error() and str(T - 1).encode() in lib.mr_last_error()
+    # (elements, gradient, threads): short rows, held ones, rows read twice, the loss alone
+    for V, grad, threads in ((2, True, 1024), (300, True, 256), (300, False, 256), (9000, True, 512), (16000, True, 512),
+                             (80000, True, 512), (82000, True, 1024), (20000, False, 256), (200000, False, 512),
+                             (1000000, False, 1024)):
+        T = (1 << 32) // threads
+        assert lib.mr_distill(far(1), 0, V, T, V, far(2), far(3), 2, far(4), ctypes.c_double(1.0), f(1.0), far(5), far(6),
+                              far(7) if grad else None, V, None) == -22, (V, grad)
+        assert b"too many rows" in lib.mr_last_error() and str(T - 1).encode() in lib.mr_last_error(), (V, grad)

@@ -361,3 +361,11 @@ def test_bindings_refuse_on_the_host():
         K.gemm_act_bwd(x, w.t().contiguous(), out.float(), out, act="silu")
     with pytest.raises(KernelError, match="dbias"):
         K.act_bwd(out.float(), out, out, act="silu", dbias=torch.zeros(3, device="cpu"))
+
+
+def test_columns_past_a_launch_are_refused_before_it():
+    """The bias gradient's sum takes 1024 threads for 64 columns, and a launch's threads are a 32-bit number."""
+    lib, N = K.lib(), 1 << 28
+    far = lambda n: P(n << 50)
+    assert lib.mr_act_bwd(1, N, far(1), 0, N, far(2), N, 0, far(3), N, far(4), far(5), ctypes.c_size_t(4 * N), None) == -22
+    assert b"large" in lib.mr_last_error()

@@ -215,3 +215,15 @@ def test_binding_refuses_on_the_host():
         K.rope_positions(x, pos, freq, out=x.half(), **kw)
     with pytest.raises(KernelError, match="ROCm device"):
         K.rope_positions(x, pos, freq, **kw)
+
+
+def test_rows_past_a_launch_are_refused_before_it():
+    """A block takes some tokens, and blocks times threads is a 32-bit number: the first row too many of each kind."""
+    lib, P = K.lib(), ctypes.c_void_p
+    for d, tokens in ((4096, 1), (128, 4), (2, 256)):
+        T = (((1 << 32) - 1) // 256) * tokens + 1
+        if T > 0x7fffffff:
+            T = 1 << 31
+        assert lib.mr_rope_positions(P(1 << 50), 1, d, T, 1, d, P(2 << 50), P(3 << 50), d, 0, ctypes.c_float(1.0), 0,
+                                     P(4 << 50), d, None) == -22, d
+        assert b"too many rows" in lib.mr_last_error()
