@@ -1242,7 +1242,7 @@ int mr_distill(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, 
   if (k < 1 || k > kMaxTop) return fail(MR_EINVAL, "mr_distill: k=%d must lie in [1, %d]", k, kMaxTop);
   if (!(temperature >= kMinTemperature && temperature <= kMaxTemperature))
     return fail(MR_EINVAL, "mr_distill: the temperature must lie in [1/1024, 1024]");
-  if (!row_loss || (T > 0 && (!logits || !top_values || !top_ids))) return fail(MR_EINVAL, "mr_distill: null pointer");
+  if (T > 0 && (!row_loss || !logits || !top_values || !top_ids)) return fail(MR_EINVAL, "mr_distill: null pointer");
   if (ld < V || (dlogits && ldd < V)) return fail(MR_EINVAL, "mr_distill: a leading dimension is smaller than V");
   if (T > 0x7fffffff) return fail(MR_EINVAL, "mr_distill: too many rows");
   const int es = dtype_bytes(dtype);

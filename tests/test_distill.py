@@ -730,3 +730,20 @@ def test_rows_past_a_launch_are_refused_before_it():
         assert lib.mr_distill(far(1), 0, V, T, V, far(2), far(3), 2, far(4), ctypes.c_double(1.0), f(1.0), far(5), far(6),
                               far(7) if grad else None, V, None) == -22, (V, grad)
         assert b"too many rows" in lib.mr_last_error() and str(T - 1).encode() in lib.mr_last_error(), (V, grad)
+
+
+def test_no_rows_have_no_addresses():
+    """Tensors without elements have none: with nothing to write, nothing is refused."""
+    lib, f = K.lib(), ctypes.c_float
+    assert lib.mr_distill(None, 0, 10, 0, 10, None, None, 3, None, ctypes.c_double(1.0), f(1.0), None, None, None, 0, None) == 0
+    assert lib.mr_top_logits(None, 0, 10, 0, 10, 3, ctypes.c_double(1.0), None, None, None, None) == 0
+    assert lib.mr_rope_positions(None, 0, 64, 0, 1, 64, None, None, 64, 0, f(1.0), 0, None, 64, None) == 0
+
+
+@pytest.mark.gpu
+def test_a_loss_of_no_rows():
+    e = lambda *s, dt=torch.float32: torch.empty(*s, dtype=dt, device=dev())
+    loss = torch.full((1,), 5.0, device=dev())
+    K.distill_loss(e(0, 10), e(0, 3), e(0, 3, dt=torch.int32), V=10, scale=1.0, row_loss=e(0), lse=e(0), loss_out=loss,
+                   dlogits=e(0, 10))
+    assert float(loss) == 0.0
