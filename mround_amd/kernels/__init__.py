@@ -213,7 +213,7 @@ def _ld(t: torch.Tensor | None) -> int:
     says nothing: torch leaves any value there."""
     if t is None:
         return 0
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _one_device(name: str, *tensors: torch.Tensor | None) -> None:

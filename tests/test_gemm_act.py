@@ -369,3 +369,29 @@ def test_columns_past_a_launch_are_refused_before_it():
     far = lambda n: P(n << 50)
     assert lib.mr_act_bwd(1, N, far(1), 0, N, far(2), N, 0, far(3), N, far(4), far(5), ctypes.c_size_t(4 * N), None) == -22
     assert b"large" in lib.mr_last_error()
+
+
+@pytest.mark.gpu
+def test_a_single_row_of_any_stride():
+    """A single row's stride leads nowhere: rows of odd, of huge and of no distance give what a row of its own gives."""
+    print("case act single row", file=sys.stderr, flush=True)
+    N, Kd, g = 64, 128, torch.Generator().manual_seed(4)
+    full = lambda n, dt: torch.randn(1, n, generator=g).to(dt).to(dev())
+    x, w, r, pre0 = full(Kd, BF), torch.randn(N, Kd, generator=g).to(BF).to(dev()), full(N, torch.float32), full(N, BF)
+    dd, wd = full(Kd, BF), torch.randn(Kd, N, generator=g).to(BF).to(dev())
+
+    def row(t, stride):  # the same values, and a stride of its own
+        return t.clone().as_strided(t.shape, (stride, 1))
+
+    def outputs(at):
+        out, pre = at(torch.zeros(1, N, device=dev())), at(torch.zeros(1, N, dtype=BF, device=dev()))
+        K.gemm_act(at(x), w, out, act="silu", pre=pre, resid=at(r))
+        d1, d2 = at(torch.zeros(1, N, dtype=BF, device=dev())), at(torch.zeros(1, N, dtype=BF, device=dev()))
+        K.gemm_act_bwd(at(dd), wd, at(pre0), d1, act="gelu")
+        K.act_bwd(at(r), at(pre0), d2, act="relu2")
+        return out, pre, d1, d2
+
+    want = outputs(lambda t: t.clone())
+    for stride in (0, 131, 1 << 30):
+        for got, ref in zip(outputs(lambda t: row(t, stride)), want):
+            assert torch.equal(got, ref), stride
