@@ -227,3 +227,16 @@ def test_rows_past_a_launch_are_refused_before_it():
         assert lib.mr_rope_positions(P(1 << 50), 1, d, T, 1, d, P(2 << 50), P(3 << 50), d, 0, ctypes.c_float(1.0), 0,
                                      P(4 << 50), d, None) == -22, d
         assert b"too many rows" in lib.mr_last_error()
+
+
+# rows enough for several tokens a block, the last block short of them, whole pieces of 16 bytes and not
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("case", [(4000, 16, 128, 64, 32, "interleaved"), (9001, 4, 0, 128, 64, "half"),
+                                  (2049, 2, 64, 64, 64, "half"), (4099, 3, 0, 64, 16, "half"),
+                                  (4099, 3, 0, 64, 16, "interleaved"), (3203, 2, 3, 80, 20, "half"),
+                                  (20001, 1, 0, 32, 32, "interleaved"), (300003, 1, 0, 16, 2, "half")],
+                         ids=lambda c: "x".join(map(str, c)))
+def test_blocks_of_several_tokens(case, backward, dtype):
+    test_rotation(case, backward, dtype)
