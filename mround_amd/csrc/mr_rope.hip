@@ -15,10 +15,19 @@
 // there: no table of positions is read or kept, at any length.
 //
 // Bound by memory: an element is read and written once. 16384 tokens of 32 bf16
-// heads of 128 take 50 us (268 MB, 5.4 TB/s; 57 us through the caches), 4000 of 16
-// float16 heads, 32 of 64 elements rotated, 6 us, and 8 tokens 3 us, where a call's own
-// 8 us on the host are what counts. A thread has 4 x 32 bytes on their way while the
-// angles are worked out.
+// heads of 128 take 50 us (268 MB, 5.4 TB/s), 4000 of 16 float16 heads, 32 of 64
+// elements rotated, 6 us, and 8 tokens 3 us, where a call's own 8 us on the host are
+// what counts. A thread has 4 x 32 bytes on their way while the angles are worked out.
+//
+// Loads and stores pass by the caches where another buffer receives whole heads whose
+// halves are whole cache lines (of 128 bytes): that call takes 50 us so and 58 through
+// the caches, of 65536 tokens 189 and 206. Elsewhere they do not. In place the product
+// that wrote the rows has left them there and attention reads them next: product,
+// rotation and attention of 16384 tokens of 16 + 2 heads of 128 (rows of 2560) took 325
+// us past the caches, and take 320; of neighbours 334 and 321; of 14 + 2 heads of 64 half
+// rotated 146 and 138. And neighbours or a head's rest, 32 bytes a thread, or halves
+// under a line are parts of lines, which the caches put together: 65536 tokens of
+// neighbours 302 us past them and 203 through them, of heads of 128 half rotated 275 and 213.
 #include "mr_common.h"
 
 namespace mr {
@@ -53,7 +62,7 @@ __device__ __forceinline__ uint4 ld16(const uint8_t* p) {
 }
 __device__ __forceinline__ void st16(uint8_t* p, uint4 v) { __builtin_memcpy(p, &v, 16); }
 
-// The same of 16-byte places.
+// The same of 16-byte places, past the caches.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint4 ld16s(const uint8_t* p) {
   const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
@@ -92,8 +101,9 @@ __device__ __forceinline__ uint4 narrow(const float (&v)[E]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// VEC: every rotated unit is whole and every unit starts on 16 bytes.
-template <int DT, bool HALF, bool BWD, bool VEC>
+// VEC: every rotated unit is whole and every unit starts on 16 bytes; PAST: and what
+// is moved passes by the caches.
+template <int DT, bool HALF, bool BWD, bool VEC, bool PAST>
 __global__ __launch_bounds__(kRopeBlock) void rope_any(RopeParams p) {
   constexpr int ES = DT == MR_F32 ? 4 : 2;  // bytes of an element
   constexpr int E = 16 / ES;                // pairs of a unit
@@ -139,7 +149,7 @@ __global__ __launch_bounds__(kRopeBlock) void rope_any(RopeParams p) {
   auto load = [&](const At& u) __attribute__((always_inline)) {
     const uint8_t* row = xb + static_cast<int64_t>(u.tok) * p.ldx * ES;
     Unit v{};
-    if (VEC && u.na == E && u.nb == E) {
+    if (PAST && u.na == E && u.nb == E) {
       v.a = ld16s(row + u.a * ES);
       v.b = ld16s(row + u.b * ES);
     } else if (u.na == E && u.nb == E) {
@@ -159,7 +169,7 @@ __global__ __launch_bounds__(kRopeBlock) void rope_any(RopeParams p) {
   };
   auto store = [&](const At& u, const Unit& v) __attribute__((always_inline)) {
     uint8_t* row = ob + static_cast<int64_t>(u.tok) * p.ldo * ES;
-    if (VEC && u.na == E && u.nb == E) {
+    if (PAST && u.na == E && u.nb == E) {
       st16s(row + u.a * ES, v.a);
       st16s(row + u.b * ES, v.b);
     } else if (u.na == E && u.nb == E) {
@@ -297,6 +307,7 @@ int mr_rope_positions(const void* x, int dtype, int64_t ldx, int64_t T, int n_he
   // whole rotated units, and pieces of 16 bytes on 16-byte addresses
   const bool vec = p.pairs % e == 0 && head_dim % e == 0 && (ldx * es) % 16 == 0 && (ldo * es) % 16 == 0 &&
                    aligned16(x) && aligned16(out);
+  const bool past = vec && half && !in_place && rotary_dim == head_dim && p.pairs * es % 128 == 0;
   // Tokens of a block: an angle for each of its threads, but blocks enough to
   // give every CU four, and 32 KB of angles at most.
   int64_t tokens = (kRopeBlock + p.pairs - 1) / p.pairs;
@@ -308,8 +319,13 @@ int mr_rope_positions(const void* x, int dtype, int64_t ldx, int64_t T, int n_he
   const dim3 grid(static_cast<unsigned>((T + tokens - 1) / tokens)), block(kRopeBlock);
   const size_t lds = static_cast<size_t>(tokens) * p.pairs * sizeof(float2);
   hipStream_t s = static_cast<hipStream_t>(stream);
-#define MR_ROPE(DT, HALF, BWD, VEC) hipLaunchKernelGGL((rope_any<DT, HALF, BWD, VEC>), grid, block, lds, s, p)
-#define MR_ROPE_V(DT, HALF, BWD) do { if (vec) MR_ROPE(DT, HALF, BWD, true); else MR_ROPE(DT, HALF, BWD, false); } while (0)
+#define MR_ROPE(DT, HALF, BWD, VEC, PAST) hipLaunchKernelGGL((rope_any<DT, HALF, BWD, VEC, PAST>), grid, block, lds, s, p)
+#define MR_ROPE_V(DT, HALF, BWD)                              \
+  do {                                                        \
+    if (HALF && past) MR_ROPE(DT, HALF, BWD, true, HALF);     \
+    else if (vec) MR_ROPE(DT, HALF, BWD, true, false);        \
+    else MR_ROPE(DT, HALF, BWD, false, false);                \
+  } while (0)
 #define MR_ROPE_D(DT)                                                                   \
   do {                                                                                  \
     if (half) { if (backward) MR_ROPE_V(DT, true, true); else MR_ROPE_V(DT, true, false); } \
