@@ -224,6 +224,18 @@ __device__ __forceinline__ T waves_sum(const T* v) {
 // values, whose exponents are no floats.
 constexpr float kMasked = -1e37f;
 
+// A sum and its mean's terms under a greater base. What was summed among masks far from zero can be infinite
+// (is_far), and times zero no number: nothing is left of it. NaN stays.
+__device__ __forceinline__ void rebase(float& s, float& ve, float& e, float f) {
+  if (f == 0.0f) {
+    if (s == s) s = 0.0f;
+    ve = e = 0.0f;
+  }
+  s *= f;
+  ve *= f;
+  e *= f;
+}
+
 // A running sum of exp(v / T), as s 2^base: base is max hi, so a term is one fused
 // multiply-add and the exponential, 2^(v hi - base). What hi lacks of log2(e) / T
 // comes back at the end, to first order, with the mean of v (from one in E of the terms).
@@ -238,9 +250,7 @@ struct RunningSum {
         // (a product past the floats is their end: an exponential above it overflows, as it should)
         const float grown = clampf(mx * c.hi, -kMaxFloat, kMaxFloat), f = max > kMasked ? __builtin_amdgcn_exp2f(base - grown) : 1.0f;
         base = grown;
-        s *= f;
-        ve *= f;
-        e *= f;
+        rebase(s, ve, e, f);
       }
       max = mx;
     }
@@ -273,9 +283,10 @@ struct RunningSum {
   __device__ __forceinline__ void publish(Shared<W>& sh) {
     const float about = wave_max(max > kMasked ? base : -kInf), f = max > kMasked ? __builtin_amdgcn_exp2f(base - about) : 1.0f;
     max = wave_max(max);
-    s = wave_sum(s * f);
-    ve = wave_sum(ve * f);
-    e = wave_sum(e * f);
+    rebase(s, ve, e, f);
+    s = wave_sum(s);
+    ve = wave_sum(ve);
+    e = wave_sum(e);
     if ((threadIdx.x & 63) == 0) {
       const int w = threadIdx.x >> 6;
       sh.max[w] = max;
@@ -296,8 +307,9 @@ struct BlockSum {
     const int w = threadIdx.x % W;
     max = waves_max<W>(sh.max);
     const float about = waves_max<W>(sh.base), f = sh.base[w] == -kInf ? 1.0f : __builtin_amdgcn_exp2f(sh.base[w] - about);
-    sum = static_cast<double>(sh.s[w] * f);
-    float v = sh.ve[w] * f, n = sh.e[w] * f;
+    float s = sh.s[w], v = sh.ve[w], n = sh.e[w];
+    rebase(s, v, n, f);
+    sum = static_cast<double>(s);
     for (int off = W / 2; off > 0; off >>= 1) {
       sum += __shfl_xor(sum, off, 64);
       v += __shfl_xor(v, off, 64);

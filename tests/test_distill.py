@@ -747,3 +747,35 @@ def test_a_loss_of_no_rows():
     K.distill_loss(e(0, 10), e(0, 3), e(0, 3, dt=torch.int32), V=10, scale=1.0, row_loss=e(0), lse=e(0), loss_out=loss,
                    dlogits=e(0, 10))
     assert float(loss) == 0.0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [300, 9000, 40001, 151936, 200003])
+@pytest.mark.parametrize("mask,dtype", [(m, t) for t in ("bf16", "f32") for m in (-1e6, -1e9, -1e10, -3e10, -1e12, -1e20, -1e30, -1e36)]
+                         + [(-1e4, "f16"), (-65504.0, "f16")])
+def test_masks_that_are_numbers(mask, dtype, V):
+    """A large negative number in the place of minus infinity, at either end of a row, in most of its pieces and in
+    nearly all: sums that began among the masks go on with what follows, and a NaN among them stays."""
+    T, k = 6, 8
+    z, values, ids, teacher = make(T, V, k, dtype, seed=V + 5)
+    listed = torch.zeros(T, V, dtype=torch.bool).scatter_(1, ids.long(), True)
+    out = torch.zeros(T, V, dtype=torch.bool)
+    out[0, : V // 2] = out[1, V // 2:] = True
+    out[2] = torch.rand(V, generator=torch.Generator().manual_seed(3)) < 0.9
+    out[3, : V - 9] = out[4, 9:] = True
+    z = torch.where(out, torch.full_like(z, mask), z)
+    for temperature in (0.7, 1.0, 2.0, 3.1):
+        check_top(z, k, temperature)
+        lse = torch.logsumexp(teacher.double() / temperature, 1).float()
+        zl = torch.where(listed, teacher.to(z.dtype), z)  # (no listed logit masked: a loss of 1e30 would hide the rest)
+        for tail in (lse, None):
+            check(zl, values, ids, scale=256.0 if dtype == "f16" else 0.37, lse=tail, temperature=temperature)
+    with_nan = z.clone()
+    with_nan[0, 1] = with_nan[1, V - 2] = with_nan[3, 2] = math.nan
+    values_, ids_, lse_ = run_top(with_nan.to(dev()), V, k)
+    assert torch.isnan(lse_.cpu()).tolist() == [True, True, False, True, False, False]
+    assert ids_[0, 0] == 1 and ids_[1, 0] == V - 2 and ids_[3, 0] == 2
+    zl = torch.where(listed, teacher.to(z.dtype), with_nan)
+    for grad in (True, False):
+        row, _, _ = run(zl, values, ids, scale=1.0, grad=grad)
+        assert torch.equal(torch.isnan(row.cpu()), torch.isnan(zl).any(1))
