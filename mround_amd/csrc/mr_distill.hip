@@ -236,6 +236,16 @@ __device__ __forceinline__ void rebase(float& s, float& ve, float& e, float f) {
   e *= f;
 }
 
+// The mean of v over a sum's terms, from one in E of them: v_e their sum of v, e of their
+// terms. Where they have under half of their share of the sum, peaks lie among the
+// others, and what these have too much lies at `peak`. (By the mean of the rest alone a
+// peak 80 above it left the sum's logarithm 4e-6 off.)
+template <int E>
+__device__ __forceinline__ float mean_logit(float sum, float v_e, float e, float peak) {
+  const float more = sum - E * e;
+  return more > 0.5f * sum ? (E * v_e + more * peak) / (E * e + more) : v_e / e;
+}
+
 // A running sum of exp(v / T), as s 2^base: base is max hi, so a term is one fused
 // multiply-add and the exponential, 2^(v hi - base). What hi lacks of log2(e) / T
 // comes back at the end, to first order, with the mean of v (from one in E of the terms).
@@ -299,7 +309,7 @@ struct RunningSum {
 };
 
 // The block's sum: sum 2^exponent, and the maximum, on every thread.
-template <int W>
+template <int W, int E>
 struct BlockSum {
   double sum, exponent;
   float max;
@@ -316,7 +326,7 @@ struct BlockSum {
       n += __shfl_xor(n, off, 64);
     }
     // (far from zero the mean of v, which ends at -1e30, is the maximum to a few steps of 2^-24)
-    const float mean = n > 0.0f && v < kInf && v > -kInf && !is_far(max, c) ? v / n : max;
+    const float mean = n > 0.0f && v < kInf && v > -kInf && !is_far(max, c) ? mean_logit<E>(static_cast<float>(sum), v, n, max) : max;
     exponent = about == -kInf ? 0.0 : static_cast<double>(about) + static_cast<double>(c.lo) * mean;
   }
 };
@@ -405,7 +415,7 @@ __global__ __launch_bounds__(THREADS, 8) void top_rows(TopParams p) {
   __syncthreads();
   bool odd;  // a NaN, an infinity, or no logit above the masks' values
   {
-    const BlockSum<W> all(s_sum, p.c);
+    const BlockSum<W, E> all(s_sum, p.c);
     odd = !(all.sum > 0.0 && all.sum < static_cast<double>(kInf) && all.max < kInf);
     // (odd: the maximum alone; a NaN is the list's first entry, which tells)
     if (tid == 0 && p.lse)
@@ -1026,11 +1036,14 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   // What the row comes to, from the block's sums (a wave or all).
   auto row_sums = [&]() __attribute__((always_inline)) {
     const double lo = static_cast<double>(p.c.lo);
-    const float v = waves_sum<W>(s_ve), e = waves_sum<W>(s_e);
+    const float v = uniform(waves_sum<W>(s_ve)), e = uniform(waves_sum<W>(s_e));
     l.finish(s);
-    return RowSums(p, l, waves_sum<W>(s.rest),
+    const double rest = waves_sum<W>(s.rest);
+    // (a peak that the sampled terms lack is one or a few logits, whose terms are the sum)
+    const float f = uniform(static_cast<float>(rest)), mean = mean_logit<E>(f, v, e, about + __builtin_amdgcn_logf(f) / p.c.hi);
+    return RowSums(p, l, rest,
                    is_far(about, p.c) ? far_base(about, p.c)
-                                      : static_cast<double>(about * p.c.hi) + lo * (e > 0.0f ? static_cast<double>(v / e) : about));
+                                      : static_cast<double>(about * p.c.hi) + lo * (rest > 0.0 ? static_cast<double>(mean) : about));
   };
   const bool none = l.n == 0;
   if (p.dz) {
@@ -1128,7 +1141,7 @@ __global__ __launch_bounds__(THREADS, 8) void distill_stream(DistillParams p) {
   l.sums(p, 0.0f, s);
   __syncthreads();  // (and the list's reads of the row are done)
   l.finish(s);
-  BlockSum<W> rest(s_sum, p.c);
+  BlockSum<W, E> rest(s_sum, p.c);
   const float about = rest.max > kMasked ? rest.max : 0.0f;
   if (is_far(about, p.c)) {
     float sum = 0.0f;

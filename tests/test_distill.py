@@ -779,3 +779,26 @@ def test_masks_that_are_numbers(mask, dtype, V):
     for grad in (True, False):
         row, _, _ = run(zl, values, ids, scale=1.0, grad=grad)
         assert torch.equal(torch.isnan(row.cpu()), torch.isnan(zl).any(1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [300, 9000, 60001, 151936, 200003])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("temperature", [0.75, 1.1, 1.25, 1.5, 2.5, 3.0])
+@pytest.mark.parametrize("gap", [20, 50, 80])
+def test_a_peak_far_above_the_rest(gap, temperature, dtype, V):
+    """One logit above all else by 20 to 80 temperatures, at places that the sum's correction samples and does not;
+    in the loss it lies off the list."""
+    T, k = 16, 4
+    g = torch.Generator().manual_seed(V)
+    z = (torch.randn(T, V, generator=g) - gap * temperature)
+    for r in range(T):
+        z[r, (r * (V - 17)) // T + r] = 0.0
+    z = z.to(DT[dtype])
+    check_top(z, k, temperature)
+    teacher = torch.randn(T, V, generator=g)
+    ids = torch.stack([torch.randperm(V, generator=g)[:k] for _ in range(T)]).int()
+    ids = torch.where(ids == z.argmax(1, keepdim=True), (ids + 1) % V, ids)
+    values = teacher.gather(1, ids.long())
+    lse = torch.logsumexp(teacher.double() / temperature, 1).float()
+    check(z, values, ids, scale=1.0, lse=lse, temperature=temperature)
