@@ -265,7 +265,7 @@ int mr_cross_entropy(const void* logits, int64_t ld, int64_t T, int64_t V, const
  * largest, 1 <= k <= min(V, 1024), in descending order, ties to the lower index
  * (the zeros are equal; NaN counts as the largest), as fp32 values [T, k] and
  * int32 ids [T, k], and, if lse is non-NULL, lse[t] = log sum_i exp(logits[t, i]
- * / temperature).
+ * / temperature). A call takes the rows of one launch: at least 4,194,303.
  */
 int mr_top_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t V, int k, double temperature,
                   float* values, int32_t* ids, float* lse, void* stream);
@@ -290,7 +290,8 @@ int mr_top_logits(const void* logits, int dtype, int64_t ld, int64_t T, int64_t 
  * q_j > 0 makes the loss infinite.
  * Unlisted logits of -1e37 and below, as masks write them, count as minus infinity;
  * a row with an unlisted logit so large that logit / temperature in powers of two is no
- * float has no finite loss. Temperatures lie in [1/1024, 1024], here and above.
+ * float has no finite loss. Temperatures lie in [1/1024, 1024], here and above; rows
+ * are limited as above.
  * Beside mr_cross_entropy as the objective the scores are gradients of
  * (mround/pipeline/scoring.py:183-192).
  */
@@ -500,6 +501,7 @@ int mr_rope(void* x_bf16, int64_t ld, int64_t T, int S, int n_heads, int head_di
  * rounding. out may be x with the same leading dimension (only the rotated
  * part is then written) or share no memory with it (the whole heads are
  * written); what lies beyond the n_heads heads is neither read nor written.
+ * T is at most 16,777,215 (more where a head rotates under 256 pairs).
  * Beside mr_rope: the mlx rope's traditional, dims, base/freqs and offset forms.
  */
 enum { MR_ROPE_HALF = 0, MR_ROPE_INTERLEAVED = 1 };

@@ -12,9 +12,11 @@
 //   loss = sum_j q_j (log q_j - log p_j) + q_R (log q_R - log p_R),
 //   dloss/dz_i = (p_i Q - q_i) / T on S,  p_i (Q - q_R / p_R) / T off S,  Q = sum q + q_R.
 //
-// Both read rows of a vocabulary and are bound by memory: a row's logits move
-// once, and its gradient once. Row sums run in fp32; the list's terms, whose
-// differences are the loss, and 1 - sum q in fp64.
+// Both read rows of a vocabulary and are bound by memory. Top logits and the loss
+// alone read a row once; with the gradient a row is read once as far as half a CU's
+// registers and LDS hold it, beyond that twice in part, past 20,480 pieces of 16 bytes
+// twice, and its gradient is written once. Row sums run in fp32; the list's terms,
+// whose differences are the loss, and 1 - sum q in fp64.
 #include <cmath>
 #include <limits>
 #include <type_traits>
@@ -807,7 +809,10 @@ __device__ __forceinline__ void lds_barrier() {
 
 // Piece i of a gradient row, laid out as piece_bytes reads it. The gradient passes by
 // the caches: 2044 rows of 151936 286 us by plain stores and loads, 254 by these
-// stores, 241 by such loads too of the pieces that are read once.
+// stores, 241 by such loads too of the pieces that are read once. Between the head's
+// product and its backward, the gradient over the logits, such rows gain 2 % of the
+// three (1247 us against 1269, 2048 rows and 896 columns of the head), rows that the
+// last-level cache would hold lose as much (of 49152, 576 columns: 374 against 368).
 template <int DT>
 __device__ __forceinline__ void store_piece(uint8_t* row, int i, int V, uint4 o) {
   constexpr int E = kPiece<DT>, ES = 16 / E;
@@ -825,8 +830,8 @@ __device__ __forceinline__ void store_piece(uint8_t* row, int i, int V, uint4 o)
   }
 }
 
-// One workgroup per row, the row held in registers: N pieces of 16 bytes per
-// thread, all loads in flight together, the row read once. A bitmap of the listed
+// One workgroup per row, the row held in registers, LDS and, past both, in memory: N,
+// M and R pieces of 16 bytes per thread. A bitmap of the listed
 // ids in LDS takes them out of it (minus infinity), so the rest's sum is formed of
 // its own terms: as the total less the listed it would have no digit left where
 // the list has nearly all the mass. The listed logits are gathered by the threads
@@ -849,8 +854,10 @@ __device__ __forceinline__ void store_piece(uint8_t* row, int i, int V, uint4 o)
 // rows of 49152 108 and 88. So M further pieces of a thread lie in LDS, and R more,
 // of rows past both, are read twice, for the sum through the registers of the held
 // ones before these come and for the gradient as they leave: 2044 rows of 151936
-// took 326 us by a CU a row, all held, and 305 so. What else the two rows took from
-// one another were their ways through the caches (store_piece): 241 us now, 5.2 TB/s.
+// took 326 us by a CU a row, all held, and 305 so, although 14 of a thread's 37 pieces
+// (38 % of the row) are read again. What else the two rows took from one another were
+// their ways through the caches (store_piece): 242 us now, 5.1 TB/s of one reading and
+// one writing, 6.1 with what is read again.
 template <int DT, int THREADS, int N, int M, int R>
 __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   constexpr int E = kPiece<DT>, ES = 16 / E, W = THREADS / 64;

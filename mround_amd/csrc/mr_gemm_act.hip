@@ -10,9 +10,12 @@
 // write and read it again.
 //
 // Bound by the matrix cores: silu of 16384 x 18944 x 3584 with the pre-activation
-// saved takes 1758 us (1265 TFLOP/s). At 4096 x 11008 x 2048, where the products
-// alone take 163 us forward and 147 backward, the epilogues come to 163 (relu) to
-// 179 us and 155 to 181 us (erf gelu), and a bias gradient to 6 us more.
+// saved takes 1758 to 1843 us (1207 to 1265 TFLOP/s, by the card). At 4096 x 11008 x
+// 2048, where the products alone take 146 us forward and 149 backward, they take with
+// these epilogues 159 (relu) to 182 us (erf gelu) and 165 to 184 with the
+// pre-activation saved; backward 161 to 185, of which reading the pre-activation is 12
+// and the erf gelu's slope 24, and a bias gradient 6 to 7 more. A slice of 32 rows
+// reads what its epilogue needs when it starts, with nothing beside it to cover the wait.
 #include "mr_gemm_tiles.h"
 
 namespace mr {

@@ -1832,7 +1832,8 @@ int dispatch(GemmParams p, hipStream_t s) {
                        : EPI == EPI_SWIGLU     ? OUT_SWIGLU
                        : EPI == EPI_SWIGLU_BWD ? OUT_SWIGLU_BWD
                        : EPI == EPI_SWIGLU_SPLIT ? OUT_F32  // the fp32 product's plan, so its bits
-                       : is_act_bwd(EPI) || (is_act(EPI) && !OB) ? OUT_RESID  // what they read besides
+                       // (fitted to no epilogue with an activation: the plain one that moves as much)
+                       : is_act_bwd(EPI) || (is_act(EPI) && !OB) ? OUT_RESID
                        : OB                    ? OUT_B16
                                                : OUT_F32;
   const Plan plan = plan_for(p.M, p.N, p.K / BK, AK, o, p.ws ? p.ws_bytes : 0);
