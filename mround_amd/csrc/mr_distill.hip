@@ -714,13 +714,14 @@ struct List {
     top = wave_max(top);
     if ((threadIdx.x & 63) == 0) s.z[threadIdx.x >> 6] = top;
   }
+  // (the row's, in scalar registers: in vector ones they would not fit beside a held row)
   __device__ __forceinline__ void collect(const Shared& s) {
-    t_max = waves_max<W>(s.t);
-    z_max = waves_max<W>(s.z);
-    n = waves_sum<W>(s.n);
+    t_max = uniform(waves_max<W>(s.t));
+    z_max = uniform(waves_max<W>(s.z));
+    n = __builtin_amdgcn_readfirstlane(waves_sum<W>(s.n));
   }
   // Sums of q (without lse: of its exponentials about the maximum), of
-  // q (log q - z / T) and of the student's exponentials about z_max. Into the
+  // q (log q - (z - z_max) / T) and of the student's exponentials about z_max. Into the
   // block's sums with the thread's share of the rest, before a barrier; then from them.
   __device__ __forceinline__ void sums(const DistillParams& p, float rest, Shared& s) {
     q_sum = a_sum = 0.0;
@@ -730,7 +731,7 @@ struct List {
     each(p, [&](int e, int, float t) {
       const double log_q = static_cast<double>(t) * p.inv_t - shift, q = exp(log_q);
       q_sum += q;
-      if (q != 0.0) a_sum += q * (log_q - static_cast<double>(z(e)) * p.inv_t);
+      if (q != 0.0) a_sum += q * (log_q - (static_cast<double>(z(e)) - base) * p.inv_t);
       zs += exp_t(z(e) - base, p.c);
     });
     // (threads' sums meet in fp64: the loss is a small difference of logarithms, and
@@ -756,6 +757,7 @@ struct List {
 // two: exp(u) = 2^(u log2 e)), the list's z_sum 2^(z_max c).
 struct RowSums {
   double rest, base, top, total;  // total: of both, times 2^-top
+  double above;                   // top, from z_max: of a list of masks no digit of 1e38 is left
   double q_rest, q_all, q_norm, p_rest, list_scale;
   template <int DT, int THREADS>
   __device__ __forceinline__ RowSums(const DistillParams& p, const List<DT, THREADS>& l, double rest_, double base_)
@@ -763,6 +765,7 @@ struct RowSums {
     const double c = static_cast<double>(p.c.hi) + p.c.lo;
     const double dz = l.z_max == -kInf ? base : l.z_max * c;
     top = rest > 0.0 ? fmax(base, dz) : dz;
+    above = top - (l.z_max == -kInf ? 0.0 : dz);
     const double r = rest > 0.0 ? rest * exp2(base - top) : rest;  // (NaN stays)
     list_scale = exp2(dz - top);
     total = r + l.z_sum * list_scale;
@@ -779,9 +782,9 @@ struct RowSums {
     if (l.n < 0) return __builtin_nanf("");
     if (l.n == 0) return 0.0f;
     constexpr double ln2 = 0.69314718055994530942;
-    const double log_total = log(total) + top * ln2;
-    double x = p.lse ? l.a_sum + l.q_sum * log_total : l.a_sum * q_norm - log(l.q_sum) + log_total;
-    if (q_rest > 0.0) x += q_rest * (log(q_rest) - (log(rest) + base * ln2 - log_total));
+    const double log_total = log(total), log_p = log_total + above * ln2;
+    double x = p.lse ? l.a_sum + l.q_sum * log_p : l.a_sum * q_norm - log(l.q_sum) + log_p;
+    if (q_rest > 0.0) x += q_rest * (log(q_rest) - (log(rest) + (base - top) * ln2 - log_total));
     return static_cast<float>(x);
   }
   // The gradient on the rest is rest_gradient * (term of the rest's sum).
@@ -916,7 +919,7 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
   };
   // (A mask is no maximum: about itself its terms would be one where its product with log2(e) / T is exact. About
   // zero each is zero.)
-  float about = waves_max<W>(s_first);
+  float about = uniform(waves_max<W>(s_first));
   if (about <= kMasked) about = 0.0f;
   float sum, ve, se;
   auto add_up = [&](auto takes) __attribute__((always_inline)) {
@@ -1032,7 +1035,7 @@ __global__ __launch_bounds__(THREADS, 4) void distill_held(DistillParams p) {
     mx = wave_max(mx);
     if (lane == 0) s_first[wave] = mx;
     __syncthreads();
-    about = waves_max<W>(s_first);
+    about = uniform(waves_max<W>(s_first));
     if (about <= kMasked) about = 0.0f;  // (every term is then zero)
     fresh();
     add_up(std::false_type{});

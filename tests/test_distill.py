@@ -802,3 +802,34 @@ def test_a_peak_far_above_the_rest(gap, temperature, dtype, V):
     values = teacher.gather(1, ids.long())
     lse = torch.logsumexp(teacher.double() / temperature, 1).float()
     check(z, values, ids, scale=1.0, lse=lse, temperature=temperature)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [5, 300, 9000, 40001, 151936, 200003])
+@pytest.mark.parametrize("low,dtype", [(m, t) for t in ("bf16", "f32") for m in (0.0, -2.0 ** 125, -1e30, -1e12, 3e12)]
+                         + [(-65504.0, "f16")])
+def test_rows_that_a_mask_takes_whole(low, dtype, V):
+    """Every logit at one value, the type's lowest (0 here) and other masks: the student's distribution is uniform over
+    the list where the value counts as minus infinity off it, else over the vocabulary, whatever the value."""
+    T, k = 3, 4
+    low = low or torch.finfo(DT[dtype]).min
+    g = torch.Generator().manual_seed(V)
+    teacher = torch.randn(T, V, generator=g)
+    ids = torch.argsort(torch.rand(T, V, generator=g), 1)[:, :k].int()
+    values = teacher.gather(1, ids.long())
+    z = torch.full((T, V), low).to(DT[dtype])
+    as_zero = torch.zeros(T, V, dtype=torch.float64)  # (a shift of a row changes nothing)
+    if float(z[0, 0]) <= -1e37:
+        as_zero.fill_(-math.inf).scatter_(1, ids.long(), 0.0)
+    for temperature in (0.7, 1.0, 2.034):
+        lse = torch.logsumexp(teacher.double() / temperature, 1).float()
+        for tail in (lse, None):
+            kw = dict(scale=0.37, lse=tail, temperature=temperature)
+            want, grad, size, weight, _ = reference(as_zero, values, ids, **kw)
+            row, _, d = run(z, values, ids, **kw)
+            alone, _, _ = run(z, values, ids, grad=False, **kw)
+            tol = 2 * weight * unit(V) + 2.0 ** -24 * want.abs() + 1e-12
+            for r in (row, alone):
+                assert bool(((r.cpu().double() - want).abs() <= tol).all()), (temperature, tail is None, r, want)
+            gtol = 2 * size * unit(V) + torch.finfo(z.dtype).eps / 2 * grad.abs() + 2.0 ** -25 * (dtype == "f16") + 2.0 ** -120
+            assert bool(((d.cpu().double() - grad).abs() <= gtol).all()), (temperature, tail is None)
