@@ -17,6 +17,7 @@ budget the average implies (api.py:1471-1695), or checks and costs a given
 from __future__ import annotations
 
 import dataclasses
+import gc
 import json
 import math
 import time
@@ -647,7 +648,8 @@ def quantize(model: str | Path, *, output_dir: str | Path, bits: int = 4, group_
     print(f"  {timing.describe()}", flush=True)
     on_gpu = torch.cuda.is_available() and str(device).startswith("cuda")
     held_before = 0
-    if on_gpu:  # the run's own peak: what the process already holds is left out
+    if on_gpu:  # the run's own peak: what the process already holds is left out, not what it dropped in cycles
+        gc.collect()
         torch.cuda.reset_peak_memory_stats(device)
         held_before = torch.cuda.memory_allocated(device)
     t0 = time.perf_counter()

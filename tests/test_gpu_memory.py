@@ -8,6 +8,7 @@ import json
 import sys
 
 import pytest
+import torch
 
 from mround_amd import api
 from mround_amd.pipeline.checkpoint import write_random_checkpoint
@@ -57,3 +58,26 @@ def test_prediction_bounds_a_pass_by_the_teacher(tmp_path):
     print(f"  predicted {predicted} measured {memory['peak_allocated']}", file=sys.stderr)
     assert rec["mixed"]["objective"] == "teacher" and memory["peak_stage"] == "scoring"
     assert 0.85 * predicted <= memory["peak_allocated"] <= 1.05 * predicted
+
+
+def test_the_measured_peak_is_the_runs_own(tmp_path):
+    """Tensors that the process has dropped in reference cycles, which a collection during the run would free, are not
+    held by it."""
+    print("case memory cycles", flush=True, file=sys.stderr)
+    src = write_random_checkpoint(tmp_path / "m", SMALL, seed=1)
+
+    class Cycle:
+        pass
+
+    def peak():
+        res = api.quantize(src, output_dir=tmp_path / "q", bits=4, symmetry=Symmetry.ASYMMETRIC, seed=2,
+                           tuning=TuningConfig(iters=2, batch_size=4, n_samples=8, seq_len=256))
+        return json.loads(res.config_path.read_text())["memory"]["peak_allocated"]
+
+    peak()  # (what a first run leaves with the process)
+    want = peak()
+    for _ in range(3):
+        c = Cycle()
+        c.itself, c.tensor = c, torch.empty(10 << 20, dtype=torch.uint8, device="cuda")
+    del c
+    assert peak() == want
