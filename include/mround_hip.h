@@ -454,6 +454,96 @@ int mr_rmsnorm_bwd(const float* dy, const float* h, const float* w, const float*
                    void* stream);
 
 /*
+ * Experts of a token (no counterpart in the reference, whose blocks are dense):
+ * p = softmax(logits row) over E experts, the k largest in descending order
+ * (equal ones: the lower index first), weights scale p, or with `normalize` scale p
+ * over the chosen ones' sum. Logits fp32, bf16 or fp16 [T, E] (leading dimension
+ * ld). A logit of -inf is never chosen; an entry that finds none has id -1, weight 0
+ * and slot -1. A NaN counts as the largest and makes its row's weights NaN.
+ * offsets [E + 1], slots [T, k] and rows [T k] (all or none): the pairs sorted by
+ * expert, tokens in order within one: expert e's places start at offsets[e],
+ * slots is a pair's place, rows a place's token (places past offsets[E] are left).
+ * E <= 512, k <= min(E, 64). workspace: mr_route_workspace_bytes(T, E) bytes when
+ * offsets are asked for.
+ * mr_route_experts_bwd: the logits' gradient (their type; may be written over
+ * them) from dweights [T, k] for the ids that were chosen, each once a row.
+ */
+size_t mr_route_workspace_bytes(int64_t T, int64_t E);
+int mr_route_experts(const void* logits, int dtype, int64_t ld, int64_t T, int64_t E, int64_t k, int normalize,
+                     float scale, float* weights, int32_t* ids, int32_t* offsets, int32_t* slots, int32_t* rows,
+                     void* workspace, size_t workspace_bytes, void* stream);
+int mr_route_experts_bwd(const float* dweights, const void* logits, int dtype, int64_t ld, const int32_t* ids,
+                         int64_t T, int64_t E, int64_t k, int normalize, float scale, void* dlogits, int64_t lddz,
+                         void* stream);
+
+/*
+ * Products grouped by expert, bf16 operands: expert e's rows are offsets[e] ..
+ * offsets[e + 1] - 1 (device memory, as mr_route_experts writes them; values
+ * outside the rows there are count as their ends).
+ *   MR_NT  C[r] = A[r] B[e]^T   B[e] is N x K at B + e b_step; with `index` [M]
+ *          A's row r is its row index[r] of a_rows (an index outside counts as the
+ *          nearest row; A within 4 GiB)
+ *   MR_NN  C[r] = A[r] B[e]     B[e] is K x N
+ *   MR_TN  C[e] = A[rows of e]^T B[rows of e], M x N fp32 at C + e c_step, K all
+ *          experts' rows; added to C with `accumulate`, else zeros without rows
+ * M x N, C fp32 or bf16, rows outside the offsets left. N (TN: and M) multiples of
+ * 8; K a positive multiple of 64 (TN: any). Operands and C 16-byte aligned, leading
+ * dimensions and steps multiples of 8 (fp32 C: 4).
+ * mr_gemm_experts_swiglu, _bwd: mr_gemm_swiglu and mr_gemm_swiglu_bwd over such
+ * rows, Wgu[e] 2N x K interleaved every 32 rows, Wd[e] K x N, M any; dgu may be gu.
+ */
+int mr_gemm_experts(int layout, int64_t experts, int64_t M, int64_t N, int64_t K, const void* A, int64_t lda,
+                    const int32_t* index, int64_t a_rows, const void* B, int64_t ldb, int64_t b_step,
+                    const int32_t* offsets, void* C, int c_dtype, int64_t ldc, int64_t c_step, int accumulate,
+                    void* stream);
+int mr_gemm_experts_swiglu(int64_t experts, int64_t M, int64_t N, int64_t K, const void* X, int64_t ldx,
+                           const int32_t* index, int64_t x_rows, const void* Wgu, int64_t ldw, int64_t w_step,
+                           const int32_t* offsets, void* act, int64_t ldact, void* gu, int64_t ldgu, void* stream);
+int mr_gemm_experts_swiglu_bwd(int64_t experts, int64_t M, int64_t N, int64_t K, const void* dy, int64_t ldd,
+                               const void* Wd, int64_t ldw, int64_t w_step, const int32_t* offsets, const void* gu,
+                               int64_t ldgu, void* dgu, int64_t lddgu, void* stream);
+
+/*
+ * Rows to their experts' places and back, fp32 or bf16, sums in fp32:
+ * mr_combine_experts: out[t] = resid[t] + sum_j weights[t, j] y[slots[t, j]], in
+ *   order of j (resid null: 0, of out's type, and may be out; weights null: 1).
+ * mr_spread_experts: out[slots[t, j]] = weights[t, j] x[t]; with y (of out's type;
+ *   may be out) and dweights [T, k]: dweights[t, j] = x[t] . y[slots[t, j]]. Places
+ *   without an entry are left.
+ * slots [T, k]; a negative one, or one past the R rows, is no entry; others occur once.
+ */
+int mr_combine_experts(const void* y, int y_dtype, int64_t ldy, int64_t R, const int32_t* slots, const float* weights,
+                       int64_t T, int64_t k, int64_t H, const void* resid, int64_t ldr, void* out, int out_dtype,
+                       int64_t ldo, void* stream);
+int mr_spread_experts(const void* x, int x_dtype, int64_t ldx, const int32_t* slots, const float* weights, int64_t T,
+                      int64_t k, int64_t H, void* out, int out_dtype, int64_t ldo, int64_t R, const void* y, int64_t ldy,
+                      float* dweights, void* stream);
+
+/*
+ * The end of a block's branch and the norm after it, rows [T, H], H <= 16384:
+ *   out = resid + scale gate rmsnorm(y) post      normed = rmsnorm(out) pre
+ * with rmsnorm(v) = v rsqrt(mean(v^2) + eps) (post null: y itself; gate [ceil(T /
+ * gate_rows), H], a row for each gate_rows rows, null: 1; pre and normed together or
+ * neither). y and normed are act_dtype (fp32, bf16 or fp16), resid and out
+ * stream_dtype (fp32 or act_dtype), weights fp32; sums in fp32, normed of out before
+ * it is rounded. out may be resid, normed may be y.
+ * The backward takes y and out as the forward read and wrote them, dnormed (with
+ * pre) and dout (either null: none), and writes dy (may be y), dresid (may be dout)
+ * and, where given, dpost, dpre [H] and dgate: sums over rows by blocks in order, the
+ * blocks' partials in the workspace. mr_norm_residual_bwd_workspace_bytes: for which
+ * of dpost, dgate and dpre are asked for, gate_rows of any value without a gate.
+ */
+int mr_norm_residual(const void* y, int act_dtype, int64_t ldy, const void* resid, int stream_dtype, int64_t ldr,
+                     int64_t T, int64_t H, float eps, const float* post, const float* gate, int64_t gate_rows,
+                     float scale, const float* pre, void* out, int64_t ldo, void* normed, int64_t ldn, void* stream);
+size_t mr_norm_residual_bwd_workspace_bytes(int64_t T, int64_t H, int64_t gate_rows, int post, int gate, int pre);
+int mr_norm_residual_bwd(const void* dnormed, int act_dtype, int64_t lddn, const void* dout, int stream_dtype,
+                         int64_t lddo, const void* y, int64_t ldy, const void* out, int64_t ldo, int64_t T, int64_t H,
+                         float eps, const float* post, const float* gate, int64_t gate_rows, float scale,
+                         const float* pre, void* dy, int64_t lddy, void* dresid, int64_t lddr, float* dpost,
+                         float* dgate, float* dpre, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Split-precision operands: the reference's remedy for the block objective's
  * subtraction of two block outputs (mround DOCUMENTATION.md:885-925, three
  * products A_hi B_hi + A_hi B_lo + A_lo B_hi), which its code documents but

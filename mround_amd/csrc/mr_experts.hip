@@ -1,0 +1,772 @@
+// The experts of a token, and its rows on their way to them and back.
+//
+// Choice. p = softmax(z) over the experts' logits; the k largest, equal ones by
+// index, with weights scale p (or scale p over their sum). A logit of -inf is never
+// chosen: an entry without an expert has id -1, weight 0 and no place.
+// Order. The (token, expert) pairs sorted by expert, tokens in order within one:
+// offsets[e] is expert e's first place, slots[pair] a pair's place, rows[place] its
+// token. Counting sort: each block counts its tokens' pairs an expert, adds what
+// the blocks before it counted, and ranks its own. No atomic's order reaches a
+// result.
+// Rows. spread: y[slots[t, j]] = w[t, j] x[t], and the weights' gradients x[t] .
+// y_old; combine: out[t] = resid[t] + sum_j w[t, j] y[slots[t, j]], in order of j.
+// Each is the other's backward.
+#include <cmath>
+
+#include "mr_rows.h"
+
+namespace mr {
+namespace {
+
+// ---- choice -----------------------------------------------------------------
+
+constexpr int kRouteThreads = 1024;
+constexpr int kRouteWaves = kRouteThreads / 64;
+constexpr int kMaxExperts = 512, kMaxTop = 64;
+
+struct RouteParams {
+  const void* z;
+  int64_t ldz;
+  int T, E, k;
+  bool normalize;
+  float scale;
+  float* weights;
+  int32_t* ids;
+  int32_t* offsets;  // null: no order is asked for
+  int32_t* slots;
+  int32_t* rows;
+  int32_t* counts;   // [blocks, E], of several blocks
+  int chunk;         // tokens of a block
+  int blocks;
+};
+
+// A float's place in the descending order as an unsigned number: NaN above all,
+// -inf (which is never chosen) at 0, zeros alike.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (x != x) return 0xffffffffu;
+  if (x == -INFINITY) return 0;
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+
+// Maximum, minimum and sum over the L lanes of a token (L = 16, 32 or 64, aligned).
+template <int L, typename T, typename F>
+__device__ __forceinline__ T lanes_reduce(T x, F f) {
+  x = f(x, dpp<kDppXor1>(x));
+  x = f(x, dpp<kDppXor2>(x));
+  x = f(x, dpp<kDppHalfMirror>(x));
+  x = f(x, dpp<kDppMirror>(x));
+  if constexpr (L >= 32) x = f(x, __shfl_xor(x, 16, 64));
+  if constexpr (L >= 64) x = f(x, __shfl_xor(x, 32, 64));
+  return x;
+}
+
+// A token's logits, V to a lane: expert i L + lane.
+template <int DT, int L, int V>
+__device__ __forceinline__ void load_logits(const RouteParams& p, int64_t t, int l, float (&z)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int e = i * L + l;
+    z[i] = e < p.E ? load_elem<DT>(p.z, t * p.ldz + e) : -INFINITY;
+  }
+}
+
+// The block's tokens t0 .. t1 - 1: ids and weights, and the count of each expert in hist (LDS).
+template <int DT, int L, int V>
+__device__ __forceinline__ void choose(const RouteParams& p, int t0, int t1, int32_t* hist) {
+  constexpr int TOKENS = kRouteThreads / L;
+  const int l = threadIdx.x % L;
+  for (int t = t0 + static_cast<int>(threadIdx.x) / L; t < t1; t += TOKENS) {
+    float z[V];
+    load_logits<DT, L, V>(p, t, l, z);
+    uint32_t key[V];
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      key[i] = order_key(z[i]);
+      m = fmaxf(m, z[i]);
+    }
+    m = lanes_reduce<L>(m, [](float a, float b) { return fmaxf(a, b); });
+    float sum = 0.0f;
+    if (!p.normalize && m > -INFINITY) {  // (of NaN and +inf: NaN, like every weight then)
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum += expf(z[i] - m);
+      sum = lanes_reduce<L>(sum, [](float a, float b) { return a + b; });
+    }
+    float own = -INFINITY;  // the logit of this lane's entry, entry l
+    int own_id = -1;
+    for (int j = 0; j < p.k; ++j) {
+      uint32_t best = 0, at = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const bool more = key[i] > best;
+        best = more ? key[i] : best;
+        at = more ? i * L + l : at;
+      }
+      const uint32_t top = lanes_reduce<L>(best, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+      at = lanes_reduce<L>(best == top ? at : 0xffffffffu, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+      float value = 0.0f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const bool it = top && at == static_cast<uint32_t>(i * L + l);
+        value = it ? z[i] : value;
+        key[i] = it ? 0 : key[i];
+      }
+      // the lane that held it is at % L of the token's
+      value = __shfl(value, (static_cast<int>(threadIdx.x) & 63 & ~(L - 1)) + static_cast<int>(at % L), 64);
+      if (l == j && top) {
+        own = value;
+        own_id = static_cast<int>(at);
+      }
+    }
+    float w = own_id >= 0 ? expf(own - m) : 0.0f;
+    if (p.normalize) sum = lanes_reduce<L>(w, [](float a, float b) { return a + b; });
+    w = own_id >= 0 ? w / sum * p.scale : 0.0f;
+    if (l < p.k) {
+      const int64_t at = static_cast<int64_t>(t) * p.k + l;
+      p.ids[at] = own_id;
+      p.weights[at] = w;
+      if (own_id >= 0 && p.offsets) atomicAdd(hist + own_id, 1);
+    }
+  }
+}
+
+// ---- order ------------------------------------------------------------------
+
+// start[e]: the place of the block's first pair of expert e. hist[e], its own
+// count, where it is the only block; else counts[.][e].
+__device__ __forceinline__ void block_starts(const RouteParams& p, const int32_t* hist, int32_t* start, int32_t* scratch) {
+  const int tid = threadIdx.x, E = p.E;
+  int32_t all = 0, before = 0;
+  if (p.blocks == 1) {
+    if (tid < E) all = hist[tid];
+  } else {
+    // runs of blocks by groups of threads (E a group), added in LDS
+    const int wide = (E + 63) / 64 * 64, groups = kRouteThreads / wide, g = tid / wide, e = tid % wide;
+    int32_t a = 0, b = 0;
+    if (g < groups && e < E) {
+      const int per = (p.blocks + groups - 1) / groups;
+      const int32_t* c = p.counts + e;
+#pragma unroll 8
+      for (int i = g * per; i < min((g + 1) * per, p.blocks); ++i) {
+        const int32_t n = c[static_cast<int64_t>(i) * E];
+        a += n;
+        b += i < static_cast<int>(blockIdx.x) ? n : 0;
+      }
+    }
+    if (tid < E) scratch[tid] = start[tid] = 0;
+    __syncthreads();
+    if (g < groups && e < E) {
+      atomicAdd(scratch + e, a);
+      atomicAdd(start + e, b);
+    }
+    __syncthreads();
+    if (tid < E) {
+      all = scratch[tid];
+      before = start[tid];
+    }
+    __syncthreads();
+  }
+  // exclusive scan of the experts' counts over the threads
+  const int lane = tid & 63;
+  int32_t upto = all;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const int32_t x = __shfl_up(upto, o, 64);
+    upto += lane >= o ? x : 0;
+  }
+  if (lane == 63) scratch[tid >> 6] = upto;
+  __syncthreads();
+  int32_t base = 0;
+  for (int w = 0; w < (tid >> 6); ++w) base += scratch[w];
+  const int32_t first = base + upto - all;
+  if (tid < E) start[tid] = first + before;
+  if (blockIdx.x == 0 && tid < E) {
+    p.offsets[tid] = first;
+    if (tid == E - 1) p.offsets[E] = first + all;
+  }
+  __syncthreads();
+}
+
+// The places of the block's pairs: its waves take runs of pairs in order. A wave
+// counts its run's experts in its row of `of_wave`; the rows become the places
+// where each wave's pairs of an expert start; then 64 pairs at a time, the lanes of
+// one expert (found bit by bit) take consecutive places.
+__device__ __forceinline__ void place(const RouteParams& p, int t0, int t1, const int32_t* start, int32_t* of_wave) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, E = p.E;
+  const int64_t first = static_cast<int64_t>(t0) * p.k;
+  const int64_t pairs = static_cast<int64_t>(t1 - t0) * p.k;
+  const int64_t per = ((pairs + kRouteWaves - 1) / kRouteWaves + 63) / 64 * 64;
+  const int64_t a = wave * per, b = min(a + per, pairs);
+  int32_t* mine = of_wave + wave * E;
+  for (int e = lane; e < E; e += 64) mine[e] = 0;
+  __syncthreads();
+  for (int64_t i = a + lane; i < b; i += 64) {
+    const int id = p.ids[first + i];
+    if (id >= 0) atomicAdd(mine + id, 1);
+  }
+  __syncthreads();
+  if (tid < E) {
+    int32_t at = start[tid];
+#pragma unroll
+    for (int w = 0; w < kRouteWaves; ++w) {
+      const int32_t n = of_wave[w * E + tid];
+      of_wave[w * E + tid] = at;
+      at += n;
+    }
+  }
+  __syncthreads();
+  int bits = 0;
+  while ((1 << bits) < E) ++bits;
+  for (int64_t i = a; i < b; i += 64) {
+    const int64_t pair = first + i + lane;
+    const int id = i + lane < b ? p.ids[pair] : -1;
+    uint64_t same = __ballot(id >= 0);
+    for (int q = 0; q < bits; ++q) {
+      const uint64_t set = __ballot((id >> q) & 1);
+      same &= ((id >> q) & 1) ? set : ~set;
+    }
+    const int leader = same ? __builtin_ctzll(same) : 0;
+    int32_t at = 0;
+    if (id >= 0 && lane == leader) at = atomicAdd(mine + id, static_cast<int32_t>(__popcll(same)));
+    at = __shfl(at, leader, 64);
+    if (i + lane < b) {
+      if (id >= 0) {
+        at += __popcll(same & ((1ull << lane) - 1));
+        p.slots[pair] = at;
+        p.rows[at] = static_cast<int32_t>(pair / p.k);
+      } else {
+        p.slots[pair] = -1;
+      }
+    }
+  }
+}
+
+// LDS of a block: counts or starts [E], scratch [E], places a wave [waves, E].
+constexpr size_t route_lds(int64_t E) { return static_cast<size_t>(E * (2 + kRouteWaves) + 16) * 4; }
+
+template <int DT, int L, int V>
+__global__ __launch_bounds__(kRouteThreads) void route_choose(RouteParams p) {
+  extern __shared__ int32_t lds[];
+  int32_t* hist = lds;
+  for (int e = threadIdx.x; e < p.E; e += kRouteThreads) hist[e] = 0;
+  __syncthreads();
+  const int t0 = static_cast<int>(blockIdx.x) * p.chunk, t1 = min(t0 + p.chunk, p.T);
+  choose<DT, L, V>(p, t0, t1, hist);
+  if (!p.offsets) return;
+  __syncthreads();  // (the block's ids too)
+  if (p.blocks > 1) {
+    for (int e = threadIdx.x; e < p.E; e += kRouteThreads) p.counts[static_cast<int64_t>(blockIdx.x) * p.E + e] = hist[e];
+    return;
+  }
+  block_starts(p, hist, lds + p.E, lds + 2 * p.E);
+  place(p, t0, t1, lds + p.E, lds + 2 * p.E);
+}
+
+__global__ __launch_bounds__(kRouteThreads) void route_place(RouteParams p) {
+  extern __shared__ int32_t lds[];
+  const int t0 = static_cast<int>(blockIdx.x) * p.chunk, t1 = min(t0 + p.chunk, p.T);
+  block_starts(p, lds, lds + p.E, lds + 2 * p.E);
+  place(p, t0, t1, lds + p.E, lds + 2 * p.E);
+}
+
+// The gradient of the logits: dz = p (d - sum p d), d the weights' gradients at
+// the chosen experts; over the chosen alone where their weights were normalized.
+struct RouteBwdParams {
+  RouteParams f;
+  const float* dw;
+  void* dz;
+  int64_t lddz;
+};
+template <int DT, int L, int V>
+__global__ __launch_bounds__(256) void route_bwd(RouteBwdParams p) {
+  const int l = threadIdx.x % L, k = p.f.k;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (256 / L) + threadIdx.x / L;
+  if (t >= p.f.T) return;  // (whole groups of L lanes, which reduce among themselves)
+  float z[V], d[V];
+  bool chosen[V];
+  load_logits<DT, L, V>(p.f, t, l, z);
+  const int my_id = l < k ? p.f.ids[t * k + l] : -1;
+  const float my_d = l < k ? p.dw[t * k + l] : 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    d[i] = 0.0f;
+    chosen[i] = false;
+  }
+  for (int j = 0; j < k; ++j) {
+    const int from = (static_cast<int>(threadIdx.x) & 63 & ~(L - 1)) + j;
+    const int id = __shfl(my_id, from, 64);
+    const float dj = __shfl(my_d, from, 64);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const bool it = id == i * L + l;
+      d[i] += it ? dj : 0.0f;
+      chosen[i] = chosen[i] || it;
+    }
+  }
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if (p.f.normalize && !chosen[i]) z[i] = -INFINITY;
+    m = fmaxf(m, z[i]);
+  }
+  m = lanes_reduce<L>(m, [](float a, float b) { return fmaxf(a, b); });
+  float e[V], sum = 0.0f, dot = 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    e[i] = m > -INFINITY ? expf(z[i] - m) : z[i] == -INFINITY ? 0.0f : z[i];  // (z a NaN: a row of them and -inf)
+    sum += e[i];
+    dot += e[i] * d[i];
+  }
+  sum = lanes_reduce<L>(sum, [](float a, float b) { return a + b; });
+  dot = lanes_reduce<L>(dot, [](float a, float b) { return a + b; });
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a row that is -inf throughout has no gradient)
+  dot *= inv;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const int at = i * L + l;
+    if (at < p.f.E) store_elem<DT>(p.dz, t * p.lddz + at, p.f.scale * (e[i] * inv) * (d[i] - dot));
+  }
+}
+
+// ---- rows -------------------------------------------------------------------
+
+struct RowsParams {
+  const void* x;    // spread: [T, H] rows; combine: resid or null
+  int64_t ldx;
+  void* y;          // the experts' rows [R, H] (spread writes, combine reads)
+  int64_t ldy;
+  const void* y_old;  // spread: what the weights' gradients multiply, or null
+  int64_t ldyo;
+  int64_t R;
+  const int32_t* slots;
+  const float* weights;  // [T, k] or null
+  float* dweights;       // spread: [T, k] or null
+  void* out;
+  int64_t ldo;
+  int64_t T;
+  int H, k, pieces;
+};
+
+// Eight places at a time are in flight; a place outside the rows counts as none.
+constexpr int kAtOnce = 8;
+
+template <int DY, int DO, int V>
+__global__ __launch_bounds__(256) void combine_kernel(RowsParams p) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t t = i / p.pieces;
+  const int c = static_cast<int>(i - t * p.pieces) * V;
+  if (t >= p.T) return;
+  float acc[V];
+  if (p.x) {
+    Piece<DO, V> r;
+    r.load(p.x, t * p.ldx + c);
+#pragma unroll
+    for (int q = 0; q < V; ++q) acc[q] = r.get(q);
+  } else {
+#pragma unroll
+    for (int q = 0; q < V; ++q) acc[q] = 0.0f;
+  }
+  const int32_t* slots = p.slots + t * p.k;
+  const float* weights = p.weights ? p.weights + t * p.k : nullptr;
+  for (int j0 = 0; j0 < p.k; j0 += kAtOnce) {
+    Piece<DY, V> y[kAtOnce];
+    float w[kAtOnce];
+    bool there[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int jj = min(j0 + j, p.k - 1);
+      const int64_t s = slots[jj];
+      there[j] = j0 + j < p.k && s >= 0 && s < p.R;
+      w[j] = weights ? weights[jj] : 1.0f;
+      if (there[j]) y[j].load(p.y, s * p.ldy + c);
+      else y[j].zero();
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j)
+#pragma unroll
+      for (int q = 0; q < V; ++q) acc[q] += there[j] ? w[j] * y[j].get(q) : 0.0f;
+  }
+  store_piece<DO, V, false>(p.out, t * p.ldo + c, acc);
+}
+
+// W waves to a token.
+template <int DX, int DY, int V, int W>
+__global__ __launch_bounds__(256) void spread_kernel(RowsParams p) {
+  __shared__ float smem[4][kAtOnce];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (4 / W) + (W == 4 ? 0 : wave);
+  if (t >= p.T) return;  // (W 4: the whole block)
+  const int first = W == 4 ? static_cast<int>(threadIdx.x) : lane;
+  const int32_t* slots = p.slots + t * p.k;
+  for (int j0 = 0; j0 < p.k; j0 += kAtOnce) {
+    int64_t s[kAtOnce];
+    float w[kAtOnce], dot[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int jj = min(j0 + j, p.k - 1);
+      s[j] = slots[jj];
+      if (j0 + j >= p.k || s[j] >= p.R) s[j] = -1;
+      w[j] = p.weights ? p.weights[t * p.k + jj] : 1.0f;
+      dot[j] = 0.0f;
+    }
+    for (int i = first; i < p.pieces; i += 64 * W) {
+      const int c = i * V;
+      Piece<DX, V> x;
+      x.load(p.x, t * p.ldx + c);
+      Piece<DY, V> y[kAtOnce];
+      if (p.dweights) {
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+          if (s[j] >= 0) y[j].load(p.y_old, s[j] * p.ldyo + c);
+          else y[j].zero();
+        }
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j)
+#pragma unroll
+          for (int q = 0; q < V; ++q) dot[j] += x.get(q) * y[j].get(q);
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        if (s[j] < 0) continue;
+        float o[V];
+#pragma unroll
+        for (int q = 0; q < V; ++q) o[q] = w[j] * x.get(q);
+        store_piece<DY, V, false>(p.y, s[j] * p.ldy + c, o);
+      }
+    }
+    if (p.dweights) {
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) dot[j] = wave_sum(dot[j]);
+      if constexpr (W == 4) {
+        if (lane == 0) {
+#pragma unroll
+          for (int j = 0; j < kAtOnce; ++j) smem[wave][j] = dot[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) dot[j] = (smem[0][j] + smem[1][j]) + (smem[2][j] + smem[3][j]);
+        __syncthreads();
+      }
+      if (first == 0) {
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j)
+          if (j0 + j < p.k) p.dweights[t * p.k + j0 + j] = s[j] >= 0 ? dot[j] : 0.0f;
+      }
+    }
+  }
+}
+
+int route_blocks(int64_t T, int64_t* chunk_out) {
+  // at most 256 blocks of 64 tokens' multiples, 128 at least
+  int64_t chunk = ((T + 255) / 256 + 63) / 64 * 64;
+  if (chunk < 128) chunk = 128;
+  *chunk_out = chunk;
+  const int64_t n = (T + chunk - 1) / chunk;
+  return static_cast<int>(n > 0 ? n : 1);
+}
+
+int check_route(const char* fn, int dtype, int64_t ldz, int64_t T, int64_t E, int64_t k, const void* z) {
+  if (T < 0 || E <= 0 || k <= 0) return fail(MR_EINVAL, "%s: no experts to choose or from, or a negative size", fn);
+  if (!valid_dtype(dtype)) return fail(MR_EINVAL, "%s: bad dtype %d", fn, dtype);
+  if (k > E || k > kMaxTop || E > kMaxExperts)
+    return fail(MR_EINVAL, "%s: at most %d of at most %d experts, no more than there are (%lld of %lld)", fn, kMaxTop,
+                kMaxExperts, static_cast<long long>(k), static_cast<long long>(E));
+  if (T * k > 0x7fffffff) return fail(MR_EINVAL, "%s: too many rows", fn);
+  if (T > 0 && ldz < E) return fail(MR_EINVAL, "%s: a leading dimension is smaller than its row", fn);
+  if (reinterpret_cast<uintptr_t>(z) % dtype_bytes(dtype))
+    return fail(MR_EINVAL, "%s: a pointer is not aligned to its elements", fn);
+  return MR_OK;
+}
+
+// Lanes to a token: one for each entry, with at most 16 logits each.
+int route_lanes(int64_t E, int64_t k) {
+  if (k <= 16 && E <= 256) return 16;
+  return k <= 32 && E <= 512 ? 32 : 64;
+}
+
+#define MR_ROUTE_V(DT, L, CALL)                           \
+  do {                                                    \
+    if (E <= 4 * L) CALL(DT, L, 4);                       \
+    else if (L == 64 || E <= 8 * L) CALL(DT, L, 8);       \
+    else CALL(DT, L, (L == 64 ? 8 : 16));                 \
+  } while (0)
+#define MR_ROUTE_L(DT, CALL)                       \
+  do {                                             \
+    if (lanes == 16) MR_ROUTE_V(DT, 16, CALL);     \
+    else if (lanes == 32) MR_ROUTE_V(DT, 32, CALL); \
+    else MR_ROUTE_V(DT, 64, CALL);                 \
+  } while (0)
+#define MR_ROUTE_CASES(CALL)                         \
+  do {                                               \
+    if (dtype == MR_F32) MR_ROUTE_L(MR_F32, CALL);   \
+    else if (dtype == MR_BF16) MR_ROUTE_L(MR_BF16, CALL); \
+    else MR_ROUTE_L(MR_F16, CALL);                   \
+  } while (0)
+
+int64_t rows_bytes(int64_t n, int64_t ld, int64_t H, int es) { return n > 0 ? ((n - 1) * ld + H) * es : 0; }
+
+struct Bytes {
+  const void* p;
+  int64_t n;
+};
+template <int NW, int NR>
+bool clash(const Bytes (&w)[NW], const Bytes (&r)[NR]) {
+  for (int a = 0; a < NW; ++a) {
+    if (!w[a].p || w[a].n <= 0) continue;
+    for (int b = 0; b < NR; ++b)
+      if (r[b].p && r[b].n > 0 && overlap(w[a].p, w[a].n, r[b].p, r[b].n)) return true;
+    for (int b = a + 1; b < NW; ++b)
+      if (w[b].p && w[b].n > 0 && overlap(w[a].p, w[a].n, w[b].p, w[b].n)) return true;
+  }
+  return false;
+}
+
+bool on4(const void* a, const void* b = nullptr, const void* c = nullptr, const void* d = nullptr) {
+  return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c) |
+           reinterpret_cast<uintptr_t>(d)) & 3) == 0;
+}
+
+bool vector_rows(const void* p, int64_t ld, int es) { return !p || (aligned16(p) && ld * es % 16 == 0); }
+
+int check_rows(const char* fn, int64_t T, int64_t k, int64_t R, int64_t H) {
+  if (T < 0 || k <= 0 || R < 0 || H < 0) return fail(MR_EINVAL, "%s: no experts, or a negative size", fn);
+  if (H > 0x7fffffff || T * k > 0x7fffffff || R > 0x7fffffff) return fail(MR_EINVAL, "%s: too large", fn);
+  return MR_OK;
+}
+
+}  // namespace
+}  // namespace mr
+
+extern "C" {
+
+size_t mr_route_workspace_bytes(int64_t T, int64_t E) {
+  int64_t chunk;
+  const int blocks = mr::route_blocks(T > 0 ? T : 0, &chunk);
+  return blocks > 1 && E > 0 ? static_cast<size_t>(blocks) * E * 4 : 0;
+}
+
+int mr_route_experts(const void* logits, int dtype, int64_t ld, int64_t T, int64_t E, int64_t k, int normalize,
+                     float scale, float* weights, int32_t* ids, int32_t* offsets, int32_t* slots, int32_t* rows,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace mr;
+  clear_error();
+  const char* fn = "mr_route_experts";
+  if (const int rc = check_route(fn, dtype, ld, T, E, k, logits)) return rc;
+  if (T > 0 && (!logits || !weights || !ids)) return fail(MR_EINVAL, "%s: null pointer", fn);
+  if (!offsets ? slots || rows : T > 0 && (!slots || !rows))
+    return fail(MR_EINVAL, "%s: offsets, slots and rows come together", fn);
+  if (T == 0 && !offsets) return MR_OK;
+  if (!on4(weights, ids) || !on4(offsets, slots, rows, workspace))
+    return fail(MR_EINVAL, "%s: a pointer is not aligned to its elements", fn);
+  const size_t need = offsets ? mr_route_workspace_bytes(T, E) : 0;
+  if (need && (!workspace || workspace_bytes < need)) return fail(MR_EINVAL, "%s: %zu bytes of workspace are needed", fn, need);
+  {
+    const int64_t n = T * k * 4;
+    const Bytes w[6] = {{weights, n}, {ids, n}, {offsets, (E + 1) * 4}, {slots, n}, {rows, n},
+                        {need ? workspace : nullptr, static_cast<int64_t>(need)}};
+    const Bytes r[1] = {{logits, rows_bytes(T, ld, E, dtype_bytes(dtype))}};
+    if (clash(w, r)) return fail(MR_EINVAL, "%s: outputs and the workspace must not overlap the logits or each other", fn);
+  }
+  RouteParams p{};
+  int64_t chunk;
+  p.blocks = route_blocks(T, &chunk);
+  p.chunk = static_cast<int>(chunk);
+  p.z = logits;
+  p.ldz = ld;
+  p.T = static_cast<int>(T);
+  p.E = static_cast<int>(E);
+  p.k = static_cast<int>(k);
+  p.normalize = normalize != 0;
+  p.scale = scale;
+  p.weights = weights;
+  p.ids = ids;
+  p.offsets = offsets;
+  p.slots = slots;
+  p.rows = rows;
+  p.counts = static_cast<int32_t*>(workspace);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid(p.blocks), block(kRouteThreads);
+  const size_t lds = route_lds(E);
+  const int lanes = route_lanes(E, k);
+#define MR_CHOOSE(DT, L, V) hipLaunchKernelGGL((route_choose<DT, L, V>), grid, block, lds, s, p)
+  MR_ROUTE_CASES(MR_CHOOSE);
+#undef MR_CHOOSE
+  MR_LAUNCH_CHECK(fn);
+  if (offsets && p.blocks > 1) {
+    hipLaunchKernelGGL(route_place, grid, block, lds, s, p);
+    MR_LAUNCH_CHECK(fn);
+  }
+  return MR_OK;
+}
+
+int mr_route_experts_bwd(const float* dweights, const void* logits, int dtype, int64_t ld, const int32_t* ids, int64_t T,
+                         int64_t E, int64_t k, int normalize, float scale, void* dlogits, int64_t lddz, void* stream) {
+  using namespace mr;
+  clear_error();
+  const char* fn = "mr_route_experts_bwd";
+  if (const int rc = check_route(fn, dtype, ld, T, E, k, logits)) return rc;
+  if (T == 0) return MR_OK;
+  if (!dweights || !logits || !ids || !dlogits) return fail(MR_EINVAL, "%s: null pointer", fn);
+  if (lddz < E) return fail(MR_EINVAL, "%s: a leading dimension is smaller than its row", fn);
+  const int es = dtype_bytes(dtype);
+  if (!on4(dweights, ids) || reinterpret_cast<uintptr_t>(dlogits) % es)
+    return fail(MR_EINVAL, "%s: a pointer is not aligned to its elements", fn);
+  {
+    const bool in_place = dlogits == logits && lddz == ld;
+    const Bytes w[1] = {{dlogits, rows_bytes(T, lddz, E, es)}};
+    const Bytes r[3] = {{in_place ? nullptr : logits, rows_bytes(T, ld, E, es)}, {dweights, T * k * 4}, {ids, T * k * 4}};
+    if (clash(w, r)) return fail(MR_EINVAL, "%s: dlogits may be the logits, and overlaps nothing else", fn);
+  }
+  RouteBwdParams p{};
+  p.f.z = logits;
+  p.f.ldz = ld;
+  p.f.T = static_cast<int>(T);
+  p.f.E = static_cast<int>(E);
+  p.f.k = static_cast<int>(k);
+  p.f.normalize = normalize != 0;
+  p.f.scale = scale;
+  p.f.ids = const_cast<int32_t*>(ids);
+  p.dw = dweights;
+  p.dz = dlogits;
+  p.lddz = lddz;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int lanes = route_lanes(E, k);
+  const int64_t blocks = (T * lanes + 255) / 256;
+  if (too_many_blocks(blocks, 256)) return fail(MR_EINVAL, "%s: too many rows", fn);
+  const dim3 grid(static_cast<unsigned>(blocks)), block(256);
+#define MR_BACK(DT, L, V) hipLaunchKernelGGL((route_bwd<DT, L, V>), grid, block, 0, s, p)
+  MR_ROUTE_CASES(MR_BACK);
+#undef MR_BACK
+  MR_LAUNCH_CHECK(fn);
+  return MR_OK;
+}
+
+int mr_combine_experts(const void* y, int y_dtype, int64_t ldy, int64_t R, const int32_t* slots, const float* weights,
+                       int64_t T, int64_t k, int64_t H, const void* resid, int64_t ldr, void* out, int out_dtype,
+                       int64_t ldo, void* stream) {
+  using namespace mr;
+  clear_error();
+  const char* fn = "mr_combine_experts";
+  if (const int rc = check_rows(fn, T, k, R, H)) return rc;
+  if ((y_dtype != MR_F32 && y_dtype != MR_BF16) || (out_dtype != MR_F32 && out_dtype != MR_BF16))
+    return fail(MR_EINVAL, "%s: rows are fp32 or bf16", fn);
+  if (T == 0 || H == 0) return MR_OK;
+  if (!slots || !out || (!y && R)) return fail(MR_EINVAL, "%s: null pointer", fn);
+  const int ey = dtype_bytes(y_dtype), eo = dtype_bytes(out_dtype);
+  if ((R > 0 && ldy < H) || ldo < H || (resid && ldr < H))
+    return fail(MR_EINVAL, "%s: a leading dimension is smaller than its row", fn);
+  if (reinterpret_cast<uintptr_t>(y) % ey || (reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(resid)) % eo ||
+      !on4(slots, weights))
+    return fail(MR_EINVAL, "%s: a pointer is not aligned to its elements", fn);
+  {
+    const bool in_place = out == resid && ldo == ldr;
+    const Bytes w[1] = {{out, rows_bytes(T, ldo, H, eo)}};
+    const Bytes r[4] = {{y, rows_bytes(R, ldy, H, ey)}, {in_place ? nullptr : resid, rows_bytes(T, ldr, H, eo)},
+                        {slots, T * k * 4}, {weights, T * k * 4}};
+    if (clash(w, r)) return fail(MR_EINVAL, "%s: out may be resid, and overlaps nothing else", fn);
+  }
+  RowsParams p{};
+  p.x = resid;
+  p.ldx = ldr;
+  p.y = const_cast<void*>(y);
+  p.ldy = ldy;
+  p.R = R;
+  p.slots = slots;
+  p.weights = weights;
+  p.out = out;
+  p.ldo = ldo;
+  p.T = T;
+  p.H = static_cast<int>(H);
+  p.k = static_cast<int>(k);
+  const bool vec = H % 8 == 0 && vector_rows(y, ldy, ey) && vector_rows(resid, ldr, eo) && vector_rows(out, ldo, eo);
+  p.pieces = static_cast<int>(vec ? H / 8 : H);
+  const int64_t blocks = (T * p.pieces + 255) / 256;
+  if (too_many_blocks(blocks, 256)) return fail(MR_EINVAL, "%s: too large", fn);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>(blocks)), block(256);
+#define MR_COMBINE(DY, DO)                                                                        \
+  do {                                                                                            \
+    if (vec) hipLaunchKernelGGL((combine_kernel<DY, DO, 8>), grid, block, 0, s, p);               \
+    else hipLaunchKernelGGL((combine_kernel<DY, DO, 1>), grid, block, 0, s, p);                   \
+  } while (0)
+  if (y_dtype == MR_BF16) {
+    if (out_dtype == MR_F32) MR_COMBINE(MR_BF16, MR_F32);
+    else MR_COMBINE(MR_BF16, MR_BF16);
+  } else {
+    if (out_dtype == MR_F32) MR_COMBINE(MR_F32, MR_F32);
+    else MR_COMBINE(MR_F32, MR_BF16);
+  }
+#undef MR_COMBINE
+  MR_LAUNCH_CHECK(fn);
+  return MR_OK;
+}
+
+int mr_spread_experts(const void* x, int x_dtype, int64_t ldx, const int32_t* slots, const float* weights, int64_t T,
+                      int64_t k, int64_t H, void* out, int out_dtype, int64_t ldo, int64_t R, const void* y, int64_t ldy,
+                      float* dweights, void* stream) {
+  using namespace mr;
+  clear_error();
+  const char* fn = "mr_spread_experts";
+  if (const int rc = check_rows(fn, T, k, R, H)) return rc;
+  if ((x_dtype != MR_F32 && x_dtype != MR_BF16) || (out_dtype != MR_F32 && out_dtype != MR_BF16))
+    return fail(MR_EINVAL, "%s: rows are fp32 or bf16", fn);
+  if (T == 0 || (H == 0 && !dweights)) return MR_OK;
+  if (!dweights != !y && R) return fail(MR_EINVAL, "%s: the weights' gradients and the rows they multiply come together", fn);
+  if (H == 0) return fail(MR_EINVAL, "%s: no columns to sum dweights over", fn);
+  if (!x || !slots || (!out && R)) return fail(MR_EINVAL, "%s: null pointer", fn);
+  const int ex = dtype_bytes(x_dtype), eo = dtype_bytes(out_dtype);
+  if (ldx < H || (R > 0 && (ldo < H || (y && ldy < H))))
+    return fail(MR_EINVAL, "%s: a leading dimension is smaller than its row", fn);
+  if (reinterpret_cast<uintptr_t>(x) % ex || (reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(y)) % eo ||
+      !on4(slots, weights, dweights))
+    return fail(MR_EINVAL, "%s: a pointer is not aligned to its elements", fn);
+  {
+    const bool in_place = out == y && ldo == ldy;
+    const Bytes w[2] = {{out, rows_bytes(R, ldo, H, eo)}, {dweights, T * k * 4}};
+    const Bytes r[4] = {{x, rows_bytes(T, ldx, H, ex)}, {in_place ? nullptr : y, rows_bytes(R, ldy, H, eo)},
+                        {slots, T * k * 4}, {weights, T * k * 4}};
+    if (clash(w, r)) return fail(MR_EINVAL, "%s: out may be y; outputs overlap nothing else", fn);
+  }
+  RowsParams p{};
+  p.x = x;
+  p.ldx = ldx;
+  p.y = out;
+  p.ldy = ldo;
+  p.y_old = y;
+  p.ldyo = ldy;
+  p.R = R;
+  p.slots = slots;
+  p.weights = weights;
+  p.dweights = dweights;
+  p.T = T;
+  p.H = static_cast<int>(H);
+  p.k = static_cast<int>(k);
+  const bool vec = H % 8 == 0 && vector_rows(x, ldx, ex) && vector_rows(out, ldo, eo) && vector_rows(y, ldy, eo);
+  p.pieces = static_cast<int>(vec ? H / 8 : H);
+  // A wave to a token where that fills the card twice over, else a block.
+  const bool one = T >= 4096 || p.pieces <= 64;
+  const int64_t blocks = one ? (T + 3) / 4 : T;
+  if (too_many_blocks(blocks, 256)) return fail(MR_EINVAL, "%s: too large", fn);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>(blocks)), block(256);
+#define MR_SPREAD(DX, DY)                                                                           \
+  do {                                                                                              \
+    if (vec && one) hipLaunchKernelGGL((spread_kernel<DX, DY, 8, 1>), grid, block, 0, s, p);        \
+    else if (vec) hipLaunchKernelGGL((spread_kernel<DX, DY, 8, 4>), grid, block, 0, s, p);          \
+    else if (one) hipLaunchKernelGGL((spread_kernel<DX, DY, 1, 1>), grid, block, 0, s, p);          \
+    else hipLaunchKernelGGL((spread_kernel<DX, DY, 1, 4>), grid, block, 0, s, p);                   \
+  } while (0)
+  if (x_dtype == MR_BF16) {
+    if (out_dtype == MR_F32) MR_SPREAD(MR_BF16, MR_F32);
+    else MR_SPREAD(MR_BF16, MR_BF16);
+  } else {
+    if (out_dtype == MR_F32) MR_SPREAD(MR_F32, MR_F32);
+    else MR_SPREAD(MR_F32, MR_BF16);
+  }
+#undef MR_SPREAD
+  MR_LAUNCH_CHECK(fn);
+  return MR_OK;
+}
+
+}  // extern "C"

@@ -110,6 +110,22 @@ struct GemmParams {
   int sub;
   float* ws;         // k-split partials (caller's workspace), or null: no split
   int64_t ws_bytes;
+  static constexpr bool kGrouped = false, kIndexed = false;
+};
+
+// A product grouped by expert: expert e's rows are offsets[e] .. offsets[e + 1] - 1
+// of A and C (K-major A; M, then, is all experts' rows) or of both operands'
+// k-rows (MN-major A: K is all rows, and C has a matrix an expert). The counts
+// are known on the device alone: the launch has the blocks of the worst case, and
+// those past the last tile leave (enter). INDEXED: row r of A is A's row index[r].
+template <bool INDEXED>
+struct GroupedParams : GemmParams {
+  const int32_t* offsets;
+  int experts;
+  const int32_t* index;
+  int64_t a_rows;          // INDEXED: the rows A has
+  int64_t b_step, c_step;  // elements between the experts' B (K-major A) and C (MN-major A)
+  static constexpr bool kGrouped = true, kIndexed = INDEXED;
 };
 
 // Logical tile -> (tile row, tile column): groups of 8 tile rows, column by
@@ -168,6 +184,11 @@ __device__ __forceinline__ rsrc_t make_rsrc(const void* base, int64_t bytes) {
                                            kRsrcFlags);
 }
 
+// The same over all that an unsigned offset of 32 bits reaches.
+__device__ __forceinline__ rsrc_t make_rsrc_all(const void* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, -1, kRsrcFlags);
+}
+
 // 16 bytes per lane from the buffer into LDS at lds + 16 * lane. (Kept out of
 // the templates: the host pass of hipcc drops the launch stubs of kernels
 // whose templates call this builtin directly.)
@@ -175,12 +196,14 @@ __device__ __forceinline__ void load_lds16(rsrc_t r, uint8_t* lds, int voff) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)lds, 16, voff, 0, 0, 0);
 }
 
-template <int ROWS>
+// index: the operand's rows lie at index[row0 + ...] of a matrix of `all` rows
+// (offsets of 32 bits from its first, unsigned; other indices go to its ends).
+template <int ROWS, bool INDEXED = false>
 struct KMajorDirect {
   static constexpr int INSTR = ROWS * 8 / 64 / kLoaders;  // instructions per loading wave
   static_assert(INSTR * kLoaders * 64 == ROWS * 8, "the loading waves must cover every chunk of the tile");
   int voff[INSTR];
-  __device__ __forceinline__ void init(int64_t ld, int row0, int rows_valid) {
+  __device__ __forceinline__ void init(int64_t ld, int row0, int rows_valid, const int32_t* index = nullptr, int64_t all = 0) {
     const int lane = threadIdx.x & 63;
     const int wave = wave_id();
     const int sub = lane >> 3;
@@ -190,11 +213,17 @@ struct KMajorDirect {
       const int row = q * 8 + sub;
       const int chunk = (lane & 7) ^ swz_bits(row);
       const int g = min(row0 + row, rows_valid - 1);
-      voff[i] = static_cast<int>(((g - row0) * ld + chunk * 8) * 2);
+      if constexpr (INDEXED) {
+        const int at = min(max(index[g], 0), static_cast<int>(all - 1));
+        voff[i] = static_cast<int>((static_cast<uint32_t>(at) * static_cast<uint32_t>(ld) + chunk * 8) * 2);
+      } else {
+        voff[i] = static_cast<int>(((g - row0) * ld + chunk * 8) * 2);
+      }
     }
   }
   // The buffer over the operand from row row0, k0 on; then load i of this wave's INSTR into a stage.
   __device__ __forceinline__ static rsrc_t at(const uint16_t* base, int64_t ld, int row0, int rows_valid, int k0) {
+    if constexpr (INDEXED) return make_rsrc_all(base + k0);
     return make_rsrc(base + row0 * ld + k0, (static_cast<int64_t>(rows_valid - row0) * ld - k0) * 2);
   }
   __device__ __forceinline__ void issue_one(rsrc_t r, int i, uint8_t* lds) const {
@@ -202,8 +231,7 @@ struct KMajorDirect {
   }
   __device__ __forceinline__ void issue(const uint16_t* base, int64_t ld, int row0, int rows_valid,
                                         int k0, uint8_t* lds) const {
-    const uint16_t* b = base + row0 * ld + k0;
-    const rsrc_t r = make_rsrc(b, (static_cast<int64_t>(rows_valid - row0) * ld - k0) * 2);
+    const rsrc_t r = at(base, ld, row0, rows_valid, k0);
     const int wave = wave_id();
     if (wave >= kLoaders) return;
 #pragma unroll
@@ -737,8 +765,90 @@ __device__ __forceinline__ void store_partial(float* out, const f32x16 (&acc)[TM
             f32x4{acc[i][j][4 * gi], acc[i][j][4 * gi + 1], acc[i][j][4 * gi + 2], acc[i][j][4 * gi + 3]};
 }
 
-template <int BM, int BN, bool A_KMAJOR, bool B_KMAJOR, int EPI, bool OUT_BF16>
-__global__ __launch_bounds__(kThreads) void gemm_kernel(GemmParams p) {
+// The tile of block `bid` of a grouped product: p becomes its expert's product
+// and (bm, bn) the tile in it. False where the block has none. Each wave counts
+// the experts' tiles by itself (64 experts at a time, a scan over the lanes,
+// 0.3 us), which is less than a launch that would write a list of them. Offsets
+// are held between 0 and the rows there are, so that no others lead outside.
+template <int BM, int BN, bool A_KMAJOR, bool OUT_BF16, bool INDEXED>
+__device__ __forceinline__ bool enter(GroupedParams<INDEXED>& p, int bid, int& bm, int& bn) {
+  const int rows = A_KMAJOR ? p.M : p.K;
+  auto at = [&](int i) __attribute__((always_inline)) { return min(max(p.offsets[i], 0), rows); };
+  p.grid_n = (p.N + BN - 1) / BN;
+  int e, first, len, lt;
+  if constexpr (A_KMAJOR) {
+    const int lane = threadIdx.x & 63;
+    auto tiles = [&](int i) __attribute__((always_inline)) {
+      return i < p.experts ? (max(at(i + 1) - at(i), 0) + BM - 1) / BM * p.grid_n : 0;
+    };
+    int total = 0;
+    for (int c = 0; c < p.experts; c += 64) total += tiles(c + lane);
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) total += __shfl_xor(total, o, 64);
+    total = __builtin_amdgcn_readfirstlane(total);
+    if (bid >= total) return false;
+    lt = xcd_order(bid, total);
+    e = -1;
+    for (int c = 0; c < p.experts && e < 0; c += 64) {
+      const int own = tiles(c + lane);
+      int upto = own;
+#pragma unroll
+      for (int o = 1; o < 64; o *= 2) {
+        const int before = __shfl_up(upto, o, 64);
+        upto += lane >= o ? before : 0;
+      }
+      const uint64_t past = __ballot(upto > lt);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        e = c + l;
+        lt -= __builtin_amdgcn_readlane(upto - own, l);
+      } else {
+        lt -= __builtin_amdgcn_readlane(upto, 63);
+      }
+    }
+    if (e < 0) return false;
+    first = __builtin_amdgcn_readfirstlane(at(e));
+    len = __builtin_amdgcn_readfirstlane(at(e + 1)) - first;
+    p.M = len;
+    p.grid_m = (len + BM - 1) / BM;
+    if constexpr (INDEXED) p.index += first;
+    else p.A += first * p.lda;
+    p.B += e * p.b_step;
+    const int64_t c0 = first * p.ldc;
+    p.C = OUT_BF16 ? static_cast<void*>(static_cast<uint16_t*>(p.C) + c0) : static_cast<void*>(static_cast<float*>(p.C) + c0);
+    if (p.gu) p.gu += first * p.ldgu;
+  } else {
+    p.grid_m = (p.M + BM - 1) / BM;
+    const int per = p.grid_m * p.grid_n;
+    lt = xcd_order(bid, per * p.experts);
+    e = lt / per;
+    lt -= e * per;
+    first = __builtin_amdgcn_readfirstlane(at(e));
+    len = max(__builtin_amdgcn_readfirstlane(at(e + 1)) - first, 0);
+    p.K = len;
+    p.A += first * p.lda;
+    p.B += first * p.ldb;
+    p.C = static_cast<float*>(p.C) + e * p.c_step;
+    if (p.resid) p.resid += e * p.c_step;
+  }
+  p.kt_per = (p.K + BK - 1) / BK;
+  tile_coords(lt, p.grid_m, p.grid_n, bm, bn);
+  return true;
+}
+
+// An expert without rows has a gradient of zeros, which its BM x BN tile gets here.
+template <int BM, int BN, int EPI>
+__device__ __forceinline__ void store_zeros(const GemmParams& p, int m0, int n0) {
+  if (EPI == EPI_RESID) return;  // (added to what is there)
+  float* const c = static_cast<float*>(p.C);
+  for (int i = threadIdx.x; i < BM * (BN / 4); i += blockDim.x) {
+    const int row = m0 + i / (BN / 4), col = n0 + i % (BN / 4) * 4;
+    if (row < p.M && col < p.N) *reinterpret_cast<float4*>(c + row * p.ldc + col) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+}
+
+template <int BM, int BN, bool A_KMAJOR, bool B_KMAJOR, int EPI, bool OUT_BF16, class P = GemmParams>
+__global__ __launch_bounds__(kThreads) void gemm_kernel(P p) {
   constexpr int WM = BM / kWaveRows, WN = BN / (kWaves / kWaveRows);
   constexpr int TM = WM / 32, TN = WN / 32;
   // Every epilogue feeds the MFMA with B as the first operand and A as the
@@ -760,14 +870,17 @@ __global__ __launch_bounds__(kThreads) void gemm_kernel(GemmParams p) {
   // XCD-aware renumbering, then the grouped order along M. Split launches take
   // the splits of one tile as consecutive blocks.
   int bid = blockIdx.x, split = 0;
-  if (p.ksplit > 1) {
+  if (P::kGrouped) {
+  } else if (p.ksplit > 1) {
     split = bid % p.ksplit;
     bid /= p.ksplit;
   } else if ((p.n_tiles & 7) == 0 || p.K > 8 * BK) {
     bid = xcd_order(bid, p.n_tiles);
   }
   int bm, bn;
-  if (p.sub) {
+  if constexpr (P::kGrouped) {
+    if (!enter<BM, BN, A_KMAJOR, OUT_BF16>(p, bid, bm, bn)) return;  // (the whole block)
+  } else if (p.sub) {
     tile_coords(p.tile0 + (bid >> 2), p.grid_m, p.grid_n, bm, bn);
     bm = 2 * bm + ((bid >> 1) & 1);
     bn = 2 * bn + (bid & 1);
@@ -777,15 +890,19 @@ __global__ __launch_bounds__(kThreads) void gemm_kernel(GemmParams p) {
   const int m0 = bm * BM;
   const int n0 = bn * BN;
   if (m0 >= p.M || n0 >= p.N) return;  // a quarter wholly past the edge (the whole block leaves)
+  if constexpr (P::kGrouped && !A_KMAJOR) {
+    if (p.K == 0) return store_zeros<BM, BN, EPI>(p, m0, n0);
+  }
 
   const int lane = threadIdx.x & 63;
   const int wave = wave_id();
   const int wm = wave / (kWaves / kWaveRows), wn = wave % (kWaves / kWaveRows);
 
   // Global loads of tile kt, straight into the given LDS stage.
-  std::conditional_t<A_KMAJOR, KMajorDirect<BM>, MNMajorDirect<BM>> ld_a;
+  std::conditional_t<A_KMAJOR, KMajorDirect<BM, P::kIndexed>, MNMajorDirect<BM>> ld_a;
   std::conditional_t<B_KMAJOR, KMajorDirect<BN>, MNMajorDirect<BN>> ld_b;
-  ld_a.init(p.lda, m0, p.M);
+  if constexpr (P::kIndexed) ld_a.init(p.lda, m0, p.M, p.index, p.a_rows);
+  else ld_a.init(p.lda, m0, p.M);
   ld_b.init(p.ldb, n0, p.N);
   auto issue_loads = [&](int kt, uint8_t* as_dst, uint8_t* bs_dst) {
     const int k0 = kt * BK;
@@ -912,7 +1029,7 @@ __global__ __launch_bounds__(kThreads) void gemm_kernel(GemmParams p) {
   };
 
   const int kt_begin = split * p.kt_per;
-  const int KT = min(p.K / BK, kt_begin + p.kt_per);
+  const int KT = P::kGrouped ? p.kt_per : min(p.K / BK, kt_begin + p.kt_per);
   if (kt_begin < KT) {
     issue_loads(kt_begin, As0, Bs0);
     __builtin_amdgcn_s_waitcnt(0);
@@ -926,7 +1043,7 @@ __global__ __launch_bounds__(kThreads) void gemm_kernel(GemmParams p) {
   }
 
   // ---- epilogue ----
-  if (p.ksplit > 1) {
+  if (!P::kGrouped && p.ksplit > 1) {
     store_partial<BM, BN>(p.ws + (static_cast<int64_t>(bid) * p.ksplit + split) * (BM * BN), acc, wm * TM, wn * TN, lane);
     return;
   }
@@ -959,8 +1076,8 @@ __global__ __launch_bounds__(kThreads) void gemm_kernel(GemmParams p) {
 // Measured on the 7B block's plain products: 3-11 % faster than the 8-wave
 // kernel (gate/up 16384 x 37888 x 3584: 1340 against 1220 TFLOP/s).
 constexpr int kWaves4 = 4;
-template <bool A_KMAJOR, bool B_KMAJOR, int EPI, bool OUT_BF16>
-__global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1, 1))) void gemm4_kernel(GemmParams p) {
+template <bool A_KMAJOR, bool B_KMAJOR, int EPI, bool OUT_BF16, class P = GemmParams>
+__global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1, 1))) void gemm4_kernel(P p) {
   constexpr int BM = 256, BN = 256, WM = 128, WN = 128, TM = WM / 32, TN = WN / 32;
   constexpr int STAGE = 256 * ROW_BYTES;  // bytes of one operand stage (either layout)
   static_assert(STAGE == MNMajorDirect<256>::ROWB * BK, "both layouts stage 32 KB");
@@ -973,25 +1090,33 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
   // A k-split launch takes the splits of one tile as consecutive blocks, each
   // over kt_per k-tiles (the last over what remains).
   int bid = blockIdx.x, split = 0;
-  if (p.ksplit > 1) {
-    split = bid % p.ksplit;
-    bid /= p.ksplit;
-  } else {
-    bid = xcd_order(bid, p.n_tiles);
-  }
   int bm, bn;
-  tile_coords(p.tile0 + bid, p.grid_m, p.grid_n, bm, bn);
+  if constexpr (P::kGrouped) {
+    if (!enter<BM, BN, A_KMAJOR, OUT_BF16>(p, bid, bm, bn)) return;  // (the whole block)
+  } else {
+    if (p.ksplit > 1) {
+      split = bid % p.ksplit;
+      bid /= p.ksplit;
+    } else {
+      bid = xcd_order(bid, p.n_tiles);
+    }
+    tile_coords(p.tile0 + bid, p.grid_m, p.grid_n, bm, bn);
+  }
   const int m0 = bm * BM, n0 = bn * BN;
+  if constexpr (P::kGrouped && !A_KMAJOR) {
+    if (p.K == 0) return store_zeros<BM, BN, EPI>(p, m0, n0);
+  }
   const int lane = threadIdx.x & 63;
   const int wave = wave_id();
   const int wm = wave >> 1, wn = wave & 1;
 
-  std::conditional_t<A_KMAJOR, KMajorDirect<BM>, MNMajorDirect<BM>> ld_a;
+  std::conditional_t<A_KMAJOR, KMajorDirect<BM, P::kIndexed>, MNMajorDirect<BM>> ld_a;
   std::conditional_t<B_KMAJOR, KMajorDirect<BN>, MNMajorDirect<BN>> ld_b;
-  ld_a.init(p.lda, m0, p.M);
+  if constexpr (P::kIndexed) ld_a.init(p.lda, m0, p.M, p.index, p.a_rows);
+  else ld_a.init(p.lda, m0, p.M);
   ld_b.init(p.ldb, n0, p.N);
   const int kt0 = split * p.kt_per;
-  const int KT = min(p.K / BK - kt0, p.kt_per);  // this block's k-tiles: kt0 .. kt0 + KT - 1
+  const int KT = P::kGrouped ? p.kt_per : min(p.K / BK - kt0, p.kt_per);  // this block's k-tiles: kt0 .. kt0 + KT - 1
   auto tk = [&](int u) { return kt0 + min(u, KT - 1); };
   auto ra_at = [&](int kt) { return ld_a.at(p.A, p.lda, m0, A_KMAJOR ? p.M : p.K, kt * BK); };
   auto rb_at = [&](int kt) { return ld_b.at(p.B, p.ldb, n0, B_KMAJOR ? p.N : p.K, kt * BK); };
@@ -1165,7 +1290,7 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
   // the repeated last loads land, every wave is past its reads: LDS is free
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  if (p.ksplit > 1) {
+  if (!P::kGrouped && p.ksplit > 1) {
     store_partial<BM, BN>(p.ws + (static_cast<int64_t>(bid) * p.ksplit + split) * (BM * BN), acc, wm * TM, wn * TN, lane);
     return;
   }

@@ -25,6 +25,7 @@ from mround_amd.exceptions import KernelError, KernelUnavailableError
 __all__ = [
     "MODE",
     "act_bwd",
+    "combine_experts",
     "copy_bytes",
     "cross_entropy",
     "delta_loss",
@@ -36,15 +37,23 @@ __all__ = [
     "fq_forward",
     "gemm_act",
     "gemm_act_bwd",
+    "gemm_experts",
+    "gemm_experts_swiglu",
+    "gemm_experts_swiglu_bwd",
     "lib",
     "lib_path",
     "loss_mse",
     "loss_outlier",
     "loss_workspace",
+    "norm_residual",
+    "norm_residual_bwd",
     "pack_codes",
     "packed_width",
     "quantize_pack",
     "rope_positions",
+    "route_experts",
+    "route_experts_bwd",
+    "spread_experts",
     "to_affine",
     "top_logits",
     "unpack_codes",
@@ -97,6 +106,18 @@ _SIGNATURES = {
     "mr_gemm_act_bwd": (_I, [_L, _L, _L, _P, _L, _P, _L, _P, _L, _I, _P, _L, _P, _P, ctypes.c_size_t, _P,
                              ctypes.c_size_t, _P]),
     "mr_act_bwd": (_I, [_L, _L, _P, _I, _L, _P, _L, _I, _P, _L, _P, _P, ctypes.c_size_t, _P]),
+    "mr_gemm_experts": (_I, [_I, _L, _L, _L, _L, _P, _L, _P, _L, _P, _L, _L, _P, _P, _I, _L, _L, _I, _P]),
+    "mr_gemm_experts_swiglu": (_I, [_L, _L, _L, _L, _P, _L, _P, _L, _P, _L, _L, _P, _P, _L, _P, _L, _P]),
+    "mr_gemm_experts_swiglu_bwd": (_I, [_L, _L, _L, _L, _P, _L, _P, _L, _L, _P, _P, _L, _P, _L, _P]),
+    "mr_route_workspace_bytes": (ctypes.c_size_t, [_L, _L]),
+    "mr_route_experts": (_I, [_P, _I, _L, _L, _L, _L, _I, _F, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
+    "mr_route_experts_bwd": (_I, [_P, _P, _I, _L, _P, _L, _L, _L, _I, _F, _P, _L, _P]),
+    "mr_combine_experts": (_I, [_P, _I, _L, _L, _P, _P, _L, _L, _L, _P, _L, _P, _I, _L, _P]),
+    "mr_spread_experts": (_I, [_P, _I, _L, _P, _P, _L, _L, _L, _P, _I, _L, _L, _P, _L, _P, _P]),
+    "mr_norm_residual": (_I, [_P, _I, _L, _P, _I, _L, _L, _L, _F, _P, _P, _L, _F, _P, _P, _L, _P, _L, _P]),
+    "mr_norm_residual_bwd_workspace_bytes": (ctypes.c_size_t, [_L, _L, _L, _I, _I, _I]),
+    "mr_norm_residual_bwd": (_I, [_P, _I, _L, _P, _I, _L, _P, _L, _P, _L, _L, _L, _F, _P, _P, _L, _F, _P, _P, _L, _P,
+                                  _L, _P, _P, _P, _P, ctypes.c_size_t, _P]),
     "mr_rmsnorm_fwd": (_I, [_P, _P, _L, _L, _F, _P, _P, _P]),
     "mr_rmsnorm_bwd": (_I, [_P, _P, _P, _P, _P, _L, _L, _P, _P, _P]),
     "mr_rmsnorm_fwd_split": (_I, [_P, _P, _L, _L, _F, _P, _P, _P, _P]),
@@ -683,6 +704,303 @@ def act_bwd(dout, pre, dpre, *, act, dbias=None) -> None:
     rc = lib().mr_act_bwd(M, N, _rows_ptr(dout), dtype_code(dout.dtype), _ld(dout), _rows_ptr(pre), _ld(pre), code,
                           _rows_ptr(dpre), _ld(dpre), _ptr(dbias), part_ptr, part_bytes, _stream(dout))
     _check(rc, "mr_act_bwd")
+
+
+# ------------------------------------------------------------------ experts --
+
+def _dense(name: str, what: str, t, dtype, shape) -> None:
+    """A contiguous tensor of one type and shape, or None."""
+    if t is not None and (t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
+        raise KernelError(f"{name}: {what} must be contiguous {str(dtype).removeprefix('torch.')} {list(shape)}, got "
+                          f"{t.dtype} {list(t.shape)}")
+
+
+def _matrix(name: str, what: str, t, dtypes, shape) -> None:
+    if t is not None and (t.dtype not in dtypes or t.dim() != 2 or tuple(t.shape) != tuple(shape)):
+        kinds = " or ".join(str(d).removeprefix("torch.") for d in dtypes)
+        raise KernelError(f"{name}: {what} must be {kinds} {list(shape)}, got {t.dtype} {list(t.shape)}")
+
+
+def _stacked(name: str, what: str, t, dtype, shape):
+    """The experts' matrices ``[E, rows, cols]``, unit stride along a row: (leading
+    dimension, elements between experts)."""
+    if t.dtype != dtype or t.dim() != 3 or tuple(t.shape) != tuple(shape) or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise KernelError(f"{name}: {what} must be {str(dtype).removeprefix('torch.')} {list(shape)} with contiguous "
+                          f"rows, got {t.dtype} {list(t.shape)}")
+    ld = t.stride(1) if t.shape[1] > 1 else t.shape[2]
+    # (one expert's step says nothing: torch leaves any value there)
+    return ld, (t.stride(0) if t.shape[0] > 1 else t.shape[1] * ld)
+
+
+def route_experts(logits, *, weights, ids, offsets=None, slots=None, rows=None, normalize=False, scale=1.0) -> None:
+    """``mr_route_experts``: each token's ``k`` likeliest experts from ``logits``
+    ``[T, E]`` (float32, bfloat16 or float16; rows may be strided), in descending
+    order, ties to the lower index: int32 ``ids`` and float32 ``weights`` ``[T,
+    k]``, ``scale`` times the softmax over all experts, or with ``normalize`` over
+    the chosen. A logit of -inf is never chosen; an entry that finds none has id -1
+    and weight 0. With ``offsets`` ``[E + 1]``, ``slots`` ``[T, k]`` and ``rows``
+    ``[T k]`` (int32) also the order of the tokens by expert that the grouped
+    products take: expert e's places are ``offsets[e] .. offsets[e + 1] - 1``,
+    ``slots`` the place of each entry (-1: none), ``rows`` the token at each place
+    (those past the last are left). E is at most 512 and k at most 64."""
+    T, E = logits.shape if logits.dim() == 2 else (-1, -1)
+    if T < 0 or weights.dim() != 2:
+        raise KernelError("route_experts: logits [T, E] and weights [T, k] are matrices")
+    k = weights.shape[1]
+    _dense("route_experts", "weights", weights, torch.float32, (T, k))
+    _dense("route_experts", "ids", ids, torch.int32, (T, k))
+    _dense("route_experts", "offsets", offsets, torch.int32, (E + 1,))
+    _dense("route_experts", "slots", slots, torch.int32, (T, k))
+    _dense("route_experts", "rows", rows, torch.int32, (T * k,))
+    if (offsets is None) != (slots is None) or (offsets is None) != (rows is None):
+        raise KernelError("route_experts: offsets, slots and rows come together")
+    _one_device("route_experts", logits, weights, ids, offsets, slots, rows)
+    nbytes = int(lib().mr_route_workspace_bytes(T, E)) if offsets is not None else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
+    rc = lib().mr_route_experts(_rows_ptr(logits), dtype_code(logits.dtype), _ld(logits), T, E, k, int(normalize), scale,
+                                _ptr(weights), _ptr(ids), _ptr(offsets), _ptr(slots), _ptr(rows), _ptr(ws), nbytes,
+                                _stream(logits))
+    _check(rc, "mr_route_experts")
+
+
+def route_experts_bwd(dweights, logits, ids, dlogits, *, normalize=False, scale=1.0) -> None:
+    """``mr_route_experts_bwd``: the gradient ``dlogits`` (the logits' type; may be
+    ``logits``) from that of the weights, ``dweights`` ``[T, k]`` float32, for the
+    ``ids`` that :func:`route_experts` chose with the same ``normalize`` and
+    ``scale``."""
+    T, E = logits.shape if logits.dim() == 2 else (-1, -1)
+    if T < 0 or ids.dim() != 2:
+        raise KernelError("route_experts_bwd: logits [T, E] and ids [T, k] are matrices")
+    k = ids.shape[1]
+    _dense("route_experts_bwd", "ids", ids, torch.int32, (T, k))
+    _dense("route_experts_bwd", "dweights", dweights, torch.float32, (T, k))
+    _matrix("route_experts_bwd", "dlogits", dlogits, (logits.dtype,), (T, E))
+    _one_device("route_experts_bwd", logits, ids, dweights, dlogits)
+    rc = lib().mr_route_experts_bwd(_ptr(dweights), _rows_ptr(logits), dtype_code(logits.dtype), _ld(logits), _ptr(ids), T,
+                                    E, k, int(normalize), scale, _rows_ptr(dlogits), _ld(dlogits), _stream(logits))
+    _check(rc, "mr_route_experts_bwd")
+
+
+def gemm_experts(layout: str, a, b, c, *, offsets, rows=None, accumulate=False) -> None:
+    """``mr_gemm_experts``: products of rows in the experts' order (``offsets``
+    int32 ``[E + 1]``, as :func:`route_experts` gives them) with each expert's matrix,
+    bfloat16 operands:
+
+    * "nt": ``c[r] = a[r] b[e]^T``, ``b`` ``[E, N, K]``, ``c`` ``[R, N]`` bfloat16 or
+      float32; with ``rows`` (int32 ``[R]``) row r of ``a`` is its row ``rows[r]``;
+    * "nn": ``c[r] = a[r] b[e]``, ``b`` ``[E, K, N]``;
+    * "tn": ``c[e] = a[rows of e]^T b[rows of e]``, ``c`` ``[E, M, N]`` float32 (zeros
+      for an expert without rows), or with ``accumulate`` added to what ``c`` holds.
+
+    Rows of ``c`` outside the offsets are left. N (and M) is a multiple of 8, K of
+    64; the experts' row counts are any."""
+    if layout not in GEMM_LAYOUT:
+        raise KernelError(f"gemm_experts: layout must be one of {', '.join(GEMM_LAYOUT)}, got {layout!r}")
+    name = "gemm_experts"
+    _bf16_matrix(name, "a", a)
+    E = offsets.numel() - 1
+    _dense(name, "offsets", offsets, torch.int32, (E + 1,))
+    a_rows = a.shape[0]
+    if layout == "tn":
+        (K, M), N = a.shape, b.shape[-1]
+        _bf16_matrix(name, "b", b, (K, N))
+        ldc, c_step = _stacked(name, "c", c, torch.float32, (E, M, N))
+        ldb, b_step = _ld(b), 0
+        if rows is not None:
+            raise KernelError("gemm_experts: only the rows of an 'nt' product may lie at an index")
+    else:
+        if b.dim() != 3:
+            raise KernelError("gemm_experts: b must hold a matrix for each expert")
+        M, K = (a_rows if rows is None else rows.numel()), a.shape[1]
+        N = b.shape[1] if layout == "nt" else b.shape[2]
+        ldb, b_step = _stacked(name, "b", b, torch.bfloat16, (E, N, K) if layout == "nt" else (E, K, N))
+        _matrix(name, "c", c, (torch.bfloat16, torch.float32), (M, N))
+        _dense(name, "rows", rows, torch.int32, (M,))
+        ldc, c_step = _ld(c), 0
+    _one_device(name, a, b, c, offsets, rows)
+    rc = lib().mr_gemm_experts(GEMM_LAYOUT[layout], E, M, N, K, _rows_ptr(a), _ld(a), _ptr(rows), a_rows, b.data_ptr(),
+                               ldb, b_step, _ptr(offsets), c.data_ptr(), dtype_code(c.dtype), ldc, c_step,
+                               int(accumulate), _stream(a))
+    _check(rc, "mr_gemm_experts")
+
+
+def gemm_experts_swiglu(x, wgu, act, gu=None, *, offsets, rows=None) -> None:
+    """``mr_gemm_experts_swiglu``: :func:`gemm_swiglu` over rows in the experts'
+    order, each with its expert's interleaved gate/up weight, ``wgu`` ``[E, 2N, K]``;
+    ``act`` ``[R, N]`` and ``gu`` ``[R, 2N]`` bfloat16. ``offsets`` and ``rows`` as
+    :func:`gemm_experts`'. N is a multiple of 32, K of 64."""
+    name = "gemm_experts_swiglu"
+    _bf16_matrix(name, "x", x)
+    E = offsets.numel() - 1
+    _dense(name, "offsets", offsets, torch.int32, (E + 1,))
+    if wgu.dim() != 3 or wgu.shape[1] % 2:
+        raise KernelError(f"{name}: wgu must be [E, 2N, K]")
+    x_rows, K = x.shape
+    R, N = (x_rows if rows is None else rows.numel()), wgu.shape[1] // 2
+    ldw, step = _stacked(name, "wgu", wgu, torch.bfloat16, (E, 2 * N, K))
+    _bf16_matrix(name, "act", act, (R, N))
+    if gu is not None:
+        _bf16_matrix(name, "gu", gu, (R, 2 * N))
+    _dense(name, "rows", rows, torch.int32, (R,))
+    _one_device(name, x, wgu, act, gu, offsets, rows)
+    rc = lib().mr_gemm_experts_swiglu(E, R, N, K, _rows_ptr(x), _ld(x), _ptr(rows), x_rows, wgu.data_ptr(), ldw, step,
+                                      _ptr(offsets), _rows_ptr(act), _ld(act), _rows_ptr(gu), _ld(gu), _stream(x))
+    _check(rc, "mr_gemm_experts_swiglu")
+
+
+def gemm_experts_swiglu_bwd(dy, wd, gu, dgu, *, offsets) -> None:
+    """``mr_gemm_experts_swiglu_bwd``: ``dgu`` from ``dact = dy[r] wd[e]`` and the saved
+    interleaved gate/up ``gu`` ``[R, 2N]`` (``dgu`` may be ``gu``); ``wd`` ``[E, K,
+    N]``, the down weights, ``dy`` ``[R, K]`` in the experts' order."""
+    name = "gemm_experts_swiglu_bwd"
+    _bf16_matrix(name, "dy", dy)
+    E = offsets.numel() - 1
+    _dense(name, "offsets", offsets, torch.int32, (E + 1,))
+    if wd.dim() != 3:
+        raise KernelError(f"{name}: wd must be [E, K, N]")
+    (R, K), N = dy.shape, wd.shape[2]
+    ldw, step = _stacked(name, "wd", wd, torch.bfloat16, (E, K, N))
+    _bf16_matrix(name, "gu", gu, (R, 2 * N))
+    _bf16_matrix(name, "dgu", dgu, (R, 2 * N))
+    _one_device(name, dy, wd, gu, dgu, offsets)
+    rc = lib().mr_gemm_experts_swiglu_bwd(E, R, N, K, _rows_ptr(dy), _ld(dy), wd.data_ptr(), ldw, step, _ptr(offsets),
+                                          _rows_ptr(gu), _ld(gu), _rows_ptr(dgu), _ld(dgu), _stream(dy))
+    _check(rc, "mr_gemm_experts_swiglu_bwd")
+
+
+_ROW_TYPES = (torch.float32, torch.bfloat16)
+
+
+def combine_experts(y, slots, out, *, weights=None, resid=None) -> None:
+    """``mr_combine_experts``: ``out[t] = resid[t] + sum_j weights[t, j] y[slots[t,
+    j]]`` (float32 sums in order of j), ``y`` ``[R, H]`` in the experts' order,
+    ``slots`` int32 ``[T, k]`` (negative: no entry), float32 ``weights`` ``[T, k]``
+    (None: 1). ``y`` and ``out`` float32 or bfloat16; ``resid`` of ``out``'s type, and
+    may be ``out``."""
+    name = "combine_experts"
+    T, k = slots.shape if slots.dim() == 2 else (-1, -1)
+    R, H = y.shape if y.dim() == 2 else (-1, -1)
+    _dense(name, "slots", slots, torch.int32, (T, k))
+    _matrix(name, "y", y, _ROW_TYPES, (R, H))
+    _matrix(name, "out", out, _ROW_TYPES, (T, H))
+    _matrix(name, "resid", resid, (out.dtype,), (T, H))
+    _dense(name, "weights", weights, torch.float32, (T, k))
+    _one_device(name, y, slots, out, weights, resid)
+    rc = lib().mr_combine_experts(_rows_ptr(y), dtype_code(y.dtype), _ld(y), R, _ptr(slots), _ptr(weights), T, k, H,
+                                  _rows_ptr(resid), _ld(resid), _rows_ptr(out), dtype_code(out.dtype), _ld(out),
+                                  _stream(y))
+    _check(rc, "mr_combine_experts")
+
+
+def spread_experts(x, slots, out, *, weights=None, y=None, dweights=None) -> None:
+    """``mr_spread_experts``: ``out[slots[t, j]] = weights[t, j] x[t]`` (weights None:
+    1), the rows ``x`` ``[T, H]`` in the experts' order (negative slots: none; places
+    without an entry are left). For the backward of :func:`combine_experts` ``x`` is its
+    output's gradient and ``dweights`` ``[T, k]`` (float32) receives ``x[t] .
+    y[slots[t, j]]``. ``x`` and ``out`` float32 or bfloat16, ``y`` of ``out``'s type and
+    shape, and may be ``out``."""
+    name = "spread_experts"
+    T, k = slots.shape if slots.dim() == 2 else (-1, -1)
+    R, H = out.shape if out.dim() == 2 else (-1, -1)
+    _dense(name, "slots", slots, torch.int32, (T, k))
+    _matrix(name, "x", x, _ROW_TYPES, (T, H))
+    _matrix(name, "out", out, _ROW_TYPES, (R, H))
+    _matrix(name, "y", y, (out.dtype,), (R, H))
+    _dense(name, "weights", weights, torch.float32, (T, k))
+    _dense(name, "dweights", dweights, torch.float32, (T, k))
+    if (y is None) != (dweights is None):
+        raise KernelError("spread_experts: the weights' gradients and the rows they multiply come together")
+    _one_device(name, x, slots, out, weights, y, dweights)
+    rc = lib().mr_spread_experts(_rows_ptr(x), dtype_code(x.dtype), _ld(x), _ptr(slots), _ptr(weights), T, k, H,
+                                 _rows_ptr(out), dtype_code(out.dtype), _ld(out), R, _rows_ptr(y), _ld(y),
+                                 _ptr(dweights), _stream(x))
+    _check(rc, "mr_spread_experts")
+
+
+# -------------------------------------------------------------------- norms --
+
+_ACT_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _norm_types(name: str, y, stream):
+    if y.dtype not in _ACT_TYPES or stream.dtype not in (torch.float32, y.dtype) or y.dim() != 2:
+        raise KernelError(f"{name}: the branch is a float32, bfloat16 or float16 matrix and the stream float32 or of its "
+                          f"type, got {y.dtype} {list(y.shape)} and {stream.dtype}")
+
+
+def _gate(name: str, gate, gate_rows, T: int, H: int) -> int:
+    """Rows a gate row applies to."""
+    if gate is None:
+        return 0
+    per = max(T, 1) if gate_rows is None else int(gate_rows)
+    if per <= 0:
+        raise KernelError(f"{name}: gate_rows must be positive, got {gate_rows}")
+    _dense(name, "gate", gate, torch.float32, (-(-T // per), H) if T else tuple(gate.shape[:1]) + (H,))
+    return per
+
+
+def norm_residual(y, resid, out, *, eps, post=None, gate=None, gate_rows=None, scale=1.0, pre=None, normed=None) -> None:
+    """``mr_norm_residual``: the end of a block's branch and the norm after it, ``out =
+    resid + scale gate rmsnorm(y) post`` and ``normed = rmsnorm(out) pre``, over rows
+    ``[T, H]`` (which may be strided). ``post`` None: ``y`` itself; ``gate`` float32
+    ``[G, H]``, a row for each ``gate_rows`` rows (None: one for all), or None: 1;
+    ``pre`` and ``normed`` together or not at all. The branch (``y``, ``normed``) is
+    float32, bfloat16 or float16, the stream (``resid``, ``out``) float32 or of the
+    same type; weights are float32 ``[H]``. Sums are float32, and ``normed`` is that of
+    ``out`` before it is rounded. ``out`` may be ``resid``, ``normed`` may be ``y``. H is
+    at most 16384."""
+    name = "norm_residual"
+    _norm_types(name, y, resid)
+    T, H = y.shape
+    _matrix(name, "resid", resid, (resid.dtype,), (T, H))
+    _matrix(name, "out", out, (resid.dtype,), (T, H))
+    _matrix(name, "normed", normed, (y.dtype,), (T, H))
+    for what, w in (("post", post), ("pre", pre)):
+        _dense(name, what, w, torch.float32, (H,))
+    if (pre is None) != (normed is None):
+        raise KernelError("norm_residual: the next norm's weight and its output come together")
+    per = _gate(name, gate, gate_rows, T, H)
+    _one_device(name, y, resid, out, post, gate, pre, normed)
+    rc = lib().mr_norm_residual(_rows_ptr(y), dtype_code(y.dtype), _ld(y), _rows_ptr(resid), dtype_code(resid.dtype),
+                                _ld(resid), T, H, eps, _ptr(post), _ptr(gate), per, scale, _ptr(pre), _rows_ptr(out),
+                                _ld(out), _rows_ptr(normed), _ld(normed), _stream(y))
+    _check(rc, "mr_norm_residual")
+
+
+def norm_residual_bwd(dnormed, dout, y, out, dy, dresid, *, eps, post=None, gate=None, gate_rows=None, scale=1.0,
+                      pre=None, dpost=None, dgate=None, dpre=None) -> None:
+    """``mr_norm_residual_bwd``: the gradients ``dy`` and ``dresid`` of
+    :func:`norm_residual` from those of ``normed`` (``dnormed``, with ``pre``) and of
+    ``out`` from elsewhere (``dout``; either may be None), its input ``y`` and its
+    output ``out``; ``dpost``, ``dpre`` ``[H]`` and ``dgate`` ``[G, H]`` (float32, None:
+    not wanted) receive the weights' gradients, sums over the rows in an order that
+    the shape fixes. ``dresid`` may be ``dout`` and ``dy`` may be ``y``."""
+    name = "norm_residual_bwd"
+    _norm_types(name, dy, dresid)
+    T, H = dy.shape
+    for what, t, dt in (("dnormed", dnormed, dy.dtype), ("y", y, dy.dtype), ("dout", dout, dresid.dtype),
+                        ("out", out, dresid.dtype), ("dresid", dresid, dresid.dtype)):
+        _matrix(name, what, t, (dt,), (T, H))
+    for what, w in (("post", post), ("pre", pre), ("dpost", dpost), ("dpre", dpre)):
+        _dense(name, what, w, torch.float32, (H,))
+    if (pre is None) != (dnormed is None):
+        raise KernelError("norm_residual_bwd: the next norm's weight and its output's gradient come together")
+    for what, g, w in (("dpost", dpost, post), ("dgate", dgate, gate), ("dpre", dpre, pre)):
+        if g is not None and w is None:
+            raise KernelError(f"norm_residual_bwd: {what} is asked for without its weight")
+    per = _gate(name, gate, gate_rows, T, H)
+    if dgate is not None:
+        _dense(name, "dgate", dgate, torch.float32, gate.shape)
+    _one_device(name, dnormed, dout, y, out, dy, dresid, post, gate, pre, dpost, dgate, dpre)
+    nbytes = int(lib().mr_norm_residual_bwd_workspace_bytes(T, H, per, dpost is not None, dgate is not None,
+                                                            dpre is not None))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes else None
+    rc = lib().mr_norm_residual_bwd(
+        _rows_ptr(dnormed), dtype_code(dy.dtype), _ld(dnormed), _rows_ptr(dout), dtype_code(dresid.dtype), _ld(dout),
+        _rows_ptr(y), _ld(y), _rows_ptr(out), _ld(out), T, H, eps, _ptr(post), _ptr(gate), per, scale, _ptr(pre),
+        _rows_ptr(dy), _ld(dy), _rows_ptr(dresid), _ld(dresid), _ptr(dpost), _ptr(dgate), _ptr(dpre), _ptr(ws), nbytes,
+        _stream(dy))
+    _check(rc, "mr_norm_residual_bwd")
 
 
 def rmsnorm_fwd(h, w, eps, y, rstd=None) -> None:
