@@ -47,6 +47,7 @@ struct NormParams {
   const void* dout;
   int64_t lddo;
   int64_t chunk, per_group;  // rows of a block; blocks of a group (0: blocks of whole groups)
+  int row_threads, teams;    // threads of a row; rows at a time (more than one: a wave each)
   float* part_pre;           // [blocks, H] or null
   float* part_post;
   float* part_gate;          // [groups per_group, H]; per_group 0: dgate itself
@@ -76,8 +77,8 @@ __device__ __forceinline__ void load_weights(const float* w, int c, float (&out)
 }
 
 // Thread t holds the pieces t, t + threads, .. (P of them) of its row.
-template <int A, int S, int V, int P>
-__global__ __launch_bounds__(1024) void norm_fwd(NormParams p) {
+template <int A, int S, int V, int P, int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_fwd(NormParams p) {
   __shared__ float smem[3][16];
   int slot = 0;
   const int threads = blockDim.x;
@@ -155,11 +156,10 @@ __global__ __launch_bounds__(1024) void norm_fwd(NormParams p) {
   }
 }
 
-// Two sums at once.
-__device__ __forceinline__ void block_sum2(float& a, float& b, float (*smem)[16][2], int& slot) {
+// Two sums at once, over the `waves` waves of a row.
+__device__ __forceinline__ void block_sum2(float& a, float& b, float (*smem)[16][2], int& slot, int waves) {
   a = wave_sum(a);
   b = wave_sum(b);
-  const int waves = blockDim.x >> 6;
   if (waves == 1) return;
   if ((threadIdx.x & 63) == 0) {
     smem[slot][threadIdx.x >> 6][0] = a;
@@ -174,52 +174,97 @@ __device__ __forceinline__ void block_sum2(float& a, float& b, float (*smem)[16]
   slot = slot == 2 ? 0 : slot + 1;
 }
 
-template <int A, int S, int V, int P>
-__global__ __launch_bounds__(1024) void norm_bwd(NormParams p) {
+// WHOLE: the block's rows are whole groups of the gate. What dgate and dw_post sum
+// differs by factors that are a group's own, dh n: one sum serves both, and the
+// factors come in when the group ends.
+// The registers of P = 1 are held to those of four waves a SIMD where they fit, two
+// rows of up to 512 pieces a CU, with the next row's loads in flight (AHEAD); rows
+// past 1024 pieces leave no room for that.
+constexpr int waves_for(int A, int V, int P, bool WHOLE) {
+  return V == 1 ? 4 : P == 1 ? (A == MR_F32 || WHOLE ? 3 : 4) : 2;
+}
+template <int A, int S, int V, int P, int THREADS, bool WHOLE>
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(waves_for(A, V, P, WHOLE)))) void norm_bwd(NormParams p) {
+  constexpr bool AHEAD = THREADS == 512;
   __shared__ float smem[3][16][2];
   int slot = 0;
-  const int threads = blockDim.x;
+  const int waves = p.row_threads >> 6, teams = p.teams;
+  const int team = teams > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  const int thread = static_cast<int>(threadIdx.x) - team * 64;  // in its row
   const float inv_h = 1.0f / static_cast<float>(p.H);
-  int col[P];
+  uint32_t col[P];
   bool in[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
-    col[i] = (static_cast<int>(threadIdx.x) + i * threads) * V;
-    in[i] = col[i] < p.H;
-    col[i] = in[i] ? col[i] : 0;
+    const int c = (thread + i * p.row_threads) * V;
+    in[i] = c < p.H;
+    col[i] = in[i] ? c : 0;
   }
-  // this block's rows: a chunk of one group, or whole groups
+  // this block's rows: a chunk of one group, whose teams take turns, or whole groups,
+  // which the teams take in turn
   int64_t row0, row1, group;
-  if (p.per_group) {
+  if constexpr (!WHOLE) {
     group = blockIdx.x / p.per_group;
     row0 = group * p.gate_rows + (blockIdx.x % p.per_group) * p.chunk;
     row1 = min(min(row0 + p.chunk, (group + 1) * p.gate_rows), p.T);
   } else {
     row0 = static_cast<int64_t>(blockIdx.x) * p.chunk;
     row1 = min(row0 + p.chunk, p.T);
-    group = row0 / p.gate_rows;
+    group = row0 / p.gate_rows + team;
   }
-  float wpost[P][V], wpre[P][V], gate[P][V];
-  float s_pre[P][V], s_post[P][V], s_gate[P][V];
-  auto load_gate = [&]() __attribute__((always_inline)) {
+  row0 += WHOLE ? team * p.gate_rows : team;
+  const bool branch = p.post || p.gate;
+  float wpre[P][V], c[P][V];  // c = scale gate w_post
+  float s_pre[P][V], s[P][V], s_post[P][V];
+  auto load_branch = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < P; ++i) load_weights<V>(p.gate + group * p.H, col[i], gate[i]);
+    for (int i = 0; i < P; ++i) {
+      float w[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) c[i][k] = p.scale;
+      if (p.gate) {
+        load_weights<V>(p.gate + group * p.H, col[i], w);
+#pragma unroll
+        for (int k = 0; k < V; ++k) c[i][k] *= w[k];
+      }
+      if (p.post) {
+        load_weights<V>(p.post, col[i], w);
+#pragma unroll
+        for (int k = 0; k < V; ++k) c[i][k] *= w[k];
+      }
+    }
   };
 #pragma unroll
   for (int i = 0; i < P; ++i) {
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      wpost[i][k] = wpre[i][k] = gate[i][k] = 1.0f;
-      s_pre[i][k] = s_post[i][k] = s_gate[i][k] = 0.0f;
+      wpre[i][k] = 1.0f;
+      s_pre[i][k] = s[i][k] = s_post[i][k] = 0.0f;
     }
-    if (p.post) load_weights<V>(p.post, col[i], wpost[i]);
     if (p.pre) load_weights<V>(p.pre, col[i], wpre[i]);
   }
-  if (p.gate && row0 < row1) load_gate();
-  auto flush = [&](float* to, int64_t at, float (&s)[P][V]) __attribute__((always_inline)) {
+  if (row0 < row1) load_branch();
+  // The end of a group: dgate = scale w_post s, and to w_post's gradient scale gate s.
+  auto end_group = [&](float* gate_to, int64_t at) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < P; ++i)
-      if (in[i]) store_piece<MR_F32, V, false>(to, at * p.H + col[i], s[i]);
+    for (int i = 0; i < P; ++i) {
+      float w[V], o[V];
+      if (gate_to) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) w[k] = 1.0f;
+        if (p.post) load_weights<V>(p.post, col[i], w);
+#pragma unroll
+        for (int k = 0; k < V; ++k) o[k] = p.scale * w[k] * s[i][k];
+        if (in[i]) store_piece<MR_F32, V, false>(gate_to, at * p.H + col[i], o);
+      }
+      if (p.part_post) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) w[k] = 1.0f;
+        if (p.gate) load_weights<V>(p.gate + group * p.H, col[i], w);
+#pragma unroll
+        for (int k = 0; k < V; ++k) s_post[i][k] += p.scale * w[k] * s[i][k];
+      }
+    }
   };
   Piece<A, V> y[P], y_next[P], g[P], g_next[P];
   Piece<S, V> h[P], h_next[P], d[P], d_next[P];
@@ -230,20 +275,28 @@ __global__ __launch_bounds__(1024) void norm_bwd(NormParams p) {
     d_next[i].zero();
     y_next[i].zero();
   }
-  auto fetch = [&](int64_t row) __attribute__((always_inline)) {
+  constexpr int ea = A == MR_F32 ? 4 : 2, es = S == MR_F32 ? 4 : 2;
+  auto fetch = [&](int64_t row) __attribute__((always_inline)) {  // (a row's address is the block's, a lane's offset 32 bits)
+    const char* gr = static_cast<const char*>(p.dx) + row * p.lddx * ea;
+    const char* hr = static_cast<const char*>(p.stream) + row * p.lds * es;
+    const char* dr = static_cast<const char*>(p.dout) + row * p.lddo * es;
+    const char* yr = static_cast<const char*>(p.y) + row * p.ldy * ea;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       if (p.pre) {
-        g_next[i].load(p.dx, row * p.lddx + col[i]);
-        h_next[i].load(p.stream, row * p.lds + col[i]);
+        g_next[i].load(gr, col[i]);
+        h_next[i].load(hr, col[i]);
       }
-      if (p.dout) d_next[i].load(p.dout, row * p.lddo + col[i]);
-      if (p.post || p.gate) y_next[i].load(p.y, row * p.ldy + col[i]);
+      if (p.dout) d_next[i].load(dr, col[i]);
+      if (branch) y_next[i].load(yr, col[i]);
     }
   };
-  if (row0 < row1) fetch(row0);
-  int64_t left = p.per_group ? 0 : p.gate_rows;  // rows until the group ends
-  for (int64_t row = row0; row < row1; ++row) {
+  if (AHEAD && row0 < row1) fetch(row0);
+  int64_t left = p.gate_rows;  // WHOLE: rows until the group ends
+  for (int64_t row = row0, next; row < row1; row = next) {
+    const bool last = WHOLE && (left == 1 || row + 1 == row1);  // of its group
+    next = !WHOLE ? row + teams : last ? (group + teams) * p.gate_rows : row + 1;
+    if (!AHEAD) fetch(row);
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       y[i] = y_next[i];
@@ -251,7 +304,7 @@ __global__ __launch_bounds__(1024) void norm_bwd(NormParams p) {
       h[i] = h_next[i];
       d[i] = d_next[i];
     }
-    if (row + 1 < row1) fetch(row + 1);
+    if (AHEAD && next < row1) fetch(next);
     float rh = 0.0f, ch = 0.0f;
     if (p.pre) {
       float ss = 0.0f, dot = 0.0f;
@@ -263,11 +316,14 @@ __global__ __launch_bounds__(1024) void norm_bwd(NormParams p) {
           ss += v * v;
           dot += g[i].get(k) * wpre[i][k] * v;
         }
-      block_sum2(ss, dot, smem, slot);
+      block_sum2(ss, dot, smem, slot, waves);
+#pragma unroll
+      for (int i = 0; i < P; ++i) g[i].hide();
       rh = rsqrtf(ss * inv_h + p.eps);
       ch = rh * rh * (dot * inv_h);
     }
     float dh[P][V];
+    char* const out_row = static_cast<char*>(p.out) + row * p.ldo * es;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
 #pragma unroll
@@ -276,7 +332,7 @@ __global__ __launch_bounds__(1024) void norm_bwd(NormParams p) {
         dh[i][k] = d[i].get(k) + rh * (gv * wpre[i][k] - v * ch);
         s_pre[i][k] += gv * (v * rh);
       }
-      if (in[i]) store_piece<S, V, false>(p.out, row * p.ldo + col[i], dh[i]);
+      if (in[i]) store_piece<S, V, false>(out_row, col[i], dh[i]);
     }
     float ry = 1.0f, cy = 0.0f;
     if (p.post) {
@@ -287,42 +343,70 @@ __global__ __launch_bounds__(1024) void norm_bwd(NormParams p) {
         for (int k = 0; k < V; ++k) {
           const float v = in[i] ? y[i].get(k) : 0.0f;
           ss += v * v;
-          dot += p.scale * dh[i][k] * gate[i][k] * wpost[i][k] * v;
+          dot += dh[i][k] * c[i][k] * v;
         }
-      block_sum2(ss, dot, smem, slot);
+      block_sum2(ss, dot, smem, slot, waves);
+#pragma unroll
+      for (int i = 0; i < P; ++i) y[i].hide();
       ry = rsqrtf(ss * inv_h + p.eps);
       cy = ry * ry * (dot * inv_h);
     }
+    char* const dy_row = static_cast<char*>(p.normed) + row * p.ldn * ea;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       float o[V];
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const float v = y[i].get(k), n = v * ry;  // (without post ry is 1 and cy 0)
-        const float e = p.scale * dh[i][k];
-        s_gate[i][k] += e * (n * wpost[i][k]);
-        const float b = e * gate[i][k];
-        s_post[i][k] += b * n;
-        o[k] = ry * (b * wpost[i][k] - v * cy);
+        const float v = y[i].get(k);  // (without post ry is 1 and cy 0)
+        s[i][k] += dh[i][k] * (v * ry);
+        o[k] = ry * (dh[i][k] * c[i][k] - v * cy);
       }
-      if (in[i]) store_piece<A, V, false>(p.normed, row * p.ldn + col[i], o);
+      if (in[i]) store_piece<A, V, false>(dy_row, col[i], o);
     }
-    if (left && (--left == 0 || row + 1 == row1)) {
-      if (p.part_gate) flush(p.part_gate, group, s_gate);
-      if (row + 1 < row1) {
-        ++group;
-        left = p.gate_rows;
-        if (p.gate) load_gate();
+    if constexpr (WHOLE) {
+      --left;
+      if (last) {
+        end_group(p.part_gate, group);
+        if (next < row1) {
+          group += teams;
+          left = p.gate_rows;
+          load_branch();
 #pragma unroll
-        for (int i = 0; i < P; ++i)
+          for (int i = 0; i < P; ++i)
 #pragma unroll
-          for (int k = 0; k < V; ++k) s_gate[i][k] = 0.0f;
+            for (int k = 0; k < V; ++k) s[i][k] = 0.0f;
+        }
       }
     }
   }
-  if (p.part_pre) flush(p.part_pre, blockIdx.x, s_pre);
-  if (p.part_post) flush(p.part_post, blockIdx.x, s_post);
-  if (p.part_gate && p.per_group) flush(p.part_gate, blockIdx.x, s_gate);
+  if constexpr (V == 8 && P == 1) {
+    if (teams > 1) {  // the first team gets the sums, in order
+      __shared__ float each[8][64][8];
+      auto meet = [&](float (&x)[P][V]) __attribute__((always_inline)) {
+        store_piece<MR_F32, V, false>(&each[team][thread][0], 0, x[0]);
+        __syncthreads();
+        if (team == 0) {
+          for (int t = 1; t < teams; ++t)
+#pragma unroll
+            for (int k = 0; k < V; ++k) x[0][k] += each[t][thread][k];
+        }
+        __syncthreads();
+      };
+      meet(s_pre);
+      meet(WHOLE ? s_post : s);
+      if (team) return;
+    }
+  }
+  if constexpr (!WHOLE) {
+    if (branch) end_group(p.part_gate, blockIdx.x);
+  }
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    if (!in[i]) continue;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * p.H + col[i];
+    if (p.part_pre) store_piece<MR_F32, V, false>(p.part_pre, at, s_pre[i]);
+    if (p.part_post) store_piece<MR_F32, V, false>(p.part_post, at, s_post[i]);
+  }
 }
 
 // out[s, c] = sum over the n rows of part from row s n on, in an order that the
@@ -358,14 +442,14 @@ __global__ __launch_bounds__(1024) void norm_sum(SumParams p) {
 }
 
 constexpr int kMaxH = 16384;
-constexpr int64_t kBlocks = 512;  // of the backward, about
-
 struct Split {
   int64_t chunk, per_group, blocks;
 };
-// The rows of a backward block: about 512 blocks, each of one group's rows or of whole groups.
-Split split_rows(int64_t T, int64_t gate_rows) {
-  const int64_t want = (T + kBlocks - 1) / kBlocks;
+// The rows of a backward block: about 512 blocks (two a CU; four, of rows of up to
+// 128 threads), each of one group's rows or of whole groups.
+Split split_rows(int64_t T, int64_t H, int64_t gate_rows) {
+  const int64_t most = H > 512 && H <= 1024 ? 1024 : 512;
+  const int64_t want = (T + most - 1) / most;
   if (gate_rows <= want) {
     const int64_t chunk = want / gate_rows * gate_rows;
     return {chunk, 0, (T + chunk - 1) / chunk};
@@ -386,6 +470,9 @@ int check_norm(const char* fn, int64_t T, int64_t H, int act, int stream_type, c
 }
 
 bool vector_rows(const void* p, int64_t ld, int es) { return !p || (aligned16(p) && ld * es % 16 == 0); }
+
+// Pieces of a row of n that a thread holds (the kernels' P).
+int pieces_a_thread(int n, bool vec) { return vec ? (n > 512 ? 2 : 1) : (n > 8192 ? 16 : n > 4096 ? 8 : 4); }
 
 // threads that hold a row of n pieces, P each
 int row_threads(int n, int P) {
@@ -459,27 +546,32 @@ int mr_norm_residual(const void* y, int act_dtype, int64_t ldy, const void* resi
   const bool vec = H % 8 == 0 && vector_rows(y, ldy, ea) && vector_rows(resid, ldr, es) && vector_rows(out, ldo, es) &&
                    vector_rows(normed, ldn, ea) && vector_rows(post, 0, 4) && vector_rows(pre, 0, 4) && vector_rows(gate, H, 4);
   const int n = static_cast<int>(vec ? H / 8 : H);
-  const int P = vec ? (n > 512 ? 2 : 1) : (n > 4096 ? 16 : 4);
+  const int P = pieces_a_thread(n, vec);
   const int threads = row_threads(n, P);
   const int64_t most = 256ll * (2048 / threads);
   const dim3 grid(static_cast<unsigned>(T < most ? T : most)), block(threads);
   hipStream_t s = static_cast<hipStream_t>(stream);
+#define MR_NORM_LAUNCH(A, S, V, P, N) hipLaunchKernelGGL((norm_fwd<A, S, V, P, N>), grid, block, 0, s, p)
 #define MR_NORM(A, S)                                                                             \
   do {                                                                                             \
-    if (vec && P == 1) hipLaunchKernelGGL((norm_fwd<A, S, 8, 1>), grid, block, 0, s, p);          \
-    else if (vec) hipLaunchKernelGGL((norm_fwd<A, S, 8, 2>), grid, block, 0, s, p);               \
-    else if (P == 4) hipLaunchKernelGGL((norm_fwd<A, S, 1, 4>), grid, block, 0, s, p);            \
-    else hipLaunchKernelGGL((norm_fwd<A, S, 1, 16>), grid, block, 0, s, p);                       \
+    if (!vec) {                                                                                   \
+      if (n <= 4096) MR_NORM_LAUNCH(A, S, 1, 4, 1024);                                            \
+      else if (n <= 8192) MR_NORM_LAUNCH(A, S, 1, 8, 1024);                                       \
+      else MR_NORM_LAUNCH(A, S, 1, 16, 1024);                                                     \
+    } else if (n <= 512) MR_NORM_LAUNCH(A, S, 8, 1, 512);                                         \
+    else if (n <= 1024) MR_NORM_LAUNCH(A, S, 8, 2, 512);                                          \
+    else MR_NORM_LAUNCH(A, S, 8, 2, 1024);                                                        \
   } while (0)
   MR_NORM_TYPES(MR_NORM);
 #undef MR_NORM
+#undef MR_NORM_LAUNCH
   MR_LAUNCH_CHECK(fn);
   return MR_OK;
 }
 
 size_t mr_norm_residual_bwd_workspace_bytes(int64_t T, int64_t H, int64_t gate_rows, int post, int gate, int pre) {
   if (T <= 0 || H <= 0) return 0;
-  const mr::Split sp = mr::split_rows(T, gate ? (gate_rows > 0 ? gate_rows : 1) : T);
+  const mr::Split sp = mr::split_rows(T, H, gate ? (gate_rows > 0 ? gate_rows : 1) : T);
   const int64_t each = sp.blocks * H * 4;
   return static_cast<size_t>((post ? each : 0) + (pre ? each : 0) + (gate && sp.per_group > 1 ? each : 0));
 }
@@ -510,7 +602,7 @@ int mr_norm_residual_bwd(const void* dnormed, int act_dtype, int64_t lddn, const
   const int64_t rows = T > 0 ? T : 1;
   const int64_t of_gate = gate ? gate_rows : rows;
   const int64_t groups = T > 0 ? (T + of_gate - 1) / of_gate : 0;
-  const Split sp = split_rows(rows, of_gate);
+  const Split sp = split_rows(rows, H, of_gate);
   const int64_t each = sp.blocks * H * 4;
   const size_t need = T > 0 ? mr_norm_residual_bwd_workspace_bytes(T, H, gate_rows, dpost != nullptr, dgate != nullptr, dpre != nullptr) : 0;
   if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need))
@@ -595,23 +687,36 @@ int mr_norm_residual_bwd(const void* dnormed, int act_dtype, int64_t lddn, const
                      vector_rows(dout, lddo, es) && vector_rows(dy, lddy, ea) && vector_rows(dresid, lddr, es) &&
                      vector_rows(post, 0, 4) && vector_rows(pre, 0, 4) && vector_rows(gate, H, 4) && vector_rows(dgate, H, 4);
     const int n = static_cast<int>(vec ? H / 8 : H);
-    const int P = vec ? (n > 1024 ? 2 : 1) : (n > 4096 ? 16 : 4);
+    const int P = pieces_a_thread(n, vec);
     const int threads = row_threads(n, P);
-    if (too_many_blocks(blocks, threads)) return fail(MR_EINVAL, "%s: too many rows", fn);
-    const dim3 grid(static_cast<unsigned>(blocks)), block(threads);
+    if (too_many_blocks(blocks, 1024)) return fail(MR_EINVAL, "%s: too many rows", fn);
+    // Eight rows at a time where a wave holds one (with one, two waves a CU were all
+    // there were: 32768 rows of 256 columns 81 us, 42 now).
+    p.row_threads = threads;
+    p.teams = vec && threads == 64 ? 8 : 1;
+    const dim3 grid(static_cast<unsigned>(blocks)), block(threads * p.teams);
+#define MR_NORM_LAUNCH(A, S, V, P, N)                                                              \
+  do {                                                                                            \
+    if (sp.per_group) hipLaunchKernelGGL((norm_bwd<A, S, V, P, N, false>), grid, block, 0, s, p); \
+    else hipLaunchKernelGGL((norm_bwd<A, S, V, P, N, true>), grid, block, 0, s, p);               \
+  } while (0)
 #define MR_NORM(A, S)                                                                             \
   do {                                                                                             \
-    if (vec && P == 1) hipLaunchKernelGGL((norm_bwd<A, S, 8, 1>), grid, block, 0, s, p);          \
-    else if (vec) hipLaunchKernelGGL((norm_bwd<A, S, 8, 2>), grid, block, 0, s, p);               \
-    else if (P == 4) hipLaunchKernelGGL((norm_bwd<A, S, 1, 4>), grid, block, 0, s, p);            \
-    else hipLaunchKernelGGL((norm_bwd<A, S, 1, 16>), grid, block, 0, s, p);                       \
+    if (!vec) {                                                                                   \
+      if (n <= 4096) MR_NORM_LAUNCH(A, S, 1, 4, 1024);                                            \
+      else if (n <= 8192) MR_NORM_LAUNCH(A, S, 1, 8, 1024);                                       \
+      else MR_NORM_LAUNCH(A, S, 1, 16, 1024);                                                     \
+    } else if (n <= 512) MR_NORM_LAUNCH(A, S, 8, 1, 512);                                         \
+    else if (n <= 1024) MR_NORM_LAUNCH(A, S, 8, 2, 512);                                          \
+    else MR_NORM_LAUNCH(A, S, 8, 2, 1024);                                                        \
   } while (0)
     MR_NORM_TYPES(MR_NORM);
 #undef MR_NORM
+#undef MR_NORM_LAUNCH
     MR_LAUNCH_CHECK(fn);
   }
   if (blocks_y) {
-    // (a gate that several blocks share has more rows than 1/512 of them: at most 513 groups)
+    // (a gate that several blocks share has more rows than 1/1024 of them: at most 1025 groups)
     hipLaunchKernelGGL(norm_sum, dim3(static_cast<unsigned>((H + 63) / 64), static_cast<unsigned>(blocks_y)), dim3(1024), 0, s, q);
     MR_LAUNCH_CHECK(fn);
   }

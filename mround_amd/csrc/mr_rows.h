@@ -31,6 +31,11 @@ struct Piece {
 #pragma unroll
     for (int k = 0; k < WORDS; ++k) w[k] = 0;
   }
+  // Its floats are to be made again from here on, not kept.
+  __device__ __forceinline__ void hide() {
+#pragma unroll
+    for (int k = 0; k < WORDS; ++k) asm volatile("" : "+v"(w[k]));
+  }
   __device__ __forceinline__ float get(int k) const {
     if constexpr (DT == MR_F32) return __uint_as_float(w[k]);
     const uint32_t x = V == 1 ? w[0] : w[k >> 1] >> (16 * (k & 1));
