@@ -28,7 +28,7 @@ struct RouteParams {
   const void* z;
   int64_t ldz;
   int T, E, k;
-  bool normalize;
+  bool normalize, whole;  // whole: a row is runs of four on addresses of their size
   float scale;
   float* weights;
   int32_t* ids;
@@ -41,15 +41,18 @@ struct RouteParams {
 };
 
 // A float's place in the descending order as an unsigned number: NaN above all,
-// -inf (which is never chosen) at 0, zeros alike.
+// -inf (which is never chosen) at 0, zeros alike. And back: the float (of a NaN, one).
 __device__ __forceinline__ uint32_t order_key(float x) {
   if (x != x) return 0xffffffffu;
   if (x == -INFINITY) return 0;
   const uint32_t b = __float_as_uint(x + 0.0f);
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
 
-// Maximum, minimum and sum over the L lanes of a token (L = 16, 32 or 64, aligned).
+// x reduced over the L lanes of a token (L = 16, 32 or 64, aligned).
 template <int L, typename T, typename F>
 __device__ __forceinline__ T lanes_reduce(T x, F f) {
   x = f(x, dpp<kDppXor1>(x));
@@ -61,21 +64,52 @@ __device__ __forceinline__ T lanes_reduce(T x, F f) {
   return x;
 }
 
-// A token's logits, V to a lane: expert i L + lane.
+// A token's logits, V to a lane, runs of four: the expert of a lane's entry i.
+template <int L>
+constexpr __device__ __forceinline__ int expert_of(int i, int l) { return i / 4 * (4 * L) + l * 4 + i % 4; }
+
 template <int DT, int L, int V>
 __device__ __forceinline__ void load_logits(const RouteParams& p, int64_t t, int l, float (&z)[V]) {
+  const char* row = static_cast<const char*>(p.z) + t * p.ldz * (DT == MR_F32 ? 4 : 2);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int e = i * L + l;
-    z[i] = e < p.E ? load_elem<DT>(p.z, t * p.ldz + e) : -INFINITY;
+  for (int i = 0; i < V; i += 4) {
+    const int e = expert_of<L>(i, l);
+    if (p.whole) {  // (runs lie wholly inside or past the row, on addresses of their size)
+      if (e < p.E) {
+        if constexpr (DT == MR_F32) {
+          const float4 v = *reinterpret_cast<const float4*>(row + e * 4);
+          z[i] = v.x, z[i + 1] = v.y, z[i + 2] = v.z, z[i + 3] = v.w;
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(row + e * 2);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t w = (k < 2 ? v.x : v.y) >> (16 * (k & 1));
+            z[i + k] = DT == MR_BF16 ? __uint_as_float(w << 16) : f16_to_f32(static_cast<uint16_t>(w));
+          }
+        }
+      } else {
+        z[i] = z[i + 1] = z[i + 2] = z[i + 3] = -INFINITY;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) z[i + k] = e + k < p.E ? load_elem<DT>(row, e + k) : -INFINITY;
+    }
   }
 }
 
-// The block's tokens t0 .. t1 - 1: ids and weights, and the count of each expert in hist (LDS).
+// The block's tokens t0 .. t1 - 1: ids and weights, and the count of each expert in
+// hist (LDS). A choice is a maximum over the lanes; what is chosen leaves the keys.
+// 16-bit logits make one key with their expert (the upper half in order, the lower
+// the expert from the top): the maximum is the choice. 32-bit ones need a second
+// reduction, over the lanes that hold the maximum, for the lowest expert. The
+// instructions bound it (16384 tokens, 8 of 128 experts: 4 us of 60 each a choice).
 template <int DT, int L, int V>
 __device__ __forceinline__ void choose(const RouteParams& p, int t0, int t1, int32_t* hist) {
   constexpr int TOKENS = kRouteThreads / L;
+  constexpr bool NARROW = DT != MR_F32;
   const int l = threadIdx.x % L;
+  auto largest = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  auto least = [](uint32_t a, uint32_t b) { return a < b ? a : b; };
   for (int t = t0 + static_cast<int>(threadIdx.x) / L; t < t1; t += TOKENS) {
     float z[V];
     load_logits<DT, L, V>(p, t, l, z);
@@ -84,6 +118,16 @@ __device__ __forceinline__ void choose(const RouteParams& p, int t0, int t1, int
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       key[i] = order_key(z[i]);
+      if constexpr (NARROW) {
+        // (a 16-bit float's key: of bf16 the upper half, of fp16, whose values need 13 bits
+        // more than the half has, the order of its own bits)
+        uint32_t k16 = key[i] >> 16;
+        if constexpr (DT == MR_F16) {
+          const uint32_t b = f32_to_f16(z[i] + 0.0f);
+          k16 = key[i] == 0 ? 0 : key[i] == 0xffffffffu ? 0xffffu : (b & 0x8000u) ? ~b & 0xffffu : b | 0x8000u;
+        }
+        key[i] = key[i] == 0 ? 0 : (k16 << 16) | (0xffffu - expert_of<L>(i, l));
+      }
       m = fmaxf(m, z[i]);
     }
     m = lanes_reduce<L>(m, [](float a, float b) { return fmaxf(a, b); });
@@ -96,26 +140,32 @@ __device__ __forceinline__ void choose(const RouteParams& p, int t0, int t1, int
     float own = -INFINITY;  // the logit of this lane's entry, entry l
     int own_id = -1;
     for (int j = 0; j < p.k; ++j) {
-      uint32_t best = 0, at = 0;
+      uint32_t best = key[0];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const bool more = key[i] > best;
-        best = more ? key[i] : best;
-        at = more ? i * L + l : at;
-      }
-      const uint32_t top = lanes_reduce<L>(best, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-      at = lanes_reduce<L>(best == top ? at : 0xffffffffu, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
-      float value = 0.0f;
+      for (int i = 1; i < V; ++i) best = largest(best, key[i]);
+      const uint32_t top = lanes_reduce<L>(best, largest);
+      uint32_t at;
+      if constexpr (NARROW) {
+        at = 0xffffu - (top & 0xffffu);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const bool it = top && at == static_cast<uint32_t>(i * L + l);
-        value = it ? z[i] : value;
-        key[i] = it ? 0 : key[i];
+        for (int i = 0; i < V; ++i) key[i] = key[i] == top ? 0 : key[i];
+      } else {
+        at = 0xffffffffu;
+#pragma unroll
+        for (int i = V - 1; i >= 0; --i) at = key[i] == top ? expert_of<L>(i, l) : at;
+        at = lanes_reduce<L>(at, least);
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[i] = at == static_cast<uint32_t>(expert_of<L>(i, l)) ? 0 : key[i];
       }
-      // the lane that held it is at % L of the token's
-      value = __shfl(value, (static_cast<int>(threadIdx.x) & 63 & ~(L - 1)) + static_cast<int>(at % L), 64);
       if (l == j && top) {
-        own = value;
+        if constexpr (DT == MR_F32) {
+          own = key_value(top);
+        } else if constexpr (DT == MR_BF16) {
+          own = key_value((top & 0xffff0000u) | ((top & 0x80000000u) ? 0 : 0xffffu));
+        } else {
+          const uint32_t k = top >> 16;
+          own = f16_to_f32(static_cast<uint16_t>((k & 0x8000u) ? k ^ 0x8000u : ~k));
+        }
         own_id = static_cast<int>(at);
       }
     }
@@ -299,7 +349,7 @@ __global__ __launch_bounds__(256) void route_bwd(RouteBwdParams p) {
     const float dj = __shfl(my_d, from, 64);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const bool it = id == i * L + l;
+      const bool it = id == expert_of<L>(i, l);
       d[i] += it ? dj : 0.0f;
       chosen[i] = chosen[i] || it;
     }
@@ -322,10 +372,29 @@ __global__ __launch_bounds__(256) void route_bwd(RouteBwdParams p) {
   dot = lanes_reduce<L>(dot, [](float a, float b) { return a + b; });
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a row that is -inf throughout has no gradient)
   dot *= inv;
+  char* const row = static_cast<char*>(p.dz) + t * p.lddz * (DT == MR_F32 ? 4 : 2);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int at = i * L + l;
-    if (at < p.f.E) store_elem<DT>(p.dz, t * p.lddz + at, p.f.scale * (e[i] * inv) * (d[i] - dot));
+  for (int i = 0; i < V; i += 4) {
+    const int at = expert_of<L>(i, l);
+    float g[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) g[q] = p.f.scale * (e[i + q] * inv) * (d[i + q] - dot);
+    if (p.f.whole) {
+      if (at >= p.f.E) continue;
+      if constexpr (DT == MR_F32) {
+        *reinterpret_cast<float4*>(row + at * 4) = make_float4(g[0], g[1], g[2], g[3]);
+      } else if constexpr (DT == MR_BF16) {
+        *reinterpret_cast<uint2*>(row + at * 2) = make_uint2(pack_bf16x2(g[0], g[1]), pack_bf16x2(g[2], g[3]));
+      } else {
+        *reinterpret_cast<uint2*>(row + at * 2) =
+            make_uint2(f32_to_f16(g[0]) | static_cast<uint32_t>(f32_to_f16(g[1])) << 16,
+                       f32_to_f16(g[2]) | static_cast<uint32_t>(f32_to_f16(g[3])) << 16);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (at + q < p.f.E) store_elem<DT>(row, at + q, g[q]);
+    }
   }
 }
 
@@ -458,9 +527,9 @@ __global__ __launch_bounds__(256) void spread_kernel(RowsParams p) {
 }
 
 int route_blocks(int64_t T, int64_t* chunk_out) {
-  // at most 256 blocks of 64 tokens' multiples, 128 at least
-  int64_t chunk = ((T + 255) / 256 + 63) / 64 * 64;
-  if (chunk < 128) chunk = 128;
+  // Multiples of 64 tokens (a pass of a block with 16 lanes each), for at most 256
+  // blocks. (128 tokens at least: 16384 tokens, 8 of 128 experts 19.4 us, 13 now.)
+  const int64_t chunk = T <= 64 ? 64 : ((T + 255) / 256 + 63) / 64 * 64;
   *chunk_out = chunk;
   const int64_t n = (T + chunk - 1) / chunk;
   return static_cast<int>(n > 0 ? n : 1);
@@ -477,6 +546,10 @@ int check_route(const char* fn, int dtype, int64_t ldz, int64_t T, int64_t E, in
   if (reinterpret_cast<uintptr_t>(z) % dtype_bytes(dtype))
     return fail(MR_EINVAL, "%s: a pointer is not aligned to its elements", fn);
   return MR_OK;
+}
+
+bool whole_runs(const void* p, int64_t ld, int64_t E, int es) {
+  return E % 4 == 0 && ld % 4 == 0 && reinterpret_cast<uintptr_t>(p) % (4 * es) == 0;
 }
 
 // Lanes to a token: one for each entry, with at most 16 logits each.
@@ -578,6 +651,7 @@ int mr_route_experts(const void* logits, int dtype, int64_t ld, int64_t T, int64
   p.E = static_cast<int>(E);
   p.k = static_cast<int>(k);
   p.normalize = normalize != 0;
+  p.whole = whole_runs(logits, ld, E, dtype_bytes(dtype));
   p.scale = scale;
   p.weights = weights;
   p.ids = ids;
@@ -625,6 +699,7 @@ int mr_route_experts_bwd(const float* dweights, const void* logits, int dtype, i
   p.f.E = static_cast<int>(E);
   p.f.k = static_cast<int>(k);
   p.f.normalize = normalize != 0;
+  p.f.whole = whole_runs(logits, ld, E, es) && whole_runs(dlogits, lddz, E, es);
   p.f.scale = scale;
   p.f.ids = const_cast<int32_t*>(ids);
   p.dw = dweights;
