@@ -491,17 +491,28 @@ int mr_route_experts_bwd(const float* dweights, const void* logits, int dtype, i
  * dimensions and steps multiples of 8 (fp32 C: 4).
  * mr_gemm_experts_swiglu, _bwd: mr_gemm_swiglu and mr_gemm_swiglu_bwd over such
  * rows, Wgu[e] 2N x K interleaved every 32 rows, Wd[e] K x N, M any; dgu may be gu.
+ * workspace: partials of products that are cut along K, which those of few tiles are:
+ * a smaller one than mr_gemm_experts_plan names, or none, leaves them whole.
+ * mr_gemm_experts_plan: how a product runs (blocks of 16 rows, 128 x 128 or 256 x 256
+ * tiles), the blocks along K of a tile and the partials' bytes, for the product's
+ * width (2N for the SwiGLU pair) and an output of mr_gemm_plan's kinds; M, or for
+ * MR_TN K, is all experts' rows.
  */
+enum { MR_EXPERTS_FEW = 0, MR_EXPERTS_SMALL = 1, MR_EXPERTS_LARGE = 2 };
+int mr_gemm_experts_plan(int layout, int output, int64_t experts, int64_t M, int64_t N, int64_t K, int* way_out,
+                         int* split_out, size_t* workspace_out);
 int mr_gemm_experts(int layout, int64_t experts, int64_t M, int64_t N, int64_t K, const void* A, int64_t lda,
                     const int32_t* index, int64_t a_rows, const void* B, int64_t ldb, int64_t b_step,
                     const int32_t* offsets, void* C, int c_dtype, int64_t ldc, int64_t c_step, int accumulate,
-                    void* stream);
+                    void* workspace, size_t workspace_bytes, void* stream);
 int mr_gemm_experts_swiglu(int64_t experts, int64_t M, int64_t N, int64_t K, const void* X, int64_t ldx,
                            const int32_t* index, int64_t x_rows, const void* Wgu, int64_t ldw, int64_t w_step,
-                           const int32_t* offsets, void* act, int64_t ldact, void* gu, int64_t ldgu, void* stream);
+                           const int32_t* offsets, void* act, int64_t ldact, void* gu, int64_t ldgu,
+                           void* workspace, size_t workspace_bytes, void* stream);
 int mr_gemm_experts_swiglu_bwd(int64_t experts, int64_t M, int64_t N, int64_t K, const void* dy, int64_t ldd,
                                const void* Wd, int64_t ldw, int64_t w_step, const int32_t* offsets, const void* gu,
-                               int64_t ldgu, void* dgu, int64_t lddgu, void* stream);
+                               int64_t ldgu, void* dgu, int64_t lddgu, void* workspace, size_t workspace_bytes,
+                               void* stream);
 
 /*
  * Rows to their experts' places and back, fp32 or bf16, sums in fp32:

@@ -320,10 +320,18 @@ __device__ __forceinline__ void store16(T* p, T v) {
 // What rounding x to bf16 leaves, exactly.
 __device__ __forceinline__ float bf16_rest(float x) { return x - bf16_to_f32(f32_to_bf16(x)); }
 
+// The first row of a wave's 32-row slice i: one run of WM rows a wave, or with HALVES
+// one run of WM / 2 in each half of the tile, so that a tile whose second half is
+// past the edge has a first half that all waves share.
+template <int WM, bool HALVES>
+constexpr __device__ __forceinline__ int slice_row(int wm, int i) {
+  return HALVES ? (i * 32) / (WM / 2) * WM + wm * (WM / 2) + i * 32 % (WM / 2) : wm * WM + i * 32;
+}
+
 // The epilogues of a wave's WM x WN share of a tile from its transposed
 // accumulators (see SWAP in the kernels), staged through the wave's REGION
 // bytes of LDS at `region` (free once the k loop has ended).
-template <int WM, int WN, int REGION, int EPI, bool OUT_BF16, int TM, int TN>
+template <int WM, int WN, int REGION, int EPI, bool OUT_BF16, bool HALVES = false, int TM, int TN>
 __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM][TN], int m0, int n0, int wm,
                                            int wn, int lane, uint8_t* region) {
   const int lrow = (lane >> 5) * 4;
@@ -365,6 +373,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
     constexpr bool SPLIT = EPI == EPI_SWIGLU_SPLIT;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
+      if (HALVES && m0 + slice_row<WM, HALVES>(wm, i) >= p.M) continue;
 #pragma unroll
       for (int jb = 0; jb < TN / JH; ++jb) {
 #pragma unroll
@@ -377,7 +386,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
         }
         // The same wave reads back what it wrote (LDS keeps a wave's accesses
         // in order), then the next slice overwrites the region.
-        const int row0 = m0 + wm * WM + i * 32;
+        const int row0 = m0 + slice_row<WM, HALVES>(wm, i);
         const int col0 = n0 + wn * WN + jb * JH * 32;  // gate/up column, a multiple of 64
         // uniform bases of the slice; lane offsets stay 32-bit (ld < 2^22, 32 rows)
         uint16_t* const act_s = act + static_cast<int64_t>(row0) * p.ldc + col0 / 2;
@@ -455,6 +464,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
     uint16_t* dgu = static_cast<uint16_t*>(p.C);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
+      if (HALVES && m0 + slice_row<WM, HALVES>(wm, i) >= p.M) continue;
 #pragma unroll
       for (int jb = 0; jb < TN / JH; ++jb) {
 #pragma unroll
@@ -468,7 +478,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
         // The same wave reads back what it wrote (LDS keeps a wave's accesses
         // in order). Loads go to clamped (always valid) places; only the
         // stores are guarded.
-        const int row0 = m0 + wm * WM + i * 32;
+        const int row0 = m0 + slice_row<WM, HALVES>(wm, i);
         const int col0 = n0 + wn * WN + jb * JH * 32;
         const uint16_t* const gu_s = p.gu + static_cast<int64_t>(row0) * p.ldgu;
         uint16_t* const dgu_s = dgu + static_cast<int64_t>(row0) * p.ldc;
@@ -549,7 +559,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
             *(lds_f32x4*)(st + lcol * PITCH + (jj * 32 + gi * 8 + lrow) * 4) =
                 f32x4{acc[i][j][4 * gi], acc[i][j][4 * gi + 1], acc[i][j][4 * gi + 2], acc[i][j][4 * gi + 3]};
         }
-        const int row0 = m0 + wm * WM + i * 32;
+        const int row0 = m0 + slice_row<WM, HALVES>(wm, i);
         const int col0 = n0 + wn * WN + jb * JH * 32;
         const int col = col0 + ch * OPC, cb = min(col, p.N - OPC);  // N is a multiple of 8
         const int64_t cbase = static_cast<int64_t>(row0) * p.ldc + col0;
@@ -676,6 +686,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
     const bool has_bias = p.bias != nullptr;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
+      if (HALVES && m0 + slice_row<WM, HALVES>(wm, i) >= p.M) continue;
 #pragma unroll
       for (int jb = 0; jb < TN / JH; ++jb) {
 #pragma unroll
@@ -686,7 +697,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
             *(lds_f32x4*)(st + lcol * PITCH + (jj * 32 + gi * 8 + lrow) * 4) =
                 f32x4{acc[i][j][4 * gi], acc[i][j][4 * gi + 1], acc[i][j][4 * gi + 2], acc[i][j][4 * gi + 3]};
         }
-        const int row0 = m0 + wm * WM + i * 32;
+        const int row0 = m0 + slice_row<WM, HALVES>(wm, i);
         const int col0 = n0 + wn * WN + jb * JH * 32;
         // uniform bases of the slice; lane offsets stay 32-bit (ld < 2^22, 32 rows)
         const int64_t cbase = static_cast<int64_t>(row0) * p.ldc + col0;
@@ -765,50 +776,92 @@ __device__ __forceinline__ void store_partial(float* out, const f32x16 (&acc)[TM
             f32x4{acc[i][j][4 * gi], acc[i][j][4 * gi + 1], acc[i][j][4 * gi + 2], acc[i][j][4 * gi + 3]};
 }
 
+// The sum of x over the lanes up to each one (row by row of 16 lanes, then across them).
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // 1, 2, 4, 8 lanes down a row
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the last of rows 0 and 2 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // the last of row 1 to rows 2 and 3
+  return x;
+}
+
+// Half octaves of a count, 0 for none: experts of one class count as alike long.
+__device__ __forceinline__ int length_class(int n) {
+  return n > 0 ? static_cast<int>(__float_as_uint(static_cast<float>(n)) >> 22) - 253 : 0;
+}
+
 // The tile of block `bid` of a grouped product: p becomes its expert's product
 // and (bm, bn) the tile in it. False where the block has none. Each wave counts
-// the experts' tiles by itself (64 experts at a time, a scan over the lanes,
-// 0.3 us), which is less than a launch that would write a list of them. Offsets
-// are held between 0 and the rows there are, so that no others lead outside.
+// the experts' tiles by itself (64 experts at a time, scans over the lanes), which
+// is less than a launch that would write a list of them. Offsets are held between
+// 0 and the rows there are, so that no others lead outside.
+//
+// Rows (K-major A): every tile takes as long, and each XCD gets a contiguous run
+// of them, experts in order. Weight gradients: an expert's tiles take as long as it
+// has rows, so each XCD gets an eighth of every expert's tiles (a contiguous run of
+// tile_coords, which shares panels), longest experts first. (A run of whole experts
+// an XCD: the XCD with the liked ones worked twice as long as the others, 16 experts
+// of 2048 x 1408 over 32764 rows 352 us.)
 template <int BM, int BN, bool A_KMAJOR, bool OUT_BF16, bool INDEXED>
 __device__ __forceinline__ bool enter(GroupedParams<INDEXED>& p, int bid, int& bm, int& bn) {
   const int rows = A_KMAJOR ? p.M : p.K;
+  const int lane = threadIdx.x & 63;
   auto at = [&](int i) __attribute__((always_inline)) { return min(max(p.offsets[i], 0), rows); };
+  auto length = [&](int i) __attribute__((always_inline)) { return i < p.experts ? max(at(i + 1) - at(i), 0) : 0; };
   p.grid_n = (p.N + BN - 1) / BN;
-  int e, first, len, lt;
+  int e = -1, lt;
   if constexpr (A_KMAJOR) {
-    const int lane = threadIdx.x & 63;
-    auto tiles = [&](int i) __attribute__((always_inline)) {
-      return i < p.experts ? (max(at(i + 1) - at(i), 0) + BM - 1) / BM * p.grid_n : 0;
-    };
+    auto tiles = [&](int i) __attribute__((always_inline)) { return (length(i) + BM - 1) / BM * p.grid_n; };
     int total = 0;
     for (int c = 0; c < p.experts; c += 64) total += tiles(c + lane);
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) total += __shfl_xor(total, o, 64);
-    total = __builtin_amdgcn_readfirstlane(total);
+    total = __builtin_amdgcn_readlane(wave_scan(total), 63);
     if (bid >= total) return false;
+    p.tile0 = bid;
     lt = xcd_order(bid, total);
-    e = -1;
-    for (int c = 0; c < p.experts && e < 0; c += 64) {
-      const int own = tiles(c + lane);
-      int upto = own;
-#pragma unroll
-      for (int o = 1; o < 64; o *= 2) {
-        const int before = __shfl_up(upto, o, 64);
-        upto += lane >= o ? before : 0;
-      }
+    for (int c = 0; c < p.experts; c += 64) {
+      const int own = tiles(c + lane), upto = wave_scan(own);
       const uint64_t past = __ballot(upto > lt);
       if (past) {
         const int l = __builtin_ctzll(past);
         e = c + l;
         lt -= __builtin_amdgcn_readlane(upto - own, l);
-      } else {
-        lt -= __builtin_amdgcn_readlane(upto, 63);
+        break;
+      }
+      lt -= __builtin_amdgcn_readlane(upto, 63);
+    }
+  } else {
+    p.grid_m = (p.M + BM - 1) / BM;
+    const int per = p.grid_m * p.grid_n, share = (per + 7) / 8;
+    const int i = bid >> 3;
+    int rank = i / share;
+    // (XCD x takes another eighth of each next expert, which evens out shares that are not full)
+    lt = ((bid + rank) & 7) * share + i % share;
+    if (lt >= per) return false;
+    p.tile0 = rank * per + lt;
+    int longest = 0;
+    for (int c = 0; c < p.experts; c += 64) longest = max(longest, length_class(length(c + lane)));
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) longest = max(longest, __shfl_xor(longest, o, 64));
+    longest = __builtin_amdgcn_readfirstlane(longest);
+    for (int cls = longest; cls >= 0 && e < 0; --cls) {
+      for (int c = 0; c < p.experts; c += 64) {
+        const bool in = c + lane < p.experts && length_class(length(c + lane)) == cls;
+        const uint64_t set = __ballot(in);
+        const int n = __popcll(set);
+        if (rank < n) {
+          e = c + __builtin_ctzll(__ballot(in && __popcll(set & ((1ull << lane) - 1)) == rank));
+          break;
+        }
+        rank -= n;
       }
     }
-    if (e < 0) return false;
-    first = __builtin_amdgcn_readfirstlane(at(e));
-    len = __builtin_amdgcn_readfirstlane(at(e + 1)) - first;
+  }
+  if (e < 0) return false;
+  const int first = __builtin_amdgcn_readfirstlane(at(e));
+  const int len = max(__builtin_amdgcn_readfirstlane(at(e + 1)) - first, 0);
+  if constexpr (A_KMAJOR) {
     p.M = len;
     p.grid_m = (len + BM - 1) / BM;
     if constexpr (INDEXED) p.index += first;
@@ -818,20 +871,13 @@ __device__ __forceinline__ bool enter(GroupedParams<INDEXED>& p, int bid, int& b
     p.C = OUT_BF16 ? static_cast<void*>(static_cast<uint16_t*>(p.C) + c0) : static_cast<void*>(static_cast<float*>(p.C) + c0);
     if (p.gu) p.gu += first * p.ldgu;
   } else {
-    p.grid_m = (p.M + BM - 1) / BM;
-    const int per = p.grid_m * p.grid_n;
-    lt = xcd_order(bid, per * p.experts);
-    e = lt / per;
-    lt -= e * per;
-    first = __builtin_amdgcn_readfirstlane(at(e));
-    len = max(__builtin_amdgcn_readfirstlane(at(e + 1)) - first, 0);
     p.K = len;
     p.A += first * p.lda;
     p.B += first * p.ldb;
     p.C = static_cast<float*>(p.C) + e * p.c_step;
     if (p.resid) p.resid += e * p.c_step;
   }
-  p.kt_per = (p.K + BK - 1) / BK;
+  p.kt_per = ((p.K + BK - 1) / BK + p.ksplit - 1) / p.ksplit;
   tile_coords(lt, p.grid_m, p.grid_n, bm, bn);
   return true;
 }
@@ -870,10 +916,10 @@ __global__ __launch_bounds__(kThreads) void gemm_kernel(P p) {
   // XCD-aware renumbering, then the grouped order along M. Split launches take
   // the splits of one tile as consecutive blocks.
   int bid = blockIdx.x, split = 0;
-  if (P::kGrouped) {
-  } else if (p.ksplit > 1) {
+  if (p.ksplit > 1) {
     split = bid % p.ksplit;
     bid /= p.ksplit;
+  } else if (P::kGrouped) {
   } else if ((p.n_tiles & 7) == 0 || p.K > 8 * BK) {
     bid = xcd_order(bid, p.n_tiles);
   }
@@ -891,7 +937,7 @@ __global__ __launch_bounds__(kThreads) void gemm_kernel(P p) {
   const int n0 = bn * BN;
   if (m0 >= p.M || n0 >= p.N) return;  // a quarter wholly past the edge (the whole block leaves)
   if constexpr (P::kGrouped && !A_KMAJOR) {
-    if (p.K == 0) return store_zeros<BM, BN, EPI>(p, m0, n0);
+    if (p.K == 0 && p.ksplit == 1) return store_zeros<BM, BN, EPI>(p, m0, n0);
   }
 
   const int lane = threadIdx.x & 63;
@@ -1029,7 +1075,7 @@ __global__ __launch_bounds__(kThreads) void gemm_kernel(P p) {
   };
 
   const int kt_begin = split * p.kt_per;
-  const int KT = P::kGrouped ? p.kt_per : min(p.K / BK, kt_begin + p.kt_per);
+  const int KT = min(P::kGrouped ? (p.K + BK - 1) / BK : p.K / BK, kt_begin + p.kt_per);
   if (kt_begin < KT) {
     issue_loads(kt_begin, As0, Bs0);
     __builtin_amdgcn_s_waitcnt(0);
@@ -1043,8 +1089,8 @@ __global__ __launch_bounds__(kThreads) void gemm_kernel(P p) {
   }
 
   // ---- epilogue ----
-  if (!P::kGrouped && p.ksplit > 1) {
-    store_partial<BM, BN>(p.ws + (static_cast<int64_t>(bid) * p.ksplit + split) * (BM * BN), acc, wm * TM, wn * TN, lane);
+  if (p.ksplit > 1) {
+    store_partial<BM, BN>(p.ws + (static_cast<int64_t>(P::kGrouped ? p.tile0 : bid) * p.ksplit + split) * (BM * BN), acc, wm * TM, wn * TN, lane);
     return;
   }
   {
@@ -1080,6 +1126,9 @@ template <bool A_KMAJOR, bool B_KMAJOR, int EPI, bool OUT_BF16, class P = GemmPa
 __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1, 1))) void gemm4_kernel(P p) {
   constexpr int BM = 256, BN = 256, WM = 128, WN = 128, TM = WM / 32, TN = WN / 32;
   constexpr int STAGE = 256 * ROW_BYTES;  // bytes of one operand stage (either layout)
+  // A group's last rows may fill only half a tile: its k-tiles then run without the
+  // second half's loads and MFMAs (see tile).
+  constexpr bool HALVES = P::kGrouped && A_KMAJOR;
   static_assert(STAGE == MNMajorDirect<256>::ROWB * BK, "both layouts stage 32 KB");
   __shared__ __attribute__((aligned(1024))) uint8_t As0[STAGE];
   __shared__ __attribute__((aligned(1024))) uint8_t As1[STAGE];
@@ -1135,7 +1184,7 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
 #pragma unroll
     for (int x = 0; x < NA; ++x) {
       if constexpr (A_KMAJOR)
-        a_reg[x] = (wm * WM + l32) * ROW_BYTES + (((2 * x + h) ^ swz_bits(l32)) << 4);
+        a_reg[x] = ((HALVES ? wm * (WM / 2) : wm * WM) + l32) * ROW_BYTES + (((2 * x + h) ^ swz_bits(l32)) << 4);
       else
         a_reg[x] = MNMajorDirect<BM>::frag_off(wm * WM + x * 32, lane);
       asm volatile("" : "+v"(a_reg[x]));
@@ -1151,11 +1200,11 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
   }
   typedef const __attribute__((address_space(3))) uint8_t* lds_ptr;
   bf16x8 af[2][TM], bfr[2][TN];
-  auto rd = [&](lds_ptr la, lds_ptr lb, int kk, int slot) __attribute__((always_inline)) {
+  auto rd = [&](lds_ptr la, lds_ptr lb, int kk, int slot, int rows = TM) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
+    for (int i = 0; i < rows; ++i) {
       if constexpr (A_KMAJOR) {
-        af[slot][i] = *(const lds_bf16x8_t*)(la + a_reg[kk] + i * 32 * ROW_BYTES);
+        af[slot][i] = *(const lds_bf16x8_t*)(la + a_reg[kk] + slice_row<WM, HALVES>(0, i) * ROW_BYTES);
       } else {
         constexpr uint32_t R = MNMajorDirect<BM>::ROWB;
         const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(la + a_reg[i] + kk * 16 * R));
@@ -1175,9 +1224,9 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
       }
     }
   };
-  auto mm = [&](int slot) __attribute__((always_inline)) {
+  auto mm = [&](int slot, int rows = TM) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int i = 0; i < rows; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bfr[slot][j], af[slot][i], acc[i][j], 0, 0, 0);
@@ -1185,7 +1234,18 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
   // The order of a k16 step: its next-step fragment reads (8, 12 or 16 LDS
   // instructions) and the loads spread between its 16 MFMAs.
   constexpr int NR = (A_KMAJOR ? TM : 2 * TM) + (B_KMAJOR ? TN : 2 * TN);
-  auto order = [](bool loads) __attribute__((always_inline)) {
+  constexpr int NR2 = TM / 2 + (B_KMAJOR ? TN : 2 * TN);  // of a half tile's step, between 8 MFMAs
+  auto order = [](bool loads, bool half = false) __attribute__((always_inline)) {
+    if (half) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        if (q < NR2 - 8) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        else if (q < NR2) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (loads && (q & 1)) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+      }
+      return;
+    }
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       if constexpr (NR == 12) {
@@ -1230,8 +1290,11 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
     }
     __builtin_amdgcn_sched_barrier(0);
   }
-  // k-tile u on A stage SA and B stage SB
-  auto tile = [&](int u, auto sac, auto sbc) __attribute__((always_inline)) {
+  // k-tile u on A stage SA and B stage SB; HALF: of a tile's first 128 rows alone
+  // (slices 0 and 1 of each wave), whose A loads are the first 4 of a wave's 8.
+  auto tile = [&](int u, auto sac, auto sbc, auto halfc) __attribute__((always_inline)) {
+    constexpr bool HALF = decltype(halfc)::value;
+    constexpr int ROWS = HALF ? TM / 2 : TM;
     constexpr int SA = decltype(sac)::value, SB = decltype(sbc)::value;
     uint8_t* la_ = SA == 0 ? As0 : SA == 1 ? As1 : As2;
     uint8_t* na_ = SA == 0 ? As1 : SA == 1 ? As2 : As0;
@@ -1240,53 +1303,68 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
     uint8_t* nb_ = SB == 0 ? Bs1 : Bs0;                  // B of k-tile u + 1
     const lds_ptr la = (lds_ptr)la_, lb = (lds_ptr)lb_;
     const rsrc_t r_b1 = rb_at(tk(u + 1)), r_a2 = ra_at(tk(u + 2)), r_b2 = rb_at(tk(u + 2));
-    rd(la, lb, 1, 1);
+    rd(la, lb, 1, 1, ROWS);
 #pragma unroll
     for (int i = 4; i < 8; ++i) ld_b.issue_one(r_b1, i, nb_);
-    mm(0);
-    order(true);
+    mm(0, ROWS);
+    order(true, HALF);
     __builtin_amdgcn_sched_barrier(0);
-    rd(la, lb, 2, 0);
+    rd(la, lb, 2, 0, ROWS);
 #pragma unroll
     for (int i = 0; i < 4; ++i) ld_a.issue_one(r_a2, i, fa_);
-    mm(1);
-    order(true);
+    mm(1, ROWS);
+    order(true, HALF);
     __builtin_amdgcn_sched_barrier(0);
-    rd(la, lb, 3, 1);
+    rd(la, lb, 3, 1, ROWS);
+    if constexpr (!HALF) {
 #pragma unroll
-    for (int i = 4; i < 8; ++i) ld_a.issue_one(r_a2, i, fa_);
-    mm(0);
-    order(true);
+      for (int i = 4; i < 8; ++i) ld_a.issue_one(r_a2, i, fa_);
+    }
+    mm(0, ROWS);
+    order(!HALF, HALF);
     __builtin_amdgcn_sched_barrier(0);
     // Every read of this stage done, k-tile u + 1 landed (the 8 A loads of
-    // k-tile u + 2 may be in flight): a plain barrier, no memory fence.
-    asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+    // k-tile u + 2, or the half tile's 4, may be in flight): a plain barrier, no
+    // memory fence.
+    if constexpr (HALF) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    rd((lds_ptr)na_, (lds_ptr)nb_, 0, 0);
+    rd((lds_ptr)na_, (lds_ptr)nb_, 0, 0, ROWS);
 #pragma unroll
     for (int i = 0; i < 4; ++i) ld_b.issue_one(r_b2, i, lb_);
-    mm(1);
-    order(true);
+    mm(1, ROWS);
+    order(true, HALF);
     __builtin_amdgcn_sched_barrier(0);
   };
-  {
-    int u = 0;
-    if (phase <= 0) tile(u++, std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
-    if (phase <= 1) tile(u++, std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-    if (phase <= 2) tile(u++, std::integral_constant<int, 2>{}, std::integral_constant<int, 0>{});
-    if (phase <= 3) tile(u++, std::integral_constant<int, 0>{}, std::integral_constant<int, 1>{});
-    if (phase <= 4) tile(u++, std::integral_constant<int, 1>{}, std::integral_constant<int, 0>{});
-    tile(u++, std::integral_constant<int, 2>{}, std::integral_constant<int, 1>{});
-    for (; u < KT; u += 6) {
-      tile(u, std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
-      tile(u + 1, std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-      tile(u + 2, std::integral_constant<int, 2>{}, std::integral_constant<int, 0>{});
-      tile(u + 3, std::integral_constant<int, 0>{}, std::integral_constant<int, 1>{});
-      tile(u + 4, std::integral_constant<int, 1>{}, std::integral_constant<int, 0>{});
-      tile(u + 5, std::integral_constant<int, 2>{}, std::integral_constant<int, 1>{});
-    }
+#define MR_TILE(U, SA, SB) tile(U, std::integral_constant<int, SA>{}, std::integral_constant<int, SB>{}, half)
+#define MR_K_LOOP()                        \
+  {                                        \
+    int u = 0;                             \
+    if (phase <= 0) MR_TILE(u++, 0, 0);    \
+    if (phase <= 1) MR_TILE(u++, 1, 1);    \
+    if (phase <= 2) MR_TILE(u++, 2, 0);    \
+    if (phase <= 3) MR_TILE(u++, 0, 1);    \
+    if (phase <= 4) MR_TILE(u++, 1, 0);    \
+    MR_TILE(u++, 2, 1);                    \
+    for (; u < KT; u += 6) {               \
+      MR_TILE(u, 0, 0);                    \
+      MR_TILE(u + 1, 1, 1);                \
+      MR_TILE(u + 2, 2, 0);                \
+      MR_TILE(u + 3, 0, 1);                \
+      MR_TILE(u + 4, 1, 0);                \
+      MR_TILE(u + 5, 2, 1);                \
+    }                                      \
   }
+  if (HALVES && p.M - m0 <= 128) {
+    constexpr std::bool_constant<HALVES> half;
+    MR_K_LOOP()
+  } else {
+    constexpr std::false_type half;
+    MR_K_LOOP()
+  }
+#undef MR_K_LOOP
+#undef MR_TILE
   // the repeated last loads land, every wave is past its reads: LDS is free
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
@@ -1295,7 +1373,7 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
     return;
   }
   uint8_t* region = wave == 0 ? As0 : wave == 1 ? As1 : wave == 2 ? As2 : Bs0;
-  store_tile<WM, WN, STAGE, EPI, OUT_BF16>(p, acc, m0, n0, wm, wn, lane, region);
+  store_tile<WM, WN, STAGE, EPI, OUT_BF16, HALVES>(p, acc, m0, n0, wm, wn, lane, region);
 }
 
 // ---- deep-pipelined 4-wave kernel, 128 x 128 or 256 x 128 tiles, one block per CU --
@@ -1548,15 +1626,19 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
 // apart), a thread 4 columns of a row: the partials and the outputs both move
 // in whole 128-byte lines. (Against row-major partials and element-wise output:
 // the 3B split-precision products' reduces 33 -> 24 and 31 -> 25 us.)
-template <int BM, int BN, int EPI, bool OUT_BF16>
-__global__ __launch_bounds__(256) void gemm_reduce(GemmParams p) {
+template <int BM, int BN, int EPI, bool OUT_BF16, bool A_KMAJOR = true, class P = GemmParams>
+__global__ __launch_bounds__(256) void gemm_reduce(P p) {
   typedef float f32x4 __attribute__((ext_vector_type(4)));
   constexpr int NB = is_swiglu(EPI) ? BN / 64 : BN / 32;  // blocks (or pairs) across a tile
   constexpr int PER_TILE = (BM / 32) * NB;
   const int t = static_cast<int>(blockIdx.x) / PER_TILE, rem = static_cast<int>(blockIdx.x) % PER_TILE;
   const int bi = rem / NB, bj = rem % NB;
   int bm, bn;
-  tile_coords(p.tile0 + t, p.grid_m, p.grid_n, bm, bn);
+  if constexpr (P::kGrouped) {
+    if (!enter<BM, BN, A_KMAJOR, OUT_BF16>(p, t, bm, bn)) return;
+  } else {
+    tile_coords(p.tile0 + t, p.grid_m, p.grid_n, bm, bn);
+  }
   const int r = threadIdx.x >> 3, c = threadIdx.x & 7;  // row and 4-column piece of the block
   const int row = bm * BM + bi * 32 + r;
   if constexpr (is_act_bwd(EPI)) {
@@ -1565,7 +1647,7 @@ __global__ __launch_bounds__(256) void gemm_reduce(GemmParams p) {
     if (row >= p.M) return;
   }
   auto sum4 = [&](int b) __attribute__((always_inline)) {  // piece of block column b, splits in order
-    const float* part = p.ws + static_cast<int64_t>(t) * p.ksplit * (BM * BN) +
+    const float* part = p.ws + static_cast<int64_t>(P::kGrouped ? p.tile0 : t) * p.ksplit * (BM * BN) +
                         ((bi * (BN / 32) + b) * 4 + (c >> 1)) * 256 + ((c & 1) * 32 + r) * 4;
     f32x4 a = *reinterpret_cast<const f32x4*>(part);
 #pragma unroll 4

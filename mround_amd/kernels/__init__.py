@@ -38,6 +38,7 @@ __all__ = [
     "gemm_act",
     "gemm_act_bwd",
     "gemm_experts",
+    "gemm_experts_plan",
     "gemm_experts_swiglu",
     "gemm_experts_swiglu_bwd",
     "lib",
@@ -106,9 +107,12 @@ _SIGNATURES = {
     "mr_gemm_act_bwd": (_I, [_L, _L, _L, _P, _L, _P, _L, _P, _L, _I, _P, _L, _P, _P, ctypes.c_size_t, _P,
                              ctypes.c_size_t, _P]),
     "mr_act_bwd": (_I, [_L, _L, _P, _I, _L, _P, _L, _I, _P, _L, _P, _P, ctypes.c_size_t, _P]),
-    "mr_gemm_experts": (_I, [_I, _L, _L, _L, _L, _P, _L, _P, _L, _P, _L, _L, _P, _P, _I, _L, _L, _I, _P]),
-    "mr_gemm_experts_swiglu": (_I, [_L, _L, _L, _L, _P, _L, _P, _L, _P, _L, _L, _P, _P, _L, _P, _L, _P]),
-    "mr_gemm_experts_swiglu_bwd": (_I, [_L, _L, _L, _L, _P, _L, _P, _L, _L, _P, _P, _L, _P, _L, _P]),
+    "mr_gemm_experts_plan": (_I, [_I, _I, _L, _L, _L, _L, _P, _P, _P]),
+    "mr_gemm_experts": (_I, [_I, _L, _L, _L, _L, _P, _L, _P, _L, _P, _L, _L, _P, _P, _I, _L, _L, _I, _P, ctypes.c_size_t,
+                             _P]),
+    "mr_gemm_experts_swiglu": (_I, [_L, _L, _L, _L, _P, _L, _P, _L, _P, _L, _L, _P, _P, _L, _P, _L, _P, ctypes.c_size_t,
+                                    _P]),
+    "mr_gemm_experts_swiglu_bwd": (_I, [_L, _L, _L, _L, _P, _L, _P, _L, _L, _P, _P, _L, _P, _L, _P, ctypes.c_size_t, _P]),
     "mr_route_workspace_bytes": (ctypes.c_size_t, [_L, _L]),
     "mr_route_experts": (_I, [_P, _I, _L, _L, _L, _L, _I, _F, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P]),
     "mr_route_experts_bwd": (_I, [_P, _P, _I, _L, _P, _L, _L, _L, _I, _F, _P, _L, _P]),
@@ -781,7 +785,28 @@ def route_experts_bwd(dweights, logits, ids, dlogits, *, normalize=False, scale=
     _check(rc, "mr_route_experts_bwd")
 
 
-def gemm_experts(layout: str, a, b, c, *, offsets, rows=None, accumulate=False) -> None:
+EXPERTS_WAYS = ("few", "small", "large")
+
+
+def gemm_experts_plan(layout: str, output: str, experts: int, M: int, N: int, K: int) -> tuple[str, int, int]:
+    """``mr_gemm_experts_plan``: (way, blocks along K of a tile, bytes of partials) of a
+    grouped product of width N; M, or for "tn" K, counts all experts' rows."""
+    way, split, nbytes = ctypes.c_int(), ctypes.c_int(), ctypes.c_size_t()
+    rc = lib().mr_gemm_experts_plan(GEMM_LAYOUT[layout], GEMM_OUTPUT[output], experts, M, N, K, ctypes.byref(way),
+                                    ctypes.byref(split), ctypes.byref(nbytes))
+    _check(rc, "mr_gemm_experts_plan")
+    return EXPERTS_WAYS[way.value], split.value, nbytes.value
+
+
+def _experts_ws(layout: str, output: str, device, experts: int, M: int, N: int, K: int, workspace):
+    """As :func:`_gemm_ws`."""
+    if workspace is not None:
+        return workspace
+    nbytes = gemm_experts_plan(layout, output, experts, M, N, K)[2]
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def gemm_experts(layout: str, a, b, c, *, offsets, rows=None, accumulate=False, workspace=None) -> None:
     """``mr_gemm_experts``: products of rows in the experts' order (``offsets``
     int32 ``[E + 1]``, as :func:`route_experts` gives them) with each expert's matrix,
     bfloat16 operands:
@@ -793,7 +818,9 @@ def gemm_experts(layout: str, a, b, c, *, offsets, rows=None, accumulate=False) 
       for an expert without rows), or with ``accumulate`` added to what ``c`` holds.
 
     Rows of ``c`` outside the offsets are left. N (and M) is a multiple of 8, K of
-    64; the experts' row counts are any."""
+    64; the experts' row counts are any. ``workspace``: partials of products of few
+    tiles, which are cut along K (a device tensor of the bytes that
+    :func:`gemm_experts_plan` names); None allocates them for the call."""
     if layout not in GEMM_LAYOUT:
         raise KernelError(f"gemm_experts: layout must be one of {', '.join(GEMM_LAYOUT)}, got {layout!r}")
     name = "gemm_experts"
@@ -817,18 +844,21 @@ def gemm_experts(layout: str, a, b, c, *, offsets, rows=None, accumulate=False) 
         _matrix(name, "c", c, (torch.bfloat16, torch.float32), (M, N))
         _dense(name, "rows", rows, torch.int32, (M,))
         ldc, c_step = _ld(c), 0
-    _one_device(name, a, b, c, offsets, rows)
+    _one_device(name, a, b, c, offsets, rows, workspace)
+    output = "resid" if accumulate else "bf16" if c.dtype == torch.bfloat16 else "f32"
+    ws = _experts_ws(layout, output, a.device, E, M, N, K, workspace)
+    ws_ptr, ws_bytes = _ws_args(ws)
     rc = lib().mr_gemm_experts(GEMM_LAYOUT[layout], E, M, N, K, _rows_ptr(a), _ld(a), _ptr(rows), a_rows, b.data_ptr(),
                                ldb, b_step, _ptr(offsets), c.data_ptr(), dtype_code(c.dtype), ldc, c_step,
-                               int(accumulate), _stream(a))
+                               int(accumulate), ws_ptr, ws_bytes, _stream(a))
     _check(rc, "mr_gemm_experts")
 
 
-def gemm_experts_swiglu(x, wgu, act, gu=None, *, offsets, rows=None) -> None:
+def gemm_experts_swiglu(x, wgu, act, gu=None, *, offsets, rows=None, workspace=None) -> None:
     """``mr_gemm_experts_swiglu``: :func:`gemm_swiglu` over rows in the experts'
     order, each with its expert's interleaved gate/up weight, ``wgu`` ``[E, 2N, K]``;
-    ``act`` ``[R, N]`` and ``gu`` ``[R, 2N]`` bfloat16. ``offsets`` and ``rows`` as
-    :func:`gemm_experts`'. N is a multiple of 32, K of 64."""
+    ``act`` ``[R, N]`` and ``gu`` ``[R, 2N]`` bfloat16. ``offsets``, ``rows`` and
+    ``workspace`` as :func:`gemm_experts`'. N is a multiple of 32, K of 64."""
     name = "gemm_experts_swiglu"
     _bf16_matrix(name, "x", x)
     E = offsets.numel() - 1
@@ -842,13 +872,16 @@ def gemm_experts_swiglu(x, wgu, act, gu=None, *, offsets, rows=None) -> None:
     if gu is not None:
         _bf16_matrix(name, "gu", gu, (R, 2 * N))
     _dense(name, "rows", rows, torch.int32, (R,))
-    _one_device(name, x, wgu, act, gu, offsets, rows)
+    _one_device(name, x, wgu, act, gu, offsets, rows, workspace)
+    ws = _experts_ws("nt", "swiglu", x.device, E, R, 2 * N, K, workspace)
+    ws_ptr, ws_bytes = _ws_args(ws)
     rc = lib().mr_gemm_experts_swiglu(E, R, N, K, _rows_ptr(x), _ld(x), _ptr(rows), x_rows, wgu.data_ptr(), ldw, step,
-                                      _ptr(offsets), _rows_ptr(act), _ld(act), _rows_ptr(gu), _ld(gu), _stream(x))
+                                      _ptr(offsets), _rows_ptr(act), _ld(act), _rows_ptr(gu), _ld(gu), ws_ptr, ws_bytes,
+                                      _stream(x))
     _check(rc, "mr_gemm_experts_swiglu")
 
 
-def gemm_experts_swiglu_bwd(dy, wd, gu, dgu, *, offsets) -> None:
+def gemm_experts_swiglu_bwd(dy, wd, gu, dgu, *, offsets, workspace=None) -> None:
     """``mr_gemm_experts_swiglu_bwd``: ``dgu`` from ``dact = dy[r] wd[e]`` and the saved
     interleaved gate/up ``gu`` ``[R, 2N]`` (``dgu`` may be ``gu``); ``wd`` ``[E, K,
     N]``, the down weights, ``dy`` ``[R, K]`` in the experts' order."""
@@ -862,9 +895,11 @@ def gemm_experts_swiglu_bwd(dy, wd, gu, dgu, *, offsets) -> None:
     ldw, step = _stacked(name, "wd", wd, torch.bfloat16, (E, K, N))
     _bf16_matrix(name, "gu", gu, (R, 2 * N))
     _bf16_matrix(name, "dgu", dgu, (R, 2 * N))
-    _one_device(name, dy, wd, gu, dgu, offsets)
+    _one_device(name, dy, wd, gu, dgu, offsets, workspace)
+    ws = _experts_ws("nn", "swiglu_bwd", dy.device, E, R, N, K, workspace)
+    ws_ptr, ws_bytes = _ws_args(ws)
     rc = lib().mr_gemm_experts_swiglu_bwd(E, R, N, K, _rows_ptr(dy), _ld(dy), wd.data_ptr(), ldw, step, _ptr(offsets),
-                                          _rows_ptr(gu), _ld(gu), _rows_ptr(dgu), _ld(dgu), _stream(dy))
+                                          _rows_ptr(gu), _ld(gu), _rows_ptr(dgu), _ld(dgu), ws_ptr, ws_bytes, _stream(dy))
     _check(rc, "mr_gemm_experts_swiglu_bwd")
 
 

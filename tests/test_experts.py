@@ -306,9 +306,25 @@ def test_places_outside_the_rows_are_none():
 # rows of each expert: none at all, one, whole tiles and not, each side of the choice of tiles
 COUNTS = {"none": [0, 0, 0], "one": [1], "few": [0, 1, 2, 0, 3, 1, 0, 0], "odd": [63, 0, 65, 1, 130, 64, 7],
           "large": [300, 0, 513, 1], "many": [(37 * i * i) % 23 for i in range(150)], "skewed": [0, 5, 1500, 2],
-          "whole": [256, 512]}
-# (N, K)
-SIZES = [(8, 64), (72, 128), (264, 192), (520, 448), (768, 2048)]
+          "whole": [256, 512], "long": [2100, 1, 1500], "tall": [1900, 130, 0, 2300, 1701]}
+WEIGHT_SIZES = [(8, 8), (72, 264), (264, 72), (520, 448), (2560, 2560)]
+SWIGLU_SIZES = [(32, 64), (96, 128), (288, 192), (704, 448), (96, 2048), (2048, 1024)]
+# (N, K): with the counts, every way that a product runs (test_products_take_every_way)
+SIZES = [(8, 64), (72, 128), (264, 192), (520, 448), (768, 2048), (2048, 1024)]
+
+
+def test_products_take_every_way():
+    rows = [(len(n), sum(n)) for n in COUNTS.values() if sum(n)]
+    for layout, output in (("nt", "bf16"), ("nt", "f32"), ("nn", "bf16"), ("nn", "f32")):
+        plans = {K.gemm_experts_plan(layout, output, E, R, N, Kd)[:2] for E, R in rows for N, Kd in SIZES}
+        assert {p[0] for p in plans} == {"few", "small", "large"} and any(s > 1 for _, s in plans), (layout, output, plans)
+    for layout, output in (("nt", "swiglu"), ("nn", "swiglu_bwd")):
+        wide = 2 if layout == "nt" else 1
+        plans = {K.gemm_experts_plan(layout, output, E, R, wide * N, Kd)[:2] for E, R in rows for N, Kd in SWIGLU_SIZES}
+        assert {p[0] for p in plans} == {"few", "small", "large"} and any(s > 1 for _, s in plans), (output, plans)
+    for output in ("f32", "resid"):
+        plans = {K.gemm_experts_plan("tn", output, E, M, N, R)[:2] for E, R in rows for M, N in WEIGHT_SIZES}
+        assert {p[0] for p in plans} == {"small", "large"} and any(s > 1 for _, s in plans), (output, plans)
 
 
 def offsets_of(counts):
@@ -365,7 +381,7 @@ def test_rows_products(counts, N, Kd):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("counts", COUNTS)
-@pytest.mark.parametrize("M,N", [(8, 8), (72, 264), (264, 72), (520, 448)])
+@pytest.mark.parametrize("M,N", WEIGHT_SIZES)
 def test_weight_products(counts, M, N):
     n = COUNTS[counts]
     E, R = len(n), sum(COUNTS[counts])
@@ -400,7 +416,7 @@ def halves(t):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("counts", COUNTS)
-@pytest.mark.parametrize("N,Kd", [(32, 64), (96, 128), (288, 192), (704, 448)])
+@pytest.mark.parametrize("N,Kd", SWIGLU_SIZES)
 def test_swiglu_products(counts, N, Kd):
     n, extra = COUNTS[counts], 4
     E, R = len(n), sum(COUNTS[counts])
@@ -661,7 +677,7 @@ def test_rows_refuse(fn, base, change, message):
 
 
 GEMM = dict(layout=0, E=4, M=100, N=64, K=128, A=address(0), lda=128, index=None, a_rows=0, B=address(1), ldb=128,
-            b_step=64 * 128, off=address(2), C=address(3), cdt=1, ldc=64, c_step=0, acc=0, stream=None)
+            b_step=64 * 128, off=address(2), C=address(3), cdt=1, ldc=64, c_step=0, acc=0, ws=None, ws_bytes=0, stream=None)
 TN = dict(GEMM, layout=2, M=64, K=100, lda=64, ldb=64, cdt=0, c_step=64 * 64)
 
 
@@ -673,6 +689,7 @@ TN = dict(GEMM, layout=2, M=64, K=100, lda=64, ldb=64, cdt=0, c_step=64 * 64)
     (GEMM, dict(C=address(0)), "overlap"), (GEMM, dict(acc=1), "added"), (GEMM, dict(lda=1 << 23), "leading dimensions above"),
     (GEMM, dict(index=address(4), a_rows=0), "4 GiB"), (GEMM, dict(index=address(4), a_rows=1 << 30), "4 GiB"),
     (GEMM, dict(index=address(4), layout=1, ldb=64), "nt"), (GEMM, dict(A=ctypes.c_void_p(A + 2)), "aligned"),
+    (GEMM, dict(ws=address(0), ws_bytes=1 << 20), "overlap"), (GEMM, dict(ws=ctypes.c_void_p(A + 8), ws_bytes=64), "aligned"),
     (TN, dict(cdt=1), "fp32"), (TN, dict(M=60, lda=64), "multiples of 8"), (TN, dict(c_step=4092), "overlap"),
     (TN, dict(index=address(4), a_rows=5), "nt"), (TN, dict(lda=56), "smaller")])
 def test_products_refuse(base, change, message):
@@ -680,9 +697,9 @@ def test_products_refuse(base, change, message):
 
 
 SWIGLU = dict(E=4, M=100, N=64, K=128, X=address(0), ldx=128, index=None, rows=0, W=address(1), ldw=128, step=128 * 128,
-              off=address(2), act=address(3), ldact=64, gu=address(4), ldgu=128, stream=None)
+              off=address(2), act=address(3), ldact=64, gu=address(4), ldgu=128, ws=None, ws_bytes=0, stream=None)
 SWIGLU_BWD = dict(E=4, M=100, N=64, K=128, dy=address(0), ldd=128, W=address(1), ldw=64, step=128 * 64, off=address(2),
-                  gu=address(3), ldgu=128, dgu=address(4), lddgu=128, stream=None)
+                  gu=address(3), ldgu=128, dgu=address(4), lddgu=128, ws=None, ws_bytes=0, stream=None)
 
 
 @pytest.mark.parametrize("fn,base,change,message", [
@@ -692,7 +709,8 @@ SWIGLU_BWD = dict(E=4, M=100, N=64, K=128, dy=address(0), ldd=128, W=address(1),
     ("mr_gemm_experts_swiglu_bwd", SWIGLU_BWD, dict(N=40), "32"), ("mr_gemm_experts_swiglu_bwd", SWIGLU_BWD, dict(K=96), "64"),
     ("mr_gemm_experts_swiglu_bwd", SWIGLU_BWD, dict(dgu=address(0)), "overlap"),
     ("mr_gemm_experts_swiglu_bwd", SWIGLU_BWD, dict(dgu=address(3), lddgu=136), "unless dgu is gu"),
-    ("mr_gemm_experts_swiglu_bwd", SWIGLU_BWD, dict(gu=None), "null")])
+    ("mr_gemm_experts_swiglu_bwd", SWIGLU_BWD, dict(gu=None), "null"),
+    ("mr_gemm_experts_swiglu_bwd", SWIGLU_BWD, dict(dgu=address(3), ws=address(3), ws_bytes=1 << 10), "workspace")])
 def test_swiglu_refuses(fn, base, change, message):
     refused(fn, list(dict(base, **change).values()), message)
 
