@@ -494,13 +494,15 @@ int mr_route_experts_bwd(const float* dweights, const void* logits, int dtype, i
  * workspace: partials of products that are cut along K, which those of few tiles are:
  * a smaller one than mr_gemm_experts_plan names, or none, leaves them whole.
  * mr_gemm_experts_plan: how a product runs (blocks of 16 rows, 128 x 128 or 256 x 256
- * tiles), the blocks along K of a tile and the partials' bytes, for the product's
+ * tiles), the blocks along K of a tile and the partials' bytes (which
+ * mr_gemm_experts_workspace_bytes returns alone), for the product's
  * width (2N for the SwiGLU pair) and an output of mr_gemm_plan's kinds; M, or for
  * MR_TN K, is all experts' rows.
  */
 enum { MR_EXPERTS_FEW = 0, MR_EXPERTS_SMALL = 1, MR_EXPERTS_LARGE = 2 };
 int mr_gemm_experts_plan(int layout, int output, int64_t experts, int64_t M, int64_t N, int64_t K, int* way_out,
                          int* split_out, size_t* workspace_out);
+size_t mr_gemm_experts_workspace_bytes(int layout, int output, int64_t experts, int64_t M, int64_t N, int64_t K);
 int mr_gemm_experts(int layout, int64_t experts, int64_t M, int64_t N, int64_t K, const void* A, int64_t lda,
                     const int32_t* index, int64_t a_rows, const void* B, int64_t ldb, int64_t b_step,
                     const int32_t* offsets, void* C, int c_dtype, int64_t ldc, int64_t c_step, int accumulate,

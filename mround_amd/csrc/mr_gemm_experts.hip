@@ -354,6 +354,12 @@ int64_t all_rows_bytes(int64_t experts, int64_t step, int64_t rows, int64_t ld, 
 
 extern "C" {
 
+size_t mr_gemm_experts_workspace_bytes(int layout, int output, int64_t experts, int64_t M, int64_t N, int64_t K) {
+  int way, split;
+  size_t bytes = 0;
+  return mr_gemm_experts_plan(layout, output, experts, M, N, K, &way, &split, &bytes) == MR_OK ? bytes : 0;
+}
+
 int mr_gemm_experts_plan(int layout, int output, int64_t experts, int64_t M, int64_t N, int64_t K, int* way_out,
                          int* split_out, size_t* workspace_out) {
   using namespace mr;

@@ -107,6 +107,7 @@ _SIGNATURES = {
     "mr_gemm_act_bwd": (_I, [_L, _L, _L, _P, _L, _P, _L, _P, _L, _I, _P, _L, _P, _P, ctypes.c_size_t, _P,
                              ctypes.c_size_t, _P]),
     "mr_act_bwd": (_I, [_L, _L, _P, _I, _L, _P, _L, _I, _P, _L, _P, _P, ctypes.c_size_t, _P]),
+    "mr_gemm_experts_workspace_bytes": (ctypes.c_size_t, [_I, _I, _L, _L, _L, _L]),
     "mr_gemm_experts_plan": (_I, [_I, _I, _L, _L, _L, _L, _P, _P, _P]),
     "mr_gemm_experts": (_I, [_I, _L, _L, _L, _L, _P, _L, _P, _L, _P, _L, _L, _P, _P, _I, _L, _L, _I, _P, ctypes.c_size_t,
                              _P]),
@@ -241,17 +242,22 @@ def _ld(t: torch.Tensor | None) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _one_device(name: str, *tensors: torch.Tensor | None) -> None:
-    """Refuse operands that do not share the current device: the launch goes to
-    its stream, and the pointers would be another device's."""
+def _one_device(name: str, *tensors: torch.Tensor | None) -> int:
+    """Refuse operands that do not share the current device (the launch goes to
+    its stream, and the pointers would be another device's); the device."""
+    device = None
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        at = t.get_device()
+        if at == device:
+            continue
+        if at < 0:
             raise KernelError("tensors passed to the HIP library must live on a ROCm device")
-        if t.get_device() != torch._C._cuda_getDevice():
-            raise KernelError(f"{name}: every tensor must live on the current device "
-                              f"(cuda:{torch._C._cuda_getDevice()}), got one on {t.device}")
+        device = torch._C._cuda_getDevice()
+        if at != device:
+            raise KernelError(f"{name}: every tensor must live on the current device (cuda:{device}), got one on {t.device}")
+    return device
 
 
 def _f32(t: torch.Tensor | None, name: str) -> torch.Tensor | None:
@@ -711,29 +717,66 @@ def act_bwd(dout, pre, dpre, *, act, dbias=None) -> None:
 
 
 # ------------------------------------------------------------------ experts --
+#
+# A call on a few tokens takes as long as its checks (the launch itself is 3 us of
+# the 6 to 8), so each operand is looked at once: its type, its shape, its strides,
+# then the devices of all.
 
-def _dense(name: str, what: str, t, dtype, shape) -> None:
-    """A contiguous tensor of one type and shape, or None."""
-    if t is not None and (t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
-        raise KernelError(f"{name}: {what} must be contiguous {str(dtype).removeprefix('torch.')} {list(shape)}, got "
-                          f"{t.dtype} {list(t.shape)}")
-
-
-def _matrix(name: str, what: str, t, dtypes, shape) -> None:
-    if t is not None and (t.dtype not in dtypes or t.dim() != 2 or tuple(t.shape) != tuple(shape)):
-        kinds = " or ".join(str(d).removeprefix("torch.") for d in dtypes)
-        raise KernelError(f"{name}: {what} must be {kinds} {list(shape)}, got {t.dtype} {list(t.shape)}")
+def _refuse(name: str, what: str, t, dtypes, shape, how: str) -> None:
+    kinds = " or ".join(str(d).removeprefix("torch.") for d in dtypes)
+    raise KernelError(f"{name}: {what} must be {how} {kinds} {list(shape)}, got {t.dtype} {list(t.shape)} of strides "
+                      f"{list(t.stride())}")
 
 
-def _stacked(name: str, what: str, t, dtype, shape):
-    """The experts' matrices ``[E, rows, cols]``, unit stride along a row: (leading
-    dimension, elements between experts)."""
-    if t.dtype != dtype or t.dim() != 3 or tuple(t.shape) != tuple(shape) or (t.shape[2] > 1 and t.stride(2) != 1):
-        raise KernelError(f"{name}: {what} must be {str(dtype).removeprefix('torch.')} {list(shape)} with contiguous "
-                          f"rows, got {t.dtype} {list(t.shape)}")
-    ld = t.stride(1) if t.shape[1] > 1 else t.shape[2]
-    # (one expert's step says nothing: torch leaves any value there)
-    return ld, (t.stride(0) if t.shape[0] > 1 else t.shape[1] * ld)
+def _dense(name: str, what: str, t, dtype, shape) -> int | None:
+    """The address of a contiguous tensor of one type and shape, or of none."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        _refuse(name, what, t, (dtype,), shape, "contiguous")
+    return t.data_ptr()
+
+
+def _matrix(name: str, what: str, t, dtypes, shape) -> tuple[int | None, int]:
+    """(address, leading dimension) of a matrix whose rows may lie apart, or of none. A
+    single row's stride says nothing: torch leaves any value there."""
+    if t is None:
+        return None, 0
+    rows, cols = shape
+    if t.dtype not in dtypes or t.shape != shape:
+        _refuse(name, what, t, dtypes, shape, "a matrix of contiguous rows,")
+    ld, step = t.stride()
+    if cols > 1 and step != 1:
+        _refuse(name, what, t, dtypes, shape, "a matrix of contiguous rows,")
+    return t.data_ptr(), ld if rows > 1 else cols
+
+
+def _stacked(name: str, what: str, t, dtype, shape) -> tuple[int, int, int]:
+    """(address, leading dimension, elements between experts) of the experts'
+    matrices ``[E, rows, cols]``."""
+    if t.dtype is not dtype or t.shape != shape:
+        _refuse(name, what, t, (dtype,), shape, "matrices of contiguous rows,")
+    E, rows, cols = shape
+    step, ld, one = t.stride()
+    if cols > 1 and one != 1:
+        _refuse(name, what, t, (dtype,), shape, "matrices of contiguous rows,")
+    ld = ld if rows > 1 else cols
+    return t.data_ptr(), ld, step if E > 1 else rows * ld
+
+
+def _size2(name: str, what: str, t) -> tuple[int, int]:
+    if t.dim() != 2:
+        raise KernelError(f"{name}: {what} must be a matrix, got {list(t.shape)}")
+    return t.shape
+
+
+def _scratch(nbytes: int, device: int):
+    """(address, tensor) of a call's own scratch memory, which the allocator ties to
+    the current stream (the tensor is held until the launch)."""
+    if not nbytes:
+        return None, None
+    t = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
+    return t.data_ptr(), t
 
 
 def route_experts(logits, *, weights, ids, offsets=None, slots=None, rows=None, normalize=False, scale=1.0) -> None:
@@ -747,22 +790,20 @@ def route_experts(logits, *, weights, ids, offsets=None, slots=None, rows=None, 
     products take: expert e's places are ``offsets[e] .. offsets[e + 1] - 1``,
     ``slots`` the place of each entry (-1: none), ``rows`` the token at each place
     (those past the last are left). E is at most 512 and k at most 64."""
-    T, E = logits.shape if logits.dim() == 2 else (-1, -1)
-    if T < 0 or weights.dim() != 2:
-        raise KernelError("route_experts: logits [T, E] and weights [T, k] are matrices")
-    k = weights.shape[1]
-    _dense("route_experts", "weights", weights, torch.float32, (T, k))
-    _dense("route_experts", "ids", ids, torch.int32, (T, k))
-    _dense("route_experts", "offsets", offsets, torch.int32, (E + 1,))
-    _dense("route_experts", "slots", slots, torch.int32, (T, k))
-    _dense("route_experts", "rows", rows, torch.int32, (T * k,))
+    name, i32 = "route_experts", torch.int32
+    T, E = _size2(name, "logits", logits)
+    k = _size2(name, "weights", weights)[1]
+    z, ld = _matrix(name, "logits", logits, (logits.dtype,), (T, E))
+    w = _dense(name, "weights", weights, torch.float32, (T, k))
+    i = _dense(name, "ids", ids, i32, (T, k))
+    o, s, r = (_dense(name, "offsets", offsets, i32, (E + 1,)), _dense(name, "slots", slots, i32, (T, k)),
+               _dense(name, "rows", rows, i32, (T * k,)))
     if (offsets is None) != (slots is None) or (offsets is None) != (rows is None):
         raise KernelError("route_experts: offsets, slots and rows come together")
-    _one_device("route_experts", logits, weights, ids, offsets, slots, rows)
-    nbytes = int(lib().mr_route_workspace_bytes(T, E)) if offsets is not None else 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
-    rc = lib().mr_route_experts(_rows_ptr(logits), dtype_code(logits.dtype), _ld(logits), T, E, k, int(normalize), scale,
-                                _ptr(weights), _ptr(ids), _ptr(offsets), _ptr(slots), _ptr(rows), _ptr(ws), nbytes,
+    device = _one_device(name, logits, weights, ids, offsets, slots, rows)
+    nbytes = lib().mr_route_workspace_bytes(T, E) if offsets is not None else 0
+    ws, hold = _scratch(nbytes, device)
+    rc = lib().mr_route_experts(z, dtype_code(logits.dtype), ld, T, E, k, int(normalize), scale, w, i, o, s, r, ws, nbytes,
                                 _stream(logits))
     _check(rc, "mr_route_experts")
 
@@ -772,16 +813,16 @@ def route_experts_bwd(dweights, logits, ids, dlogits, *, normalize=False, scale=
     ``logits``) from that of the weights, ``dweights`` ``[T, k]`` float32, for the
     ``ids`` that :func:`route_experts` chose with the same ``normalize`` and
     ``scale``."""
-    T, E = logits.shape if logits.dim() == 2 else (-1, -1)
-    if T < 0 or ids.dim() != 2:
-        raise KernelError("route_experts_bwd: logits [T, E] and ids [T, k] are matrices")
-    k = ids.shape[1]
-    _dense("route_experts_bwd", "ids", ids, torch.int32, (T, k))
-    _dense("route_experts_bwd", "dweights", dweights, torch.float32, (T, k))
-    _matrix("route_experts_bwd", "dlogits", dlogits, (logits.dtype,), (T, E))
-    _one_device("route_experts_bwd", logits, ids, dweights, dlogits)
-    rc = lib().mr_route_experts_bwd(_ptr(dweights), _rows_ptr(logits), dtype_code(logits.dtype), _ld(logits), _ptr(ids), T,
-                                    E, k, int(normalize), scale, _rows_ptr(dlogits), _ld(dlogits), _stream(logits))
+    name = "route_experts_bwd"
+    T, E = _size2(name, "logits", logits)
+    k = _size2(name, "ids", ids)[1]
+    z, ld = _matrix(name, "logits", logits, (logits.dtype,), (T, E))
+    i = _dense(name, "ids", ids, torch.int32, (T, k))
+    dw = _dense(name, "dweights", dweights, torch.float32, (T, k))
+    dz, lddz = _matrix(name, "dlogits", dlogits, (logits.dtype,), (T, E))
+    _one_device(name, logits, ids, dweights, dlogits)
+    rc = lib().mr_route_experts_bwd(dw, z, dtype_code(logits.dtype), ld, i, T, E, k, int(normalize), scale, dz, lddz,
+                                    _stream(logits))
     _check(rc, "mr_route_experts_bwd")
 
 
@@ -798,12 +839,18 @@ def gemm_experts_plan(layout: str, output: str, experts: int, M: int, N: int, K:
     return EXPERTS_WAYS[way.value], split.value, nbytes.value
 
 
-def _experts_ws(layout: str, output: str, device, experts: int, M: int, N: int, K: int, workspace):
-    """As :func:`_gemm_ws`."""
+def _experts_ws(layout: int, output: int, device: int, experts: int, M: int, N: int, K: int, workspace):
+    """(address, bytes, tensor) of a grouped product's partials: the caller's, or as
+    :func:`_scratch`."""
     if workspace is not None:
-        return workspace
-    nbytes = gemm_experts_plan(layout, output, experts, M, N, K)[2]
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        return *_ws_args(workspace), workspace
+    nbytes = lib().mr_gemm_experts_workspace_bytes(layout, output, experts, M, N, K)
+    at, hold = _scratch(nbytes, device)
+    return at, nbytes, hold
+
+
+_BF16 = (torch.bfloat16,)
+_ROW_TYPES = (torch.float32, torch.bfloat16)
 
 
 def gemm_experts(layout: str, a, b, c, *, offsets, rows=None, accumulate=False, workspace=None) -> None:
@@ -821,36 +868,33 @@ def gemm_experts(layout: str, a, b, c, *, offsets, rows=None, accumulate=False, 
     64; the experts' row counts are any. ``workspace``: partials of products of few
     tiles, which are cut along K (a device tensor of the bytes that
     :func:`gemm_experts_plan` names); None allocates them for the call."""
+    name = "gemm_experts"
     if layout not in GEMM_LAYOUT:
         raise KernelError(f"gemm_experts: layout must be one of {', '.join(GEMM_LAYOUT)}, got {layout!r}")
-    name = "gemm_experts"
-    _bf16_matrix(name, "a", a)
     E = offsets.numel() - 1
-    _dense(name, "offsets", offsets, torch.int32, (E + 1,))
-    a_rows = a.shape[0]
+    off = _dense(name, "offsets", offsets, torch.int32, (E + 1,))
+    a_rows, cols = _size2(name, "a", a)
+    at_a, lda = _matrix(name, "a", a, _BF16, (a_rows, cols))
     if layout == "tn":
-        (K, M), N = a.shape, b.shape[-1]
-        _bf16_matrix(name, "b", b, (K, N))
-        ldc, c_step = _stacked(name, "c", c, torch.float32, (E, M, N))
-        ldb, b_step = _ld(b), 0
         if rows is not None:
             raise KernelError("gemm_experts: only the rows of an 'nt' product may lie at an index")
+        K, M, N = a_rows, cols, _size2(name, "b", b)[1]
+        at_b, ldb = _matrix(name, "b", b, _BF16, (K, N))
+        at_c, ldc, c_step = _stacked(name, "c", c, torch.float32, (E, M, N))
+        index, b_step = None, 0
     else:
         if b.dim() != 3:
             raise KernelError("gemm_experts: b must hold a matrix for each expert")
-        M, K = (a_rows if rows is None else rows.numel()), a.shape[1]
+        M, K = (a_rows if rows is None else rows.numel()), cols
         N = b.shape[1] if layout == "nt" else b.shape[2]
-        ldb, b_step = _stacked(name, "b", b, torch.bfloat16, (E, N, K) if layout == "nt" else (E, K, N))
-        _matrix(name, "c", c, (torch.bfloat16, torch.float32), (M, N))
-        _dense(name, "rows", rows, torch.int32, (M,))
-        ldc, c_step = _ld(c), 0
-    _one_device(name, a, b, c, offsets, rows, workspace)
-    output = "resid" if accumulate else "bf16" if c.dtype == torch.bfloat16 else "f32"
-    ws = _experts_ws(layout, output, a.device, E, M, N, K, workspace)
-    ws_ptr, ws_bytes = _ws_args(ws)
-    rc = lib().mr_gemm_experts(GEMM_LAYOUT[layout], E, M, N, K, _rows_ptr(a), _ld(a), _ptr(rows), a_rows, b.data_ptr(),
-                               ldb, b_step, _ptr(offsets), c.data_ptr(), dtype_code(c.dtype), ldc, c_step,
-                               int(accumulate), ws_ptr, ws_bytes, _stream(a))
+        at_b, ldb, b_step = _stacked(name, "b", b, torch.bfloat16, (E, N, K) if layout == "nt" else (E, K, N))
+        at_c, ldc = _matrix(name, "c", c, _ROW_TYPES, (M, N))
+        index, c_step = _dense(name, "rows", rows, torch.int32, (M,)), 0
+    device = _one_device(name, a, b, c, offsets, rows, workspace)
+    kind, dtype = GEMM_LAYOUT[layout], dtype_code(c.dtype)
+    ws, ws_bytes, hold = _experts_ws(kind, 2 if accumulate else dtype, device, E, M, N, K, workspace)
+    rc = lib().mr_gemm_experts(kind, E, M, N, K, at_a, lda, index, a_rows, at_b, ldb, b_step, off, at_c, dtype, ldc, c_step,
+                               int(accumulate), ws, ws_bytes, _stream(a))
     _check(rc, "mr_gemm_experts")
 
 
@@ -860,24 +904,21 @@ def gemm_experts_swiglu(x, wgu, act, gu=None, *, offsets, rows=None, workspace=N
     ``act`` ``[R, N]`` and ``gu`` ``[R, 2N]`` bfloat16. ``offsets``, ``rows`` and
     ``workspace`` as :func:`gemm_experts`'. N is a multiple of 32, K of 64."""
     name = "gemm_experts_swiglu"
-    _bf16_matrix(name, "x", x)
     E = offsets.numel() - 1
-    _dense(name, "offsets", offsets, torch.int32, (E + 1,))
+    off = _dense(name, "offsets", offsets, torch.int32, (E + 1,))
     if wgu.dim() != 3 or wgu.shape[1] % 2:
         raise KernelError(f"{name}: wgu must be [E, 2N, K]")
-    x_rows, K = x.shape
+    x_rows, K = _size2(name, "x", x)
     R, N = (x_rows if rows is None else rows.numel()), wgu.shape[1] // 2
-    ldw, step = _stacked(name, "wgu", wgu, torch.bfloat16, (E, 2 * N, K))
-    _bf16_matrix(name, "act", act, (R, N))
-    if gu is not None:
-        _bf16_matrix(name, "gu", gu, (R, 2 * N))
-    _dense(name, "rows", rows, torch.int32, (R,))
-    _one_device(name, x, wgu, act, gu, offsets, rows, workspace)
-    ws = _experts_ws("nt", "swiglu", x.device, E, R, 2 * N, K, workspace)
-    ws_ptr, ws_bytes = _ws_args(ws)
-    rc = lib().mr_gemm_experts_swiglu(E, R, N, K, _rows_ptr(x), _ld(x), _ptr(rows), x_rows, wgu.data_ptr(), ldw, step,
-                                      _ptr(offsets), _rows_ptr(act), _ld(act), _rows_ptr(gu), _ld(gu), ws_ptr, ws_bytes,
-                                      _stream(x))
+    at_x, ldx = _matrix(name, "x", x, _BF16, (x_rows, K))
+    w, ldw, step = _stacked(name, "wgu", wgu, torch.bfloat16, (E, 2 * N, K))
+    at_act, ldact = _matrix(name, "act", act, _BF16, (R, N))
+    at_gu, ldgu = _matrix(name, "gu", gu, _BF16, (R, 2 * N))
+    index = _dense(name, "rows", rows, torch.int32, (R,))
+    device = _one_device(name, x, wgu, act, gu, offsets, rows, workspace)
+    ws, ws_bytes, hold = _experts_ws(0, 3, device, E, R, 2 * N, K, workspace)
+    rc = lib().mr_gemm_experts_swiglu(E, R, N, K, at_x, ldx, index, x_rows, w, ldw, step, off, at_act, ldact, at_gu, ldgu,
+                                      ws, ws_bytes, _stream(x))
     _check(rc, "mr_gemm_experts_swiglu")
 
 
@@ -886,24 +927,20 @@ def gemm_experts_swiglu_bwd(dy, wd, gu, dgu, *, offsets, workspace=None) -> None
     interleaved gate/up ``gu`` ``[R, 2N]`` (``dgu`` may be ``gu``); ``wd`` ``[E, K,
     N]``, the down weights, ``dy`` ``[R, K]`` in the experts' order."""
     name = "gemm_experts_swiglu_bwd"
-    _bf16_matrix(name, "dy", dy)
     E = offsets.numel() - 1
-    _dense(name, "offsets", offsets, torch.int32, (E + 1,))
+    off = _dense(name, "offsets", offsets, torch.int32, (E + 1,))
     if wd.dim() != 3:
         raise KernelError(f"{name}: wd must be [E, K, N]")
-    (R, K), N = dy.shape, wd.shape[2]
-    ldw, step = _stacked(name, "wd", wd, torch.bfloat16, (E, K, N))
-    _bf16_matrix(name, "gu", gu, (R, 2 * N))
-    _bf16_matrix(name, "dgu", dgu, (R, 2 * N))
-    _one_device(name, dy, wd, gu, dgu, offsets, workspace)
-    ws = _experts_ws("nn", "swiglu_bwd", dy.device, E, R, N, K, workspace)
-    ws_ptr, ws_bytes = _ws_args(ws)
-    rc = lib().mr_gemm_experts_swiglu_bwd(E, R, N, K, _rows_ptr(dy), _ld(dy), wd.data_ptr(), ldw, step, _ptr(offsets),
-                                          _rows_ptr(gu), _ld(gu), _rows_ptr(dgu), _ld(dgu), ws_ptr, ws_bytes, _stream(dy))
+    (R, K), N = _size2(name, "dy", dy), wd.shape[2]
+    at_dy, ldd = _matrix(name, "dy", dy, _BF16, (R, K))
+    w, ldw, step = _stacked(name, "wd", wd, torch.bfloat16, (E, K, N))
+    at_gu, ldgu = _matrix(name, "gu", gu, _BF16, (R, 2 * N))
+    at_dgu, lddgu = _matrix(name, "dgu", dgu, _BF16, (R, 2 * N))
+    device = _one_device(name, dy, wd, gu, dgu, offsets, workspace)
+    ws, ws_bytes, hold = _experts_ws(1, 5, device, E, R, N, K, workspace)
+    rc = lib().mr_gemm_experts_swiglu_bwd(E, R, N, K, at_dy, ldd, w, ldw, step, off, at_gu, ldgu, at_dgu, lddgu, ws,
+                                          ws_bytes, _stream(dy))
     _check(rc, "mr_gemm_experts_swiglu_bwd")
-
-
-_ROW_TYPES = (torch.float32, torch.bfloat16)
 
 
 def combine_experts(y, slots, out, *, weights=None, resid=None) -> None:
@@ -913,17 +950,15 @@ def combine_experts(y, slots, out, *, weights=None, resid=None) -> None:
     (None: 1). ``y`` and ``out`` float32 or bfloat16; ``resid`` of ``out``'s type, and
     may be ``out``."""
     name = "combine_experts"
-    T, k = slots.shape if slots.dim() == 2 else (-1, -1)
-    R, H = y.shape if y.dim() == 2 else (-1, -1)
-    _dense(name, "slots", slots, torch.int32, (T, k))
-    _matrix(name, "y", y, _ROW_TYPES, (R, H))
-    _matrix(name, "out", out, _ROW_TYPES, (T, H))
-    _matrix(name, "resid", resid, (out.dtype,), (T, H))
-    _dense(name, "weights", weights, torch.float32, (T, k))
+    (T, k), (R, H) = _size2(name, "slots", slots), _size2(name, "y", y)
+    s = _dense(name, "slots", slots, torch.int32, (T, k))
+    at_y, ldy = _matrix(name, "y", y, _ROW_TYPES, (R, H))
+    at_out, ldo = _matrix(name, "out", out, _ROW_TYPES, (T, H))
+    at_r, ldr = _matrix(name, "resid", resid, (out.dtype,), (T, H))
+    w = _dense(name, "weights", weights, torch.float32, (T, k))
     _one_device(name, y, slots, out, weights, resid)
-    rc = lib().mr_combine_experts(_rows_ptr(y), dtype_code(y.dtype), _ld(y), R, _ptr(slots), _ptr(weights), T, k, H,
-                                  _rows_ptr(resid), _ld(resid), _rows_ptr(out), dtype_code(out.dtype), _ld(out),
-                                  _stream(y))
+    rc = lib().mr_combine_experts(at_y, dtype_code(y.dtype), ldy, R, s, w, T, k, H, at_r, ldr, at_out,
+                                  dtype_code(out.dtype), ldo, _stream(y))
     _check(rc, "mr_combine_experts")
 
 
@@ -935,20 +970,18 @@ def spread_experts(x, slots, out, *, weights=None, y=None, dweights=None) -> Non
     y[slots[t, j]]``. ``x`` and ``out`` float32 or bfloat16, ``y`` of ``out``'s type and
     shape, and may be ``out``."""
     name = "spread_experts"
-    T, k = slots.shape if slots.dim() == 2 else (-1, -1)
-    R, H = out.shape if out.dim() == 2 else (-1, -1)
-    _dense(name, "slots", slots, torch.int32, (T, k))
-    _matrix(name, "x", x, _ROW_TYPES, (T, H))
-    _matrix(name, "out", out, _ROW_TYPES, (R, H))
-    _matrix(name, "y", y, (out.dtype,), (R, H))
-    _dense(name, "weights", weights, torch.float32, (T, k))
-    _dense(name, "dweights", dweights, torch.float32, (T, k))
+    (T, k), (R, H) = _size2(name, "slots", slots), _size2(name, "out", out)
+    s = _dense(name, "slots", slots, torch.int32, (T, k))
+    at_x, ldx = _matrix(name, "x", x, _ROW_TYPES, (T, H))
+    at_out, ldo = _matrix(name, "out", out, _ROW_TYPES, (R, H))
+    at_y, ldy = _matrix(name, "y", y, (out.dtype,), (R, H))
+    w = _dense(name, "weights", weights, torch.float32, (T, k))
+    dw = _dense(name, "dweights", dweights, torch.float32, (T, k))
     if (y is None) != (dweights is None):
         raise KernelError("spread_experts: the weights' gradients and the rows they multiply come together")
     _one_device(name, x, slots, out, weights, y, dweights)
-    rc = lib().mr_spread_experts(_rows_ptr(x), dtype_code(x.dtype), _ld(x), _ptr(slots), _ptr(weights), T, k, H,
-                                 _rows_ptr(out), dtype_code(out.dtype), _ld(out), R, _rows_ptr(y), _ld(y),
-                                 _ptr(dweights), _stream(x))
+    rc = lib().mr_spread_experts(at_x, dtype_code(x.dtype), ldx, s, w, T, k, H, at_out, dtype_code(out.dtype), ldo, R, at_y,
+                                 ldy, dw, _stream(x))
     _check(rc, "mr_spread_experts")
 
 
@@ -957,21 +990,21 @@ def spread_experts(x, slots, out, *, weights=None, y=None, dweights=None) -> Non
 _ACT_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _norm_types(name: str, y, stream):
-    if y.dtype not in _ACT_TYPES or stream.dtype not in (torch.float32, y.dtype) or y.dim() != 2:
+def _norm_types(name: str, y, stream) -> tuple[int, int]:
+    if y.dtype not in _ACT_TYPES or (stream.dtype is not torch.float32 and stream.dtype is not y.dtype) or y.dim() != 2:
         raise KernelError(f"{name}: the branch is a float32, bfloat16 or float16 matrix and the stream float32 or of its "
                           f"type, got {y.dtype} {list(y.shape)} and {stream.dtype}")
+    return y.shape
 
 
-def _gate(name: str, gate, gate_rows, T: int, H: int) -> int:
-    """Rows a gate row applies to."""
+def _gate(name: str, gate, gate_rows, T: int, H: int) -> tuple[int | None, int]:
+    """(address, rows a gate row applies to)."""
     if gate is None:
-        return 0
+        return None, 0
     per = max(T, 1) if gate_rows is None else int(gate_rows)
     if per <= 0:
         raise KernelError(f"{name}: gate_rows must be positive, got {gate_rows}")
-    _dense(name, "gate", gate, torch.float32, (-(-T // per), H) if T else tuple(gate.shape[:1]) + (H,))
-    return per
+    return _dense(name, "gate", gate, torch.float32, (-(-T // per), H) if T else (gate.shape[0], H)), per
 
 
 def norm_residual(y, resid, out, *, eps, post=None, gate=None, gate_rows=None, scale=1.0, pre=None, normed=None) -> None:
@@ -984,21 +1017,19 @@ def norm_residual(y, resid, out, *, eps, post=None, gate=None, gate_rows=None, s
     same type; weights are float32 ``[H]``. Sums are float32, and ``normed`` is that of
     ``out`` before it is rounded. ``out`` may be ``resid``, ``normed`` may be ``y``. H is
     at most 16384."""
-    name = "norm_residual"
-    _norm_types(name, y, resid)
-    T, H = y.shape
-    _matrix(name, "resid", resid, (resid.dtype,), (T, H))
-    _matrix(name, "out", out, (resid.dtype,), (T, H))
-    _matrix(name, "normed", normed, (y.dtype,), (T, H))
-    for what, w in (("post", post), ("pre", pre)):
-        _dense(name, what, w, torch.float32, (H,))
+    name, f32 = "norm_residual", torch.float32
+    T, H = _norm_types(name, y, resid)
+    at_y, ldy = _matrix(name, "y", y, (y.dtype,), (T, H))
+    at_r, ldr = _matrix(name, "resid", resid, (resid.dtype,), (T, H))
+    at_out, ldo = _matrix(name, "out", out, (resid.dtype,), (T, H))
+    at_x, ldx = _matrix(name, "normed", normed, (y.dtype,), (T, H))
+    w_post, w_pre = _dense(name, "post", post, f32, (H,)), _dense(name, "pre", pre, f32, (H,))
     if (pre is None) != (normed is None):
         raise KernelError("norm_residual: the next norm's weight and its output come together")
-    per = _gate(name, gate, gate_rows, T, H)
+    g, per = _gate(name, gate, gate_rows, T, H)
     _one_device(name, y, resid, out, post, gate, pre, normed)
-    rc = lib().mr_norm_residual(_rows_ptr(y), dtype_code(y.dtype), _ld(y), _rows_ptr(resid), dtype_code(resid.dtype),
-                                _ld(resid), T, H, eps, _ptr(post), _ptr(gate), per, scale, _ptr(pre), _rows_ptr(out),
-                                _ld(out), _rows_ptr(normed), _ld(normed), _stream(y))
+    rc = lib().mr_norm_residual(at_y, dtype_code(y.dtype), ldy, at_r, dtype_code(resid.dtype), ldr, T, H, eps, w_post, g, per,
+                                scale, w_pre, at_out, ldo, at_x, ldx, _stream(y))
     _check(rc, "mr_norm_residual")
 
 
@@ -1010,31 +1041,31 @@ def norm_residual_bwd(dnormed, dout, y, out, dy, dresid, *, eps, post=None, gate
     output ``out``; ``dpost``, ``dpre`` ``[H]`` and ``dgate`` ``[G, H]`` (float32, None:
     not wanted) receive the weights' gradients, sums over the rows in an order that
     the shape fixes. ``dresid`` may be ``dout`` and ``dy`` may be ``y``."""
-    name = "norm_residual_bwd"
-    _norm_types(name, dy, dresid)
-    T, H = dy.shape
-    for what, t, dt in (("dnormed", dnormed, dy.dtype), ("y", y, dy.dtype), ("dout", dout, dresid.dtype),
-                        ("out", out, dresid.dtype), ("dresid", dresid, dresid.dtype)):
-        _matrix(name, what, t, (dt,), (T, H))
-    for what, w in (("post", post), ("pre", pre), ("dpost", dpost), ("dpre", dpre)):
-        _dense(name, what, w, torch.float32, (H,))
+    name, f32 = "norm_residual_bwd", torch.float32
+    T, H = shape = tuple(_norm_types(name, dy, dresid))
+    act, stream = (dy.dtype,), (dresid.dtype,)
+    at_dx, lddx = _matrix(name, "dnormed", dnormed, act, shape)
+    at_d, ldd = _matrix(name, "dout", dout, stream, shape)
+    at_y, ldy = _matrix(name, "y", y, act, shape)
+    at_h, ldh = _matrix(name, "out", out, stream, shape)
+    at_dy, lddy = _matrix(name, "dy", dy, act, shape)
+    at_dr, lddr = _matrix(name, "dresid", dresid, stream, shape)
+    w_post, w_pre = _dense(name, "post", post, f32, (H,)), _dense(name, "pre", pre, f32, (H,))
+    g_post, g_pre = _dense(name, "dpost", dpost, f32, (H,)), _dense(name, "dpre", dpre, f32, (H,))
     if (pre is None) != (dnormed is None):
         raise KernelError("norm_residual_bwd: the next norm's weight and its output's gradient come together")
-    for what, g, w in (("dpost", dpost, post), ("dgate", dgate, gate), ("dpre", dpre, pre)):
-        if g is not None and w is None:
-            raise KernelError(f"norm_residual_bwd: {what} is asked for without its weight")
-    per = _gate(name, gate, gate_rows, T, H)
-    if dgate is not None:
-        _dense(name, "dgate", dgate, torch.float32, gate.shape)
-    _one_device(name, dnormed, dout, y, out, dy, dresid, post, gate, pre, dpost, dgate, dpre)
-    nbytes = int(lib().mr_norm_residual_bwd_workspace_bytes(T, H, per, dpost is not None, dgate is not None,
-                                                            dpre is not None))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device) if nbytes else None
-    rc = lib().mr_norm_residual_bwd(
-        _rows_ptr(dnormed), dtype_code(dy.dtype), _ld(dnormed), _rows_ptr(dout), dtype_code(dresid.dtype), _ld(dout),
-        _rows_ptr(y), _ld(y), _rows_ptr(out), _ld(out), T, H, eps, _ptr(post), _ptr(gate), per, scale, _ptr(pre),
-        _rows_ptr(dy), _ld(dy), _rows_ptr(dresid), _ld(dresid), _ptr(dpost), _ptr(dgate), _ptr(dpre), _ptr(ws), nbytes,
-        _stream(dy))
+    if (dpost is not None and post is None) or (dgate is not None and gate is None) or (dpre is not None and pre is None):
+        raise KernelError("norm_residual_bwd: a gradient is asked for of a weight that is not there")
+    g, per = _gate(name, gate, gate_rows, T, H)
+    g_gate = None if dgate is None else _dense(name, "dgate", dgate, f32, gate.shape)
+    device = _one_device(name, dnormed, dout, y, out, dy, dresid, post, gate, pre, dpost, dgate, dpre)
+    nbytes = 0
+    if dpost is not None or dgate is not None or dpre is not None:
+        nbytes = lib().mr_norm_residual_bwd_workspace_bytes(T, H, per, dpost is not None, dgate is not None, dpre is not None)
+    ws, hold = _scratch(nbytes, device)
+    rc = lib().mr_norm_residual_bwd(at_dx, dtype_code(dy.dtype), lddx, at_d, dtype_code(dresid.dtype), ldd, at_y, ldy, at_h,
+                                    ldh, T, H, eps, w_post, g, per, scale, w_pre, at_dy, lddy, at_dr, lddr, g_post, g_gate,
+                                    g_pre, ws, nbytes, _stream(dy))
     _check(rc, "mr_norm_residual_bwd")
 
 
