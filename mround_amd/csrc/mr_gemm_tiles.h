@@ -320,9 +320,9 @@ __device__ __forceinline__ void store16(T* p, T v) {
 // What rounding x to bf16 leaves, exactly.
 __device__ __forceinline__ float bf16_rest(float x) { return x - bf16_to_f32(f32_to_bf16(x)); }
 
-// The first row of a wave's 32-row slice i: one run of WM rows a wave, or with HALVES
-// one run of WM / 2 in each half of the tile, so that a tile whose second half is
-// past the edge has a first half that all waves share.
+// The first row (column) of a wave's 32-wide slice i: one run of WM a wave, or with
+// HALVES one run of WM / 2 in each half of the tile, so that a tile whose second half
+// is past the edge has a first half that all waves share.
 template <int WM, bool HALVES>
 constexpr __device__ __forceinline__ int slice_row(int wm, int i) {
   return HALVES ? (i * 32) / (WM / 2) * WM + wm * (WM / 2) + i * 32 % (WM / 2) : wm * WM + i * 32;
@@ -336,6 +336,8 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
                                            int wn, int lane, uint8_t* region) {
   const int lrow = (lane >> 5) * 4;
   const int lcol = lane & 31;
+  // HALVES: where column c of the wave's lies from its first one.
+  auto apart = [](int c) __attribute__((always_inline)) { return HALVES && c >= WN / 2 ? c + WN / 2 : c; };
   if constexpr (is_swiglu(EPI)) {
     // B rows interleave 32 gate rows and 32 up rows, and a wave's column
     // range starts on a multiple of 64: block j = 2q holds gate columns and
@@ -387,7 +389,8 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
         // The same wave reads back what it wrote (LDS keeps a wave's accesses
         // in order), then the next slice overwrites the region.
         const int row0 = m0 + slice_row<WM, HALVES>(wm, i);
-        const int col0 = n0 + wn * WN + jb * JH * 32;  // gate/up column, a multiple of 64
+        const int col0 = n0 + slice_row<WN, HALVES>(wn, jb * JH);  // gate/up column, a multiple of 64
+        static_assert(!HALVES || JH == TN, "a slice holds both of a wave's runs");
         // uniform bases of the slice; lane offsets stay 32-bit (ld < 2^22, 32 rows)
         uint16_t* const act_s = act + static_cast<int64_t>(row0) * p.ldc + col0 / 2;
         uint16_t* const gu_s = p.gu + static_cast<int64_t>(row0) * p.ldgu + col0;
@@ -401,9 +404,10 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
           for (int it = 0; it < NIT; ++it) {
             const int idx = it * 64 + lane, r = idx / CH, ch = idx % CH;
             const int gc = (ch >> 2) * 64 + (ch & 3) * 8;  // staged gate column; up 32 further
+            const int gcol = apart(gc), acol = HALVES ? (gcol >> 6) * 32 + (gcol & 31) : ch * 8;  // of gu and act, from col0
             const f32x4 g0 = *(const lds_f32x4*)(st + at(r, gc / 4)), g1 = *(const lds_f32x4*)(st + at(r, gc / 4 + 1));
             const f32x4 u0 = *(const lds_f32x4*)(st + at(r, gc / 4 + 8)), u1 = *(const lds_f32x4*)(st + at(r, gc / 4 + 9));
-            if (!GUARD || (row0 + r < p.M && col0 / 2 + ch * 8 < p.n_out)) {
+            if (!GUARD || (row0 + r < p.M && col0 / 2 + acol < p.n_out)) {
               float a[8];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -412,7 +416,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
               }
               const u32x4 hi = {pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(a[4], a[5]),
                                 pack_bf16x2(a[6], a[7])};
-              uint16_t* const ao = act_s + static_cast<uint32_t>(r * static_cast<int>(p.ldc) + ch * 8);
+              uint16_t* const ao = act_s + static_cast<uint32_t>(r * static_cast<int>(p.ldc) + acol);
               store16<false>(reinterpret_cast<u32x4*>(ao), hi);
               if constexpr (SPLIT) {
                 store16<false>(reinterpret_cast<u32x4*>(ao + p.n_out), hi);
@@ -423,7 +427,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
                   store16<false>(reinterpret_cast<u32x4*>(hi_s + static_cast<uint32_t>(r * static_cast<int>(p.ldact) + ch * 8)), hi);
               }
               if constexpr (GU) {
-                uint16_t* const o = gu_s + static_cast<uint32_t>(r * static_cast<int>(p.ldgu) + gc);
+                uint16_t* const o = gu_s + static_cast<uint32_t>(r * static_cast<int>(p.ldgu) + gcol);
                 store16<false>(reinterpret_cast<u32x4*>(o), u32x4{pack_bf16x2(g0[0], g0[1]), pack_bf16x2(g0[2], g0[3]),
                                                            pack_bf16x2(g1[0], g1[1]), pack_bf16x2(g1[2], g1[3])});
                 store16<false>(reinterpret_cast<u32x4*>(o + 32), u32x4{pack_bf16x2(u0[0], u0[1]), pack_bf16x2(u0[2], u0[3]),
@@ -432,7 +436,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
             }
           }
         };
-        const bool full = row0 + 32 <= p.M && col0 / 2 + JH * 16 <= p.n_out;
+        const bool full = row0 + 32 <= p.M && (HALVES ? n0 + 2 * WN <= p.N : col0 / 2 + JH * 16 <= p.n_out);
         if (has_gu) {
           if (full) out(std::false_type{}, std::true_type{});
           else out(std::true_type{}, std::true_type{});
@@ -479,14 +483,15 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
         // in order). Loads go to clamped (always valid) places; only the
         // stores are guarded.
         const int row0 = m0 + slice_row<WM, HALVES>(wm, i);
-        const int col0 = n0 + wn * WN + jb * JH * 32;
+        const int col0 = n0 + slice_row<WN, HALVES>(wn, jb * JH);
+        static_assert(!HALVES || JH == TN, "a slice holds both of a wave's runs");
         const uint16_t* const gu_s = p.gu + static_cast<int64_t>(row0) * p.ldgu;
         uint16_t* const dgu_s = dgu + static_cast<int64_t>(row0) * p.ldc;
         u32x4 gv[NIT], uv[NIT];
 #pragma unroll
         for (int it = 0; it < NIT; ++it) {
           const int idx = it * 64 + lane, r = idx / CH, ch = idx % CH;
-          const int row = min(row0 + r, p.M - 1), col = min(col0 + ch * 8, p.N - 8);
+          const int row = min(row0 + r, p.M - 1), col = min(col0 + apart(ch * 8), p.N - 8);
           // signed: a slice wholly past the edge clamps to row M - 1, below row0
           const int o = (row - row0) * static_cast<int>(p.ldgu) + (col >> 5) * 64 + (col & 31);
           gv[it] = *reinterpret_cast<const u32x4*>(gu_s + o);
@@ -497,7 +502,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
 #pragma unroll
         for (int it = 0; it < NIT; ++it) {
           const int idx = it * 64 + lane, r = idx / CH, ch = idx % CH;
-          const int row = row0 + r, col = col0 + ch * 8;
+          const int row = row0 + r, col = col0 + apart(ch * 8);
           const f32x4 d0 = *(__attribute__((address_space(3))) f32x4*)(st + r * PITCH + ch * 32);
           const f32x4 d1 = *(__attribute__((address_space(3))) f32x4*)(st + r * PITCH + ch * 32 + 16);
           const float da[8] = {d0[0], d0[1], d0[2], d0[3], d1[0], d1[1], d1[2], d1[3]};
@@ -521,7 +526,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
           }
         }
         };
-        if (row0 + 32 <= p.M && col0 + JH * 32 <= p.N) out(std::false_type{});
+        if (row0 + 32 <= p.M && (HALVES ? n0 + 2 * WN : col0 + JH * 32) <= p.N) out(std::false_type{});
         else out(std::true_type{});
       }
     }
@@ -698,7 +703,8 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
                 f32x4{acc[i][j][4 * gi], acc[i][j][4 * gi + 1], acc[i][j][4 * gi + 2], acc[i][j][4 * gi + 3]};
         }
         const int row0 = m0 + slice_row<WM, HALVES>(wm, i);
-        const int col0 = n0 + wn * WN + jb * JH * 32;
+        const int col0 = n0 + slice_row<WN, HALVES>(wn, jb * JH);
+        static_assert(!HALVES || JH == TN, "a slice holds both of a wave's runs");
         // uniform bases of the slice; lane offsets stay 32-bit (ld < 2^22, 32 rows)
         const int64_t cbase = static_cast<int64_t>(row0) * p.ldc + col0;
         uint16_t* const cb16 = static_cast<uint16_t*>(p.C) + cbase;
@@ -711,7 +717,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
 #pragma unroll
           for (int it = 0; it < NIT; ++it) {
             const int idx = it * 64 + lane, r = idx / CH, ch = idx % CH;
-            const int row = min(row0 + r, p.M - 1), col = min(col0 + ch * 4, p.N - 4);
+            const int row = min(row0 + r, p.M - 1), col = min(col0 + apart(ch * 4), p.N - 4);
             // signed: a slice wholly past the edge clamps to row M - 1, below row0
             res[it] = *reinterpret_cast<const f32x4*>(rs + ((row - row0) * static_cast<int>(p.ldr) + col));
           }
@@ -724,8 +730,8 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
 #pragma unroll
           for (int it = 0; it < NIT; ++it) {
             const int idx = it * 64 + lane, r = idx / CH, ch = idx % CH;
-            const int row = row0 + r, col = col0 + ch * OPC;
-            const uint32_t oc = static_cast<uint32_t>(r * static_cast<int>(p.ldc) + ch * OPC);
+            const int row = row0 + r, col = col0 + apart(ch * OPC);
+            const uint32_t oc = static_cast<uint32_t>(r * static_cast<int>(p.ldc) + apart(ch * OPC));
             if (!GUARD || (row < p.M && col < p.N)) {
               // N is a multiple of 8: a store's columns lie wholly inside or past the edge
               const int cb = GUARD ? min(col, p.N - OPC) : col;
@@ -746,7 +752,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
             }
           }
         };
-        const bool full = row0 + 32 <= p.M && col0 + JH * 32 <= p.N;
+        const bool full = row0 + 32 <= p.M && (HALVES ? n0 + 2 * WN : col0 + JH * 32) <= p.N;
         if (has_bias) {
           if (full) out(std::true_type{}, std::false_type{});
           else out(std::true_type{}, std::true_type{});
@@ -799,7 +805,8 @@ __device__ __forceinline__ int length_class(int n) {
 // 0 and the rows there are, so that no others lead outside.
 //
 // Rows (K-major A): every tile takes as long, and each XCD gets a contiguous run
-// of them, experts in order. Weight gradients: an expert's tiles take as long as it
+// of them, experts in order. (Tiles past the last whole round as quarters on a launch
+// of their own gained 2 % of 2.2 rounds and lost as much of 13.) Weight gradients: an expert's tiles take as long as it
 // has rows, so each XCD gets an eighth of every expert's tiles (a contiguous run of
 // tile_coords, which shares panels), longest experts first. (A run of whole experts
 // an XCD: the XCD with the liked ones worked twice as long as the others, 16 experts
@@ -1126,9 +1133,9 @@ template <bool A_KMAJOR, bool B_KMAJOR, int EPI, bool OUT_BF16, class P = GemmPa
 __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1, 1))) void gemm4_kernel(P p) {
   constexpr int BM = 256, BN = 256, WM = 128, WN = 128, TM = WM / 32, TN = WN / 32;
   constexpr int STAGE = 256 * ROW_BYTES;  // bytes of one operand stage (either layout)
-  // A group's last rows may fill only half a tile: its k-tiles then run without the
-  // second half's loads and MFMAs (see tile).
-  constexpr bool HALVES = P::kGrouped && A_KMAJOR;
+  // An expert's last rows, and the last columns, may fill only half a tile: its k-tiles
+  // then run without the second half's MFMAs and, of K-major operands, loads (see tile).
+  constexpr bool HALVES = P::kGrouped;
   static_assert(STAGE == MNMajorDirect<256>::ROWB * BK, "both layouts stage 32 KB");
   __shared__ __attribute__((aligned(1024))) uint8_t As0[STAGE];
   __shared__ __attribute__((aligned(1024))) uint8_t As1[STAGE];
@@ -1186,21 +1193,21 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
       if constexpr (A_KMAJOR)
         a_reg[x] = ((HALVES ? wm * (WM / 2) : wm * WM) + l32) * ROW_BYTES + (((2 * x + h) ^ swz_bits(l32)) << 4);
       else
-        a_reg[x] = MNMajorDirect<BM>::frag_off(wm * WM + x * 32, lane);
+        a_reg[x] = MNMajorDirect<BM>::frag_off(slice_row<WM, HALVES>(wm, x), lane);
       asm volatile("" : "+v"(a_reg[x]));
     }
 #pragma unroll
     for (int x = 0; x < NB; ++x) {
       if constexpr (B_KMAJOR)
-        b_reg[x] = (wn * WN + l32) * ROW_BYTES + (((2 * x + h) ^ swz_bits(l32)) << 4);
+        b_reg[x] = ((HALVES ? wn * (WN / 2) : wn * WN) + l32) * ROW_BYTES + (((2 * x + h) ^ swz_bits(l32)) << 4);
       else
-        b_reg[x] = MNMajorDirect<BN>::frag_off(wn * WN + x * 32, lane);
+        b_reg[x] = MNMajorDirect<BN>::frag_off(slice_row<WN, HALVES>(wn, x), lane);
       asm volatile("" : "+v"(b_reg[x]));
     }
   }
   typedef const __attribute__((address_space(3))) uint8_t* lds_ptr;
   bf16x8 af[2][TM], bfr[2][TN];
-  auto rd = [&](lds_ptr la, lds_ptr lb, int kk, int slot, int rows = TM) __attribute__((always_inline)) {
+  auto rd = [&](lds_ptr la, lds_ptr lb, int kk, int slot, int rows = TM, int cols = TN) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < rows; ++i) {
       if constexpr (A_KMAJOR) {
@@ -1213,9 +1220,9 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
       }
     }
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
+    for (int j = 0; j < cols; ++j) {
       if constexpr (B_KMAJOR) {
-        bfr[slot][j] = *(const lds_bf16x8_t*)(lb + b_reg[kk] + j * 32 * ROW_BYTES);
+        bfr[slot][j] = *(const lds_bf16x8_t*)(lb + b_reg[kk] + slice_row<WN, HALVES>(0, j) * ROW_BYTES);
       } else {
         constexpr uint32_t R = MNMajorDirect<BN>::ROWB;
         const v4i16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16_t*)(lb + b_reg[j] + kk * 16 * R));
@@ -1224,25 +1231,27 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
       }
     }
   };
-  auto mm = [&](int slot, int rows = TM) __attribute__((always_inline)) {
+  auto mm = [&](int slot, int rows = TM, int cols = TN) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < rows; ++i)
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
+      for (int j = 0; j < cols; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bfr[slot][j], af[slot][i], acc[i][j], 0, 0, 0);
   };
   // The order of a k16 step: its next-step fragment reads (8, 12 or 16 LDS
   // instructions) and the loads spread between its 16 MFMAs.
   constexpr int NR = (A_KMAJOR ? TM : 2 * TM) + (B_KMAJOR ? TN : 2 * TN);
-  constexpr int NR2 = TM / 2 + (B_KMAJOR ? TN : 2 * TN);  // of a half tile's step, between 8 MFMAs
-  auto order = [](bool loads, bool half = false) __attribute__((always_inline)) {
-    if (half) {
+  // Of rows x cols MFMAs, fewer than 16, in a half tile: its reads spread evenly.
+  auto order = [](bool loads, int rows = TM, int cols = TN) __attribute__((always_inline)) {
+    if (rows * cols < 16) {
+      const int n = rows * cols, reads = (A_KMAJOR ? rows : 2 * rows) + (B_KMAJOR ? cols : 2 * cols);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        if (q < NR2 - 8) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-        else if (q < NR2) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      for (int q = 0; q < n; ++q) {
+        const int now = reads * (q + 1) / n - reads * q / n;
+        if (now == 1) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        if (now == 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        if (loads && (q & 1)) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+        if (loads && (n == 4 || (q & 1))) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
       }
       return;
     }
@@ -1290,11 +1299,12 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
     }
     __builtin_amdgcn_sched_barrier(0);
   }
-  // k-tile u on A stage SA and B stage SB; HALF: of a tile's first 128 rows alone
-  // (slices 0 and 1 of each wave), whose A loads are the first 4 of a wave's 8.
-  auto tile = [&](int u, auto sac, auto sbc, auto halfc) __attribute__((always_inline)) {
-    constexpr bool HALF = decltype(halfc)::value;
-    constexpr int ROWS = HALF ? TM / 2 : TM;
+  // k-tile u on A stage SA and B stage SB; of a half tile's first 128 rows or columns
+  // alone (slices 0 and 1 of each wave), whose K-major loads are the first 4 of a
+  // wave's 8.
+  auto tile = [&](int u, auto sac, auto sbc, auto half_mc, auto half_nc) __attribute__((always_inline)) {
+    constexpr int ROWS = decltype(half_mc)::value ? TM / 2 : TM, COLS = decltype(half_nc)::value ? TN / 2 : TN;
+    constexpr bool SKIP_A = ROWS < TM && A_KMAJOR, SKIP_B = COLS < TN && B_KMAJOR;
     constexpr int SA = decltype(sac)::value, SB = decltype(sbc)::value;
     uint8_t* la_ = SA == 0 ? As0 : SA == 1 ? As1 : As2;
     uint8_t* na_ = SA == 0 ? As1 : SA == 1 ? As2 : As0;
@@ -1303,41 +1313,43 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
     uint8_t* nb_ = SB == 0 ? Bs1 : Bs0;                  // B of k-tile u + 1
     const lds_ptr la = (lds_ptr)la_, lb = (lds_ptr)lb_;
     const rsrc_t r_b1 = rb_at(tk(u + 1)), r_a2 = ra_at(tk(u + 2)), r_b2 = rb_at(tk(u + 2));
-    rd(la, lb, 1, 1, ROWS);
+    rd(la, lb, 1, 1, ROWS, COLS);
+    if constexpr (!SKIP_B) {
 #pragma unroll
-    for (int i = 4; i < 8; ++i) ld_b.issue_one(r_b1, i, nb_);
-    mm(0, ROWS);
-    order(true, HALF);
+      for (int i = 4; i < 8; ++i) ld_b.issue_one(r_b1, i, nb_);
+    }
+    mm(0, ROWS, COLS);
+    order(!SKIP_B, ROWS, COLS);
     __builtin_amdgcn_sched_barrier(0);
-    rd(la, lb, 2, 0, ROWS);
+    rd(la, lb, 2, 0, ROWS, COLS);
 #pragma unroll
     for (int i = 0; i < 4; ++i) ld_a.issue_one(r_a2, i, fa_);
-    mm(1, ROWS);
-    order(true, HALF);
+    mm(1, ROWS, COLS);
+    order(true, ROWS, COLS);
     __builtin_amdgcn_sched_barrier(0);
-    rd(la, lb, 3, 1, ROWS);
-    if constexpr (!HALF) {
+    rd(la, lb, 3, 1, ROWS, COLS);
+    if constexpr (!SKIP_A) {
 #pragma unroll
       for (int i = 4; i < 8; ++i) ld_a.issue_one(r_a2, i, fa_);
     }
-    mm(0, ROWS);
-    order(!HALF, HALF);
+    mm(0, ROWS, COLS);
+    order(!SKIP_A, ROWS, COLS);
     __builtin_amdgcn_sched_barrier(0);
     // Every read of this stage done, k-tile u + 1 landed (the 8 A loads of
     // k-tile u + 2, or the half tile's 4, may be in flight): a plain barrier, no
     // memory fence.
-    if constexpr (HALF) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
+    if constexpr (SKIP_A) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
     else asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    rd((lds_ptr)na_, (lds_ptr)nb_, 0, 0, ROWS);
+    rd((lds_ptr)na_, (lds_ptr)nb_, 0, 0, ROWS, COLS);
 #pragma unroll
     for (int i = 0; i < 4; ++i) ld_b.issue_one(r_b2, i, lb_);
-    mm(1, ROWS);
-    order(true, HALF);
+    mm(1, ROWS, COLS);
+    order(true, ROWS, COLS);
     __builtin_amdgcn_sched_barrier(0);
   };
-#define MR_TILE(U, SA, SB) tile(U, std::integral_constant<int, SA>{}, std::integral_constant<int, SB>{}, half)
+#define MR_TILE(U, SA, SB) tile(U, std::integral_constant<int, SA>{}, std::integral_constant<int, SB>{}, half_m, half_n)
 #define MR_K_LOOP()                        \
   {                                        \
     int u = 0;                             \
@@ -1356,11 +1368,22 @@ __global__ __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(1,
       MR_TILE(u + 5, 2, 1);                \
     }                                      \
   }
-  if (HALVES && p.M - m0 <= 128) {
-    constexpr std::bool_constant<HALVES> half;
+  constexpr std::bool_constant<HALVES> yes;
+  constexpr std::false_type no;
+  const bool half_rows = HALVES && p.M - m0 <= 128, half_cols = HALVES && p.N - n0 <= 128;
+  if (half_rows && half_cols) {
+    constexpr auto half_m = yes, half_n = yes;
+    MR_K_LOOP()
+  } else if (half_rows) {
+    constexpr auto half_m = yes;
+    constexpr auto half_n = no;
+    MR_K_LOOP()
+  } else if (half_cols) {
+    constexpr auto half_m = no;
+    constexpr auto half_n = yes;
     MR_K_LOOP()
   } else {
-    constexpr std::false_type half;
+    constexpr auto half_m = no, half_n = no;
     MR_K_LOOP()
   }
 #undef MR_K_LOOP
