@@ -227,18 +227,18 @@ int64_t real_tiles_of(bool ak, int64_t bm, int64_t bn, int64_t experts, int64_t 
 }
 
 // How a grouped product runs. The row counts are on the device alone, so this goes by
-// their average. Measured on 150 products of random sizes (2 .. 256 experts, 1 ..
-// 16384 tokens, matrices of 128 .. 8192), each by every way: the way chosen is on average
-// 2 % slower than the best of them, 128 x 128 tiles alone 20 %, 256 x 256 alone 30 %.
+// their average; half a tile's rows of an expert's last tile are taken to be empty.
 // FEW (few_rows_kernel): at most 4 rows an expert, or 14 where 128 x 128 tiles make less
 //   than three rounds of them, or no more of its blocks than two a CU (64 experts of 2 x
 //   768 x 2048: 4 rows 59 us, on tiles 87; 10 rows 70 and 91; 32 rows 142 and 97).
 // SMALL, BIG: 128 x 128 tiles, two a CU, cut along K where that pays for the partials'
-//   round trip, or 256 x 256, whichever the ungrouped products' times expect to take
-//   less of (large ones for 9 % or more): half a tile's rows of an expert's last tile
-//   are taken to be empty, of which a large tile saves a quarter. Many rounds read
-//   their operands over and over, and large tiles do so less (125 experts of 439 rows,
-//   3136 x 512: 283 us on large tiles, 368 on small).
+//   round trip, or 256 x 256, whichever is expected to take less. Up to a round of
+//   either the ungrouped products' times hold; over more, tiles of unlike length overlap
+//   and it is their number that counts, with part of a round for the ends. Measured on
+//   460 products of 2 .. 128 experts and 40 rows and more an expert, by both: the one
+//   chosen is on average 0.8 % slower than the faster one, small tiles alone 5 %, large
+//   alone 25 % (8 experts of 4096 rows, 1024 x 9728: 495 us on large tiles; 125 of 439,
+//   3136 x 512: 283, on small 368; 35 experts of 493 rows' 448 x 1024 gradients: 62 and 44).
 enum Way { FEW, SMALL_TILES, BIG_TILES };
 struct GroupedPlan {
   Way way;
@@ -255,7 +255,7 @@ GroupedPlan grouped_plan(bool ak, bool bkm, int64_t experts, int64_t M, int64_t 
         (M <= 128 * experts && few <= 512))
       return {FEW, 1};
     small = used * (rows / 128 + 0.5 > 1 ? rows / 128 + 0.5 : 1.0) * ((N + 127) / 128);
-    big = used * (rows / 256 + 0.375 > 1 ? rows / 256 + 0.375 : 1.0) * ((N + 255) / 256);
+    big = used * (rows / 256 + 0.5 > 1 ? rows / 256 + 0.5 : 1.0) * ((N + 255) / 256);
   } else {
     KT = (K / experts + BK - 1) / BK;
     small = static_cast<double>(real_tiles_of(ak, 128, 128, experts, M, N));
@@ -263,8 +263,13 @@ GroupedPlan grouped_plan(bool ak, bool bkm, int64_t experts, int64_t M, int64_t 
   }
   if (KT < 1) KT = 1;
   auto whole = [](double tiles) { return static_cast<int64_t>(tiles + 0.999); };
+  const int kt = static_cast<int>(KT);
+  double t_small = small_time(512, kt, o) * (1.28 * small / 512 + 0.27);
+  if (small <= 512) t_small = small_time(whole(small), kt, o);
+  double t_big = (big_time(256, kt, 1, o) + 0.1 * big_time(256, 0, 1, o)) * (big / 256 + 0.63);
+  if (big <= 256) t_big = big_time(whole(big), kt, 1, o);
+  if (!ak && small >= 4096) t_big *= 0.8;  // (short sums: the outputs' bytes, which small tiles write less well)
   int split = 1;
-  double t_small = small_time(whole(small), static_cast<int>(KT), o);
   for (int sp = 2; sp <= 64 && sp * 4 <= KT && small * sp <= 512; ++sp) {
     const double t = small_time(whole(small * sp), static_cast<int>((KT + sp - 1) / sp), o) + 3.0 + 0.02 * small * sp;
     if (t < t_small) {
@@ -272,8 +277,6 @@ GroupedPlan grouped_plan(bool ak, bool bkm, int64_t experts, int64_t M, int64_t 
       split = sp;
     }
   }
-  double t_big = (o == OUT_SWIGLU_BWD ? 0.95 : 1.1) * big_time(whole(big), static_cast<int>(KT), 1, o);
-  if (small >= (ak ? 4096 : 5120)) t_big *= 0.7;
   return t_big < t_small ? GroupedPlan{BIG_TILES, 1} : GroupedPlan{SMALL_TILES, split};
 }
 int64_t split_bytes_of(bool ak, int64_t experts, int64_t M, int64_t N, int split) {

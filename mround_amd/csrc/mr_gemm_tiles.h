@@ -805,12 +805,13 @@ __device__ __forceinline__ int length_class(int n) {
 // 0 and the rows there are, so that no others lead outside.
 //
 // Rows (K-major A): every tile takes as long, and each XCD gets a contiguous run
-// of them, experts in order. (Tiles past the last whole round as quarters on a launch
-// of their own gained 2 % of 2.2 rounds and lost as much of 13.) Weight gradients: an expert's tiles take as long as it
-// has rows, so each XCD gets an eighth of every expert's tiles (a contiguous run of
-// tile_coords, which shares panels), longest experts first. (A run of whole experts
-// an XCD: the XCD with the liked ones worked twice as long as the others, 16 experts
-// of 2048 x 1408 over 32764 rows 352 us.)
+// of them, experts in order. (The large tiles past the last whole round as quarters,
+// on a launch of their own, gained 0.5 % over 400 products and lost 2 % of many.)
+// Weight gradients: an expert's tiles take as long as it has rows, so each XCD gets
+// an eighth of every expert's tiles (a contiguous run of tile_coords, which shares
+// panels), longest experts first. (A run of whole experts an XCD: the XCD with the
+// liked ones worked twice as long as the others, 16 experts of 2048 x 1408 over 32764
+// rows 352 us, 196 now.)
 template <int BM, int BN, bool A_KMAJOR, bool OUT_BF16, bool INDEXED>
 __device__ __forceinline__ bool enter(GroupedParams<INDEXED>& p, int bid, int& bm, int& bn) {
   const int rows = A_KMAJOR ? p.M : p.K;
