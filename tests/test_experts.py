@@ -476,6 +476,41 @@ def test_offsets_and_indices_outside_lead_nowhere():
         assert torch.allclose(c[r], one[0], rtol=0, atol=1e-4)
 
 
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Rows that start past 2^31 elements are those that the same call on few rows
+    gives."""
+    R, H, T = 70000, 32768, 40
+    y = torch.zeros(R, H, dtype=BF, device=dev())
+    slots = torch.arange(R - 2 * T, R, dtype=I32, device=dev()).view(T, 2)
+    y[R - 2 * T:] = normal(2 * T, H, seed=1).to(BF)
+    w = normal(T, 2, seed=2)
+    out, near = torch.empty(T, H, device=dev()), torch.empty(T, H, device=dev())
+    K.combine_experts(y, slots, out, weights=w)
+    K.combine_experts(y[R - 2 * T:], slots - (R - 2 * T), near, weights=w)
+    assert torch.equal(out, near)
+    back, dw, dw_near = torch.empty(2 * T, H, dtype=BF, device=dev()), torch.empty_like(w), torch.empty_like(w)
+    K.spread_experts(near, slots - (R - 2 * T), back, weights=w, y=y[R - 2 * T:].clone(), dweights=dw_near)
+    K.spread_experts(out, slots, y, weights=w, y=y, dweights=dw)
+    assert torch.equal(y[R - 2 * T:], back) and torch.equal(dw, dw_near)
+    del y, back
+    R, Kd, N = 1 << 20, 2112, 40  # the second expert's rows start past 2^31 elements of a
+    a = torch.zeros(R, Kd, dtype=BF, device=dev())
+    a[R - 300:] = normal(300, Kd, seed=3).to(BF)
+    b = normal(2, N, Kd, seed=4).to(BF)
+    c = torch.empty(R, N, device=dev())
+    K.gemm_experts("nt", a, b, c, offsets=torch.tensor([0, R - 200, R], dtype=I32, device=dev()))
+    want, tol = product(a[R - 300:], b.transpose(1, 2), [100, 200])
+    within(c[R - 300:], want, tol + rounding(want, F32), "far rows")
+    dw = torch.empty(2, N, Kd, device=dev())
+    g = torch.zeros(R, N, dtype=BF, device=dev())
+    g[R - 300:] = normal(300, N, seed=5).to(BF)
+    K.gemm_experts("tn", g, a, dw, offsets=torch.tensor([0, R - 200, R], dtype=I32, device=dev()))
+    for e, r in ((0, slice(R - 300, R - 200)), (1, slice(R - 200, R))):
+        want, mag = g[r].double().t() @ a[r].double(), g[r].double().abs().t() @ a[r].double().abs()
+        within(dw[e], want, 300 * 2.0 ** -24 * mag + rounding(want, F32), "far rows' gradients")
+
+
 # -------------------------------------------------------------- an expert MLP --
 
 class ExpertMLP:
@@ -504,9 +539,10 @@ class ExpertMLP:
                         normalize=True)
         K.gemm_experts_swiglu(x16, self.wgu, self.act, self.gu, offsets=self.off, rows=self.rows)
         K.gemm_experts("nt", self.act, self.wd, self.y, offsets=self.off)
-        K.combine_experts(self.y, self.slots, self.out, weights=self.w, resid=x)
+        if x is not None:
+            K.combine_experts(self.y, self.slots, self.out, weights=self.w, resid=x)
 
-    def backward(self, dout, x16):
+    def backward(self, dout, x16, resid=True):
         K.spread_experts(dout, self.slots, self.dy, weights=self.w, y=self.y, dweights=self.dw)
         K.gemm_experts("tn", self.dy, self.act, self.dwd, offsets=self.off)
         K.gemm_experts_swiglu_bwd(self.dy, self.wd, self.gu, self.dgu, offsets=self.off)
@@ -514,7 +550,7 @@ class ExpertMLP:
         K.gemm_experts("tn", self.dgu, self.xs, self.dwgu, offsets=self.off)
         K.gemm_experts("nn", self.dgu, self.wgu, self.dxs, offsets=self.off)
         K.route_experts_bwd(self.dw, self.logits, self.ids, self.dlogits, normalize=True)
-        K.combine_experts(self.dxs, self.slots, self.dx, resid=dout)
+        K.combine_experts(self.dxs, self.slots, self.dx, resid=dout if resid else None)
         self.dx += self.dlogits @ self.router.float()
 
     def outputs(self):
@@ -559,6 +595,53 @@ def test_expert_mlp(T, E, k, h, inter):
     for name, g in got.items():
         err = (g.double() - want[name]).norm() / want[name].norm()
         assert float(err.detach()) <= 4 * 2.0 ** -8, (name, float(err.detach()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,E,k,h,inter", MLPS)
+def test_expert_mlp_between_norms(T, E, k, h, inter):
+    """The MLP's half of a decoder block with norms before and behind the branch, a
+    gate and a scale, forward and back, against float64. The roundings on a value's way
+    are the MLP's four and those of x, the branch and their gradients: at most eight."""
+    m = ExpertMLP(T, E, k, h, inter)
+    stream, y0 = normal(T, h, seed=11), normal(T, h, seed=12).to(BF)
+    pre, post, gate = (1 + normal(h, seed=s, std=0.2) for s in (13, 14, 15))
+    dout = normal(T, h, seed=16)
+    e = lambda dt: torch.full((T, h), 3.0, dtype=dt, device=dev())
+    h1, x16, y1, out = e(F32), e(BF), e(BF), e(F32)
+    K.norm_residual(y0, stream, h1, eps=1e-6, pre=pre, normed=x16)
+    m.forward(None, x16)
+    K.combine_experts(m.y, m.slots, y1, weights=m.w)
+    K.norm_residual(y1, h1, out, eps=1e-6, post=post, gate=gate[None], scale=0.5)
+    dy1, dh1, dx16, dy0, dstream = e(BF), e(F32), e(BF), e(BF), e(F32)
+    dpost, dgate, dpre = (torch.empty(h, device=dev()) for _ in range(3))
+    K.norm_residual_bwd(None, dout, y1, out, dy1, dh1, eps=1e-6, post=post, gate=gate[None], scale=0.5, dpost=dpost,
+                        dgate=dgate[None])
+    m.backward(dy1, x16, resid=False)
+    dx16.copy_(m.dx)
+    K.norm_residual_bwd(dx16, dh1, y0, h1, dy0, dstream, eps=1e-6, pre=pre, dpre=dpre)
+    got = dict(out=out, dy0=dy0, dstream=dstream, dpost=dpost, dgate=dgate, dpre=dpre, dwd=m.dwd, dwgu=m.dwgu)
+
+    leaf = {n: t.double().requires_grad_() for n, t in dict(y0=y0, stream=stream, pre=pre, post=post, gate=gate, wgu=m.wgu,
+                                                             wd=m.wd).items()}
+    rms = lambda v: v * (v.square().mean(1, keepdim=True) + 1e-6).rsqrt()
+    r1 = leaf["stream"] + leaf["y0"]
+    x = rms(r1) * leaf["pre"]
+    w = torch.softmax((x @ m.router.double().t()).gather(1, m.ids.long()), 1)
+    branch = torch.zeros_like(r1)
+    for i in range(E):
+        t, j = torch.nonzero(m.ids == i, as_tuple=True)
+        if t.numel():
+            g, u = halves(x[t] @ leaf["wgu"][i].t())
+            branch = branch.index_add(0, t, w[t, j, None] * ((torch.nn.functional.silu(g) * u) @ leaf["wd"][i].t()))
+    r2 = r1 + 0.5 * leaf["gate"] * (rms(branch) * leaf["post"])
+    r2.backward(dout.double())
+    grad = {n: t.grad for n, t in leaf.items()}
+    want = dict(out=r2.detach(), dy0=grad["y0"], dstream=grad["stream"], dpost=grad["post"], dgate=grad["gate"],
+                dpre=grad["pre"], dwd=grad["wd"], dwgu=grad["wgu"])
+    for name, v in got.items():
+        err = (v.double() - want[name]).norm() / want[name].norm()
+        assert float(err) <= 8 * 2.0 ** -8, (name, float(err))
 
 
 @pytest.mark.gpu

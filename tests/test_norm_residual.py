@@ -223,6 +223,23 @@ def test_rows_of_zeros_and_rows_that_are_not_finite():
 
 
 @pytest.mark.gpu
+def test_offsets_past_32_bits():
+    T, H, n = 140000, 16384, 30
+    y, r = torch.zeros(T, H, dtype=BF, device=dev()), torch.zeros(T, H, dtype=BF, device=dev())
+    near = inputs(n, H, BF, BF, seed=70)
+    y[T - n:], r[T - n:] = near[0], near[1]
+    post, pre = near[2:]
+    out, x = torch.empty_like(r), torch.empty_like(y)
+    K.norm_residual(y, r, out, eps=EPS, post=post, pre=pre, normed=x)
+    few = run_forward(near[0], near[1], post, None, None, 1.0, pre)
+    assert torch.equal(out[T - n:], few[0]) and torch.equal(x[T - n:], few[1])
+    dy, dr = torch.empty(n, H, dtype=BF, device=dev()), torch.empty(n, H, dtype=BF, device=dev())
+    K.norm_residual_bwd(near[0], near[1], near[0], few[0].contiguous(), dy, dr, eps=EPS, post=post, pre=pre)
+    K.norm_residual_bwd(x.copy_(y), r, y, out, y, r, eps=EPS, post=post, pre=pre)
+    assert torch.equal(y[T - n:], dy) and torch.equal(r[T - n:], dr)
+
+
+@pytest.mark.gpu
 def test_no_rows():
     y, post = torch.empty(0, 64, device=dev()), torch.ones(64, device=dev())
     K.norm_residual(y, y, y.clone(), eps=EPS, post=post, pre=post, normed=y.clone())
