@@ -199,7 +199,7 @@ __device__ __forceinline__ void block_starts(const RouteParams& p, const int32_t
     if (g < groups && e < E) {
       const int per = (p.blocks + groups - 1) / groups;
       const int32_t* c = p.counts + e;
-#pragma unroll 8
+#pragma unroll 16
       for (int i = g * per; i < min((g + 1) * per, p.blocks); ++i) {
         const int32_t n = c[static_cast<int64_t>(i) * E];
         a += n;

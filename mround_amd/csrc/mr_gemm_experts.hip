@@ -296,7 +296,9 @@ int launch_grouped(const char* fn, const Grouped& g, hipStream_t s) {
   const int bm = way == FEW ? 16 : way == BIG_TILES ? 256 : 128;
   const int bn = way == FEW ? few_cols(BKM) : bm;
   const int64_t tiles = tiles_of(AK, bm, bn, g.experts, g.M, g.N);
-  if (too_many_blocks(tiles * (split > 8 ? split : 8), kThreads)) return fail(MR_EINVAL, "%s: too large", fn);
+  constexpr int PER_TILE = 4 * (is_swiglu(EPI) ? 2 : 4);  // blocks of a tile's reduction
+  if (too_many_blocks(tiles, 64 * kWaves) || (split > 1 && (too_many_blocks(tiles * split, kThreads) || too_many_blocks(tiles * PER_TILE, 256))))
+    return fail(MR_EINVAL, "%s: too large", fn);
   dim3 grid(static_cast<unsigned>(tiles));
   if (way == FEW) {
     if constexpr (AK) {
@@ -313,7 +315,6 @@ int launch_grouped(const char* fn, const Grouped& g, hipStream_t s) {
     p.ws = static_cast<float*>(g.ws);
     grid.x *= split;
     hipLaunchKernelGGL((gemm_kernel<128, 128, AK, BKM, EPI, OB, G>), grid, dim3(kThreads), 0, s, p);
-    constexpr int PER_TILE = 4 * (is_swiglu(EPI) ? 2 : 4);
     if (split > 1)
       hipLaunchKernelGGL((gemm_reduce<128, 128, EPI, OB, AK, G>), dim3(static_cast<unsigned>(tiles) * PER_TILE), dim3(256), 0, s, p);
   }

@@ -887,7 +887,8 @@ __device__ __forceinline__ bool enter(GroupedParams<INDEXED>& p, int bid, int& b
   }
   p.kt_per = ((p.K + BK - 1) / BK + p.ksplit - 1) / p.ksplit;
   tile_coords(lt, p.grid_m, p.grid_n, bm, bn);
-  return true;
+  // (of offsets that descend the counts may not add up)
+  return bm >= 0 && bn >= 0 && bm < p.grid_m && bn < p.grid_n;
 }
 
 // An expert without rows has a gradient of zeros, which its BM x BN tile gets here.

@@ -409,6 +409,21 @@ def test_weight_products(counts, M, N):
         assert torch.equal(whole[:, M:], start[:, M:]) and torch.equal(whole[:, :, N:], start[:, :, N:])
 
 
+@pytest.mark.gpu
+def test_weight_products_of_few_rows_each():
+    """Large tiles of one short k-tile or of none."""
+    n, M, N = COUNTS["many"], 1024, 1032
+    assert K.gemm_experts_plan("tn", "f32", len(n), M, N, sum(n))[0] == "large"
+    dy, x = normal(sum(n), M, seed=1).to(BF), normal(sum(n), N, seed=2).to(BF)
+    c = torch.full((len(n), M, N), 7.0, device=dev())
+    K.gemm_experts("tn", dy, x, c, offsets=offsets_of(n))
+    at = 0
+    for e, rows in enumerate(n):
+        a, b = dy[at:at + rows].double(), x[at:at + rows].double()
+        within(c[e], a.t() @ b, rows * 2.0 ** -24 * (a.abs().t() @ b.abs()) + rounding(a.t() @ b, F32), f"dW of {rows} rows")
+        at += rows
+
+
 def halves(t):
     v = t.unflatten(-1, (-1, 2, 32))
     return v[..., 0, :].flatten(-2), v[..., 1, :].flatten(-2)
@@ -456,6 +471,23 @@ def test_swiglu_products(counts, N, Kd):
     over = gu.clone()
     K.gemm_experts_swiglu_bwd(dy, wd, over, over, offsets=off)
     assert torch.equal(over, dgu)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,N,Kd", [(100, 40, 64), (3000, 264, 128), (8000, 2048, 1024)])
+def test_offsets_that_descend_stay_inside(R, N, Kd):
+    """Nothing but the product's own rows is written, whatever the offsets say."""
+    off = torch.tensor([R, 0, R // 2, 7, R, -3, R, 1 << 30, 0, R], dtype=I32, device=dev())
+    E = off.numel() - 1
+    a, b = normal(R, Kd, seed=1).to(BF), normal(E, N, Kd, seed=2).to(BF)
+    whole = torch.full((R + 16, N), 7.0, dtype=BF, device=dev())
+    K.gemm_experts("nt", a, b, whole[8:R + 8], offsets=off)
+    torch.cuda.synchronize()
+    assert bool((whole[:8] == 7.0).all()) and bool((whole[R + 8:] == 7.0).all())
+    dw = torch.full((E + 2, Kd, N), 7.0, device=dev())
+    K.gemm_experts("tn", a, normal(R, N, seed=3).to(BF), dw[1:E + 1], offsets=off)
+    torch.cuda.synchronize()
+    assert bool((dw[0] == 7.0).all()) and bool((dw[E + 1] == 7.0).all())
 
 
 @pytest.mark.gpu
