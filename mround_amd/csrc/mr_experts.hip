@@ -431,7 +431,9 @@ struct RowsParams {
   int H, k, pieces;
 };
 
-// Eight places at a time are in flight; a place outside the rows counts as none.
+// Eight places at a time are in flight; a place outside the rows counts as none. A
+// thread owns eight columns (or one) of a token. Bound by HBM: 16384 tokens, 8 rows of
+// 2048 each, 157 us (5.1 TB/s).
 constexpr int kAtOnce = 8;
 
 template <int DY, int DO, int V>
@@ -473,7 +475,9 @@ __global__ __launch_bounds__(256) void combine_kernel(RowsParams p) {
   store_piece<DO, V, false>(p.out, t * p.ldo + c, acc);
 }
 
-// W waves to a token.
+// W waves to a token: each of its rows is read once for its dot product and written
+// once, x from the caches after its first reading. Bound by HBM: 4005 tokens, 2 rows of
+// 3584 each, with the dots 41 us (4.2 TB/s), 16384 of 8 of 2048 272 (4.5).
 template <int DX, int DY, int V, int W>
 __global__ __launch_bounds__(256) void spread_kernel(RowsParams p) {
   __shared__ float smem[4][kAtOnce];

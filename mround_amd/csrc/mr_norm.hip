@@ -76,7 +76,9 @@ __device__ __forceinline__ void load_weights(const float* w, int c, float (&out)
   }
 }
 
-// Thread t holds the pieces t, t + threads, .. (P of them) of its row.
+// Thread t holds the pieces t, t + threads, .. (P of them) of its row. As many
+// blocks as the card holds go over the rows in turn. Bound by HBM:
+// 4005 x 2048 bf16 onto fp32 22.6 us (4.3 TB/s), 16384 x 3584 143 (4.9).
 template <int A, int S, int V, int P, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_fwd(NormParams p) {
   __shared__ float smem[3][16];
@@ -174,6 +176,9 @@ __device__ __forceinline__ void block_sum2(float& a, float& b, float (*smem)[16]
   slot = slot == 2 ? 0 : slot + 1;
 }
 
+// Bound by HBM: 16384 x 3584, bf16 and fp32, all gradients 228 us (4.6 TB/s; with an
+// accumulator for each gradient, which spilled, 343), 4005 x 2048 41 (28 and the sums'
+// launch), 32768 x 256 39 (a row a block 81).
 // WHOLE: the block's rows are whole groups of the gate. What dgate and dw_post sum
 // differs by factors that are a group's own, dh n: one sum serves both, and the
 // factors come in when the group ends.
@@ -410,7 +415,8 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(waves_f
 }
 
 // out[s, c] = sum over the n rows of part from row s n on, in an order that the
-// launch fixes: 64 columns a block, 16 runs of rows.
+// launch fixes: 64 columns a block, 16 runs of rows (10 sums of 3584 columns over 512
+// rows 6 us).
 struct SumParams {
   const float* part[3];
   float* out[3];
@@ -691,7 +697,7 @@ int mr_norm_residual_bwd(const void* dnormed, int act_dtype, int64_t lddn, const
     const int threads = row_threads(n, P);
     if (too_many_blocks(blocks, 1024)) return fail(MR_EINVAL, "%s: too many rows", fn);
     // Eight rows at a time where a wave holds one (with one, two waves a CU were all
-    // there were: 32768 rows of 256 columns 81 us, 42 now).
+    // there were: 32768 rows of 256 columns 81 us, 39 now).
     p.row_threads = threads;
     p.teams = vec && threads == 64 ? 8 : 1;
     const dim3 grid(static_cast<unsigned>(blocks)), block(threads * p.teams);
