@@ -520,7 +520,7 @@ int mr_norm_residual(const void* y, int act_dtype, int64_t ldy, const void* resi
   {
     const int64_t no = bytes_of(T, ldo, H, es), nn = normed ? bytes_of(T, ldn, H, ea) : 0;
     const int64_t ny = bytes_of(T, ldy, H, ea), nr = bytes_of(T, ldr, H, es);
-    const int64_t ng = gate ? (T + gate_rows - 1) / gate_rows * H * 4 : 0;
+    const int64_t ng = gate ? ((T - 1) / gate_rows + 1) * H * 4 : 0;
     auto hit = [&](const void* a, int64_t na, const void* b, int64_t nb) { return a && b && overlap(a, na, b, nb); };
     const bool over_resid = out == resid && ldo == ldr, over_y = normed == y && ldn == ldy;
     bool bad = hit(out, no, y, ny) || (!over_resid && hit(out, no, resid, nr)) || hit(out, no, normed, nn) ||
@@ -577,7 +577,7 @@ int mr_norm_residual(const void* y, int act_dtype, int64_t ldy, const void* resi
 
 size_t mr_norm_residual_bwd_workspace_bytes(int64_t T, int64_t H, int64_t gate_rows, int post, int gate, int pre) {
   if (T <= 0 || H <= 0) return 0;
-  const mr::Split sp = mr::split_rows(T, H, gate ? (gate_rows > 0 ? gate_rows : 1) : T);
+  const mr::Split sp = mr::split_rows(T, H, gate ? (gate_rows < 1 ? 1 : gate_rows < T ? gate_rows : T) : T);
   const int64_t each = sp.blocks * H * 4;
   return static_cast<size_t>((post ? each : 0) + (pre ? each : 0) + (gate && sp.per_group > 1 ? each : 0));
 }
@@ -606,7 +606,7 @@ int mr_norm_residual_bwd(const void* dnormed, int act_dtype, int64_t lddn, const
        reinterpret_cast<uintptr_t>(dpost) | reinterpret_cast<uintptr_t>(dgate) | reinterpret_cast<uintptr_t>(dpre)) % 4)
     return fail(MR_EINVAL, "%s: a pointer is not aligned to its elements", fn);
   const int64_t rows = T > 0 ? T : 1;
-  const int64_t of_gate = gate ? gate_rows : rows;
+  const int64_t of_gate = gate && gate_rows < rows ? gate_rows : rows;
   const int64_t groups = T > 0 ? (T + of_gate - 1) / of_gate : 0;
   const Split sp = split_rows(rows, H, of_gate);
   const int64_t each = sp.blocks * H * 4;

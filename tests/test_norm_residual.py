@@ -240,6 +240,26 @@ def test_offsets_past_32_bits():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 5, 700])
+def test_a_gate_for_more_rows_than_there_are(T):
+    y, r, post, pre = inputs(T, 72, BF, F32, seed=80)
+    gate = normal(1, 72, seed=84)
+    dx, d = normal(T, 72, seed=85).to(BF), normal(T, 72, seed=86)
+    got = []
+    for per in (None, T, 4096, 1 << 40):
+        out, x = run_forward(y, r, post, gate, per, 0.5, pre)
+        e = lambda *s, dt=F32: torch.empty(*s, dtype=dt, device=dev())
+        g = [e(T, 72, dt=BF), e(T, 72), e(72), e(1, 72), e(72)]
+        K.norm_residual_bwd(dx, d, y, out, g[0], g[1], eps=EPS, post=post, gate=gate, gate_rows=per, scale=0.5, pre=pre,
+                            dpost=g[2], dgate=g[3], dpre=g[4])
+        got.append([out, x] + g)
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+    assert K.lib().mr_norm_residual_bwd_workspace_bytes(T, 72, 1 << 40, 1, 1, 1) == \
+        K.lib().mr_norm_residual_bwd_workspace_bytes(T, 72, T, 1, 1, 1)
+
+
+@pytest.mark.gpu
 def test_no_rows():
     y, post = torch.empty(0, 64, device=dev()), torch.ones(64, device=dev())
     K.norm_residual(y, y, y.clone(), eps=EPS, post=post, pre=post, normed=y.clone())
