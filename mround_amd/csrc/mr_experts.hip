@@ -221,12 +221,7 @@ __device__ __forceinline__ void block_starts(const RouteParams& p, const int32_t
   }
   // exclusive scan of the experts' counts over the threads
   const int lane = tid & 63;
-  int32_t upto = all;
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const int32_t x = __shfl_up(upto, o, 64);
-    upto += lane >= o ? x : 0;
-  }
+  const int32_t upto = wave_scan(all);
   if (lane == 63) scratch[tid >> 6] = upto;
   __syncthreads();
   int32_t base = 0;
@@ -253,18 +248,21 @@ __device__ __forceinline__ void place(const RouteParams& p, int t0, int t1, cons
   int32_t* mine = of_wave + wave * E;
   for (int e = lane; e < E; e += 64) mine[e] = 0;
   __syncthreads();
+  int first_id = -1;  // of the run's first 64 pairs, which is all there are of most runs
   for (int64_t i = a + lane; i < b; i += 64) {
     const int id = p.ids[first + i];
+    first_id = i < a + 64 ? id : first_id;
     if (id >= 0) atomicAdd(mine + id, 1);
   }
   __syncthreads();
   if (tid < E) {
-    int32_t at = start[tid];
+    int32_t at = start[tid], n[kRouteWaves];
+#pragma unroll
+    for (int w = 0; w < kRouteWaves; ++w) n[w] = of_wave[w * E + tid];
 #pragma unroll
     for (int w = 0; w < kRouteWaves; ++w) {
-      const int32_t n = of_wave[w * E + tid];
       of_wave[w * E + tid] = at;
-      at += n;
+      at += n[w];
     }
   }
   __syncthreads();
@@ -272,7 +270,7 @@ __device__ __forceinline__ void place(const RouteParams& p, int t0, int t1, cons
   while ((1 << bits) < E) ++bits;
   for (int64_t i = a; i < b; i += 64) {
     const int64_t pair = first + i + lane;
-    const int id = i + lane < b ? p.ids[pair] : -1;
+    const int id = i == a ? first_id : i + lane < b ? p.ids[pair] : -1;
     uint64_t same = __ballot(id >= 0);
     for (int q = 0; q < bits; ++q) {
       const uint64_t set = __ballot((id >> q) & 1);

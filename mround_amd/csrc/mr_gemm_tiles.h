@@ -36,6 +36,7 @@
 
 #include "mr_act.h"
 #include "mr_common.h"
+#include "mr_rows.h"
 
 namespace mr {
 namespace {
@@ -780,17 +781,6 @@ __device__ __forceinline__ void store_partial(float* out, const f32x16 (&acc)[TM
       for (int gi = 0; gi < 4; ++gi)
         *reinterpret_cast<f32x4*>(out + (((bi + i) * (BN / 32) + bj + j) * 4 + gi) * 256 + lane * 4) =
             f32x4{acc[i][j][4 * gi], acc[i][j][4 * gi + 1], acc[i][j][4 * gi + 2], acc[i][j][4 * gi + 3]};
-}
-
-// The sum of x over the lanes up to each one (row by row of 16 lanes, then across them).
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // 1, 2, 4, 8 lanes down a row
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the last of rows 0 and 2 to rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // the last of row 1 to rows 2 and 3
-  return x;
 }
 
 // Half octaves of a count, 0 for none: experts of one class count as alike long.

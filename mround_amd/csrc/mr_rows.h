@@ -100,4 +100,15 @@ __device__ __forceinline__ float wave_sum(float x) {
   return (of(0) + of(16)) + (of(32) + of(48));
 }
 
+// The sum of x over the lanes up to each one (row by row of 16 lanes, then across them).
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // 1, 2, 4, 8 lanes down a row
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the last of rows 0 and 2 to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // the last of row 1 to rows 2 and 3
+  return x;
+}
+
 }  // namespace mr
