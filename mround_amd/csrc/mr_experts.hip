@@ -558,7 +558,7 @@ int check_route(const char* fn, int dtype, int64_t ldz, int64_t T, int64_t E, in
   if (k > E || k > kMaxTop || E > kMaxExperts)
     return fail(MR_EINVAL, "%s: at most %d of at most %d experts, no more than there are (%lld of %lld)", fn, kMaxTop,
                 kMaxExperts, static_cast<long long>(k), static_cast<long long>(E));
-  if (T * k > 0x7fffffff) return fail(MR_EINVAL, "%s: too many rows", fn);
+  if (T > 0x7fffffff / k) return fail(MR_EINVAL, "%s: too many rows", fn);
   if (T > 0 && ldz < E) return fail(MR_EINVAL, "%s: a leading dimension is smaller than its row", fn);
   if (reinterpret_cast<uintptr_t>(z) % dtype_bytes(dtype))
     return fail(MR_EINVAL, "%s: a pointer is not aligned to its elements", fn);
@@ -621,7 +621,7 @@ bool vector_rows(const void* p, int64_t ld, int es) { return !p || (aligned16(p)
 
 int check_rows(const char* fn, int64_t T, int64_t k, int64_t R, int64_t H) {
   if (T < 0 || k <= 0 || R < 0 || H < 0) return fail(MR_EINVAL, "%s: no experts, or a negative size", fn);
-  if (H > 0x7fffffff || T * k > 0x7fffffff || R > 0x7fffffff) return fail(MR_EINVAL, "%s: too large", fn);
+  if (H > 0x7fffffff || T > 0x7fffffff / k || R > 0x7fffffff) return fail(MR_EINVAL, "%s: too large", fn);
   return MR_OK;
 }
 

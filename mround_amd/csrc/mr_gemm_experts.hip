@@ -378,6 +378,8 @@ int mr_gemm_experts_plan(int layout, int output, int64_t experts, int64_t M, int
   *split_out = 1;
   *workspace_out = 0;
   if (experts <= 0 || M < 0 || N < 0 || K < 0) return fail(MR_EINVAL, "mr_gemm_experts_plan: no experts, or a negative size");
+  if (experts > 0x7ffffffe || M > 0x7fffffff || N > 0x7fffffff || K > 0x7fffffff)
+    return fail(MR_EINVAL, "mr_gemm_experts_plan: too large");
   if (M == 0 || N == 0) return MR_OK;
   constexpr Output kinds[] = {OUT_F32, OUT_B16, OUT_RESID, OUT_SWIGLU, OUT_F32, OUT_SWIGLU_BWD};
   const bool ak = layout != MR_TN;

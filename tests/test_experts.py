@@ -791,6 +791,19 @@ def test_rows_refuse(fn, base, change, message):
     refused(fn, list(dict(base, **change).values()), message)
 
 
+@pytest.mark.parametrize("fn,base,k", [("mr_route_experts", ROUTE, 8), ("mr_route_experts_bwd", BACK, 8),
+                                       ("mr_combine_experts", COMBINE, 4), ("mr_spread_experts", SPREAD, 4)])
+def test_products_of_sizes_that_pass_64_bits_are_refused(fn, base, k):
+    refused(fn, list(dict(base, T=1 << 62, k=k).values()), "too")
+
+
+@pytest.mark.parametrize("sizes", [(1 << 62, 8, 64, 64), (4, 1 << 62, 64, 64), (4, 8, 1 << 62, 64), (4, 8, 64, 1 << 62)])
+def test_plans_of_sizes_past_32_bits_are_refused(sizes):
+    out = [ctypes.byref(ctypes.c_int()), ctypes.byref(ctypes.c_int()), ctypes.byref(ctypes.c_size_t())]
+    refused("mr_gemm_experts_plan", [0, 1, *sizes, *out], "too large")
+    assert K.lib().mr_gemm_experts_workspace_bytes(0, 1, *sizes) == 0
+
+
 GEMM = dict(layout=0, E=4, M=100, N=64, K=128, A=address(0), lda=128, index=None, a_rows=0, B=address(1), ldb=128,
             b_step=64 * 128, off=address(2), C=address(3), cdt=1, ldc=64, c_step=0, acc=0, ws=None, ws_bytes=0, stream=None)
 TN = dict(GEMM, layout=2, M=64, K=100, lda=64, ldb=64, cdt=0, c_step=64 * 64)
