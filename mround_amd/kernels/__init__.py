@@ -998,7 +998,7 @@ def _norm_types(name: str, y, stream) -> tuple[int, int]:
 
 
 def _gate(name: str, gate, gate_rows, T: int, H: int) -> tuple[int | None, int]:
-    """(address, rows a gate row applies to)."""
+    """(address, rows a gate row applies to). Of no rows, a gate of any number of them."""
     if gate is None:
         return None, 0
     per = max(T, 1) if gate_rows is None else int(gate_rows)
@@ -1067,6 +1067,8 @@ def norm_residual_bwd(dnormed, dout, y, out, dy, dresid, *, eps, post=None, gate
                                     ldh, T, H, eps, w_post, g, per, scale, w_pre, at_dy, lddy, at_dr, lddr, g_post, g_gate,
                                     g_pre, ws, nbytes, _stream(dy))
     _check(rc, "mr_norm_residual_bwd")
+    if dgate is not None and not T:
+        dgate.zero_()
 
 
 def rmsnorm_fwd(h, w, eps, y, rstd=None) -> None:

@@ -269,6 +269,15 @@ def test_no_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("G,per", [(1, None), (3, 5)])
+def test_the_gate_of_no_rows_has_no_gradient(G, per):
+    y, gate = torch.empty(0, 64, device=dev()), torch.ones(G, 64, device=dev())
+    dgate = torch.full_like(gate, 7.0)
+    K.norm_residual_bwd(None, y, y, y, y.clone(), y.clone(), eps=EPS, gate=gate, gate_rows=per, dgate=dgate)
+    assert not dgate.any()
+
+
+@pytest.mark.gpu
 def test_two_blocks_in_a_graph():
     """Two branches' ends forward and back, captured once and replayed over other
     inputs between eager runs of the same chain."""
