@@ -103,7 +103,7 @@ __device__ __forceinline__ void load_logits(const RouteParams& p, int64_t t, int
 // the expert from the top): the maximum is the choice. 32-bit ones need a second
 // reduction, over the lanes that hold the maximum, for the lowest expert. The
 // instructions of the choices bound it, 30 to 50 each (16384 tokens, 8 of 128 experts:
-// 14 us with the order; with the value fetched from its lane and 64 tokens for half the
+// 13 us with the order; with the value fetched from its lane and 64 tokens for half the
 // CUs 20).
 template <int DT, int L, int V>
 __device__ __forceinline__ void choose(const RouteParams& p, int t0, int t1, int32_t* hist) {
