@@ -465,6 +465,11 @@ Split split_rows(int64_t T, int64_t H, int64_t gate_rows) {
   return {(gate_rows + per - 1) / per, per, groups * per};
 }
 
+// What a backward's blocks leave for the sums' launch (a gate's rows that one block sums are sums already).
+size_t partials_bytes(const Split& sp, int64_t H, bool post, bool gate, bool pre) {
+  return static_cast<size_t>((post ? 1 : 0) + (pre ? 1 : 0) + (gate && sp.per_group > 1 ? 1 : 0)) * sp.blocks * H * 4;
+}
+
 int check_norm(const char* fn, int64_t T, int64_t H, int act, int stream_type, const float* gate, int64_t gate_rows) {
   if (T < 0 || H < 0) return fail(MR_EINVAL, "%s: negative size", fn);
   if (!valid_dtype(act) || (stream_type != MR_F32 && stream_type != act))
@@ -577,9 +582,14 @@ int mr_norm_residual(const void* y, int act_dtype, int64_t ldy, const void* resi
 
 size_t mr_norm_residual_bwd_workspace_bytes(int64_t T, int64_t H, int64_t gate_rows, int post, int gate, int pre) {
   if (T <= 0 || H <= 0) return 0;
-  const mr::Split sp = mr::split_rows(T, H, gate ? (gate_rows < 1 ? 1 : gate_rows < T ? gate_rows : T) : T);
-  const int64_t each = sp.blocks * H * 4;
-  return static_cast<size_t>((post ? each : 0) + (pre ? each : 0) + (gate && sp.per_group > 1 ? each : 0));
+  const mr::Split sp = mr::split_rows(T, H, gate_rows < 1 ? (gate ? 1 : T) : gate_rows < T ? gate_rows : T);
+  size_t n = mr::partials_bytes(sp, H, post, gate, pre);
+  // A gate whose gradient is not wanted splits the rows as any other, and none does not.
+  if (!gate) {
+    const size_t without = mr::partials_bytes(mr::split_rows(T, H, T), H, post, false, pre);
+    n = n > without ? n : without;
+  }
+  return n;
 }
 
 int mr_norm_residual_bwd(const void* dnormed, int act_dtype, int64_t lddn, const void* dout, int stream_dtype,
@@ -610,7 +620,7 @@ int mr_norm_residual_bwd(const void* dnormed, int act_dtype, int64_t lddn, const
   const int64_t groups = T > 0 ? (T + of_gate - 1) / of_gate : 0;
   const Split sp = split_rows(rows, H, of_gate);
   const int64_t each = sp.blocks * H * 4;
-  const size_t need = T > 0 ? mr_norm_residual_bwd_workspace_bytes(T, H, gate_rows, dpost != nullptr, dgate != nullptr, dpre != nullptr) : 0;
+  const size_t need = T > 0 ? partials_bytes(sp, H, dpost != nullptr, dgate != nullptr, dpre != nullptr) : 0;
   if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need))
     return fail(MR_EINVAL, "%s: %zu bytes of workspace are needed, on an address of 16 bytes", fn, need);
   {

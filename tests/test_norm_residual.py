@@ -319,6 +319,62 @@ def test_two_blocks_in_a_graph():
             assert torch.equal(a[name], b[name]), (seed, name)
 
 
+# The gradients that may be asked for beside a gate, each with and without the others.
+SUBSETS = [(a, b, c) for a in (0, 1) for b in (0, 1) for c in (0, 1) if a or b or c]
+
+
+def blocks_of(T, H, rows):
+    """(blocks of the backward, blocks that share a gate's row): about 512, of narrow
+    rows 1024, each of whole groups or of one group's rows."""
+    want = -(-T // (1024 if 512 < H <= 1024 else 512))
+    if rows <= want:
+        return -(-T // (want // rows * rows)), 1
+    per = -(-rows // want)
+    return -(-T // rows) * per, per
+
+
+@pytest.mark.parametrize("T,H", [(1, 64), (600, 256), (1000, 256), (1000, 1024), (4005, 2048), (16384, 3584), (300000, 64)])
+@pytest.mark.parametrize("rows", [1, 2, 3, 33, 100, 2048, 1 << 40])
+def test_the_workspace_holds_what_the_blocks_leave(T, H, rows):
+    """Of any gradients, with a gate or without one."""
+    size = K.lib().mr_norm_residual_bwd_workspace_bytes
+    gated, shared = blocks_of(T, H, min(rows, T))
+    plain = blocks_of(T, H, T)[0]
+    for dpost, dgate, dpre in SUBSETS:
+        n = dpost + dpre + (dgate and shared > 1)
+        assert size(T, H, rows, dpost, dgate, dpre) >= 4 * H * n * gated
+        if not dgate:
+            for any_rows in (0, rows):
+                assert size(T, H, any_rows, dpost, 0, dpre) >= 4 * H * n * plain
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,rows", [(1000, 256, 3), (1000, 256, 100), (2049, 72, 33), (1500, 1000, 2), (700, 4104, 3), (900, 201, 5)])
+def test_any_of_the_gradients_beside_a_gate(T, H, rows):
+    """The same bits as of all of them, and nothing behind the workspace."""
+    y, h, post, pre = inputs(T, H, BF, F32, seed=90)
+    gate, _, per = gates(T, H, rows)
+    dx, d = normal(T, H, seed=95).to(BF), normal(T, H, seed=96)
+    args = dict(eps=EPS, post=post, gate=gate, gate_rows=per, scale=0.7, pre=pre)
+    f = lambda t: torch.full_like(t, 7.0)
+    want = [f(y), f(h), f(post), f(gate), f(pre)]
+    K.norm_residual_bwd(dx, d, y, h, want[0], want[1], dpost=want[2], dgate=want[3], dpre=want[4], **args)
+    lib = K.lib()
+    for subset in SUBSETS:
+        got = [f(y), f(h)] + [f(t) if on else None for t, on in zip((post, gate, pre), subset)]
+        K.norm_residual_bwd(dx, d, y, h, got[0], got[1], dpost=got[2], dgate=got[3], dpre=got[4], **args)
+        assert all(b is None or torch.equal(a, b) for a, b in zip(want, got)), subset
+        size = lib.mr_norm_residual_bwd_workspace_bytes(T, H, rows, *subset)
+        ws = torch.full((size + 4096,), 0x5a, dtype=torch.uint8, device=dev())
+        ptr = lambda t: None if t is None else t.data_ptr()
+        again = [None if t is None else f(t) for t in got]
+        assert lib.mr_norm_residual_bwd(ptr(dx), 1, H, ptr(d), 0, H, ptr(y), H, ptr(h), H, T, H, EPS, ptr(post), ptr(gate), rows,
+                                        0.7, ptr(pre), ptr(again[0]), H, ptr(again[1]), H, *map(ptr, again[2:]), ptr(ws), size,
+                                        torch.cuda.current_stream().cuda_stream) == 0
+        assert bool((ws[size:] == 0x5a).all()), subset
+        assert all(a is None or torch.equal(a, b) for a, b in zip(again, got)), subset
+
+
 # ---------------------------------------------------------------- refusals --
 
 FORWARD = dict(y=address(0), act=1, ldy=64, r=address(1), st=0, ldr=64, T=10, H=64, eps=1e-6, post=address(2),
@@ -348,6 +404,19 @@ def test_forward_refuses(change, message):
     (dict(ws=address(2)), "no memory"), (dict(dpre=ctypes.c_void_p((1 << 20) + 2)), "aligned"), (dict(rows=0), "gate")])
 def test_backward_refuses(change, message):
     refused("mr_norm_residual_bwd", list(dict(BACKWARD, **change).values()), message)
+
+
+@pytest.mark.parametrize("T,H,rows", [(1000, 256, 3), (4005, 2048, 100), (16384, 3584, 33)])
+def test_a_workspace_too_small_for_the_blocks_beside_a_gate_is_refused(T, H, rows):
+    """Where dgate is not asked for: the blocks are still those of the gate's groups."""
+    lds = {n: H for n in ("lddx", "ldd", "ldy", "ldh", "lddy", "lddr")}
+    far = {n: ctypes.c_void_p((i + 1) << 40) for i, n in enumerate(
+        ("dx", "d", "y", "h", "post", "gate", "pre", "dy", "dr", "dpost", "dpre", "ws"))}
+    base = dict(BACKWARD, **far, **lds, T=T, H=H, rows=rows, dgate=None)
+    assert blocks_of(T, H, rows)[0] > blocks_of(T, H, T)[0]
+    for change, n in ((dict(), 2), (dict(dpre=None), 1), (dict(dpost=None), 1)):
+        for blocks in (blocks_of(T, H, T)[0], blocks_of(T, H, rows)[0] - 1):
+            refused("mr_norm_residual_bwd", list(dict(base, **change, bytes=4 * H * n * blocks).values()), "workspace")
 
 
 def test_bindings_refuse():
