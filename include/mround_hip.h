@@ -463,8 +463,8 @@ int mr_rmsnorm_bwd(const float* dy, const float* h, const float* w, const float*
  * offsets [E + 1], slots [T, k] and rows [T k] (all or none): the pairs sorted by
  * expert, tokens in order within one: expert e's places start at offsets[e],
  * slots is a pair's place, rows a place's token (places past offsets[E] are left).
- * E <= 512, k <= min(E, 64). workspace: mr_route_workspace_bytes(T, E) bytes when
- * offsets are asked for.
+ * E <= 512, k <= min(E, 64), T k < 2^31, T <= 2^31 - 2^14.
+ * workspace: mr_route_workspace_bytes(T, E) bytes when offsets are asked for.
  * mr_route_experts_bwd: the logits' gradient (their type; may be written over
  * them) from dweights [T, k] for the ids that were chosen, each once a row.
  */

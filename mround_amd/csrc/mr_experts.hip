@@ -558,7 +558,8 @@ int check_route(const char* fn, int dtype, int64_t ldz, int64_t T, int64_t E, in
   if (k > E || k > kMaxTop || E > kMaxExperts)
     return fail(MR_EINVAL, "%s: at most %d of at most %d experts, no more than there are (%lld of %lld)", fn, kMaxTop,
                 kMaxExperts, static_cast<long long>(k), static_cast<long long>(E));
-  if (T > 0x7fffffff / k) return fail(MR_EINVAL, "%s: too many rows", fn);
+  // (the last block's chunk, of at most 2^23 tokens in 64s, may end past T and must end within 31 bits)
+  if (T > 0x7fffffff / k || T > 0x80000000ll - (1 << 14)) return fail(MR_EINVAL, "%s: too many rows", fn);
   if (T > 0 && ldz < E) return fail(MR_EINVAL, "%s: a leading dimension is smaller than its row", fn);
   if (reinterpret_cast<uintptr_t>(z) % dtype_bytes(dtype))
     return fail(MR_EINVAL, "%s: a pointer is not aligned to its elements", fn);

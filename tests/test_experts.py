@@ -761,6 +761,18 @@ def test_route_refuses(change, message):
     refused("mr_route_experts", list(dict(ROUTE, **change).values()), message)
 
 
+def test_route_refuses_tokens_whose_blocks_end_past_31_bits():
+    """256 blocks of whole runs of 64 tokens: the last one ends at 2^31 from 2^31 - 2^14 + 1 tokens on."""
+    most = 2 ** 31 - 2 ** 14
+    ends = lambda T: -(-T // 256 // 64) * 64 * 256
+    assert ends(most) < 2 ** 31 <= ends(most + 1)
+    far = {n: ctypes.c_void_p((i + 1) << 40) for i, n in enumerate(("z", "w", "ids", "off", "slots", "rows", "ws"))}
+    base = dict(ROUTE, **far, E=1, k=1, ld=1)
+    for T in (most + 1, 2 ** 31 - 1, 2 ** 31):
+        refused("mr_route_experts", list(dict(base, T=T).values()), "too many")
+    refused("mr_route_experts", list(dict(base, T=most, ws_bytes=8).values()), "workspace")
+
+
 BACK = dict(dw=address(1), z=address(0), dtype=0, ld=64, ids=address(2), T=300, E=64, k=8, normalize=0, scale=1.0,
             dz=address(3), lddz=64, stream=None)
 
