@@ -524,6 +524,7 @@ int mr_gemm_experts_swiglu_bwd(int64_t experts, int64_t M, int64_t N, int64_t K,
  *   may be out) and dweights [T, k]: dweights[t, j] = x[t] . y[slots[t, j]]. Places
  *   without an entry are left.
  * slots [T, k]; a negative one, or one past the R rows, is no entry; others occur once.
+ * T k and R < 2^31, H < 2^31 - 256.
  */
 int mr_combine_experts(const void* y, int y_dtype, int64_t ldy, int64_t R, const int32_t* slots, const float* weights,
                        int64_t T, int64_t k, int64_t H, const void* resid, int64_t ldr, void* out, int out_dtype,

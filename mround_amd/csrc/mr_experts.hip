@@ -802,6 +802,7 @@ int mr_spread_experts(const void* x, int x_dtype, int64_t ldx, const int32_t* sl
   clear_error();
   const char* fn = "mr_spread_experts";
   if (const int rc = check_rows(fn, T, k, R, H)) return rc;
+  if (H > 0x7fffffff - 256) return fail(MR_EINVAL, "%s: too large", fn);  // (a block's steps over the columns: 31 bits)
   if ((x_dtype != MR_F32 && x_dtype != MR_BF16) || (out_dtype != MR_F32 && out_dtype != MR_BF16))
     return fail(MR_EINVAL, "%s: rows are fp32 or bf16", fn);
   if (T == 0 || (H == 0 && !dweights)) return MR_OK;

@@ -809,6 +809,15 @@ def test_products_of_sizes_that_pass_64_bits_are_refused(fn, base, k):
     refused(fn, list(dict(base, T=1 << 62, k=k).values()), "too")
 
 
+def test_spread_refuses_columns_whose_steps_pass_31_bits():
+    """A block goes over a row 256 columns at a time, and past its end by less than one step."""
+    far = {n: ctypes.c_void_p((i + 1) << 40) for i, n in enumerate(("x", "slots", "w", "out", "y", "dw"))}
+    for H in (2 ** 31 - 1, 2 ** 31 - 256):
+        refused("mr_spread_experts", list(dict(SPREAD, **far, T=1, k=1, R=1, H=H, ldx=H, ldo=H, ldy=H).values()), "too large")
+    H = 2 ** 31 - 257
+    refused("mr_spread_experts", list(dict(SPREAD, **far, T=1, k=1, R=1, H=H, ldx=H, ldo=H, ldy=H - 1).values()), "leading")
+
+
 @pytest.mark.parametrize("sizes", [(1 << 62, 8, 64, 64), (4, 1 << 62, 64, 64), (4, 8, 1 << 62, 64), (4, 8, 64, 1 << 62)])
 def test_plans_of_sizes_past_32_bits_are_refused(sizes):
     out = [ctypes.byref(ctypes.c_int()), ctypes.byref(ctypes.c_int()), ctypes.byref(ctypes.c_size_t())]
