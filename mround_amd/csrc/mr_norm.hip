@@ -448,6 +448,7 @@ __global__ __launch_bounds__(1024) void norm_sum(SumParams p) {
 }
 
 constexpr int kMaxH = 16384;
+constexpr int64_t kMaxT = int64_t{1} << 40;  // (more than any memory holds; products of sizes stay in 64 bits)
 struct Split {
   int64_t chunk, per_group, blocks;
 };
@@ -472,6 +473,7 @@ size_t partials_bytes(const Split& sp, int64_t H, bool post, bool gate, bool pre
 
 int check_norm(const char* fn, int64_t T, int64_t H, int act, int stream_type, const float* gate, int64_t gate_rows) {
   if (T < 0 || H < 0) return fail(MR_EINVAL, "%s: negative size", fn);
+  if (T > kMaxT) return fail(MR_EINVAL, "%s: too many rows", fn);
   if (!valid_dtype(act) || (stream_type != MR_F32 && stream_type != act))
     return fail(MR_EINVAL, "%s: the stream is fp32 or of the branch's type (%d, %d)", fn, stream_type, act);
   if (H > kMaxH) return fail(MR_EINVAL, "%s: rows of more than %d columns are not supported (%lld)", fn, kMaxH,
@@ -581,7 +583,7 @@ int mr_norm_residual(const void* y, int act_dtype, int64_t ldy, const void* resi
 }
 
 size_t mr_norm_residual_bwd_workspace_bytes(int64_t T, int64_t H, int64_t gate_rows, int post, int gate, int pre) {
-  if (T <= 0 || H <= 0) return 0;
+  if (T <= 0 || T > mr::kMaxT || H <= 0 || H > mr::kMaxH) return 0;
   const mr::Split sp = mr::split_rows(T, H, gate_rows < 1 ? (gate ? 1 : T) : gate_rows < T ? gate_rows : T);
   size_t n = mr::partials_bytes(sp, H, post, gate, pre);
   // A gate whose gradient is not wanted splits the rows as any other, and none does not.

@@ -419,6 +419,13 @@ def test_a_workspace_too_small_for_the_blocks_beside_a_gate_is_refused(T, H, row
             refused("mr_norm_residual_bwd", list(dict(base, **change, bytes=4 * H * n * blocks).values()), "workspace")
 
 
+@pytest.mark.parametrize("fn,base", [("mr_norm_residual", FORWARD), ("mr_norm_residual_bwd", BACKWARD)])
+@pytest.mark.parametrize("T", [2 ** 40 + 1, 1 << 62, 2 ** 63 - 1])
+def test_rows_whose_bytes_pass_64_bits_are_refused(fn, base, T):
+    refused(fn, list(dict(base, T=T).values()), "too many rows")
+    assert K.lib().mr_norm_residual_bwd_workspace_bytes(T, 64, 5, 1, 1, 1) == 0
+
+
 def test_bindings_refuse():
     y, r, w = torch.zeros(4, 8, dtype=BF), torch.zeros(4, 8), torch.zeros(8)
     for call in (
