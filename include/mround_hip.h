@@ -547,6 +547,8 @@ int mr_spread_experts(const void* x, int x_dtype, int64_t ldx, const int32_t* sl
  * blocks' partials in the workspace. mr_norm_residual_bwd_workspace_bytes: for which
  * of dpost, dgate and dpre are asked for (post, gate, pre), and gate_rows as the call
  * has them, also where the gate's gradient is not asked for; any value without a gate.
+ * With T = 0 dpost and dpre are zeros, and dgate has no rows, ceil(0 / gate_rows), and
+ * is left: whoever keeps a gate of more rows for such a batch clears its gradient.
  */
 int mr_norm_residual(const void* y, int act_dtype, int64_t ldy, const void* resid, int stream_dtype, int64_t ldr,
                      int64_t T, int64_t H, float eps, const float* post, const float* gate, int64_t gate_rows,

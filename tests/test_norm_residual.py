@@ -278,6 +278,17 @@ def test_the_gate_of_no_rows_has_no_gradient(G, per):
 
 
 @pytest.mark.gpu
+def test_no_rows_through_the_c_interface():
+    """dpost and dpre are zeros; dgate, which has no rows then, is left."""
+    w, got = torch.ones(64, device=dev()), [torch.full((64,), 7.0, device=dev()) for _ in range(3)]
+    at = w.data_ptr()
+    assert K.lib().mr_norm_residual_bwd(None, 0, 64, None, 0, 64, None, 64, None, 64, 0, 64, EPS, at, at, 5, 1.0, at, None, 64,
+                                        None, 64, *(t.data_ptr() for t in got), None, 0, torch.cuda.current_stream().cuda_stream) == 0
+    dpost, dgate, dpre = got
+    assert not dpost.any() and not dpre.any() and bool((dgate == 7.0).all())
+
+
+@pytest.mark.gpu
 def test_two_blocks_in_a_graph():
     """Two branches' ends forward and back, captured once and replayed over other
     inputs between eager runs of the same chain."""
