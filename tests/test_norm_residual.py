@@ -174,6 +174,37 @@ def test_backward(T, H, act, stream):
         assert torch.equal(a, dy) and torch.equal(b, dr)
 
 
+# Rows enough that each block goes on to others, for each number of pieces a thread: one
+# column at a time (4, 8 and 16 a thread) and eight (one, two, and those past 8192 columns).
+MANY = [(2600, 1001), (1300, 5003), (1100, 16383), (2100, 2048), (2100, 4104), (1100, 8200), (1100, 16384)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act,stream", PAIRS)
+@pytest.mark.parametrize("T,H", MANY)
+def test_blocks_that_go_on_to_other_rows(T, H, act, stream):
+    """Forward and backward with every weight's gradient."""
+    y, r, post, pre = inputs(T, H, act, stream, seed=100)
+    dx, d = normal(T, H, seed=110).to(act), normal(T, H, seed=111).to(stream)
+    for g, rows, per in (gates(T, H, 1), gates(T, H, 3), gates(T, H, 700), (None, None, None)):
+        out, x = run_forward(y, r, post, g, per, 0.7, pre)
+        h, eh, want, ex = forward64(y, r, post, rows, 0.7, pre)
+        within(out, h, eh + rounding(h, stream), "out")
+        within(x, want, ex + rounding(want, act), "normed")
+        f = lambda t: None if t is None else torch.full_like(t, 7.0)
+        got = dict(dy=f(y), dresid=f(r), dpost=f(post), dgate=f(g), dpre=f(pre))
+        K.norm_residual_bwd(dx, d, y, r, got["dy"], got["dresid"], eps=EPS, post=post, gate=g, gate_rows=per, scale=0.7,
+                            pre=pre, dpost=got["dpost"], dgate=got["dgate"], dpre=got["dpre"])
+        want = backward64(dx, d, y, r, post, rows, 0.7, pre)
+        for name, dtype in (("dy", act), ("dresid", stream)):
+            v, tol = want[name]
+            within(got[name], v, tol + rounding(v, dtype), name)
+        for name in ("dpost", "dpre"):
+            within(got[name], want[name][0], want[name][1] + 1e-30, name)
+        if g is not None:
+            within(got["dgate"], by_group(want["dgate"][0], per), by_group(want["dgate"][1], per) + 1e-30, "dgate")
+
+
 @pytest.mark.gpu
 def test_backward_against_differences():
     """Central differences of sum(out d) + sum(normed dx) in float64 arithmetic of
