@@ -551,6 +551,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
     constexpr int NIT = 32 * CH / 64;
     static_assert(32 * PITCH <= REGION && TN % JH == 0 && NIT * 64 == 32 * CH && 64 % CH == 0, "staging does not fit");
     static_assert(!BWD || OUT_BF16, "the backward writes bf16");
+    static_assert(!HALVES, "products with an activation have whole tiles");
     lds_u8* st = (lds_u8*)region;
     const int ch = lane % CH;
     // (slices by StaticFor: with an erf in it the body is past what the unroller
@@ -565,7 +566,7 @@ __device__ __forceinline__ void store_tile(const GemmParams& p, f32x16 (&acc)[TM
             *(lds_f32x4*)(st + lcol * PITCH + (jj * 32 + gi * 8 + lrow) * 4) =
                 f32x4{acc[i][j][4 * gi], acc[i][j][4 * gi + 1], acc[i][j][4 * gi + 2], acc[i][j][4 * gi + 3]};
         }
-        const int row0 = m0 + slice_row<WM, HALVES>(wm, i);
+        const int row0 = m0 + wm * WM + i * 32;
         const int col0 = n0 + wn * WN + jb * JH * 32;
         const int col = col0 + ch * OPC, cb = min(col, p.N - OPC);  // N is a multiple of 8
         const int64_t cbase = static_cast<int64_t>(row0) * p.ldc + col0;
