@@ -1004,7 +1004,7 @@ def _gate(name: str, gate, gate_rows, T: int, H: int) -> tuple[int | None, int]:
     per = max(T, 1) if gate_rows is None else int(gate_rows)
     if per <= 0:
         raise KernelError(f"{name}: gate_rows must be positive, got {gate_rows}")
-    return _dense(name, "gate", gate, torch.float32, (-(-T // per), H) if T else (gate.shape[0], H)), per
+    return _dense(name, "gate", gate, torch.float32, (-(-T // per) if T else _size2(name, "gate", gate)[0], H)), per
 
 
 def norm_residual(y, resid, out, *, eps, post=None, gate=None, gate_rows=None, scale=1.0, pre=None, normed=None) -> None:

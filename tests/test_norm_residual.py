@@ -487,3 +487,11 @@ def test_bindings_refuse():
             lambda: K.norm_residual(y, r, r, eps=EPS)):  # (host tensors)
         with pytest.raises(KernelError):
             call()
+
+
+def test_the_gate_of_no_rows_is_a_matrix():
+    """Also where there is no row to apply it to."""
+    y, r = torch.zeros(0, 8, dtype=BF), torch.zeros(0, 8)
+    for gate in (torch.tensor(1.0), torch.ones(8), torch.ones(1, 1, 8), torch.ones(1, 4)):
+        with pytest.raises(KernelError, match="gate must be"):
+            K.norm_residual(y, r, r, eps=EPS, gate=gate)
