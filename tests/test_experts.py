@@ -543,6 +543,43 @@ def test_offsets_past_32_bits():
         within(dw[e], want, 300 * 2.0 ** -24 * mag + rounding(want, F32), "far rows' gradients")
 
 
+# (rows, N, experts), a way of products each
+FAR = {"few": (40, 72, 12), "small": (1500, 264, 3), "large": (8192, 2048, 2)}
+
+
+def test_far_products_take_every_way():
+    for way, (R, N, E) in FAR.items():
+        assert K.gemm_experts_plan("nt", "bf16", E, R, N, 2048)[0] == way
+        assert K.gemm_experts_plan("nt", "swiglu", E, R, 2 * N // 64 * 64, 2048)[0] == way
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", FAR)
+def test_rows_at_an_index_up_to_4_gib(way):
+    """The same bits as of those rows side by side, to the last row that an index reaches."""
+    R, N, E = FAR[way]
+    rows, H, near = 2 ** 20 - 1, 2048, 500
+    x = torch.zeros(rows, H, dtype=BF, device=dev())
+    x[:near], x[rows - near:] = normal(near, H, seed=1).to(BF), normal(near, H, seed=2).to(BF)
+    x[2 ** 19 - near:2 ** 19 + near] = normal(2 * near, H, seed=3).to(BF)  # either side of 2^31 bytes
+    pick = torch.randint(0, 4 * near, (R,), generator=torch.Generator().manual_seed(4)).to(dev())
+    pick[0], pick[-1] = 4 * near - 1, 0
+    index = torch.cat([torch.arange(near), torch.arange(2 ** 19 - near, 2 ** 19 + near), torch.arange(rows - near, rows)]).to(dev())[pick]
+    side = x[index]
+    assert not bool((side.abs().amax(1) == 0).any())
+    off = offsets_of([R // E] * (E - 1) + [R - R // E * (E - 1)])
+    b = normal(E, N, H, seed=5, std=H ** -0.5).to(BF)
+    got, want = torch.full((R, N), 7.0, dtype=BF, device=dev()), torch.full((R, N), 5.0, dtype=BF, device=dev())
+    K.gemm_experts("nt", x, b, got, offsets=off, rows=index.to(I32))
+    K.gemm_experts("nt", side, b, want, offsets=off)
+    assert torch.equal(got, want)
+    n = N // 64 * 32
+    act, same = torch.full((R, n), 7.0, dtype=BF, device=dev()), torch.full((R, n), 5.0, dtype=BF, device=dev())
+    K.gemm_experts_swiglu(x, b[:, :2 * n], act, offsets=off, rows=index.to(I32))
+    K.gemm_experts_swiglu(side, b[:, :2 * n], same, offsets=off)
+    assert torch.equal(act, same)
+
+
 # -------------------------------------------------------------- an expert MLP --
 
 class ExpertMLP:
