@@ -475,7 +475,8 @@ __global__ __launch_bounds__(256) void combine_kernel(RowsParams p) {
 
 // W waves to a token: each of its rows is read once for its dot product and written
 // once, x from the caches after its first reading. Bound by HBM: 4005 tokens, 2 rows of
-// 3584 each, with the dots 41 us (4.2 TB/s), 16384 of 8 of 2048 272 (4.5).
+// 3584 each, with the dots 41 us (4.2 TB/s), 16384 of 8 of 2048 272 (4.5) and 123 (4.9)
+// without them.
 template <int DX, int DY, int V, int W>
 __global__ __launch_bounds__(256) void spread_kernel(RowsParams p) {
   __shared__ float smem[4][kAtOnce];

@@ -47,7 +47,9 @@ struct Grouped {
 // 8 MFMAs, which take columns 8 apart (one v_perm a register).
 // Bound by the weights' bytes: 8 tokens of 8 of 64 experts of 2 x 768 x 2048 40 us (6.6
 // TB/s, part of it from the last-level cache; on 128 x 128 tiles 47), one token each of
-// 8 experts of 3584 x 4864 34 (72).
+// 8 experts of 3584 x 4864 34 (72). Where a long K has few columns beside it there are
+// fewer blocks than CUs, and a block's steps bound it: 8 tokens of 2 of 8 experts of 896 x
+// 4864 22 us, 14 at the weights' rate.
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -230,7 +232,10 @@ int64_t real_tiles_of(bool ak, int64_t bm, int64_t bn, int64_t experts, int64_t 
 }
 
 // How a grouped product runs. The row counts are on the device alone, so this goes by
-// their average; half a tile's rows of an expert's last tile are taken to be empty.
+// their average; half a tile's rows of an expert's last tile are taken to be empty. Rows
+// that all go to one expert cost less than the same number dealt evenly, whichever way
+// is taken: gate/up of 2 x 768 x 2048, 64 experts, 256 rows (FEW) 21 and 71 us, 512 rows
+// (FEW) 31 and 73, 4096 (SMALL) 31 and 96, 131072 of 128 experts (BIG) 650 and 685.
 // FEW (few_rows_kernel): at most 4 rows an expert, or 14 where 128 x 128 tiles make less
 //   than three rounds of them, or no more of its blocks than two a CU (64 experts of 2 x
 //   768 x 2048: 4 rows 59 us, on tiles 87; 10 rows 70 and 91; 32 rows 142 and 97).

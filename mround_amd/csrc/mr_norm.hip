@@ -78,7 +78,9 @@ __device__ __forceinline__ void load_weights(const float* w, int c, float (&out)
 
 // Thread t holds the pieces t, t + threads, .. (P of them) of its row. As many
 // blocks as the card holds go over the rows in turn. Bound by HBM:
-// 4005 x 2048 bf16 onto fp32 22.6 us (4.3 TB/s), 16384 x 3584 143 (4.9).
+// 4005 x 2048 bf16 onto fp32 22.6 us (4.3 TB/s), 16384 x 3584 143 (4.9), 4096 x 16384
+// 164 (4.9). Of rows of no whole 16 bytes past 8192 columns the registers of 16 columns a
+// thread bound it, 57 to 75 of them spilled: 4096 x 16383 358, x 8191 80.
 template <int A, int S, int V, int P, int THREADS>
 __global__ __launch_bounds__(THREADS) void norm_fwd(NormParams p) {
   __shared__ float smem[3][16];
@@ -183,8 +185,13 @@ __device__ __forceinline__ void block_sum2(float& a, float& b, float (*smem)[16]
 // differs by factors that are a group's own, dh n: one sum serves both, and the
 // factors come in when the group ends.
 // The registers of P = 1 are held to those of four waves a SIMD where they fit, two
-// rows of up to 512 pieces a CU, with the next row's loads in flight (AHEAD); rows
-// past 1024 pieces leave no room for that.
+// rows of up to 512 pieces a CU, with the next row's loads in flight (AHEAD; of 16-bit
+// rows onto fp32 5 registers are spilled for it, in the 228 us). Rows past 1024 pieces
+// leave no room for that, and registers bound them: a thread of 1024 has 128, and of
+// its weights, sums and inputs of 16 columns 116 to 262 are spilled (4096 x 8192 150 us,
+// x 8200 408, x 12288 484, x 16384 609, 2.0 TB/s). One column at a time 23 to 114 are
+// where a thread holds 8 and 272 to 470 where it holds 16 (4096 x 8191 266 us, x 12287
+// 1399, x 16383 1702).
 constexpr int waves_for(int A, int V, int P, bool WHOLE) {
   return V == 1 ? 4 : P == 1 ? (A == MR_F32 || WHOLE ? 3 : 4) : 2;
 }
