@@ -337,7 +337,8 @@ int check_grouped(const char* fn, const Grouped& g, bool ak, bool bkm, int es) {
     return fail(MR_EINVAL, ak ? "%s: N must be a multiple of 8 and K a positive multiple of 64 (N=%lld K=%lld)"
                               : "%s: N and M must be multiples of 8 (N=%lld M=%lld)",
                 fn, static_cast<long long>(g.N), static_cast<long long>(ak ? g.K : g.M));
-  if (g.M > 0x7fffffff || g.N > 0x7fffffff || g.K > 0x7fffffff || g.experts > 0x7ffffffe)
+  // (K in whole k-tiles is a 31-bit number too; tiles of that many rows are more than a launch has)
+  if (g.M > 0x7fffffff || g.N > 0x7fffffff || g.K > 0x7fffffff - (BK - 1) || g.experts > 0x7ffffffe)
     return fail(MR_EINVAL, "%s: too large", fn);
   if (g.lda > kMaxLd || g.ldb > kMaxLd || g.ldc > kMaxLd || g.ldgu > kMaxLd)
     return fail(MR_EINVAL, "%s: leading dimensions above %d are not supported", fn, kMaxLd);

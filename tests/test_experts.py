@@ -882,6 +882,15 @@ def test_products_refuse(base, change, message):
     refused("mr_gemm_experts", list(dict(base, **change).values()), message)
 
 
+def test_weight_products_refuse_rows_whose_tiles_end_past_31_bits():
+    """An expert with every row has k-tiles of 64 up to the next multiple of 64."""
+    far = {n: ctypes.c_void_p((i + 1) << 40) for i, n in enumerate(("A", "B", "off", "C"))}
+    base = dict(TN, **far, M=8, N=8, lda=8, ldb=8, ldc=8, c_step=64)
+    for rows in (2 ** 31 - 63, 2 ** 31 - 1):
+        refused("mr_gemm_experts", list(dict(base, K=rows).values()), "too large")
+    refused("mr_gemm_experts", list(dict(base, K=2 ** 31 - 64, c_step=56).values()), "overlap")
+
+
 SWIGLU = dict(E=4, M=100, N=64, K=128, X=address(0), ldx=128, index=None, rows=0, W=address(1), ldw=128, step=128 * 128,
               off=address(2), act=address(3), ldact=64, gu=address(4), ldgu=128, ws=None, ws_bytes=0, stream=None)
 SWIGLU_BWD = dict(E=4, M=100, N=64, K=128, dy=address(0), ldd=128, W=address(1), ldw=64, step=128 * 64, off=address(2),
